@@ -64,7 +64,7 @@
 extern "C" {
 #endif
 
-#define NKV_ABI_VERSION 8
+#define NKV_ABI_VERSION 9
 
 enum nkv_status {
     NKV_OK = 0,
@@ -749,6 +749,162 @@ typedef struct nkv_finish_args {
 } nkv_finish_args;
 
 int nkv_finish(void* stream, const nkv_finish_args* args);
+
+/*
+ * The 8-bit key/value cache (no counterpart in the reference, whose caches are
+ * codec payloads): the K and V rows of B batch items and H key heads in 8
+ * bits with one fp32 scale for each block of 64 rows and head; value = code *
+ * scale.  Row n of head h of item b is k[((b*H + h)*cap + n)*P + d], d < D,
+ * with P = 64 for D <= 64 and 128 above (columns D .. P hold zero), and its
+ * scale k_scale[(b*H + h)*(cap/64) + n/64]; v likewise.  D % 8 == 0, D <= 128;
+ * cap % 64 == 0, cap < 2^31.  k and v are 16-byte aligned.
+ * The caller keeps each item's length.  Rows at or past it may hold anything:
+ * no call lets them into a result.
+ */
+#define NKV_CACHE8_BLOCK 64
+enum nkv_cache8_format { NKV_CACHE8_INT8 = 0, NKV_CACHE8_E4M3 = 1 };
+enum nkv_row_dtype { NKV_ROWS_BF16 = 0, NKV_ROWS_FP16 = 1, NKV_ROWS_FP32 = 2 };
+
+typedef struct nkv_cache8 {
+    void* k;                      /* [B, H, cap, P] codes */
+    void* v;
+    float* k_scale;               /* [B, H, cap/64] */
+    float* v_scale;
+    int64_t cap;
+    int B;
+    int H;
+    int D;
+    int format;                   /* nkv_cache8_format */
+} nkv_cache8;
+
+/*
+ * Writes T new rows per item behind the `start` rows it has: row t of k and v
+ * ([B, T, H, D] of dtype, addressed as k[b*k_sb + t*k_st + h*k_sh + d]) goes
+ * to row start + t.  Per block and head, over the new rows' finite values:
+ *   s = max(amax|x|, 2^-64) / TOP       TOP = 127 (int8), 448 (e4m3)
+ * rounded once (IEEE fp32 division); a block that holds rows before `start`
+ * keeps its scale s0 if that is larger, and its codes become round(code *
+ * (s0 / s)) if it is not.  New codes are round(x / s) to the nearest, ties to
+ * even; infinities give the largest code, NaN zero.  Rows past those written
+ * are left as they were (a block's scale may have grown over them).
+ * start_dev (device, [B]; NULL: `start` for every item) is clamped to [0,
+ * cap]; counts (device, [B]; NULL: T for every item) says how many of an
+ * item's rows are written.  Rows past cap are dropped where start or counts
+ * are in device memory, and refused where start is not.
+ * k and v are 16-byte aligned with strides divisible by 8.
+ */
+typedef struct nkv_cache8_write_args {
+    nkv_cache8 cache;
+    const void* k;
+    int64_t k_sb, k_st, k_sh;
+    const void* v;
+    int64_t v_sb, v_st, v_sh;
+    int64_t T;
+    int64_t start;
+    const int32_t* start_dev;
+    const int32_t* counts;
+    int dtype;                    /* nkv_row_dtype */
+    int _pad;
+} nkv_cache8_write_args;
+
+int nkv_cache8_write(void* stream, const nkv_cache8_write_args* args);
+
+/*
+ * Attention of q [B, Q, H*G, D] (bf16 or fp16; q[b*q_sb + t*q_st + h*q_sh + d])
+ * over a cache: query head h reads key head h / G, softmax(q k^T *
+ * softmax_scale) v over the item's first `length` rows; with causal, query t
+ * sees the first length - Q + 1 + t of them (the queries are the last Q
+ * tokens).  A query that sees no key gets out = 0 and lse = -inf.
+ *   out  [B, Q, H*G, D] of q's type (o_sb/o_st/o_sh)
+ *   lse  [B, H*G, Q] fp32 natural-log row log-sum-exp, or NULL
+ * length: device [B], clamped to [0, n] (NULL: n for every item); n <= cap is
+ * also what the work is divided by.  Scores, softmax and sums are fp32; the
+ * probabilities are rounded to q's type for their product with the codes.
+ * q and out are 16-byte aligned with strides divisible by 8.
+ */
+typedef struct nkv_cache8_attend_args {
+    nkv_cache8 cache;
+    int G;
+    int dtype;                    /* NKV_ROWS_BF16 or NKV_ROWS_FP16 */
+    int64_t Q;
+    int64_t n;
+    const int32_t* length;
+    const void* q;
+    int64_t q_sb, q_st, q_sh;
+    void* out;
+    int64_t o_sb, o_st, o_sh;
+    float* lse;
+    float softmax_scale;
+    int causal;
+} nkv_cache8_attend_args;
+
+/* Bytes of workspace nkv_cache8_attend needs for these arguments (0 if none);
+ * a smaller one fails with NKV_ERR_WORKSPACE and launches nothing. */
+size_t nkv_cache8_attend_workspace_size(const nkv_cache8_attend_args* args);
+int nkv_cache8_attend(void* stream, const nkv_cache8_attend_args* args, void* workspace,
+                      size_t workspace_bytes);
+
+/*
+ * The attention weight each cached row receives:
+ *   out[b, h, n] = mass[b, h, n] + sum over the queries that see row n, and
+ *                  the G query heads of h, of exp(q.k_n * softmax_scale - lse)
+ * with lse of nkv_cache8_attend on the same arguments (a row with lse = -inf
+ * adds nothing).  mass and out are [B, H, cap] fp32 and may be the same
+ * array, whose entries past the length are then not touched (otherwise they
+ * are copied).  Deterministic: no atomics.
+ */
+typedef struct nkv_cache8_mass_args {
+    nkv_cache8 cache;             /* v and v_scale are not read */
+    int G;
+    int dtype;
+    int64_t Q;
+    int64_t n;
+    const int32_t* length;
+    const void* q;
+    int64_t q_sb, q_st, q_sh;
+    const float* lse;             /* [B, H*G, Q] */
+    const float* mass;
+    float* out;
+    float softmax_scale;
+    int causal;
+} nkv_cache8_mass_args;
+
+size_t nkv_cache8_mass_workspace_size(const nkv_cache8_mass_args* args);
+int nkv_cache8_mass(void* stream, const nkv_cache8_mass_args* args, void* workspace,
+                    size_t workspace_bytes);
+
+/*
+ * Evicts tokens head by head: of an item longer than `keep`, each head keeps
+ * the first `sink` rows, the last `recent` and, of those between, the keep -
+ * sink - recent of the largest mass (equal masses: the lower row; NaN above
+ * all), in the order they had; a shorter one keeps all.  sink + recent <= keep.
+ * The kept rows go to the front of `out`, another cache of the same heads,
+ * width and format with out.cap >= keep: a block's scale there is the largest
+ * of its rows' scales, and a row whose scale was smaller gets codes round(code
+ * * (s0 / s)) (rows that had the block's scale keep their codes).
+ *   out_mass    [B, H, out.cap] fp32, the kept rows' masses
+ *   rows        [B, H, keep] int32, the rows kept, -1 past the last
+ *   out_length  [B] int32, min(length, keep)
+ * Rows of out and out_mass past the kept ones are left as they were.  Nothing
+ * of out or out_mass may overlap the cache or mass.
+ */
+typedef struct nkv_cache8_evict_args {
+    nkv_cache8 cache;
+    nkv_cache8 out;
+    const float* mass;            /* [B, H, cap] */
+    float* out_mass;
+    int32_t* rows;
+    int32_t* out_length;
+    const int32_t* length;        /* device [B], or NULL: n */
+    int64_t n;
+    int64_t keep;
+    int64_t sink;
+    int64_t recent;
+} nkv_cache8_evict_args;
+
+size_t nkv_cache8_evict_workspace_size(const nkv_cache8_evict_args* args);
+int nkv_cache8_evict(void* stream, const nkv_cache8_evict_args* args, void* workspace,
+                     size_t workspace_bytes);
 
 #ifdef __cplusplus
 }

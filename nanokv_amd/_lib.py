@@ -13,7 +13,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libnanokv_hip.so"
 
-NKV_ABI_VERSION = 8
+NKV_ABI_VERSION = 9
 NKV_OK = 0
 NKV_ERR_INVALID = -1
 NKV_ERR_UNSUPPORTED = -2
@@ -27,6 +27,12 @@ NKV_QUANT_BF16 = 1
 NKV_SCHEDULE_AUTO = 0
 NKV_SCHEDULE_QUERY_TILES = 1
 NKV_SCHEDULE_KEY_CHUNKS = 2
+NKV_CACHE8_BLOCK = 64
+NKV_CACHE8_INT8 = 0
+NKV_CACHE8_E4M3 = 1
+NKV_ROWS_BF16 = 0
+NKV_ROWS_FP16 = 1
+NKV_ROWS_FP32 = 2
 
 # Every symbol include/nanokv.h declares (checked by tests/test_abi.py).
 EXPORTED = (
@@ -36,6 +42,9 @@ EXPORTED = (
     "nkv_int8_dequant", "nkv_c64_fit_workspace_size", "nkv_c64_fit", "nkv_camera_apply",
     "nkv_attend_static", "nkv_lift_lse_combine", "nkv_finish", "nkv_reader_rows",
     "nkv_decode_batch", "nkv_c64_fit_rows", "nkv_encode_workspace_size",
+    "nkv_cache8_write", "nkv_cache8_attend_workspace_size", "nkv_cache8_attend",
+    "nkv_cache8_mass_workspace_size", "nkv_cache8_mass", "nkv_cache8_evict_workspace_size",
+    "nkv_cache8_evict",
 )
 NKV_STATIC_SCRATCH_BYTES = 64 << 20
 
@@ -197,6 +206,53 @@ class NanoKVError(RuntimeError):
         self.code = code
 
 
+
+class NkvCache8(Structure):
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("cap", c_int64), ("B", c_int), ("H", c_int), ("D", c_int), ("format", c_int),
+    ]
+
+
+class NkvCache8WriteArgs(Structure):
+    _fields_ = [
+        ("cache", NkvCache8),
+        ("k", c_void_p), ("k_sb", c_int64), ("k_st", c_int64), ("k_sh", c_int64),
+        ("v", c_void_p), ("v_sb", c_int64), ("v_st", c_int64), ("v_sh", c_int64),
+        ("T", c_int64), ("start", c_int64), ("start_dev", c_void_p), ("counts", c_void_p),
+        ("dtype", c_int), ("_pad", c_int),
+    ]
+
+
+class NkvCache8AttendArgs(Structure):
+    _fields_ = [
+        ("cache", NkvCache8), ("G", c_int), ("dtype", c_int), ("Q", c_int64), ("n", c_int64),
+        ("length", c_void_p),
+        ("q", c_void_p), ("q_sb", c_int64), ("q_st", c_int64), ("q_sh", c_int64),
+        ("out", c_void_p), ("o_sb", c_int64), ("o_st", c_int64), ("o_sh", c_int64),
+        ("lse", c_void_p), ("softmax_scale", c_float), ("causal", c_int),
+    ]
+
+
+class NkvCache8MassArgs(Structure):
+    _fields_ = [
+        ("cache", NkvCache8), ("G", c_int), ("dtype", c_int), ("Q", c_int64), ("n", c_int64),
+        ("length", c_void_p),
+        ("q", c_void_p), ("q_sb", c_int64), ("q_st", c_int64), ("q_sh", c_int64),
+        ("lse", c_void_p), ("mass", c_void_p), ("out", c_void_p),
+        ("softmax_scale", c_float), ("causal", c_int),
+    ]
+
+
+class NkvCache8EvictArgs(Structure):
+    _fields_ = [
+        ("cache", NkvCache8), ("out", NkvCache8),
+        ("mass", c_void_p), ("out_mass", c_void_p), ("rows", c_void_p), ("out_length", c_void_p),
+        ("length", c_void_p),
+        ("n", c_int64), ("keep", c_int64), ("sink", c_int64), ("recent", c_int64),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -264,6 +320,16 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.nkv_lift_lse_combine.argtypes = [c_void_p, POINTER(NkvLiftCombineArgs)]
     lib.nkv_finish.restype = c_int
     lib.nkv_finish.argtypes = [c_void_p, POINTER(NkvFinishArgs)]
+    lib.nkv_cache8_write.restype = c_int
+    lib.nkv_cache8_write.argtypes = [c_void_p, POINTER(NkvCache8WriteArgs)]
+    for name, args in (("attend", NkvCache8AttendArgs), ("mass", NkvCache8MassArgs),
+                       ("evict", NkvCache8EvictArgs)):
+        size = getattr(lib, f"nkv_cache8_{name}_workspace_size")
+        size.restype = c_size_t
+        size.argtypes = [POINTER(args)]
+        run = getattr(lib, f"nkv_cache8_{name}")
+        run.restype = c_int
+        run.argtypes = [c_void_p, POINTER(args), c_void_p, c_size_t]
 
 
 def lib() -> ctypes.CDLL:

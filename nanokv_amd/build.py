@@ -37,6 +37,9 @@ SOURCES = {
     # RoPE rounds every fp64 product and sum separately, as the oracle does
     "nkv_rope.hip": ["-ffp-contract=off"],
     "nkv_camera.hip": ["-ffp-contract=off"],
+    # 8-bit codes are a function of their inputs to the last bit
+    "nkv_cache8.hip": ["-ffp-contract=off"],
+    "nkv_cache8_attend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 COMMON = [

@@ -1,0 +1,128 @@
+// nkv_cache8.h -- types and conversions shared by the kernels of the 8-bit
+// key/value cache (nkv_cache8.hip, nkv_cache8_attend.hip).
+//
+// A cache holds, per batch item and key head, `cap` rows of 8-bit codes at a
+// pitch of P = 64 or 128 bytes (the head width D rounded up, the columns past
+// D zero) and one fp32 scale for each block of 64 rows: value = code * scale.
+#pragma once
+
+#include "nkv_common.h"
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+namespace nkv {
+
+constexpr int C8_BLOCK = 64;                   // rows that share a scale
+constexpr float C8_TINY = 0x1p-64f;            // the least amplitude a scale stands for
+
+__host__ __device__ constexpr int c8_pitch(int D) { return D <= 64 ? 64 : 128; }
+
+template <int FMT>
+struct Fmt8 {
+    static constexpr float TOP = FMT == NKV_CACHE8_INT8 ? 127.0f : 448.0f;
+};
+
+// Four values, already divided by their scale, as four codes: to the nearest,
+// ties to even, clamped to the largest code; NaN gives the zero code, so that
+// a cache never holds anything but finite numbers.
+template <int FMT>
+__device__ __forceinline__ uint32_t to_codes(float a, float b, float c, float d) {
+    float x[4] = {a, b, c, d};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[i] = x[i] == x[i] ? x[i] : 0.0f;
+        x[i] = fminf(fmaxf(x[i], -Fmt8<FMT>::TOP), Fmt8<FMT>::TOP);
+    }
+    if constexpr (FMT == NKV_CACHE8_INT8) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w |= ((uint32_t)(int)rintf(x[i]) & 0xffu) << (8 * i);
+        return w;
+    } else {
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
+    }
+}
+
+// The values of codes 2 h and 2 h + 1 of a word (exact).
+template <int FMT>
+__device__ __forceinline__ f32x2 code_pair(uint32_t w, int h) {
+    if constexpr (FMT == NKV_CACHE8_INT8) {
+        return f32x2{(float)(int8_t)(w >> (16 * h)), (float)(int8_t)(w >> (16 * h + 8))};
+    } else {
+        return h ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true)
+                 : __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+    }
+}
+
+// The 16-bit types of queries and outputs.  Both hold every code exactly, so
+// products of queries and codes are formed in the queries' own type.
+struct Bf16 {
+    using x8 = bf16x8;
+    static constexpr int DTYPE = NKV_ROWS_BF16;
+    static __device__ __forceinline__ float load(uint16_t b) { return bf16_bits_to_f32(b); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
+    static __device__ __forceinline__ f32x4 mfma16(x8 a, x8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+};
+
+struct Fp16 {
+    using x8 = f16x8;
+    static constexpr int DTYPE = NKV_ROWS_FP16;
+    static __device__ __forceinline__ float load(uint16_t b) { return f16_bits_to_f32(b); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        f16x2 v;
+        v[0] = (_Float16)a;
+        v[1] = (_Float16)b;
+        uint32_t u;
+        __builtin_memcpy(&u, &v, 4);
+        return u;
+    }
+    static __device__ __forceinline__ f32x4 mfma16(x8 a, x8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+template <typename X8>
+__device__ __forceinline__ X8 as_x8(u32x4 v) {
+    X8 r;
+    __builtin_memcpy(&r, &v, 16);
+    return r;
+}
+
+// Eight consecutive codes as an MFMA operand of type T.
+template <typename T, int FMT>
+__device__ __forceinline__ typename T::x8 codes_x8(uint32_t lo, uint32_t hi) {
+    const f32x2 a = code_pair<FMT>(lo, 0), b = code_pair<FMT>(lo, 1);
+    const f32x2 c = code_pair<FMT>(hi, 0), d = code_pair<FMT>(hi, 1);
+    return as_x8<typename T::x8>(
+        u32x4{T::pack(a[0], a[1]), T::pack(b[0], b[1]), T::pack(c[0], c[1]), T::pack(d[0], d[1])});
+}
+
+// Sequence length of batch item b: its own entry clamped to [0, n], or n.
+__device__ __forceinline__ int c8_length(const int32_t* length, int b, int n) {
+    return length ? min(max(length[b], 0), n) : n;
+}
+
+// max / sum over the four 16-lane rows of a wave (lanes l, l ^ 16, l ^ 32,
+// l ^ 48): v_permlane16_swap exchanges odd rows of one copy with even rows of
+// the other, so the pair holds both rows' values in either order.
+__device__ __forceinline__ float rows4_max(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                    false);
+    return halfwave_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+
+__device__ __forceinline__ float rows4_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                    false);
+    return halfwave_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// Validates a cache and its shapes (host).
+int cache8_check(const nkv_cache8* c, const char* who);
+
+}  // namespace nkv

@@ -1,0 +1,438 @@
+// nkv_cache8.hip -- the 8-bit key/value cache: writing rows into it and
+// evicting rows from it (nkv_cache8_write, nkv_cache8_evict).
+//
+// Compiled without fp contraction: codes are a function of their inputs to the
+// last bit (IEEE division by the scale, one rounding to the code).
+#include "nkv_cache8.h"
+
+#include <math.h>
+
+#include <algorithm>
+
+namespace nkv {
+
+int cache8_check(const nkv_cache8* c, const char* who) {
+    auto bad = [&](int code, const char* what) {
+        set_error(std::string(who) + ": " + what);
+        return code;
+    };
+    if (c->B < 0 || c->H < 1 || c->D < 1) return bad(NKV_ERR_INVALID, "cache needs B >= 0, H >= 1, D >= 1");
+    if (c->D % 8 || c->D > 128)
+        return bad(NKV_ERR_UNSUPPORTED, "head width must be a multiple of 8, at most 128");
+    if (c->format != NKV_CACHE8_INT8 && c->format != NKV_CACHE8_E4M3)
+        return bad(NKV_ERR_INVALID, "unknown cache format");
+    if (c->cap < C8_BLOCK || c->cap % C8_BLOCK || c->cap > INT32_MAX - C8_BLOCK)
+        return bad(NKV_ERR_INVALID, "cap must be a positive multiple of 64 below 2^31");
+    if ((int64_t)c->B * c->H > INT32_MAX / 4) return bad(NKV_ERR_UNSUPPORTED, "too many heads");
+    if (c->B == 0) return NKV_OK;
+    if (!c->k || !c->v || !c->k_scale || !c->v_scale)
+        return bad(NKV_ERR_INVALID, "cache codes and scales are required");
+    if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) % 16)
+        return bad(NKV_ERR_INVALID, "cache codes must be 16-byte aligned");
+    return NKV_OK;
+}
+
+namespace {
+
+// ---------------------------------------------------------------- write
+struct WriteParams {
+    uint8_t* codes[2];            // K, V
+    float* scale[2];
+    const void* x[2];
+    int64_t sb[2], st[2], sh[2];
+    const int32_t* start_dev;
+    const int32_t* counts;
+    int64_t cap;
+    int64_t start;
+    int64_t T;
+    int B, H, D;
+};
+
+// Eight consecutive elements of a row as fp32.
+template <int DTYPE>
+__device__ __forceinline__ void load8(const void* x, int64_t at, float (&f)[8]) {
+    if constexpr (DTYPE == NKV_ROWS_FP32) {
+        const f32x4* p = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(x) + at);
+        const f32x4 a = p[0], b = p[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = a[i], f[4 + i] = b[i];
+    } else {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(x) + at);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint16_t u = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+            f[i] = DTYPE == NKV_ROWS_BF16 ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
+        }
+    }
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
+    return x;
+}
+
+// One workgroup per (block of 64 rows, head, K or V, item): the block's new
+// rows are read once into registers, eight elements a thread and piece, their
+// amplitude is reduced, and the codes are written.  Bound by HBM: three bytes
+// move per bf16 element.
+template <int DTYPE, int FMT, int P>
+__global__ void __launch_bounds__(256) write_kernel(WriteParams p) {
+    constexpr int CH = P / 8, STEP = 256 / CH, N = C8_BLOCK / STEP;
+    const int kv = blockIdx.z & 1, b = blockIdx.z >> 1, h = blockIdx.y;
+    const int64_t start =
+        p.start_dev ? min(max((int64_t)p.start_dev[b], (int64_t)0), p.cap) : p.start;
+    const int64_t count = p.counts ? min(max((int64_t)p.counts[b], (int64_t)0), p.T) : p.T;
+    const int64_t end = min(start + count, p.cap);
+    const int64_t blk = start / C8_BLOCK + blockIdx.x;
+    const int64_t row0 = blk * C8_BLOCK;               // the block's first row
+    if (row0 >= end || start >= end) return;
+    const int64_t bh = (int64_t)b * p.H + h;
+    uint8_t* codes = p.codes[kv] + (bh * p.cap + row0) * P;
+    float* scale = p.scale[kv] + bh * (p.cap / C8_BLOCK) + blk;
+    const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
+    const int lo = (int)max(start - row0, (int64_t)0), hi = (int)min(end - row0, (int64_t)C8_BLOCK);
+    float x[N][8];
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int r = r0 + STEP * i;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
+        if (r >= lo && r < hi && 8 * c < p.D)
+            load8<DTYPE>(p.x[kv], b * p.sb[kv] + (row0 + r - start) * p.st[kv] + h * p.sh[kv] + 8 * c,
+                         x[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float a = fabsf(x[i][e]);
+            top = fmaxf(top, a < INFINITY ? a : 0.0f);  // finite values alone
+        }
+    __shared__ float part[4];
+    top = wave_max(top);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    float s = fmaxf(top, C8_TINY) / Fmt8<FMT>::TOP;
+    if (lo > 0) {
+        const float s0 = *scale;
+        if (s0 >= s) {
+            s = s0;
+        } else {
+            const float ratio = s0 / s;
+            for (int r = r0; r < lo; r += STEP) {
+                u32x2* at = reinterpret_cast<u32x2*>(codes + r * P + 8 * c);
+                u32x2 w = *at;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const f32x2 a = code_pair<FMT>(w[k], 0), d = code_pair<FMT>(w[k], 1);
+                    w[k] = to_codes<FMT>(a[0] * ratio, a[1] * ratio, d[0] * ratio, d[1] * ratio);
+                }
+                *at = w;
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int r = r0 + STEP * i;
+        if (r < lo || r >= hi) continue;
+        const float(&f)[8] = x[i];
+        u32x2 w;
+        w[0] = to_codes<FMT>(f[0] / s, f[1] / s, f[2] / s, f[3] / s);
+        w[1] = to_codes<FMT>(f[4] / s, f[5] / s, f[6] / s, f[7] / s);
+        *reinterpret_cast<u32x2*>(codes + r * P + 8 * c) = w;
+    }
+    __syncthreads();  // every thread has read the old scale
+    if (threadIdx.x == 0) *scale = s;
+}
+
+template <int DTYPE>
+void write_launch(const WriteParams& p, int format, dim3 grid, hipStream_t s) {
+    const bool wide = c8_pitch(p.D) == 128;
+    if (format == NKV_CACHE8_INT8) {
+        if (wide) write_kernel<DTYPE, NKV_CACHE8_INT8, 128><<<grid, 256, 0, s>>>(p);
+        else write_kernel<DTYPE, NKV_CACHE8_INT8, 64><<<grid, 256, 0, s>>>(p);
+    } else {
+        if (wide) write_kernel<DTYPE, NKV_CACHE8_E4M3, 128><<<grid, 256, 0, s>>>(p);
+        else write_kernel<DTYPE, NKV_CACHE8_E4M3, 64><<<grid, 256, 0, s>>>(p);
+    }
+}
+
+// ---------------------------------------------------------------- evict
+struct EvictParams {
+    const uint8_t* codes[2];
+    const float* scale[2];
+    uint8_t* out[2];
+    float* out_scale[2];
+    const float* mass;
+    float* out_mass;
+    int32_t* rows;
+    int32_t* out_length;
+    const int32_t* length;
+    int64_t cap, out_cap;
+    int B, H, n, keep, sink, recent;
+};
+
+// A mass as an integer that orders as the masses do: NaN above all, -0 as +0.
+__device__ __forceinline__ uint32_t order_key(float x) {
+    if (x != x) return 0xffffffffu;
+    uint32_t u = __float_as_uint(x);
+    if (u == 0x80000000u) u = 0;
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+constexpr int SEL_THREADS = 1024;
+
+// One workgroup per (item, head): the key of the last row kept is found digit
+// by digit (8 bits a pass, counts in LDS), then the kept rows are listed in
+// order, those equal to the last key from the lowest up.
+__global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
+    const int b = blockIdx.x / p.H;
+    const int64_t bh = blockIdx.x;
+    const int n = c8_length(p.length, b, p.n);
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    int32_t* rows = p.rows + bh * p.keep;
+    if (blockIdx.x % p.H == 0 && tid == 0) p.out_length[b] = min(n, p.keep);
+    if (n <= p.keep) {
+        for (int i = tid; i < p.keep; i += SEL_THREADS) rows[i] = i < n ? i : -1;
+        return;
+    }
+    const float* mass = p.mass + bh * p.cap;
+    const int lo = p.sink, hi = n - p.recent;
+    const int want = p.keep - p.sink - p.recent;
+    __shared__ uint32_t hist[256];
+    __shared__ uint32_t pick[2];  // digit, rows still wanted below it
+    uint32_t prefix = 0, left = want;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (tid < 256) hist[tid] = 0;
+        __syncthreads();
+        for (int i = lo + tid; i < hi; i += SEL_THREADS) {
+            const uint32_t k = order_key(mass[i]);
+            if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
+                atomicAdd(&hist[(k >> shift) & 255u], 1u);
+        }
+        __syncthreads();
+        if (tid == 0) {
+            // the digit at which the count from above reaches `left`
+            uint32_t above = 0;
+            int d = 255;
+            for (; d > 0 && above + hist[d] < left; --d) above += hist[d];
+            pick[0] = (uint32_t)d;
+            pick[1] = left - above;
+        }
+        __syncthreads();
+        prefix |= pick[0] << shift;
+        left = pick[1];
+        __syncthreads();
+    }
+    // `left` rows of key `prefix` are kept (none wanted: left = 0)
+    __shared__ uint32_t sums[2][SEL_THREADS / 64];
+    uint32_t base = 0, ties = 0;
+    for (int i0 = 0; i0 < n; i0 += SEL_THREADS) {
+        const int i = i0 + tid;
+        const bool in = i < n, fixed = in && (i < lo || i >= hi);
+        const uint32_t k = in && !fixed ? order_key(mass[i]) : 0;
+        const bool tie = in && !fixed && k == prefix;
+        const uint64_t tb = __ballot(tie);
+        if (lane == 0) sums[0][wave] = (uint32_t)__popcll(tb);
+        __syncthreads();
+        uint32_t before = ties, all = 0;
+        for (int w = 0; w < SEL_THREADS / 64; ++w) {
+            if (w < wave) before += sums[0][w];
+            all += sums[0][w];
+        }
+        const uint64_t below = (1ull << lane) - 1;
+        const uint32_t tr = before + (uint32_t)__popcll(tb & below);
+        const bool keep = fixed || (in && !fixed && want > 0 && (k > prefix || (tie && tr < left)));
+        const uint64_t kb = __ballot(keep);
+        if (lane == 0) sums[1][wave] = (uint32_t)__popcll(kb);
+        __syncthreads();
+        uint32_t at = base, kept = 0;
+        for (int w = 0; w < SEL_THREADS / 64; ++w) {
+            if (w < wave) at += sums[1][w];
+            kept += sums[1][w];
+        }
+        at += (uint32_t)__popcll(kb & below);
+        if (keep && at < (uint32_t)p.keep) rows[at] = i;
+        base += kept;
+        ties += all;
+        __syncthreads();
+    }
+}
+
+// One workgroup per (block of 64 kept rows, head, K or V, item): gathers the
+// rows' codes onto the largest of their scales.
+template <int FMT, int P>
+__global__ void __launch_bounds__(256) compact_kernel(EvictParams p) {
+    constexpr int CH = P / 8, STEP = 256 / CH, N = C8_BLOCK / STEP;
+    const int kv = blockIdx.z & 1, b = blockIdx.z >> 1, h = blockIdx.y;
+    const int left = min(c8_length(p.length, b, p.n), p.keep);
+    const int row0 = blockIdx.x * C8_BLOCK;
+    if (row0 >= left) return;
+    const int hi = min(left - row0, C8_BLOCK);
+    const int64_t bh = (int64_t)b * p.H + h;
+    __shared__ int src[C8_BLOCK];
+    __shared__ float from[C8_BLOCK];
+    __shared__ float top;
+    if (threadIdx.x < 64) {
+        const int r = threadIdx.x;
+        int at = 0;
+        float s = 0.0f;
+        if (r < hi) {
+            at = p.rows[bh * p.keep + row0 + r];
+            s = p.scale[kv][bh * (p.cap / C8_BLOCK) + at / C8_BLOCK];
+            if (kv == 0) p.out_mass[bh * p.out_cap + row0 + r] = p.mass[bh * p.cap + at];
+        }
+        src[r] = at;
+        from[r] = s;
+        const float m = wave_max(s);
+        if (r == 0) {
+            top = m;
+            p.out_scale[kv][bh * (p.out_cap / C8_BLOCK) + blockIdx.x] = m;
+        }
+    }
+    __syncthreads();
+    const uint8_t* codes = p.codes[kv] + bh * p.cap * P;
+    uint8_t* out = p.out[kv] + (bh * p.out_cap + row0) * P;
+    const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
+    const float s = top;
+    u32x2 w[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int r = r0 + STEP * i;
+        if (r < hi) w[i] = *reinterpret_cast<const u32x2*>(codes + (int64_t)src[r] * P + 8 * c);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int r = r0 + STEP * i;
+        if (r >= hi) continue;
+        const float s0 = from[r];
+        if (s0 != s) {
+            const float ratio = s0 / s;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const f32x2 a = code_pair<FMT>(w[i][k], 0), d = code_pair<FMT>(w[i][k], 1);
+                w[i][k] = to_codes<FMT>(a[0] * ratio, a[1] * ratio, d[0] * ratio, d[1] * ratio);
+            }
+        }
+        *reinterpret_cast<u32x2*>(out + r * P + 8 * c) = w[i];
+    }
+}
+
+struct Range {
+    uintptr_t lo, hi;
+    Range(const void* p, int64_t bytes)
+        : lo(reinterpret_cast<uintptr_t>(p)), hi(reinterpret_cast<uintptr_t>(p) + (uintptr_t)bytes) {}
+    bool meets(const Range& o) const { return lo < o.hi && o.lo < hi; }
+};
+
+int check_evict(const nkv_cache8_evict_args* a) {
+    NKV_REQUIRE(a, NKV_ERR_INVALID, "args is null");
+    int rc = cache8_check(&a->cache, __func__);
+    if (rc) return rc;
+    rc = cache8_check(&a->out, __func__);
+    if (rc) return rc;
+    const nkv_cache8 &c = a->cache, &o = a->out;
+    NKV_REQUIRE(c.B == o.B && c.H == o.H && c.D == o.D && c.format == o.format, NKV_ERR_INVALID,
+                "out must be a cache of the same items, heads, width and format");
+    NKV_REQUIRE(a->n >= 0 && a->n <= c.cap, NKV_ERR_INVALID, "n must be in [0, cap]");
+    NKV_REQUIRE(a->keep >= 1 && a->keep <= o.cap, NKV_ERR_INVALID, "keep must be in [1, out.cap]");
+    NKV_REQUIRE(a->sink >= 0 && a->recent >= 0 && a->sink <= a->keep && a->recent <= a->keep - a->sink,
+                NKV_ERR_INVALID, "sink + recent must be at most keep");
+    NKV_REQUIRE(c.H <= 65535 && c.B <= 32767, NKV_ERR_UNSUPPORTED, "too many heads or items");
+    if (c.B == 0) return NKV_OK;
+    NKV_REQUIRE(a->mass && a->out_mass && a->rows && a->out_length, NKV_ERR_INVALID,
+                "mass, out_mass, rows and out_length are required");
+    const int64_t heads = (int64_t)c.B * c.H, P = c8_pitch(c.D);
+    const Range in[5] = {{c.k, heads * c.cap * P}, {c.v, heads * c.cap * P},
+                         {c.k_scale, heads * c.cap / 16}, {c.v_scale, heads * c.cap / 16},
+                         {a->mass, heads * c.cap * 4}};
+    const Range out[6] = {{o.k, heads * o.cap * P}, {o.v, heads * o.cap * P},
+                          {o.k_scale, heads * o.cap / 16}, {o.v_scale, heads * o.cap / 16},
+                          {a->out_mass, heads * o.cap * 4}, {a->rows, heads * a->keep * 4}};
+    for (int i = 0; i < 6; ++i) {
+        for (const Range& r : in)
+            NKV_REQUIRE(!out[i].meets(r), NKV_ERR_INVALID, "the outputs overlap the cache or mass");
+        for (int j = 0; j < i; ++j)
+            NKV_REQUIRE(!out[i].meets(out[j]), NKV_ERR_INVALID, "the outputs overlap each other");
+    }
+    return NKV_OK;
+}
+
+}  // namespace
+}  // namespace nkv
+
+using namespace nkv;
+
+extern "C" int nkv_cache8_write(void* stream, const nkv_cache8_write_args* a) {
+    clear_error();
+    NKV_REQUIRE(a, NKV_ERR_INVALID, "args is null");
+    int rc = cache8_check(&a->cache, __func__);
+    if (rc) return rc;
+    const nkv_cache8& c = a->cache;
+    NKV_REQUIRE(a->T >= 0 && a->T <= INT32_MAX, NKV_ERR_INVALID, "T must be in [0, 2^31)");
+    NKV_REQUIRE(a->dtype >= NKV_ROWS_BF16 && a->dtype <= NKV_ROWS_FP32, NKV_ERR_INVALID,
+                "unknown row dtype");
+    if (!a->start_dev)
+        NKV_REQUIRE(a->start >= 0 && a->start <= c.cap && (a->counts || a->T <= c.cap - a->start),
+                    NKV_ERR_INVALID, "rows start .. start + T must lie in [0, cap]");
+    NKV_REQUIRE(c.H <= 65535 && c.B <= 32767, NKV_ERR_UNSUPPORTED, "too many heads or items");
+    if (c.B == 0 || a->T == 0) return NKV_OK;
+    NKV_REQUIRE(a->k && a->v, NKV_ERR_INVALID, "k and v are required");
+    NKV_REQUIRE((reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v)) % 16 == 0 &&
+                    (a->k_sb | a->k_st | a->k_sh | a->v_sb | a->v_st | a->v_sh) % 8 == 0,
+                NKV_ERR_INVALID, "k and v must be 16-byte aligned with strides divisible by 8");
+    WriteParams p{{(uint8_t*)c.k, (uint8_t*)c.v}, {c.k_scale, c.v_scale}, {a->k, a->v},
+                  {a->k_sb, a->v_sb}, {a->k_st, a->v_st}, {a->k_sh, a->v_sh},
+                  a->start_dev, a->counts, c.cap, a->start, a->T, c.B, c.H, c.D};
+    // blocks that rows start .. start + T may touch, start anywhere in a block
+    int64_t blocks = (std::min<int64_t>(a->T, c.cap) + C8_BLOCK - 2) / C8_BLOCK + 1;
+    if (!a->start_dev)
+        blocks = cdiv(std::min<int64_t>(a->start + a->T, c.cap), C8_BLOCK) - a->start / C8_BLOCK;
+    if (blocks <= 0) return NKV_OK;
+    const dim3 grid((unsigned)blocks, (unsigned)c.H, (unsigned)(2 * c.B));
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    if (a->dtype == NKV_ROWS_BF16) write_launch<NKV_ROWS_BF16>(p, c.format, grid, s);
+    else if (a->dtype == NKV_ROWS_FP16) write_launch<NKV_ROWS_FP16>(p, c.format, grid, s);
+    else write_launch<NKV_ROWS_FP32>(p, c.format, grid, s);
+    NKV_LAUNCH_CHECK();
+    return NKV_OK;
+}
+
+extern "C" size_t nkv_cache8_evict_workspace_size(const nkv_cache8_evict_args* a) {
+    clear_error();
+    check_evict(a);
+    return 0;
+}
+
+extern "C" int nkv_cache8_evict(void* stream, const nkv_cache8_evict_args* a, void* workspace,
+                                size_t workspace_bytes) {
+    clear_error();
+    int rc = check_evict(a);
+    if (rc) return rc;
+    const nkv_cache8 &c = a->cache, &o = a->out;
+    if (c.B == 0) return NKV_OK;
+    EvictParams p{{(const uint8_t*)c.k, (const uint8_t*)c.v}, {c.k_scale, c.v_scale},
+                  {(uint8_t*)o.k, (uint8_t*)o.v}, {o.k_scale, o.v_scale}, a->mass, a->out_mass,
+                  a->rows, a->out_length, a->length, c.cap, o.cap, c.B, c.H, (int)a->n,
+                  (int)a->keep, (int)a->sink, (int)a->recent};
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    select_kernel<<<(unsigned)(c.B * c.H), SEL_THREADS, 0, s>>>(p);
+    NKV_LAUNCH_CHECK();
+    const int64_t blocks = cdiv(std::min(a->keep, a->n), C8_BLOCK);
+    if (blocks) {
+        const dim3 grid((unsigned)blocks, (unsigned)c.H, (unsigned)(2 * c.B));
+        const bool wide = c8_pitch(c.D) == 128;
+        if (c.format == NKV_CACHE8_INT8) {
+            if (wide) compact_kernel<NKV_CACHE8_INT8, 128><<<grid, 256, 0, s>>>(p);
+            else compact_kernel<NKV_CACHE8_INT8, 64><<<grid, 256, 0, s>>>(p);
+        } else {
+            if (wide) compact_kernel<NKV_CACHE8_E4M3, 128><<<grid, 256, 0, s>>>(p);
+            else compact_kernel<NKV_CACHE8_E4M3, 64><<<grid, 256, 0, s>>>(p);
+        }
+        NKV_LAUNCH_CHECK();
+    }
+    return NKV_OK;
+}

@@ -20,7 +20,8 @@ from ._lib import (NKV_DTYPE_BF16, NKV_DTYPE_FP16, NKV_QUANT_BF16, NKV_QUANT_FP3
                    NKV_SCHEDULE_AUTO, NKV_SCHEDULE_KEY_CHUNKS, NKV_SCHEDULE_QUERY_TILES,
                    NkvAttendArgs, NkvCodec, NkvDecodeArgs, NkvEncodeArgs, NkvFastArgs,
                    NkvCamera, NkvFinishArgs, NkvLiftCombineArgs, NkvReaderGroup, NkvC64FitArgs,
-                   NkvReaderRowsArgs, NkvRope,
+                   NkvReaderRowsArgs, NkvRope, NkvCache8, NkvCache8AttendArgs,
+                   NkvCache8EvictArgs, NkvCache8MassArgs, NkvCache8WriteArgs,
                    NkvSegment, check, lib)
 
 _SCALE_CODES = {torch.bfloat16: NKV_DTYPE_BF16, torch.float16: NKV_DTYPE_FP16}
@@ -1367,3 +1368,261 @@ def finish(native: torch.Tensor, native_lse: torch.Tensor, lifted: torch.Tensor,
     a.y_sb, a.y_sh, a.y_ss, a.y_sd = result.stride()
     check("nkv_finish", lib().nkv_finish(_stream(device), byref(a)))
     return result
+
+
+# ---------------------------------------------------------------- 8-bit cache
+CACHE8_BLOCK = _lib.NKV_CACHE8_BLOCK
+_CACHE8_FORMATS = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+_CACHE8_CODES = {torch.int8: _lib.NKV_CACHE8_INT8, torch.float8_e4m3fn: _lib.NKV_CACHE8_E4M3}
+_ROW_CODES = {torch.bfloat16: _lib.NKV_ROWS_BF16, torch.float16: _lib.NKV_ROWS_FP16,
+              torch.float32: _lib.NKV_ROWS_FP32}
+
+
+@dataclass
+class Cache8:
+    """Keys and values in 8 bits (nkv_cache8): k and v [B, H, cap, pitch] int8 or
+    float8_e4m3fn codes, k_scale and v_scale [B, H, cap / 64] fp32, one scale for
+    each block of 64 rows and head; value = code * scale.  head_dim is the row
+    width D (a multiple of 8, at most 128); pitch is 64 for D <= 64 and 128
+    above, and the columns from D on hold zero.  The caller keeps each
+    sequence's length; rows at or past it are never read into a result."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    head_dim: int
+
+    @classmethod
+    def empty(cls, B: int, H: int, cap: int, head_dim: int, device: torch.device,
+              format: str = "int8") -> "Cache8":
+        """A cache of no rows with room for cap of them (rounded up to whole
+        blocks); format "int8" or "e4m3"."""
+        if format not in _CACHE8_FORMATS:
+            raise ValueError(f"format must be one of {sorted(_CACHE8_FORMATS)}")
+        if head_dim < 1 or head_dim % 8 or head_dim > 128:
+            raise ValueError("head_dim must be a multiple of 8, at most 128")
+        if cap < 1:
+            raise ValueError("cap must be positive")
+        blocks = -(-int(cap) // CACHE8_BLOCK)
+        shape = (B, H, blocks * CACHE8_BLOCK, 64 if head_dim <= 64 else 128)
+        k, v = (torch.zeros(shape, device=device, dtype=torch.uint8)
+                .view(_CACHE8_FORMATS[format]) for _ in range(2))
+        ks, vs = (torch.ones((B, H, blocks), device=device) for _ in range(2))
+        return cls(k, v, ks, vs, int(head_dim))
+
+    @property
+    def cap(self) -> int:
+        return int(self.k.shape[2])
+
+    def struct(self) -> NkvCache8:
+        k, v, ks, vs, D = self.k, self.v, self.k_scale, self.v_scale, self.head_dim
+        code = _CACHE8_CODES.get(k.dtype)
+        if code is None or v.dtype != k.dtype:
+            raise TypeError("cache codes must be int8 or float8_e4m3fn, k and v alike")
+        shape = k.shape
+        if len(shape) != 4 or v.shape != shape or shape[3] != (64 if D <= 64 else 128):
+            raise ValueError("cache codes must be [B, H, cap, pitch], pitch 64 for head_dim <= 64 "
+                             "and 128 above")
+        B, H, cap, _ = shape
+        if cap % CACHE8_BLOCK or ks.shape != (B, H, cap // CACHE8_BLOCK) or vs.shape != ks.shape:
+            raise ValueError("cache scales must be [B, H, cap / 64] with cap a multiple of 64")
+        if ks.dtype != torch.float32 or vs.dtype != torch.float32:
+            raise TypeError("cache scales must be float32")
+        if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous()
+                and vs.is_contiguous()):
+            raise ValueError("cache codes and scales must be contiguous")
+        return NkvCache8(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), cap, B, H, D,
+                         code)
+
+
+def _cache8_call(name: str, device: torch.device, *args) -> None:
+    """One C call with its tensors' device current (a launch on another device's
+    stream would go to the current one)."""
+    fn = getattr(lib(), name)
+    if torch.cuda.current_device() == device.index:
+        check(name, fn(_stream(device), *args))
+    else:
+        with torch.cuda.device(device):
+            check(name, fn(_stream(device), *args))
+
+
+def _cache8_scratch(name: str, args, device: torch.device, workspace: Optional[torch.Tensor]):
+    """The workspace of a call: the caller's if given, else one from torch's
+    allocator, which orders its reuse behind the launch's stream."""
+    size = getattr(lib(), name + "_workspace_size")
+    need = size(byref(args))
+    if need == 0:
+        return None, 0
+    if workspace is None:
+        workspace = torch.empty(need, device=device, dtype=torch.uint8)
+    elif workspace.device != device or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous tensor on the inputs' device")
+    return workspace, workspace.numel() * workspace.element_size()
+
+
+def _cache8_lengths(t: Optional[torch.Tensor], B: int, name: str) -> Optional[int]:
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.shape != (B,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of one entry per sequence")
+    return t.data_ptr()
+
+
+def _cache8_bound(cache: Cache8, length, max_length: Optional[int]):
+    """(length tensor or None, the bound n) of a call's length: an int for all
+    sequences, or an int32 tensor [B] with entries in [0, max_length]."""
+    if isinstance(length, torch.Tensor):
+        n = cache.cap if max_length is None else int(max_length)
+        lengths = length
+    else:
+        n, lengths = int(length), None
+        if max_length is not None and n > max_length:
+            raise ValueError("length is above max_length")
+    if not 0 <= n <= cache.cap:
+        raise ValueError(f"length must be in [0, {cache.cap}]")
+    return lengths, n
+
+
+def cache8_write(cache: Cache8, k: torch.Tensor, v: torch.Tensor, start,
+                 counts: Optional[torch.Tensor] = None) -> None:
+    """Quantise new rows into a cache, in place (see nkv_cache8_write).
+
+    k, v: [B, T, H, head_dim] bf16, fp16 or fp32 (any strides divisible by 8,
+    contiguous columns).  start: the row of each sequence's first new token, an
+    int for all or an int32 tensor [B] on the device (so that a captured graph
+    can move on); a tensor's entries are clamped to [0, cap] and rows past cap
+    dropped, an int that does not leave room for T rows is refused.  counts:
+    int32 [B], how many of a sequence's T rows are written (a padded batch)."""
+    given = start if isinstance(start, torch.Tensor) else None
+    device = _require_gpu(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, given, counts)
+    a = NkvCache8WriteArgs()
+    a.cache = c = cache.struct()
+    if k.dtype not in _ROW_CODES or v.dtype != k.dtype:
+        raise TypeError("k and v must both be bf16, fp16 or fp32")
+    if k.dim() != 4 or v.shape != k.shape or k.shape[0] != c.B or k.shape[2] != c.H \
+            or k.shape[3] != c.D:
+        raise ValueError("k and v must be [B, T, H, head_dim] of the cache's B, H and head_dim")
+    a.T, a.dtype = k.shape[1], _ROW_CODES[k.dtype]
+    if k.numel() == 0:
+        return
+    a.k, a.v = k.data_ptr(), v.data_ptr()
+    a.k_sb, a.k_st, a.k_sh = _strides_bthd(k, "k")
+    a.v_sb, a.v_st, a.v_sh = _strides_bthd(v, "v")
+    a.counts = _cache8_lengths(counts, c.B, "counts")
+    if given is not None:
+        a.start_dev = _cache8_lengths(given, c.B, "start")
+    else:
+        a.start = int(start)
+    _cache8_call("nkv_cache8_write", device, byref(a))
+
+
+def _cache8_query(a, q: torch.Tensor, cache: Cache8, length, max_length, softmax_scale, causal):
+    """Fills the query half of attend's and mass's arguments."""
+    a.cache = c = cache.struct()
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("q must be bf16 or fp16")
+    if q.dim() != 4 or q.shape[0] != c.B or q.shape[3] != c.D or q.shape[2] == 0 \
+            or q.shape[2] % c.H:
+        raise ValueError("q must be [B, Q, heads, head_dim] with heads a multiple of the cache's")
+    a.G, a.dtype, a.Q = q.shape[2] // c.H, _ROW_CODES[q.dtype], q.shape[1]
+    lengths, a.n = _cache8_bound(cache, length, max_length)
+    a.length = _cache8_lengths(lengths, c.B, "length")
+    a.q = q.data_ptr()
+    if q.numel():
+        a.q_sb, a.q_st, a.q_sh = _strides_bthd(q, "q")
+    a.softmax_scale = c.D ** -0.5 if softmax_scale is None else float(softmax_scale)
+    a.causal = 1 if causal else 0
+    return c
+
+
+def cache8_attend(q: torch.Tensor, cache: Cache8, length, *, max_length: Optional[int] = None,
+                  softmax_scale: Optional[float] = None, causal: bool = False,
+                  return_lse: bool = True, out: Optional[torch.Tensor] = None,
+                  workspace: Optional[torch.Tensor] = None):
+    """Attention over an 8-bit cache (see nkv_cache8_attend).
+
+    q [B, Q, heads, head_dim] bf16 or fp16, heads a multiple of the cache's
+    (grouped heads: query head h reads key head h // (heads / H)).  length: the
+    rows visible, an int for every sequence or an int32 tensor [B] on the
+    device, clamped to [0, max_length] (default: cap), by which the work is
+    divided.  causal: the queries are the last Q tokens, query t sees the first
+    length - Q + 1 + t rows.  Returns (out like q, lse [B, heads, Q] fp32 or
+    None); a query that sees nothing gets 0 and -inf.  workspace: optional
+    uint8 buffer of nkv_cache8_attend_workspace_size bytes."""
+    device = _require_gpu(q, cache.k, cache.v, cache.k_scale, cache.v_scale, out,
+                          length if isinstance(length, torch.Tensor) else None)
+    a = NkvCache8AttendArgs()
+    c = _cache8_query(a, q, cache, length, max_length, softmax_scale, causal)
+    if out is None:
+        out = torch.empty(q.shape, device=device, dtype=q.dtype)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out must have q's shape and type")
+    a.out = out.data_ptr()
+    if q.numel():
+        a.o_sb, a.o_st, a.o_sh = _strides_bthd(out, "out")
+    lse = None
+    if return_lse:
+        lse = torch.empty((c.B, q.shape[2], q.shape[1]), device=device, dtype=torch.float32)
+        a.lse = lse.data_ptr()
+    scratch, nbytes = _cache8_scratch("nkv_cache8_attend", a, device, workspace)
+    _cache8_call("nkv_cache8_attend", device, byref(a), _ptr(scratch), nbytes)
+    return out, lse
+
+
+def cache8_mass(q: torch.Tensor, cache: Cache8, lse: torch.Tensor, mass: torch.Tensor, length, *,
+                out: Optional[torch.Tensor] = None, max_length: Optional[int] = None,
+                softmax_scale: Optional[float] = None, causal: bool = False,
+                workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Adds to mass [B, H, cap] fp32 the attention weight that each cached row
+    receives from q, summed over the queries and the heads of its group (see
+    nkv_cache8_mass).  lse: cache8_attend's, on the same arguments.  out: where
+    the sums go (default: mass itself); returned."""
+    out = mass if out is None else out
+    device = _require_gpu(q, cache.k, cache.v, cache.k_scale, cache.v_scale, lse, mass, out,
+                          length if isinstance(length, torch.Tensor) else None)
+    a = NkvCache8MassArgs()
+    c = _cache8_query(a, q, cache, length, max_length, softmax_scale, causal)
+    _contig(lse, torch.float32, "lse")
+    if lse.shape != (c.B, q.shape[2], q.shape[1]):
+        raise ValueError("lse must be [B, heads, Q]")
+    for name, t in (("mass", mass), ("out", out)):
+        _contig(t, torch.float32, name)
+        if t.shape != (c.B, c.H, c.cap):
+            raise ValueError(f"{name} must be [B, H, cap]")
+    a.lse, a.mass, a.out = lse.data_ptr(), mass.data_ptr(), out.data_ptr()
+    scratch, nbytes = _cache8_scratch("nkv_cache8_mass", a, device, workspace)
+    _cache8_call("nkv_cache8_mass", device, byref(a), _ptr(scratch), nbytes)
+    return out
+
+
+def cache8_evict(cache: Cache8, mass: torch.Tensor, length, out: Cache8, out_mass: torch.Tensor,
+                 *, keep: int, sink: int = 0, recent: int = 0, max_length: Optional[int] = None,
+                 workspace: Optional[torch.Tensor] = None):
+    """Evicts the tokens of least mass, head by head (see nkv_cache8_evict).
+
+    Of a sequence longer than keep, each head keeps its first `sink` rows, its
+    last `recent` and those of the largest mass [B, H, cap] between, in order;
+    they go to the front of `out` (another cache, cap >= keep) and their masses
+    to out_mass [B, H, out.cap].  Returns (rows [B, H, keep] int32: the rows
+    kept, -1 past the last; lengths [B] int32)."""
+    device = _require_gpu(cache.k, cache.v, cache.k_scale, cache.v_scale, mass, out.k, out.v,
+                          out.k_scale, out.v_scale, out_mass,
+                          length if isinstance(length, torch.Tensor) else None)
+    a = NkvCache8EvictArgs()
+    a.cache, a.out = c, o = cache.struct(), out.struct()
+    for name, t, cap in (("mass", mass, c.cap), ("out_mass", out_mass, o.cap)):
+        _contig(t, torch.float32, name)
+        if t.shape != (c.B, c.H, cap):
+            raise ValueError(f"{name} must be [B, H, cap] of its cache")
+    lengths, a.n = _cache8_bound(cache, length, max_length)
+    a.length = _cache8_lengths(lengths, c.B, "length")
+    a.keep, a.sink, a.recent = int(keep), int(sink), int(recent)
+    if a.keep < 1:
+        raise ValueError("keep must be positive")
+    rows = torch.empty((c.B, c.H, a.keep), device=device, dtype=torch.int32)
+    left = torch.empty((c.B,), device=device, dtype=torch.int32)
+    a.mass, a.out_mass = mass.data_ptr(), out_mass.data_ptr()
+    a.rows, a.out_length = rows.data_ptr(), left.data_ptr()
+    scratch, nbytes = _cache8_scratch("nkv_cache8_evict", a, device, workspace)
+    _cache8_call("nkv_cache8_evict", device, byref(a), _ptr(scratch), nbytes)
+    return rows, left
