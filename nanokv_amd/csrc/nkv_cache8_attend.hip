@@ -5,6 +5,14 @@
 // (q . code), and with v = sv * code the output is sum p * sv * code / sum p:
 // neither scale meets a 16-bit operand.  Codes are exact in bf16 and fp16, so
 // the scores are those of the dequantised rows with one rounding less.
+//
+// The weights p * sv of the second product are rounded to fp16 whatever the
+// queries' type: with bf16 their rounding is as large as the output's own (2^-9
+// relative; over 262,144 keys the output was 0.0026 off in norm where its own
+// rounding makes 0.0017).  fp16's range is enough because they are held in
+// units: w = 2^(z - m + LIFT) * sv / 2^unit, where unit is the log2 of the
+// largest sv so far and m is at most TAU below the row's maximum, is at most
+// 2^(LIFT + TAU) and keeps all 11 bits down to p = 2^-(14 + LIFT).
 #include "nkv_cache8.h"
 
 #include <math.h>
@@ -16,7 +24,8 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
-constexpr float TAU = 8.0f;           // a row's maximum is moved when it is off by 2^TAU
+constexpr float TAU = 3.0f;           // a row's maximum is moved when it is off by 2^TAU
+constexpr float LIFT = 12.0f;         // 2^(LIFT + TAU) < 65504
 constexpr float SCALE_MIN = 0x1p-100f;  // keeps an unwritten block's scale out of log2(0)
 
 struct AttendParams {
@@ -28,12 +37,16 @@ struct AttendParams {
     const uint16_t* q;
     uint16_t* out;
     float* lse;
-    float* part;                  // [item][16 rows][P] fp32 unnormalised outputs
-    float* part_ml;               // [item][16 rows][2] running maximum (log2) and sum
+    // partial results of the splits, [B*H][splits][rows]: the output in units of
+    // 2^unit (at most the largest code, so fp16 holds it), the maximum (log2),
+    // the sum and the unit
+    uint16_t* part;               // [..][P] fp16
+    f32x4* part_ml;
     int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;
     int64_t cap, items;
     float scale_log2;
-    int B, H, G, D, Q, n, causal, splits, groups;
+    int B, H, G, D, Q, n, causal, splits, groups, rows;
+    int per_group;                // tile kernel: 32-row blocks of a group
 };
 
 // The 16 query rows of one group: row r of key head hk is query t = r / G of
@@ -61,6 +74,41 @@ __device__ __forceinline__ void load_q(typename T::x8 (&qf)[P / 32], const uint1
         if (there && d < D) w = *reinterpret_cast<const u32x4*>(q + d);
         qf[s] = as_x8<typename T::x8>(w);
     }
+}
+
+// Eight columns of a row's result: o is in units of 2^(U + LIFT) (a merge's:
+// 2^U, with `lift` 1), l its sum.
+template <typename T>
+__device__ __forceinline__ void store_row(const AttendParams& p, int b, int hk, int row, int d,
+                                          float M, float L, float U, const float (&o)[8],
+                                          float lift = 1.0f / 4096.0f) {
+    const RowAt at = row_at(row, hk, p.G, p.Q);
+    if (!at.there) return;
+    const float f = L > 0.0f ? lift / L * __builtin_amdgcn_exp2f(U) : 0.0f;
+    if (d < p.D)
+        *reinterpret_cast<u32x4*>(p.out + b * p.o_sb + at.t * p.o_st + at.head * p.o_sh + d) =
+            u32x4{T::pack(o[0] * f, o[1] * f), T::pack(o[2] * f, o[3] * f),
+                  T::pack(o[4] * f, o[5] * f), T::pack(o[6] * f, o[7] * f)};
+    if (d == 0 && p.lse)
+        p.lse[((int64_t)b * p.H * p.G + at.head) * p.Q + at.t] =
+            L > 0.0f ? M * LN2 + logf(L) : -INFINITY;
+}
+static_assert(LIFT == 12.0f, "store_row's and store_partial's lift");
+
+// The same as one split's partial result: the output over its sum is at most
+// the largest code, and its rounding to fp16 an eighth of bf16's.
+template <int P>
+__device__ __forceinline__ void store_partial(const AttendParams& p, int bh, int split, int row,
+                                              int d, float M, float L, float U,
+                                              const float (&o)[8]) {
+    if (row >= p.rows) return;
+    const int64_t i = ((int64_t)bh * p.splits + split) * p.rows + row;
+    const float f = L > 0.0f ? 1.0f / 4096.0f / L : 0.0f;
+    if (d < P)
+        *reinterpret_cast<u32x4*>(p.part + i * P + d) =
+            u32x4{Fp16::pack(o[0] * f, o[1] * f), Fp16::pack(o[2] * f, o[3] * f),
+                  Fp16::pack(o[4] * f, o[5] * f), Fp16::pack(o[6] * f, o[7] * f)};
+    if (d == 0) p.part_ml[i] = f32x4{M, L, U, 0.0f};
 }
 
 // Four waves of a workgroup share 16 query rows and a range of 64-row blocks;
@@ -174,7 +222,7 @@ __global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
         const float mn = up ? tm : m;
         const float alpha = up ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
         m = mn;
-        const float off = (mn == -INFINITY ? 0.0f : mn) + (unit - lsv);
+        const float off = (mn == -INFINITY ? 0.0f : mn) + (unit - lsv) - LIFT;
         float lsum = 0.0f;
         uint32_t pw[2][4];
 #pragma unroll
@@ -185,10 +233,10 @@ __global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
                 w[e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, -off));
                 lsum += w[e];
             }
-            pw[t >> 1][2 * (t & 1)] = T::pack(w[0], w[1]);
-            pw[t >> 1][2 * (t & 1) + 1] = T::pack(w[2], w[3]);
+            pw[t >> 1][2 * (t & 1)] = Fp16::pack(w[0], w[1]);
+            pw[t >> 1][2 * (t & 1) + 1] = Fp16::pack(w[2], w[3]);
         }
-        l = l * alpha + lsum * __builtin_amdgcn_exp2f(unit - lsv);
+        l = l * alpha + lsum * __builtin_amdgcn_exp2f(unit - lsv - LIFT);
         if (__any(up)) {
 #pragma unroll
             for (int i = 0; i < DB; ++i)
@@ -197,7 +245,7 @@ __global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const x8 pf = as_x8<x8>(u32x4{pw[k][0], pw[k][1], pw[k][2], pw[k][3]});
+            const f16x8 pf = as_x8<f16x8>(u32x4{pw[k][0], pw[k][1], pw[k][2], pw[k][3]});
 #pragma unroll
             for (int w = 0; w < DB / 4; ++w)
 #pragma unroll
@@ -207,9 +255,10 @@ __global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
                     for (int j = 0; j < 8; ++j) a[j] = code_pair<FMT>(vr[k][j][w], h);
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const x8 vf = as_x8<x8>(u32x4{T::pack(a[0][e], a[1][e]), T::pack(a[2][e], a[3][e]),
-                                                      T::pack(a[4][e], a[5][e]), T::pack(a[6][e], a[7][e])});
-                        o[4 * w + 2 * h + e] = T::mfma16(vf, pf, o[4 * w + 2 * h + e]);
+                        const f16x8 vf = as_x8<f16x8>(
+                            u32x4{Fp16::pack(a[0][e], a[1][e]), Fp16::pack(a[2][e], a[3][e]),
+                                  Fp16::pack(a[4][e], a[5][e]), Fp16::pack(a[6][e], a[7][e])});
+                        o[4 * w + 2 * h + e] = Fp16::mfma16(vf, pf, o[4 * w + 2 * h + e]);
                     }
                 }
         }
@@ -218,95 +267,362 @@ __global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
     // merge of the four waves: o[i][e] is column DB (4 g + e) + i of row r
     __shared__ float so[4][16][P + 4];
     __shared__ float sml[4][16][2];
-    const float f = unit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(unit);
+    __shared__ float su[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int i = 0; i < DB; i += 4)
             *reinterpret_cast<f32x4*>(&so[wave][r][DB * (4 * g + e) + i]) =
-                f32x4{o[i][e] * f, o[i + 1][e] * f, o[i + 2][e] * f, o[i + 3][e] * f};
+                f32x4{o[i][e], o[i + 1][e], o[i + 2][e], o[i + 3][e]};
     if (g == 0) {
         sml[wave][r][0] = m;
         sml[wave][r][1] = l;
     }
+    if (lane == 0) su[wave] = unit;
     __syncthreads();
     const int mr = threadIdx.x / 16, d = (threadIdx.x % 16) * 8;
-    float M = -INFINITY;
+    float M = -INFINITY, U = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, sml[w][mr][0]);
+    for (int w = 0; w < 4; ++w) {
+        M = fmaxf(M, sml[w][mr][0]);
+        U = fmaxf(U, su[w]);
+    }
     float L = 0.0f, acc[8] = {};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         const float mw = sml[w][mr][0];
-        const float a = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - M);
-        L += a * sml[w][mr][1];
-        if (d < P)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] += a * so[w][mr][d + i];
-    }
-    if (p.splits > 1) {
-        const int64_t at = item * 16 + mr;
-        if (d < P) {
-            f32x4* dst = reinterpret_cast<f32x4*>(p.part + at * P + d);
-            dst[0] = f32x4{acc[0], acc[1], acc[2], acc[3]};
-            dst[1] = f32x4{acc[4], acc[5], acc[6], acc[7]};
-        }
-        if (d == 0) {
-            p.part_ml[2 * at] = M;
-            p.part_ml[2 * at + 1] = L;
-        }
-        return;
-    }
-    const RowAt ro = row_at(row0 + mr, hk, p.G, p.Q);
-    if (!ro.there) return;
-    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-    if (d < p.D)
-        *reinterpret_cast<u32x4*>(p.out + b * p.o_sb + ro.t * p.o_st + ro.head * p.o_sh + d) =
-            u32x4{T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv),
-                  T::pack(acc[4] * inv, acc[5] * inv), T::pack(acc[6] * inv, acc[7] * inv)};
-    if (d == 0 && p.lse)
-        p.lse[((int64_t)b * p.H * p.G + ro.head) * p.Q + ro.t] =
-            L > 0.0f ? M * LN2 + logf(L) : -INFINITY;
-}
-
-// The merge of the splits' partial results: 16 threads a row, eight columns
-// each; out = sum 2^(m - M) o / sum 2^(m - M) l.
-template <typename T, int P>
-__global__ void __launch_bounds__(256) merge_kernel(AttendParams p) {
-    const int64_t rows = (int64_t)p.groups * 16;
-    const int64_t at = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
-    const int d = (threadIdx.x % 16) * 8;
-    const int64_t bh = at / rows;
-    if (bh >= (int64_t)p.B * p.H) return;
-    const int row = (int)(at % rows), b = (int)(bh / p.H), hk = (int)(bh % p.H);
-    const RowAt ro = row_at(row, hk, p.G, p.Q);
-    if (!ro.there) return;
-    const int64_t step = (int64_t)p.groups * 16;
-    const int64_t first = bh * p.splits * step + row;
-    float M = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.part_ml[2 * (first + s * step)]);
-    float L = 0.0f, acc[8] = {};
-    for (int s = 0; s < p.splits; ++s) {
-        const int64_t i = first + s * step;
-        const float mw = p.part_ml[2 * i];
         if (mw == -INFINITY) continue;
         const float a = __builtin_amdgcn_exp2f(mw - M);
-        L += a * p.part_ml[2 * i + 1];
-        if (d < P) {
-            const f32x4* src = reinterpret_cast<const f32x4*>(p.part + i * P + d);
-            const f32x4 x = src[0], y = src[1];
+        L += a * sml[w][mr][1];
+        const float f = a * __builtin_amdgcn_exp2f(su[w] - U);
+        if (d < P)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) acc[k] += a * x[k], acc[4 + k] += a * y[k];
+            for (int i = 0; i < 8; ++i) acc[i] += f * so[w][mr][d + i];
+    }
+    const int row = row0 + mr;
+    if (p.splits > 1) store_partial<P>(p, bh, split, row, d, M, L, U, acc);
+    else store_row<T>(p, b, hk, row, d, M, L, U, acc);
+}
+
+// ---------------------------------------------------------------- many rows
+// Eight waves of 32 query rows each share every block of 64 keys: the
+// workgroup loads its codes into registers a block ahead, converts them once
+// and leaves K rows and V columns in LDS as MFMA operands, double-buffered,
+// with one barrier a block.  S^T = K Q^T puts a query in a lane's column (16 of
+// the scores of each 32 keys, the other 16 in lane ^ 32), and its weights are
+// then the operand of O^T += V^T W^T without leaving the registers.
+//
+// LDS: K row k at 2 P k, its 16-byte chunk c at c ^ (k mod chunks); V^T row of
+// column d at 128 R, R = d with bits 2 and 3 swapped (a lane's results are then
+// eight consecutive columns), its chunk 4 j + 2 s + h (keys of 32-key half j,
+// product s, lane half h) at chunk ^ vsw(R): reads of eight consecutive rows,
+// and writes of every fourth row, meet eight different chunks.
+constexpr int TILE_WAVES = 8;
+
+__device__ __forceinline__ int vsw(int R) { return ((R >> 2) ^ ((R & 3) << 1)) & 7; }
+
+template <typename T, int FMT, int P>
+struct TileCodes {
+    static constexpr int CH = P / 8;                     // chunks of a K row
+    static constexpr int K_BYTES = C8_BLOCK * P * 2, V_BYTES = P * C8_BLOCK * 2;
+    u32x4 k;
+    uint32_t v[4];
+    // P = 128: every thread brings 16 bytes of K and 4 x 4 bytes of V; P = 64:
+    // the first half of the workgroup K, the other V
+    static __device__ __forceinline__ bool has_k() { return P == 128 || threadIdx.x < 256; }
+    static __device__ __forceinline__ bool has_v() { return P == 128 || threadIdx.x >= 256; }
+    static __device__ __forceinline__ int kt() { return threadIdx.x; }
+    static __device__ __forceinline__ int vt() { return P == 128 ? threadIdx.x : threadIdx.x - 256; }
+
+    // the codes of the block at row key0 of this head (kb, vb: its first row)
+    __device__ __forceinline__ void load(const uint8_t* kb, const uint8_t* vb, int64_t key0) {
+        if (has_k())
+            k = *reinterpret_cast<const u32x4*>(kb + (key0 + kt() / (P / 16)) * P + 16 * (kt() % (P / 16)));
+        if (has_v())
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[i] = *reinterpret_cast<const uint32_t*>(vb + (key0 + 4 * (vt() / (P / 4)) + i) * P +
+                                                          4 * (vt() % (P / 4)));
+    }
+    // valid: the block's rows below the length; V rows past it become zero
+    // (they may hold NaN, which a zero weight does not remove)
+    __device__ __forceinline__ void store(unsigned char* buf, int valid) {
+        if (has_k()) {
+            const int row = kt() / (P / 16), c = 2 * (kt() % (P / 16)), x = row & (CH - 1);
+            unsigned char* at = buf + row * 2 * P;
+            *reinterpret_cast<typename T::x8*>(at + 16 * (c ^ x)) = codes_x8<T, FMT>(k[0], k[1]);
+            *reinterpret_cast<typename T::x8*>(at + 16 * ((c + 1) ^ x)) = codes_x8<T, FMT>(k[2], k[3]);
+        }
+        if (has_v()) {
+            const int kq = vt() / (P / 4), dq = vt() % (P / 4);
+            if (valid < C8_BLOCK)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (4 * kq + i >= valid) v[i] = 0;
+            const int R0 = 4 * ((dq & ~3) | ((dq & 1) << 1) | ((dq >> 1) & 1));
+            const int q = kq & 7, chunk = 4 * (kq >> 3) + 2 * (q >> 2) + (q & 1), half = (q >> 1) & 1;
+            f32x2 a[4][2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) a[i][h] = code_pair<FMT>(v[i], h);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                *reinterpret_cast<u32x2*>(buf + K_BYTES + (R0 + c) * 128 +
+                                          16 * (chunk ^ vsw(R0 + c)) + 8 * half) =
+                    u32x2{Fp16::pack(a[0][c >> 1][c & 1], a[1][c >> 1][c & 1]),
+                          Fp16::pack(a[2][c >> 1][c & 1], a[3][c >> 1][c & 1])};
         }
     }
-    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-    if (d < p.D)
-        *reinterpret_cast<u32x4*>(p.out + b * p.o_sb + ro.t * p.o_st + ro.head * p.o_sh + d) =
-            u32x4{T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv),
-                  T::pack(acc[4] * inv, acc[5] * inv), T::pack(acc[6] * inv, acc[7] * inv)};
-    if (d == 0 && p.lse)
-        p.lse[((int64_t)b * p.H * p.G + ro.head) * p.Q + ro.t] =
-            L > 0.0f ? M * LN2 + logf(L) : -INFINITY;
+};
+
+template <typename T, int FMT, int P>
+__global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendParams p) {
+    constexpr int KS = P / 16, DB = P / 32;
+    using x8 = typename T::x8;
+    using Codes = TileCodes<T, FMT, P>;
+    constexpr int BUF = Codes::K_BYTES + Codes::V_BYTES;
+    __shared__ __align__(16) unsigned char smem[2 * BUF];
+    const int lane = threadIdx.x & 63, hf = lane >> 5, l32 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // groups of one head and split run on one XCD in consecutive slots (block
+    // i goes to XCD i % 8), so its L2 serves all but the first read of a block
+    const int64_t per = (p.items + 7) >> 3;
+    const int64_t item = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (item >= p.items) return;
+    const int rg = (int)(item % p.groups);
+    const int64_t rest = item / p.groups;
+    const int64_t BH = (int64_t)p.B * p.H;
+    const int split = (int)(rest / BH), bh = (int)(rest % BH), b = bh / p.H, hk = bh % p.H;
+    const int len = c8_length(p.length, b, p.n);
+    const int row0 = rg * p.per_group * 32;
+    const int rows_end = min(row0 + p.per_group * 32, p.rows);
+    // keys that the group's last row sees
+    const int last = max(0, p.causal ? len - p.Q + 1 + (rows_end - 1) / p.G : len);
+    const int nb = (last + C8_BLOCK - 1) / C8_BLOCK;
+    const int b0 = (int)((int64_t)split * nb / p.splits);
+    const int b1 = (int)((int64_t)(split + 1) * nb / p.splits);
+    const int wrow = row0 + 32 * wave, row = wrow + l32;
+    const bool active = wrow < rows_end;
+    const RowAt mine = row_at(row, hk, p.G, p.Q);
+    const int end = !mine.there ? 0 : p.causal ? len - p.Q + 1 + mine.t : len;
+    const int first = p.causal ? len - p.Q + 1 + wrow / p.G : len;  // what the wave's first row sees
+    const int wlast = p.causal ? len - p.Q + 1 + (min(wrow + 32, p.rows) - 1) / p.G : len;
+    x8 qf[KS];
+    {
+        const uint16_t* q = p.q + b * p.q_sb + mine.t * p.q_st + mine.head * p.q_sh;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = 16 * s + 8 * hf;
+            u32x4 w{};
+            if (active && mine.there && d < p.D) w = *reinterpret_cast<const u32x4*>(q + d);
+            qf[s] = as_x8<x8>(w);
+        }
+    }
+    const uint8_t* kb = p.k + (int64_t)bh * p.cap * P;
+    const uint8_t* vb = p.v + (int64_t)bh * p.cap * P;
+    const float* ks = p.ks + (int64_t)bh * (p.cap / C8_BLOCK);
+    const float* vs = p.vs + (int64_t)bh * (p.cap / C8_BLOCK);
+    f32x16 o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; ++i) o[i] = f32x16{};
+    float m = -INFINITY, l = 0.0f, unit = -INFINITY;
+    Codes codes;
+    if (b0 < b1) {
+        codes.load(kb, vb, (int64_t)b0 * C8_BLOCK);
+        codes.store(smem, len - b0 * C8_BLOCK);
+        if (b0 + 1 < b1) codes.load(kb, vb, (int64_t)(b0 + 1) * C8_BLOCK);
+    }
+    lds_barrier();
+    for (int blk = b0; blk < b1; ++blk) {
+        const unsigned char* buf = smem + ((blk - b0) & 1) * BUF;
+        unsigned char* next = smem + ((blk - b0 + 1) & 1) * BUF;
+        const int key0 = blk * C8_BLOCK;
+        const bool work = active && key0 < wlast;
+        f32x16 s[2];
+        if (work) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                s[j] = f32x16{};
+#pragma unroll
+                for (int kk = 0; kk < KS; ++kk) {
+                    const int r = 32 * j + l32;
+                    const x8 kf = *reinterpret_cast<const x8*>(
+                        buf + r * 2 * P + 16 * ((2 * kk + hf) ^ (r & (Codes::CH - 1))));
+                    s[j] = T::mfma32(kf, qf[kk], s[j]);
+                }
+            }
+        }
+        if (blk + 1 < b1) {
+            codes.store(next, len - key0 - C8_BLOCK);
+            if (blk + 2 < b1) codes.load(kb, vb, (int64_t)key0 + 2 * C8_BLOCK);
+        }
+        if (work) {
+            const float sk = fmaxf(ks[blk], SCALE_MIN), sv = fmaxf(vs[blk], SCALE_MIN);
+            if (key0 + C8_BLOCK > first) {
+                const int seen = end - key0;
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (32 * j + 8 * (i >> 2) + 4 * hf + (i & 3) >= seen) s[j][i] = -INFINITY;
+            }
+            const float c = p.scale_log2 * sk, lsv = __builtin_amdgcn_logf(sv);
+            if (lsv > unit) {
+                const float f = __builtin_amdgcn_exp2f(unit - lsv);
+#pragma unroll
+                for (int i = 0; i < DB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[i][e] *= f;
+                unit = lsv;
+            }
+            float tm = s[0][0];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) tm = fmaxf(tm, s[j][i]);
+            tm = halfwave_max(tm) * c;
+            const bool up = tm > m + TAU;
+            const float mn = up ? tm : m;
+            const float alpha = up ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+            m = mn;
+            const float off = (mn == -INFINITY ? 0.0f : mn) + (unit - lsv) - LIFT;
+            float lsum = 0.0f;
+            uint32_t pw[2][8];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float w0 = __builtin_amdgcn_exp2f(fmaf(s[j][i], c, -off));
+                    const float w1 = __builtin_amdgcn_exp2f(fmaf(s[j][i + 1], c, -off));
+                    lsum += w0 + w1;
+                    pw[j][i >> 1] = Fp16::pack(w0, w1);
+                }
+            l = l * alpha + lsum * __builtin_amdgcn_exp2f(unit - lsv - LIFT);
+            if (__any(up)) {
+#pragma unroll
+                for (int i = 0; i < DB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const f16x8 pf = as_x8<f16x8>(
+                        u32x4{pw[j][4 * k], pw[j][4 * k + 1], pw[j][4 * k + 2], pw[j][4 * k + 3]});
+#pragma unroll
+                    for (int i = 0; i < DB; ++i) {
+                        const int R = 32 * i + l32;
+                        const f16x8 vf = *reinterpret_cast<const f16x8*>(
+                            buf + Codes::K_BYTES + R * 128 + 16 * ((4 * j + 2 * k + hf) ^ vsw(R)));
+                        o[i] = Fp16::mfma32(vf, pf, o[i]);
+                    }
+                }
+        }
+        lds_barrier();
+    }
+    l = halfwave_sum(l);
+    if (!active) return;
+#pragma unroll
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int d = 32 * i + 16 * e + 8 * hf;
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = o[i][8 * e + k];
+            if (p.splits > 1) store_partial<P>(p, bh, split, row, d, m, l, unit, x);
+            else store_row<T>(p, b, hk, row, d, m, l, unit, x);
+        }
+}
+
+// The merge of the splits' partial results: 16 threads a row and group of
+// splits, eight columns each; out = sum a 2^unit o / sum a with a = 2^(m - M) l.
+// SG groups share a row's splits and are joined in LDS.
+template <typename T, int P, int SG>
+__global__ void __launch_bounds__(256) merge_kernel(AttendParams p) {
+    constexpr int ROWS = 16 / SG;
+    const int64_t at = (int64_t)blockIdx.x * ROWS + threadIdx.x / (16 * SG);
+    const int sg = threadIdx.x / 16 % SG, d = (threadIdx.x % 16) * 8;
+    const int64_t bh = at / p.rows;
+    const bool in = bh < (int64_t)p.B * p.H;
+    const int row = in ? (int)(at % p.rows) : 0, b = (int)(bh / p.H), hk = (int)(bh % p.H);
+    const int64_t first = bh * p.splits * p.rows + row;
+    float M = -INFINITY, U = -INFINITY, L = 0.0f, acc[8] = {};
+    if (in) {
+        // AHEAD splits' loads in flight, then folded into the running result
+        constexpr int AHEAD = 8;
+        for (int s0 = sg; s0 < p.splits; s0 += SG * AHEAD) {
+            f32x4 ml[AHEAD];
+            u32x4 x[AHEAD];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const int s = min(s0 + SG * j, p.splits - 1);
+                const int64_t i = first + (int64_t)s * p.rows;
+                ml[j] = p.part_ml[i];
+                x[j] = d < P ? *reinterpret_cast<const u32x4*>(p.part + i * P + d) : u32x4{};
+                if (s0 + SG * j >= p.splits) ml[j][0] = ml[j][2] = -INFINITY;
+            }
+            float m1 = M, u1 = U;
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                m1 = fmaxf(m1, ml[j][0]);
+                u1 = fmaxf(u1, ml[j][2]);
+            }
+            if (m1 == -INFINITY) continue;
+            const float b0 = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - m1);
+            const float c0 = M == -INFINITY ? 0.0f : b0 * __builtin_amdgcn_exp2f(U - u1);
+            L *= b0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[k] *= c0;
+            M = m1;
+            U = u1;
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const float a =
+                    ml[j][0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[j][0] - M) * ml[j][1];
+                L += a;
+                const float f = a == 0.0f ? 0.0f : a * __builtin_amdgcn_exp2f(ml[j][2] - U);
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    acc[k] += f * f16_bits_to_f32((uint16_t)(x[j][k >> 1] >> (16 * (k & 1))));
+            }
+        }
+    }
+    if constexpr (SG > 1) {
+        __shared__ float sh[ROWS][SG][16][8];
+        __shared__ float sml[ROWS][SG][3];
+        const int lr = threadIdx.x / (16 * SG), part = threadIdx.x % 16;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sh[lr][sg][part][k] = acc[k];
+        if (part == 0) {
+            sml[lr][sg][0] = M;
+            sml[lr][sg][1] = L;
+            sml[lr][sg][2] = U;
+        }
+        __syncthreads();
+        if (sg) return;
+#pragma unroll
+        for (int s = 0; s < SG; ++s) {
+            M = fmaxf(M, sml[lr][s][0]);
+            U = fmaxf(U, sml[lr][s][2]);
+        }
+        L = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < SG; ++s) {
+            const float ms = sml[lr][s][0];
+            if (ms == -INFINITY) continue;
+            const float a = __builtin_amdgcn_exp2f(ms - M);
+            L += a * sml[lr][s][1];
+            const float f = a * __builtin_amdgcn_exp2f(sml[lr][s][2] - U);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[k] += f * sh[lr][s][part][k];
+        }
+    }
+    if (in) store_row<T>(p, b, hk, row, d, M, L, U, acc, 1.0f);
 }
 
 // ---------------------------------------------------------------- mass
@@ -422,26 +738,54 @@ int check_query(const nkv_cache8& c, int G, int dtype, int64_t Q, int64_t n, flo
 }
 
 struct Plan {
-    int groups, splits;
-    int64_t items;
+    bool tile;
+    int groups, splits, per_group;
+    int64_t items, rows;
     size_t part, ml;              // bytes
 };
 
-// Key splits: enough workgroups to fill the chip, each with at least four
-// blocks of keys (one a wave).
+// From this many rows of a key head on, the tile kernel.
+constexpr int64_t TILE_ROWS = 64;
+
 Plan attend_plan(const nkv_cache8_attend_args* a) {
     const nkv_cache8& c = a->cache;
     Plan pl{};
-    pl.groups = (int)cdiv(a->Q * a->G, 16);
-    const int64_t base = (int64_t)c.B * c.H * pl.groups;
-    const int64_t blocks = cdiv(a->n, C8_BLOCK);
+    pl.rows = a->Q * a->G;
+    const int64_t heads = (int64_t)c.B * c.H, blocks = cdiv(a->n, C8_BLOCK);
     pl.splits = 1;
-    if (base > 0 && base < 1024)
-        pl.splits = (int)std::max<int64_t>(1, std::min(cdiv(1024, base), blocks / 4));
-    pl.items = base * pl.splits;
+    pl.tile = pl.rows >= TILE_ROWS;
+    if (pl.tile) {
+        // the fewest groups of up to eight 32-row blocks, of even size
+        const int64_t qb = cdiv(pl.rows, 32);
+        pl.groups = (int)cdiv(qb, TILE_WAVES);
+        pl.per_group = (int)cdiv(qb, pl.groups);
+        const int64_t base = heads * pl.groups;
+        // splits whose rounds of 256 workgroups take least, in units of a
+        // block's time; a workgroup's start and end cost some blocks, and a
+        // merge its partials' traffic
+        double best = 0.0;
+        for (int64_t s = 1; s <= 16 && (s == 1 || blocks >= 4 * s); ++s) {
+            const double merge = s == 1 ? 0.0 : 4.0 + (double)heads * pl.rows * s * 2e-4;
+            const double t = (double)cdiv(base * s, 256) * ((double)blocks / s + 6.0) + merge;
+            if (s == 1 || t < best) {
+                best = t;
+                pl.splits = (int)s;
+            }
+        }
+        pl.items = base * pl.splits;
+    } else {
+        // enough workgroups to fill the chip, each with at least four blocks
+        // of keys (one a wave)
+        pl.groups = (int)cdiv(pl.rows, 16);
+        const int64_t base = heads * pl.groups;
+        if (base > 0 && base < 512)
+            pl.splits = (int)std::max<int64_t>(1, std::min(cdiv(512, base), blocks / 4));
+        pl.items = base * pl.splits;
+    }
     if (pl.splits > 1) {
-        pl.part = (size_t)pl.items * 16 * c8_pitch(c.D) * 4;
-        pl.ml = (size_t)pl.items * 16 * 8;
+        const size_t rows = (size_t)heads * pl.splits * pl.rows;
+        pl.ml = rows * sizeof(f32x4);
+        pl.part = rows * c8_pitch(c.D) * 2;
     }
     return pl;
 }
@@ -454,13 +798,23 @@ int check_attend(const nkv_cache8_attend_args* a) {
     NKV_REQUIRE(a->out, NKV_ERR_INVALID, "out is required");
     NKV_REQUIRE(reinterpret_cast<uintptr_t>(a->out) % 16 == 0 && (a->o_sb | a->o_st | a->o_sh) % 8 == 0,
                 NKV_ERR_INVALID, "out must be 16-byte aligned with strides divisible by 8");
-    NKV_REQUIRE(attend_plan(a).items <= INT32_MAX, NKV_ERR_UNSUPPORTED, "too many query rows");
+    NKV_REQUIRE(attend_plan(a).items <= INT32_MAX - 8, NKV_ERR_UNSUPPORTED, "too many query rows");
     return NKV_OK;
 }
 
 template <typename T, int FMT, int P>
-void attend_run(const AttendParams& p, hipStream_t s) {
-    attend_kernel<T, FMT, P><<<(unsigned)p.items, 256, 0, s>>>(p);
+void attend_run(const AttendParams& p, bool tile, hipStream_t s) {
+    if (tile)
+        attend_tile_kernel<T, FMT, P><<<(unsigned)(8 * cdiv(p.items, 8)), 64 * TILE_WAVES, 0, s>>>(p);
+    else
+        attend_kernel<T, FMT, P><<<(unsigned)p.items, 256, 0, s>>>(p);
+}
+
+template <typename T, int P>
+void merge_run(const AttendParams& p, hipStream_t s) {
+    const int64_t rows = (int64_t)p.B * p.H * p.rows;
+    if (p.splits > 8) merge_kernel<T, P, 16><<<(unsigned)rows, 256, 0, s>>>(p);
+    else merge_kernel<T, P, 1><<<(unsigned)cdiv(rows, 16), 256, 0, s>>>(p);
 }
 
 template <typename T, int FMT, int P>
@@ -489,6 +843,7 @@ void dispatch(int dtype, int format, int D, F f) {
     }
 }
 static_assert(NKV_CACHE8_INT8 == 0 && NKV_CACHE8_E4M3 == 1, "dispatch");
+static_assert(sizeof(f32x4) == 16, "partials");
 
 }  // namespace
 }  // namespace nkv
@@ -522,8 +877,8 @@ extern "C" int nkv_cache8_attend(void* stream, const nkv_cache8_attend_args* a, 
     p.q = (const uint16_t*)a->q;
     p.out = (uint16_t*)a->out;
     p.lse = a->lse;
-    p.part = (float*)workspace;
-    p.part_ml = (float*)((char*)workspace + pl.part);
+    p.part_ml = (f32x4*)workspace;
+    p.part = (uint16_t*)((char*)workspace + pl.ml);
     p.q_sb = a->q_sb, p.q_st = a->q_st, p.q_sh = a->q_sh;
     p.o_sb = a->o_sb, p.o_st = a->o_st, p.o_sh = a->o_sh;
     p.cap = c.cap;
@@ -533,18 +888,19 @@ extern "C" int nkv_cache8_attend(void* stream, const nkv_cache8_attend_args* a, 
     p.causal = a->causal != 0;
     p.splits = pl.splits;
     p.groups = pl.groups;
+    p.rows = (int)pl.rows;
+    p.per_group = pl.per_group;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     dispatch(a->dtype, c.format, c.D, [&](auto t, auto f, auto w) {
-        attend_run<decltype(t), decltype(f)::value, decltype(w)::value>(p, s);
+        attend_run<decltype(t), decltype(f)::value, decltype(w)::value>(p, pl.tile, s);
     });
     NKV_LAUNCH_CHECK();
     if (pl.splits > 1) {
-        const int64_t blocks = (int64_t)c.B * c.H * pl.groups;
         const bool wide = c8_pitch(c.D) == 128, bf16 = a->dtype == NKV_ROWS_BF16;
-        if (wide && bf16) merge_kernel<Bf16, 128><<<(unsigned)blocks, 256, 0, s>>>(p);
-        else if (wide) merge_kernel<Fp16, 128><<<(unsigned)blocks, 256, 0, s>>>(p);
-        else if (bf16) merge_kernel<Bf16, 64><<<(unsigned)blocks, 256, 0, s>>>(p);
-        else merge_kernel<Fp16, 64><<<(unsigned)blocks, 256, 0, s>>>(p);
+        if (wide && bf16) merge_run<Bf16, 128>(p, s);
+        else if (wide) merge_run<Fp16, 128>(p, s);
+        else if (bf16) merge_run<Bf16, 64>(p, s);
+        else merge_run<Fp16, 64>(p, s);
         NKV_LAUNCH_CHECK();
     }
     return NKV_OK;
