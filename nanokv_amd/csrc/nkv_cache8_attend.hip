@@ -325,8 +325,10 @@ template <typename T, int FMT, int P>
 struct TileCodes {
     static constexpr int CH = P / 8;                     // chunks of a K row
     static constexpr int K_BYTES = C8_BLOCK * P * 2, V_BYTES = P * C8_BLOCK * 2;
+    static constexpr int SMEM = 2 * K_BYTES + 3 * V_BYTES;
     u32x4 k;
     uint32_t v[4];
+    float sk, sv;                                        // the block's scales
     // P = 128: every thread brings 16 bytes of K and 4 x 4 bytes of V; P = 64:
     // the first half of the workgroup K, the other V
     static __device__ __forceinline__ bool has_k() { return P == 128 || threadIdx.x < 256; }
@@ -334,8 +336,13 @@ struct TileCodes {
     static __device__ __forceinline__ int kt() { return threadIdx.x; }
     static __device__ __forceinline__ int vt() { return P == 128 ? threadIdx.x : threadIdx.x - 256; }
 
-    // the codes of the block at row key0 of this head (kb, vb: its first row)
-    __device__ __forceinline__ void load(const uint8_t* kb, const uint8_t* vb, int64_t key0) {
+    // block blk of a head, whose first row is kb, vb.  The scales come along: a
+    // load where they are used would wait for the next block's codes with it.
+    __device__ __forceinline__ void load(const uint8_t* kb, const uint8_t* vb, const float* ks,
+                                         const float* vs, int blk) {
+        const int64_t key0 = (int64_t)blk * C8_BLOCK;
+        sk = ks[blk];
+        sv = vs[blk];
         if (has_k())
             k = *reinterpret_cast<const u32x4*>(kb + (key0 + kt() / (P / 16)) * P + 16 * (kt() % (P / 16)));
         if (has_v())
@@ -346,10 +353,10 @@ struct TileCodes {
     }
     // valid: the block's rows below the length; V rows past it become zero
     // (they may hold NaN, which a zero weight does not remove)
-    __device__ __forceinline__ void store(unsigned char* buf, int valid) {
+    __device__ __forceinline__ void store(unsigned char* kd, unsigned char* vd, int valid) {
         if (has_k()) {
             const int row = kt() / (P / 16), c = 2 * (kt() % (P / 16)), x = row & (CH - 1);
-            unsigned char* at = buf + row * 2 * P;
+            unsigned char* at = kd + row * 2 * P;
             *reinterpret_cast<typename T::x8*>(at + 16 * (c ^ x)) = codes_x8<T, FMT>(k[0], k[1]);
             *reinterpret_cast<typename T::x8*>(at + 16 * ((c + 1) ^ x)) = codes_x8<T, FMT>(k[2], k[3]);
         }
@@ -368,8 +375,8 @@ struct TileCodes {
                 for (int h = 0; h < 2; ++h) a[i][h] = code_pair<FMT>(v[i], h);
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-                *reinterpret_cast<u32x2*>(buf + K_BYTES + (R0 + c) * 128 +
-                                          16 * (chunk ^ vsw(R0 + c)) + 8 * half) =
+                *reinterpret_cast<u32x2*>(vd + (R0 + c) * 128 + 16 * (chunk ^ vsw(R0 + c)) +
+                                          8 * half) =
                     u32x2{Fp16::pack(a[0][c >> 1][c & 1], a[1][c >> 1][c & 1]),
                           Fp16::pack(a[2][c >> 1][c & 1], a[3][c >> 1][c & 1])};
         }
@@ -381,8 +388,7 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
     constexpr int KS = P / 16, DB = P / 32;
     using x8 = typename T::x8;
     using Codes = TileCodes<T, FMT, P>;
-    constexpr int BUF = Codes::K_BYTES + Codes::V_BYTES;
-    __shared__ __align__(16) unsigned char smem[2 * BUF];
+    extern __shared__ __align__(16) unsigned char smem[];  // TileCodes::SMEM
     const int lane = threadIdx.x & 63, hf = lane >> 5, l32 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // groups of one head and split run on one XCD in consecutive slots (block
@@ -428,37 +434,77 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
     for (int i = 0; i < DB; ++i) o[i] = f32x16{};
     float m = -INFINITY, l = 0.0f, unit = -INFINITY;
     Codes codes;
+    float sk = 1.0f, sv = 1.0f;  // scales of the current block
     if (b0 < b1) {
-        codes.load(kb, vb, (int64_t)b0 * C8_BLOCK);
-        codes.store(smem, len - b0 * C8_BLOCK);
-        if (b0 + 1 < b1) codes.load(kb, vb, (int64_t)(b0 + 1) * C8_BLOCK);
+        codes.load(kb, vb, ks, vs, b0);
+        codes.store(smem, smem + 2 * Codes::K_BYTES, len - b0 * C8_BLOCK);
+        sk = codes.sk, sv = codes.sv;
+        codes.load(kb, vb, ks, vs, min(b0 + 1, b1 - 1));
+    }
+    // the queries have arrived before the loop: a wait for them inside would
+    // wait for the codes in flight
+#pragma unroll
+    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s]));
+    // this lane's operand offsets in the current slots (kept in registers)
+    uint32_t kofs[KS], vofs[4];
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) {
+        kofs[kk] = l32 * 2 * P + 16 * ((2 * kk + hf) ^ (l32 & (Codes::CH - 1)));
+        asm volatile("" : "+v"(kofs[kk]));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        vofs[i] = 2 * Codes::K_BYTES + l32 * 128 + 16 * ((2 * i + hf) ^ vsw(l32));
+        asm volatile("" : "+v"(vofs[i]));
     }
     lds_barrier();
+    // Waves w and w + 4 share a SIMD.  Waves 4-7 meet a block's barrier before
+    // its softmax, waves 0-3 after it, so that one's softmax runs beside the
+    // other's products.  At barrier i every wave has stored its part of block
+    // i + 1 and is done with K of block i and V of block i - 1: two slots for
+    // K and three for V.
+    const bool lag = wave >= TILE_WAVES / 2;
+    int slot = 0;  // V's
     for (int blk = b0; blk < b1; ++blk) {
-        const unsigned char* buf = smem + ((blk - b0) & 1) * BUF;
-        unsigned char* next = smem + ((blk - b0 + 1) & 1) * BUF;
-        const int key0 = blk * C8_BLOCK;
+        const int key0 = blk * C8_BLOCK, kslot = (blk - b0) & 1;
+        const int next = slot == 2 ? 0 : slot + 1;
         const bool work = active && key0 < wlast;
         f32x16 s[2];
+        f16x8 vf[2][2 * DB];
+        auto lds_v = [&](int j) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < DB; ++i)
+                    vf[j][k * DB + i] = *reinterpret_cast<const f16x8*>(smem + vofs[2 * j + k] + i * 4096);
+        };
         if (work) {
+            x8 kf[2][KS];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int kk = 0; kk < KS; ++kk)
+                    kf[j][kk] = *reinterpret_cast<const x8*>(smem + kofs[kk] + j * 64 * P);
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                s[j] = f32x16{};
+                s[j] = T::mfma32(kf[j][0], qf[0], f32x16{});
 #pragma unroll
-                for (int kk = 0; kk < KS; ++kk) {
-                    const int r = 32 * j + l32;
-                    const x8 kf = *reinterpret_cast<const x8*>(
-                        buf + r * 2 * P + 16 * ((2 * kk + hf) ^ (r & (Codes::CH - 1))));
-                    s[j] = T::mfma32(kf, qf[kk], s[j]);
-                }
+                for (int kk = 1; kk < KS; ++kk) s[j] = T::mfma32(kf[j][kk], qf[kk], s[j]);
             }
+            __builtin_amdgcn_s_setprio(0);
+            lds_v(0);
         }
-        if (blk + 1 < b1) {
-            codes.store(next, len - key0 - C8_BLOCK);
-            if (blk + 2 < b1) codes.load(kb, vb, (int64_t)key0 + 2 * C8_BLOCK);
-        }
+        const float c = p.scale_log2 * fmaxf(sk, SCALE_MIN);
+        const float lsv = __builtin_amdgcn_logf(fmaxf(sv, SCALE_MIN));
+        // block blk + 1 (behind the last, the last again, for no one)
+        codes.store(smem + (kslot ^ 1) * Codes::K_BYTES,
+                    smem + 2 * Codes::K_BYTES + next * Codes::V_BYTES,
+                    len - min(key0 + C8_BLOCK, (b1 - 1) * C8_BLOCK));
+        sk = codes.sk, sv = codes.sv;
+        codes.load(kb, vb, ks, vs, min(blk + 2, b1 - 1));
+        if (lag) lds_barrier();
         if (work) {
-            const float sk = fmaxf(ks[blk], SCALE_MIN), sv = fmaxf(vs[blk], SCALE_MIN);
             if (key0 + C8_BLOCK > first) {
                 const int seen = end - key0;
 #pragma unroll
@@ -467,7 +513,6 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
                     for (int i = 0; i < 16; ++i)
                         if (32 * j + 8 * (i >> 2) + 4 * hf + (i & 3) >= seen) s[j][i] = -INFINITY;
             }
-            const float c = p.scale_log2 * sk, lsv = __builtin_amdgcn_logf(sv);
             if (lsv > unit) {
                 const float f = __builtin_amdgcn_exp2f(unit - lsv);
 #pragma unroll
@@ -499,6 +544,8 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
                     pw[j][i >> 1] = Fp16::pack(w0, w1);
                 }
             l = l * alpha + lsum * __builtin_amdgcn_exp2f(unit - lsv - LIFT);
+            lds_v(1);
+            __builtin_amdgcn_s_setprio(1);
             if (__any(up)) {
 #pragma unroll
                 for (int i = 0; i < DB; ++i)
@@ -512,15 +559,24 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
                     const f16x8 pf = as_x8<f16x8>(
                         u32x4{pw[j][4 * k], pw[j][4 * k + 1], pw[j][4 * k + 2], pw[j][4 * k + 3]});
 #pragma unroll
-                    for (int i = 0; i < DB; ++i) {
-                        const int R = 32 * i + l32;
-                        const f16x8 vf = *reinterpret_cast<const f16x8*>(
-                            buf + Codes::K_BYTES + R * 128 + 16 * ((4 * j + 2 * k + hf) ^ vsw(R)));
-                        o[i] = Fp16::mfma32(vf, pf, o[i]);
-                    }
+                    for (int i = 0; i < DB; ++i) o[i] = Fp16::mfma32(vf[j][k * DB + i], pf, o[i]);
                 }
+            __builtin_amdgcn_s_setprio(0);
         }
-        lds_barrier();
+        const uint32_t kstep = kslot ? -Codes::K_BYTES : Codes::K_BYTES;
+        const uint32_t vstep = slot == 2 ? -2 * Codes::V_BYTES : Codes::V_BYTES;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+            kofs[kk] += kstep;
+            asm volatile("" : "+v"(kofs[kk]));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            vofs[i] += vstep;
+            asm volatile("" : "+v"(vofs[i]));
+        }
+        slot = next;
+        if (!lag) lds_barrier();
     }
     l = halfwave_sum(l);
     if (!active) return;
@@ -803,11 +859,16 @@ int check_attend(const nkv_cache8_attend_args* a) {
 }
 
 template <typename T, int FMT, int P>
-void attend_run(const AttendParams& p, bool tile, hipStream_t s) {
-    if (tile)
-        attend_tile_kernel<T, FMT, P><<<(unsigned)(8 * cdiv(p.items, 8)), 64 * TILE_WAVES, 0, s>>>(p);
-    else
+int attend_run(const AttendParams& p, bool tile, hipStream_t s) {
+    if (tile) {
+        constexpr int SMEM = TileCodes<T, FMT, P>::SMEM;
+        if (int rc = set_smem(attend_tile_kernel<T, FMT, P>, SMEM)) return rc;
+        attend_tile_kernel<T, FMT, P>
+            <<<(unsigned)(8 * cdiv(p.items, 8)), 64 * TILE_WAVES, SMEM, s>>>(p);
+    } else {
         attend_kernel<T, FMT, P><<<(unsigned)p.items, 256, 0, s>>>(p);
+    }
+    return NKV_OK;
 }
 
 template <typename T, int P>
@@ -892,8 +953,9 @@ extern "C" int nkv_cache8_attend(void* stream, const nkv_cache8_attend_args* a, 
     p.per_group = pl.per_group;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     dispatch(a->dtype, c.format, c.D, [&](auto t, auto f, auto w) {
-        attend_run<decltype(t), decltype(f)::value, decltype(w)::value>(p, pl.tile, s);
+        rc = attend_run<decltype(t), decltype(f)::value, decltype(w)::value>(p, pl.tile, s);
     });
+    if (rc) return rc;
     NKV_LAUNCH_CHECK();
     if (pl.splits > 1) {
         const bool wide = c8_pitch(c.D) == 128, bf16 = a->dtype == NKV_ROWS_BF16;

@@ -75,10 +75,12 @@ def visible(B, Q, lengths, causal):
 
 def attend(q, k, v, lengths, causal, scale, u):
     """q [B, Q, Hq, D], k/v [B, H, cap, D] float64 -> out, lse, and bounds on
-    the error of a kernel whose probabilities and outputs have half-step u:
-    a probability and the output are off by u each, a score by the fp32 sum of
-    its D products and one fused multiply-add (D + 4 roundings of 2^-24 of the
-    sum of their magnitudes, an exponential twice that)."""
+    the error of a kernel whose outputs have half-step u: a weight is rounded to
+    fp16 (W, half a step; absolutely below its normal range), the results of key
+    splits to fp16 once more, the output by u, a score by the fp32 sum of its D
+    products and one fused multiply-add (D + 4 roundings of 2^-24 of the sum of
+    their magnitudes, an exponential twice that)."""
+    W = 2 * 2.0 ** -11
     B, Q, Hq, D = q.shape
     H = k.shape[1]
     G = Hq // H
@@ -87,24 +89,28 @@ def attend(q, k, v, lengths, causal, scale, u):
     lse, ltol = np.full((B, Hq, Q), -np.inf), np.zeros((B, Hq, Q))
     for b in range(B):
         for h in range(Hq):
-            for t in range(Q):
-                n = end[b, t]
-                if n == 0:
-                    continue
-                kk, vv = k[b, h // G, :n], v[b, h // G, :n]
-                z = kk @ q[b, t, h] * scale
-                mag = (np.abs(kk) @ np.abs(q[b, t, h]) * scale).max()
-                ez = (D + 4) * 2.0 ** -24 * mag + 2.0 ** -21
-                m = z.max()
-                p = np.exp(z - m)
-                tot = p.sum()
-                out[b, t, h] = p @ vv / tot
-                lse[b, h, t] = m + np.log(tot)
-                a = p @ np.abs(vv) / tot
-                # the last term: probabilities below fp16's normal range
-                small = n * 2.0 ** -25 * np.abs(vv).max() if u == 2.0 ** -11 else 0.0
-                otol[b, t, h] = (u + 4 * ez) * a * 1.01 + u * np.abs(out[b, t, h]) + small + 1e-30
-                ltol[b, h, t] = 2 * ez + 2.0 ** -22 * (abs(m) + abs(np.log(tot)) + 1)
+            n = int(end[b].max())
+            if n == 0:
+                continue
+            kk, vv = k[b, h // G, :n], v[b, h // G, :n]
+            hidden = np.arange(n)[None] >= end[b][:, None]
+            some = end[b] > 0
+            z = np.where(hidden, -np.inf, q[b, :, h] @ kk.T * scale)
+            mag = np.where(hidden, 0, np.abs(q[b, :, h]) @ np.abs(kk).T * scale).max(1)
+            ez = (D + 4) * 2.0 ** -24 * mag + 2.0 ** -21
+            m = np.where(some, z.max(1), 0)
+            p = np.exp(z - m[:, None])
+            tot = np.where(some, p.sum(1), 1)
+            out[b, :, h] = p @ vv / tot[:, None]
+            a = p @ np.abs(vv) / tot[:, None]
+            # weights below fp16's normal range (they are lifted by 2^12), and
+            # fp16 outputs below it: a number under 2^-14 is rounded to a
+            # multiple of 2^-24, so it is off by up to 2^-25, not by u of itself
+            small = n * 2.0 ** -37 * np.abs(vv).max() + (2.0 ** -25 if u == 2.0 ** -11 else 0)
+            otol[b, :, h] = ((W + 4 * ez)[:, None] * a * 1.01 + u * np.abs(out[b, :, h])
+                             + small + 1e-30)
+            lse[b, h] = np.where(some, m + np.log(tot), -np.inf)
+            ltol[b, h] = 2 * ez + 2.0 ** -22 * (np.abs(m) + np.abs(np.log(tot)) + 1)
     return out, lse, otol, ltol
 
 
@@ -116,17 +122,17 @@ def mass(q, k, lse, start, lengths, causal, scale):
     out, tol = start.astype(np.float64).copy(), np.abs(start).astype(np.float64) * 2.0 ** -23
     for b in range(B):
         for h in range(Hq):
-            for t in range(Q):
-                n = end[b, t]
-                if n == 0 or lse[b, h, t] == -np.inf:
-                    continue
-                kk = k[b, h // (Hq // H), :n]
-                z = kk @ q[b, t, h] * scale
-                mag = np.abs(kk) @ np.abs(q[b, t, h]) * scale
-                p = np.exp(z - float(lse[b, h, t]))
-                ez = (D + 4) * 2.0 ** -24 * mag + 2.0 ** -22 * (np.abs(lse[b, h, t]) + 2)
-                out[b, h // (Hq // H), :n] += p
-                tol[b, h // (Hq // H), :n] += p * (2 * ez + (Q * Hq // H + 2) * 2.0 ** -24)
+            n = int(end[b].max())
+            some = (end[b] > 0) & ~np.isneginf(lse[b, h])
+            kk, hk = k[b, h // (Hq // H), :n], h // (Hq // H)
+            seen = (np.arange(n)[None] < end[b][:, None]) & some[:, None]
+            off = np.where(some, lse[b, h], 0.0)[:, None]
+            z = q[b, :, h] @ kk.T * scale
+            mag = np.abs(q[b, :, h]) @ np.abs(kk).T * scale
+            p = np.where(seen, np.exp(np.where(seen, z - off, 0.0)), 0.0)
+            ez = (D + 4) * 2.0 ** -24 * mag + 2.0 ** -22 * (np.abs(off) + 2)
+            out[b, hk, :n] += p.sum(0)
+            tol[b, hk, :n] += (p * (2 * ez + (Q * Hq // H + 2) * 2.0 ** -24)).sum(0)
     return out, tol + 1e-30
 
 
