@@ -21,8 +21,8 @@ int cache8_check(const nkv_cache8* c, const char* who) {
         return bad(NKV_ERR_UNSUPPORTED, "head width must be a multiple of 8, at most 128");
     if (c->format != NKV_CACHE8_INT8 && c->format != NKV_CACHE8_E4M3)
         return bad(NKV_ERR_INVALID, "unknown cache format");
-    if (c->cap < C8_BLOCK || c->cap % C8_BLOCK || c->cap > INT32_MAX - C8_BLOCK)
-        return bad(NKV_ERR_INVALID, "cap must be a positive multiple of 64 below 2^31");
+    if (c->cap < C8_BLOCK || c->cap % C8_BLOCK || c->cap > (1 << 30))
+        return bad(NKV_ERR_INVALID, "cap must be a positive multiple of 64, at most 2^30");
     if ((int64_t)c->B * c->H > INT32_MAX / 4) return bad(NKV_ERR_UNSUPPORTED, "too many heads");
     if (c->B == 0) return NKV_OK;
     if (!c->k || !c->v || !c->k_scale || !c->v_scale)
@@ -183,16 +183,24 @@ __device__ __forceinline__ uint32_t order_key(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int SEL_THREADS = 1024;
+// One workgroup per (item, head).  The key of the last row kept is found digit
+// by digit (11, 11 and 10 bits, counts in LDS); then every wave lists the kept
+// rows of its own contiguous part in order, behind those of the waves before
+// it, rows equal to the last key from the lowest up.  Up to SEL_REG rows the
+// keys stay in registers (one read of the masses), longer heads are read again
+// for each digit and for the list.
+constexpr int SEL_WAVES = 16, SEL_THREADS = 64 * SEL_WAVES, SEL_PER = 32;
+constexpr int SEL_REG = SEL_THREADS * SEL_PER;
+constexpr int SEL_BINS = 2048;
+constexpr int SEL_AHEAD = 8;          // loads in flight where keys are read again
 
-// One workgroup per (item, head): the key of the last row kept is found digit
-// by digit (8 bits a pass, counts in LDS), then the kept rows are listed in
-// order, those equal to the last key from the lowest up.
+template <bool REG>
 __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
     const int b = blockIdx.x / p.H;
     const int64_t bh = blockIdx.x;
     const int n = c8_length(p.length, b, p.n);
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int32_t* rows = p.rows + bh * p.keep;
     if (blockIdx.x % p.H == 0 && tid == 0) p.out_length[b] = min(n, p.keep);
     if (n <= p.keep) {
@@ -200,66 +208,130 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
         return;
     }
     const float* mass = p.mass + bh * p.cap;
-    const int lo = p.sink, hi = n - p.recent;
-    const int want = p.keep - p.sink - p.recent;
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t pick[2];  // digit, rows still wanted below it
-    uint32_t prefix = 0, left = want;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (int i = lo + tid; i < hi; i += SEL_THREADS) {
-            const uint32_t k = order_key(mass[i]);
-            if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
-                atomicAdd(&hist[(k >> shift) & 255u], 1u);
+    const int lo = p.sink, hi = n - p.recent;           // the rows between are chosen from
+    const uint32_t want = p.keep - p.sink - p.recent;
+    // this wave's part: rows part .. part_end in steps of 64
+    const int steps = (n + SEL_THREADS - 1) / SEL_THREADS;
+    const int part = wave * steps * 64, part_end = min(part + steps * 64, n);
+    __shared__ uint32_t hist[SEL_BINS];
+    __shared__ uint32_t sums[SEL_WAVES];
+    __shared__ uint32_t pick[2];                        // digit, rows still wanted in it
+    uint32_t keys[REG ? SEL_PER : 1];
+    if constexpr (REG) {
+#pragma unroll
+        for (int j = 0; j < SEL_PER; ++j) {
+            const int i = part + 64 * j + lane;
+            keys[j] = j < steps && i < part_end ? order_key(mass[i]) : 0;
         }
+    }
+    // f(key, row, inside this wave's part) over the part, in order
+    auto each = [&](auto f) {
+        if constexpr (REG) {
+#pragma unroll
+            for (int j = 0; j < SEL_PER; ++j) {
+                if (j >= steps) break;
+                const int i = part + 64 * j + lane;
+                f(keys[j], i, i < part_end);
+            }
+        } else {
+            for (int j0 = 0; j0 < steps; j0 += SEL_AHEAD) {
+                float x[SEL_AHEAD];
+#pragma unroll
+                for (int j = 0; j < SEL_AHEAD; ++j) {
+                    const int i = part + 64 * (j0 + j) + lane;
+                    x[j] = j0 + j < steps && i < part_end ? mass[i] : 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < SEL_AHEAD; ++j) {
+                    if (j0 + j >= steps) break;
+                    const int i = part + 64 * (j0 + j) + lane;
+                    f(order_key(x[j]), i, i < part_end);
+                }
+            }
+        }
+    };
+    uint32_t prefix = 0, left = want, mask = 0;
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t top = pass == 2 ? 1023u : 2047u;
+        for (int i = tid; i < SEL_BINS; i += SEL_THREADS) hist[i] = 0;
         __syncthreads();
-        if (tid == 0) {
-            // the digit at which the count from above reaches `left`
-            uint32_t above = 0;
-            int d = 255;
-            for (; d > 0 && above + hist[d] < left; --d) above += hist[d];
-            pick[0] = (uint32_t)d;
+        each([&](uint32_t k, int i, bool in) {
+            const bool count = in && i >= lo && i < hi && (k & mask) == prefix;
+            const uint32_t d = (k >> shift) & top;
+            // one add where the whole wave has one digit (equal masses)
+            const uint64_t all = __ballot(count);
+            if (!all) return;
+            const uint32_t d0 = __builtin_amdgcn_readlane(d, __builtin_ctzll(all));
+            if (__ballot(count && d == d0) == all) {
+                if (lane == 0) atomicAdd(&hist[d0], (uint32_t)__popcll(all));
+            } else if (count) {
+                atomicAdd(&hist[d], 1u);
+            }
+        });
+        __syncthreads();
+        // the digit at which the count from above reaches `left`: thread t has
+        // the digits 2047 - 2 t and 2046 - 2 t
+        const uint32_t d1 = SEL_BINS - 1 - 2 * tid;
+        const uint32_t h1 = hist[d1], h0 = hist[d1 - 1];
+        uint32_t run = h1 + h0;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t x = __shfl_up(run, o);
+            if (lane >= o) run += x;
+        }
+        if (lane == 63) sums[wave] = run;
+        __syncthreads();
+        uint32_t above = run - h1 - h0;
+        for (int w = 0; w < wave; ++w) above += sums[w];
+        if (above < left && above + h1 >= left) {
+            pick[0] = d1;
             pick[1] = left - above;
+        } else if (above + h1 < left && above + h1 + h0 >= left) {
+            pick[0] = d1 - 1;
+            pick[1] = left - above - h1;
         }
+        if (tid == 0 && left == 0) pick[0] = top, pick[1] = 0;  // none wanted
         __syncthreads();
         prefix |= pick[0] << shift;
+        mask |= top << shift;
         left = pick[1];
         __syncthreads();
     }
-    // `left` rows of key `prefix` are kept (none wanted: left = 0)
-    __shared__ uint32_t sums[2][SEL_THREADS / 64];
-    uint32_t base = 0, ties = 0;
-    for (int i0 = 0; i0 < n; i0 += SEL_THREADS) {
-        const int i = i0 + tid;
-        const bool in = i < n, fixed = in && (i < lo || i >= hi);
-        const uint32_t k = in && !fixed ? order_key(mass[i]) : 0;
-        const bool tie = in && !fixed && k == prefix;
-        const uint64_t tb = __ballot(tie);
-        if (lane == 0) sums[0][wave] = (uint32_t)__popcll(tb);
-        __syncthreads();
-        uint32_t before = ties, all = 0;
-        for (int w = 0; w < SEL_THREADS / 64; ++w) {
-            if (w < wave) before += sums[0][w];
-            all += sums[0][w];
-        }
-        const uint64_t below = (1ull << lane) - 1;
-        const uint32_t tr = before + (uint32_t)__popcll(tb & below);
-        const bool keep = fixed || (in && !fixed && want > 0 && (k > prefix || (tie && tr < left)));
-        const uint64_t kb = __ballot(keep);
-        if (lane == 0) sums[1][wave] = (uint32_t)__popcll(kb);
-        __syncthreads();
-        uint32_t at = base, kept = 0;
-        for (int w = 0; w < SEL_THREADS / 64; ++w) {
-            if (w < wave) at += sums[1][w];
-            kept += sums[1][w];
-        }
-        at += (uint32_t)__popcll(kb & below);
-        if (keep && at < (uint32_t)p.keep) rows[at] = i;
-        base += kept;
-        ties += all;
-        __syncthreads();
+    // `left` of the rows whose key is `prefix` are kept, and all above it
+    __shared__ uint32_t kept[SEL_WAVES], tied[SEL_WAVES];
+    uint32_t nk = 0, nt = 0;
+    auto is_kept = [&](uint32_t k, int i, bool in) {
+        return in && (i < lo || i >= hi || (want > 0 && k > prefix));
+    };
+    auto is_tie = [&](uint32_t k, int i, bool in) {
+        return in && i >= lo && i < hi && k == prefix;
+    };
+    each([&](uint32_t k, int i, bool in) {
+        nk += (uint32_t)__popcll(__ballot(is_kept(k, i, in)));
+        nt += (uint32_t)__popcll(__ballot(is_tie(k, i, in)));
+    });
+    if (lane == 0) {
+        kept[wave] = nk;
+        tied[wave] = nt;
     }
+    __syncthreads();
+    uint32_t bk = 0, bt = 0;
+    for (int w = 0; w < wave; ++w) {
+        bk += kept[w];
+        bt += tied[w];
+    }
+    const uint64_t below = (1ull << lane) - 1;
+    each([&](uint32_t k, int i, bool in) {
+        const bool a = is_kept(k, i, in), t = is_tie(k, i, in);
+        const uint64_t ab = __ballot(a), tb = __ballot(t);
+        const uint32_t ra = bk + (uint32_t)__popcll(ab & below);
+        const uint32_t rt = bt + (uint32_t)__popcll(tb & below);
+        if (a || (t && rt < left)) rows[ra + min(rt, left)] = i;
+        bk += (uint32_t)__popcll(ab);
+        bt += (uint32_t)__popcll(tb);
+    });
 }
 
 // One workgroup per (block of 64 kept rows, head, K or V, item): gathers the
@@ -419,7 +491,8 @@ extern "C" int nkv_cache8_evict(void* stream, const nkv_cache8_evict_args* a, vo
                   a->rows, a->out_length, a->length, c.cap, o.cap, c.B, c.H, (int)a->n,
                   (int)a->keep, (int)a->sink, (int)a->recent};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    select_kernel<<<(unsigned)(c.B * c.H), SEL_THREADS, 0, s>>>(p);
+    if (a->n <= SEL_REG) select_kernel<true><<<(unsigned)(c.B * c.H), SEL_THREADS, 0, s>>>(p);
+    else select_kernel<false><<<(unsigned)(c.B * c.H), SEL_THREADS, 0, s>>>(p);
     NKV_LAUNCH_CHECK();
     const int64_t blocks = cdiv(std::min(a->keep, a->n), C8_BLOCK);
     if (blocks) {

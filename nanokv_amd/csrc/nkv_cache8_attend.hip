@@ -690,45 +690,66 @@ struct MassParams {
     const float* lse;
     const float* mass;
     float* out;
+    float* part;                  // [splits][B*H][n64] sums of the row splits
     int64_t q_sb, q_st, q_sh;
-    int64_t cap;
+    int64_t cap, n64;             // n64: n in whole blocks
     float scale_log2;
-    int B, H, G, D, Q, n, causal, groups;
+    int B, H, G, D, Q, n, causal, rows, splits, blocks;
 };
 
-// One workgroup per block of 64 cached rows and head: the waves hold the
-// block's codes as operands and take the groups of 16 query rows in turn; the
-// sums over rows stay in registers and are joined in LDS in a fixed order.
+// The result of one block's row i: the sum goes to this split's partial sums, or
+// with one split on top of the mass.
+__device__ __forceinline__ void mass_store(const MassParams& p, int bh, int64_t row, int len,
+                                           int split, float x) {
+    const int64_t at = (int64_t)bh * p.cap + row;
+    if (p.splits > 1) {
+        if (row < len) p.part[((int64_t)split * p.B * p.H + bh) * p.n64 + row] = x;
+    } else if (row < len) {
+        p.out[at] = p.mass[at] + x;
+    } else if (p.out != p.mass) {
+        p.out[at] = p.mass[at];
+    }
+}
+
+// Few query rows: a wave holds a block of 64 cached rows as operands (four
+// tiles of 16 keys) and takes the groups of 16 query rows in turn; the sums
+// over queries stay in registers until the end.  Bound by the read of K.
 template <typename T, int FMT, int P>
 __global__ void __launch_bounds__(256) mass_kernel(MassParams p) {
     constexpr int STEPS = P / 32, PIECES = P / 64;
     using x8 = typename T::x8;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int blk = blockIdx.x, bh = blockIdx.y, b = bh / p.H, hk = bh % p.H;
+    const int blk = blockIdx.x * 4 + wave, bh = blockIdx.y, b = bh / p.H, hk = bh % p.H;
+    if (blk >= p.blocks) return;
     const int len = c8_length(p.length, b, p.n);
     const int64_t key0 = (int64_t)blk * C8_BLOCK;
-    const int64_t at = (int64_t)bh * p.cap + key0;
     if (key0 >= len) {
-        if (p.out != p.mass && threadIdx.x < C8_BLOCK)
-            p.out[at + threadIdx.x] = p.mass[at + threadIdx.x];
+        mass_store(p, bh, key0 + lane, len, 0, 0.0f);
         return;
     }
+    const int64_t at = (int64_t)bh * p.cap + key0;
+    u32x4 kr[4][PIECES];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+            kr[t][i] = *reinterpret_cast<const u32x4*>(p.k + (at + 16 * t + r) * P + 64 * i + 16 * g);
+    const float c = p.scale_log2 * fmaxf(p.ks[(int64_t)bh * (p.cap / C8_BLOCK) + blk], SCALE_MIN);
     x8 kf[4][STEPS];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(p.k + (at + 16 * t + r) * P + 64 * i + 16 * g);
-            kf[t][2 * i] = codes_x8<T, FMT>(w[0], w[1]);
-            kf[t][2 * i + 1] = codes_x8<T, FMT>(w[2], w[3]);
+            kf[t][2 * i] = codes_x8<T, FMT>(kr[t][i][0], kr[t][i][1]);
+            kf[t][2 * i + 1] = codes_x8<T, FMT>(kr[t][i][2], kr[t][i][3]);
         }
-    const float c = p.scale_log2 * fmaxf(p.ks[(int64_t)bh * (p.cap / C8_BLOCK) + blk], SCALE_MIN);
     f32x4 sum[4] = {};
     // the first group with a row that sees the block's first key
     int rg0 = 0;
     if (p.causal) rg0 = max(0, (int)key0 - (len - p.Q)) * p.G / 16;
-    for (int rg = rg0 + wave; rg < p.groups; rg += 4) {
+    const int groups = (p.rows + 15) / 16;
+    for (int rg = rg0; rg < groups; ++rg) {
         const RowAt mine = row_at(rg * 16 + r, hk, p.G, p.Q);
         const int seen = (!mine.there ? 0 : p.causal ? len - p.Q + 1 + mine.t : len) - (int)key0;
         x8 qf[STEPS];
@@ -750,7 +771,6 @@ __global__ void __launch_bounds__(256) mass_kernel(MassParams p) {
             }
         }
     }
-    __shared__ float part[4][C8_BLOCK];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -758,15 +778,161 @@ __global__ void __launch_bounds__(256) mass_kernel(MassParams p) {
             float x = sum[t][e];
 #pragma unroll
             for (int k = 1; k < 16; k <<= 1) x += __shfl_xor(x, k);
-            if (r == 0) part[wave][16 * t + 4 * g + e] = x;
+            if (r == 0) mass_store(p, bh, key0 + 16 * t + 4 * g + e, len, 0, x);
         }
-    __syncthreads();
-    const int i = threadIdx.x;
-    if (i < C8_BLOCK && (key0 + i < len || p.out != p.mass)) {
-        float x = p.mass[at + i];
-        if (key0 + i < len) x += (part[0][i] + part[1][i]) + (part[2][i] + part[3][i]);
-        p.out[at + i] = x;
+}
+
+// Many query rows: four waves hold a block of 64 cached rows each (two tiles of
+// 32 keys) and share the queries, 64 rows a step, through LDS (double-buffered,
+// loaded into registers a step ahead, one barrier a step): read by every wave
+// from the cache, they would take all of its bandwidth.  Rows are split over
+// workgroups where there are few blocks of keys.
+constexpr int MT_ROWS = 64;
+
+template <typename T, int P>
+struct MassRows {
+    static constexpr int CH = P / 8, PER = CH / 4;      // chunks of a row, a thread's
+    u32x4 q[PER];
+    float off;
+    int end;
+    // rows row0 .. + 64: thread t brings chunks t % 4 + 4 i of row t / 4
+    __device__ __forceinline__ void load(const MassParams& p, int b, int hk, int len, int row0) {
+        const int part = threadIdx.x & 3;
+        const RowAt at = row_at(row0 + (threadIdx.x >> 2), hk, p.G, p.Q);
+        const uint16_t* src = p.q + b * p.q_sb + at.t * p.q_st + at.head * p.q_sh;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int d = 8 * (part + 4 * i);
+            q[i] = u32x4{};
+            if (at.there && d < p.D) q[i] = *reinterpret_cast<const u32x4*>(src + d);
+        }
+        off = at.there ? p.lse[((int64_t)b * p.H * p.G + at.head) * p.Q + at.t] : -INFINITY;
+        end = p.causal ? len - p.Q + 1 + at.t : len;
     }
+    __device__ __forceinline__ void store(unsigned char* buf, float* offs, int* ends) const {
+        const int row = threadIdx.x >> 2, part = threadIdx.x & 3;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            *reinterpret_cast<u32x4*>(buf + row * 2 * P + 16 * ((part + 4 * i) ^ (row & (CH - 1)))) = q[i];
+        if (part == 0) {
+            offs[row] = off == -INFINITY ? INFINITY : off * LOG2E;
+            ends[row] = end;
+        }
+    }
+};
+
+template <typename T, int FMT, int P>
+__global__ void __launch_bounds__(256, 2) mass_tile_kernel(MassParams p) {
+    constexpr int KS = P / 16, CH = P / 8;
+    using x8 = typename T::x8;
+    __shared__ __align__(16) unsigned char smem[2][MT_ROWS * P * 2];
+    __shared__ float offs[2][MT_ROWS];
+    __shared__ int ends[2][MT_ROWS];
+    const int lane = threadIdx.x & 63, hf = lane >> 5, l32 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int bh = blockIdx.y, b = bh / p.H, hk = bh % p.H, split = blockIdx.z;
+    const int len = c8_length(p.length, b, p.n);
+    const int first_key = blockIdx.x * 4 * C8_BLOCK;    // of the workgroup
+    const int blk = blockIdx.x * 4 + wave, key0 = blk * C8_BLOCK;
+    if (first_key >= len) {
+        if (blk < p.blocks) mass_store(p, bh, (int64_t)key0 + lane, len, split, 0.0f);
+        return;
+    }
+    const int64_t kblk = min(blk, (len - 1) / C8_BLOCK);  // a block that is there
+    x8 kf[2][KS];
+    {
+        const uint8_t* src = p.k + ((int64_t)bh * p.cap + kblk * C8_BLOCK + l32) * P + 16 * hf;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < KS / 2; ++i) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(src + 32 * t * P + 32 * i);
+                kf[t][2 * i] = codes_x8<T, FMT>(w[0], w[1]);
+                kf[t][2 * i + 1] = codes_x8<T, FMT>(w[2], w[3]);
+            }
+    }
+    const float c = p.scale_log2 * fmaxf(p.ks[(int64_t)bh * (p.cap / C8_BLOCK) + kblk], SCALE_MIN);
+    f32x16 sum[2] = {};
+    // steps with a row that sees the workgroup's first key, this split's share
+    const int steps = (p.rows + MT_ROWS - 1) / MT_ROWS;
+    int s0 = 0;
+    if (p.causal) s0 = min((int64_t)steps, (int64_t)max(0, first_key - (len - p.Q)) * p.G / MT_ROWS);
+    const int st0 = s0 + (int)((int64_t)split * (steps - s0) / p.splits);
+    const int st1 = s0 + (int)((int64_t)(split + 1) * (steps - s0) / p.splits);
+    if (st0 < st1) {
+        MassRows<T, P> rows;
+        rows.load(p, b, hk, len, st0 * MT_ROWS);
+        rows.store(smem[0], offs[0], ends[0]);
+        rows.load(p, b, hk, len, min(st0 + 1, st1 - 1) * MT_ROWS);
+        uint32_t qofs[KS];
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+            qofs[s] = l32 * 2 * P + 16 * ((4 * (s >> 1) + 2 * hf + (s & 1)) ^ (l32 & (CH - 1)));
+        lds_barrier();
+        for (int st = st0; st < st1; ++st) {
+            const int cur = (st - st0) & 1;
+            // what the step's first row sees
+            const int first = p.causal ? len - p.Q + 1 + st * MT_ROWS / p.G : len;
+            const bool masked = key0 + C8_BLOCK > first;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                f32x16 s[2];
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    const x8 qf = *reinterpret_cast<const x8*>(&smem[cur][qofs[i] + u * 64 * P]);
+                    s[0] = T::mfma32(kf[0][i], qf, i ? s[0] : f32x16{});
+                    s[1] = T::mfma32(kf[1][i], qf, i ? s[1] : f32x16{});
+                }
+                const float off = offs[cur][32 * u + l32];
+                if (masked) {
+                    const int seen = ends[cur][32 * u + l32] - key0;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float w = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, -off));
+                            sum[t][e] += 32 * t + 8 * (e >> 2) + 4 * hf + (e & 3) < seen ? w : 0.0f;
+                        }
+                } else {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            sum[t][e] += __builtin_amdgcn_exp2f(fmaf(s[t][e], c, -off));
+                }
+            }
+            rows.store(smem[cur ^ 1], offs[cur ^ 1], ends[cur ^ 1]);
+            rows.load(p, b, hk, len, min(st + 2, st1 - 1) * MT_ROWS);
+            lds_barrier();
+        }
+    }
+    if (blk >= p.blocks) return;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            float x = sum[t][e];
+#pragma unroll
+            for (int k = 1; k < 32; k <<= 1) x += __shfl_xor(x, k);
+            if (l32 == 0)
+                mass_store(p, bh, (int64_t)key0 + 32 * t + 8 * (e >> 2) + 4 * hf + (e & 3), len, split, x);
+        }
+}
+
+// Joins the row splits' partial sums, in their order.
+__global__ void __launch_bounds__(256) mass_join_kernel(MassParams p) {
+    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int bh = blockIdx.y;
+    if (row >= (int64_t)p.blocks * C8_BLOCK) return;
+    const int len = c8_length(p.length, bh / p.H, p.n);
+    const int64_t at = (int64_t)bh * p.cap + row;
+    if (row >= len) {
+        if (p.out != p.mass) p.out[at] = p.mass[at];
+        return;
+    }
+    float x = 0.0f;
+    for (int s = 0; s < p.splits; ++s) x += p.part[((int64_t)s * p.B * p.H + bh) * p.n64 + row];
+    p.out[at] = p.mass[at] + x;
 }
 
 // ---------------------------------------------------------------- host
@@ -879,12 +1045,10 @@ void merge_run(const AttendParams& p, hipStream_t s) {
 }
 
 template <typename T, int FMT, int P>
-void mass_run(const MassParams& p, hipStream_t s) {
-    // in place, blocks past n have nothing to do
-    const int64_t blocks = p.out == p.mass ? cdiv(p.n, C8_BLOCK) : p.cap / C8_BLOCK;
-    if (!blocks) return;
-    const dim3 grid((unsigned)blocks, (unsigned)(p.B * p.H));
-    mass_kernel<T, FMT, P><<<grid, 256, 0, s>>>(p);
+void mass_run(const MassParams& p, bool tile, hipStream_t s) {
+    const dim3 grid((unsigned)cdiv(p.blocks, 4), (unsigned)(p.B * p.H), (unsigned)p.splits);
+    if (tile) mass_tile_kernel<T, FMT, P><<<grid, 256, 0, s>>>(p);
+    else mass_kernel<T, FMT, P><<<grid, 256, 0, s>>>(p);
 }
 
 // f.template operator()<T, FMT, P>() of a call's types and pitch.
@@ -984,13 +1148,36 @@ int check_mass(const nkv_cache8_mass_args* a) {
     NKV_REQUIRE((int64_t)a->cache.B * a->cache.H <= 65535, NKV_ERR_UNSUPPORTED, "too many heads");
     return NKV_OK;
 }
+
+struct MassPlan {
+    bool tile;
+    int splits;
+    int64_t n64;
+    size_t bytes;
+};
+
+// Row splits: where the blocks of keys fill less than two workgroups a CU, as
+// many as do, each with at least four steps.
+MassPlan mass_plan(const nkv_cache8_mass_args* a) {
+    MassPlan pl{};
+    const int64_t rows = a->Q * a->G, heads = (int64_t)a->cache.B * a->cache.H;
+    pl.n64 = cdiv(a->n, C8_BLOCK) * C8_BLOCK;
+    pl.tile = rows >= MT_ROWS;
+    pl.splits = 1;
+    const int64_t base = heads * cdiv(pl.n64, 4 * C8_BLOCK);
+    if (pl.tile && base > 0 && base < 512)
+        pl.splits = (int)std::max<int64_t>(
+            1, std::min<int64_t>({cdiv(512, base), cdiv(rows, MT_ROWS) / 4, 256}));
+    if (pl.splits > 1) pl.bytes = (size_t)pl.splits * heads * pl.n64 * sizeof(float);
+    return pl;
+}
 }  // namespace
 }  // namespace nkv
 
 extern "C" size_t nkv_cache8_mass_workspace_size(const nkv_cache8_mass_args* a) {
     clear_error();
-    check_mass(a);
-    return 0;
+    if (check_mass(a) || a->cache.B == 0) return 0;
+    return mass_plan(a).bytes;
 }
 
 extern "C" int nkv_cache8_mass(void* stream, const nkv_cache8_mass_args* a, void* workspace,
@@ -999,6 +1186,11 @@ extern "C" int nkv_cache8_mass(void* stream, const nkv_cache8_mass_args* a, void
     int rc = check_mass(a);
     if (rc || a->cache.B == 0) return rc;
     const nkv_cache8& c = a->cache;
+    const MassPlan pl = mass_plan(a);
+    NKV_REQUIRE(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes), NKV_ERR_WORKSPACE,
+                "workspace missing or too small");
+    NKV_REQUIRE(pl.bytes == 0 || reinterpret_cast<uintptr_t>(workspace) % 4 == 0, NKV_ERR_INVALID,
+                "workspace must be 4-byte aligned");
     MassParams p{};
     p.k = (const uint8_t*)c.k;
     p.ks = c.k_scale;
@@ -1012,11 +1204,22 @@ extern "C" int nkv_cache8_mass(void* stream, const nkv_cache8_mass_args* a, void
     p.scale_log2 = a->softmax_scale * LOG2E;
     p.B = c.B, p.H = c.H, p.G = a->G, p.D = c.D, p.Q = (int)a->Q, p.n = (int)a->n;
     p.causal = a->causal != 0;
-    p.groups = (int)cdiv(a->Q * a->G, 16);
+    p.rows = (int)(a->Q * a->G);
+    p.splits = pl.splits;
+    p.n64 = pl.n64;
+    p.part = (float*)workspace;
+    // in place, blocks past n have nothing to do
+    p.blocks = (int)(p.out == p.mass ? cdiv(a->n, C8_BLOCK) : c.cap / C8_BLOCK);
+    if (p.blocks == 0) return NKV_OK;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     dispatch(a->dtype, c.format, c.D, [&](auto t, auto f, auto w) {
-        mass_run<decltype(t), decltype(f)::value, decltype(w)::value>(p, s);
+        mass_run<decltype(t), decltype(f)::value, decltype(w)::value>(p, pl.tile, s);
     });
     NKV_LAUNCH_CHECK();
+    if (pl.splits > 1) {
+        const dim3 grid((unsigned)cdiv((int64_t)p.blocks * C8_BLOCK, 256), (unsigned)(c.B * c.H));
+        mass_join_kernel<<<grid, 256, 0, s>>>(p);
+        NKV_LAUNCH_CHECK();
+    }
     return NKV_OK;
 }
