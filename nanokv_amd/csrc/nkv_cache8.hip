@@ -186,15 +186,15 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 // One workgroup per (item, head).  The key of the last row kept is found digit
 // by digit (11, 11 and 10 bits, counts in LDS); then every wave lists the kept
 // rows of its own contiguous part in order, behind those of the waves before
-// it, rows equal to the last key from the lowest up.  Up to SEL_REG rows the
-// keys stay in registers (one read of the masses), longer heads are read again
-// for each digit and for the list.
-constexpr int SEL_WAVES = 16, SEL_THREADS = 64 * SEL_WAVES, SEL_PER = 32;
-constexpr int SEL_REG = SEL_THREADS * SEL_PER;
+// it, rows equal to the last key from the lowest up.  Up to SEL_LDS rows the
+// keys stay in LDS (one read of the masses), longer heads are read again for
+// each digit and for the list.
+constexpr int SEL_WAVES = 16, SEL_THREADS = 64 * SEL_WAVES;
+constexpr int SEL_LDS = 32768;
 constexpr int SEL_BINS = 2048;
-constexpr int SEL_AHEAD = 8;          // loads in flight where keys are read again
+constexpr int SEL_AHEAD = 8;          // keys of a lane in flight
 
-template <bool REG>
+template <bool LDS>
 __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
     const int b = blockIdx.x / p.H;
     const int64_t bh = blockIdx.x;
@@ -213,59 +213,44 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
     // this wave's part: rows part .. part_end in steps of 64
     const int steps = (n + SEL_THREADS - 1) / SEL_THREADS;
     const int part = wave * steps * 64, part_end = min(part + steps * 64, n);
+    extern __shared__ uint32_t held[];                  // the keys, in row order (LDS)
     __shared__ uint32_t hist[SEL_BINS];
     __shared__ uint32_t sums[SEL_WAVES];
     __shared__ uint32_t pick[2];                        // digit, rows still wanted in it
-    uint32_t keys[REG ? SEL_PER : 1];
-    if constexpr (REG) {
+    // f(key, row) over the part in order, SEL_AHEAD loads in flight; rows past
+    // the part's end come with any key
+    auto each = [&](bool first, auto f) {
+        for (int j0 = 0; j0 < steps; j0 += SEL_AHEAD) {
+            uint32_t k[SEL_AHEAD];
 #pragma unroll
-        for (int j = 0; j < SEL_PER; ++j) {
-            const int i = part + 64 * j + lane;
-            keys[j] = j < steps && i < part_end ? order_key(mass[i]) : 0;
-        }
-    }
-    // f(key, row, inside this wave's part) over the part, in order
-    auto each = [&](auto f) {
-        if constexpr (REG) {
-#pragma unroll
-            for (int j = 0; j < SEL_PER; ++j) {
-                if (j >= steps) break;
-                const int i = part + 64 * j + lane;
-                f(keys[j], i, i < part_end);
+            for (int j = 0; j < SEL_AHEAD; ++j) {
+                const int i = min(part + 64 * (j0 + j) + lane, n - 1);
+                k[j] = LDS && !first ? held[i] : __float_as_uint(mass[i]);
             }
-        } else {
-            for (int j0 = 0; j0 < steps; j0 += SEL_AHEAD) {
-                float x[SEL_AHEAD];
 #pragma unroll
-                for (int j = 0; j < SEL_AHEAD; ++j) {
-                    const int i = part + 64 * (j0 + j) + lane;
-                    x[j] = j0 + j < steps && i < part_end ? mass[i] : 0.0f;
-                }
-#pragma unroll
-                for (int j = 0; j < SEL_AHEAD; ++j) {
-                    if (j0 + j >= steps) break;
-                    const int i = part + 64 * (j0 + j) + lane;
-                    f(order_key(x[j]), i, i < part_end);
-                }
+            for (int j = 0; j < SEL_AHEAD; ++j) {
+                if (j0 + j >= steps) break;
+                const int i = part + 64 * (j0 + j) + lane;
+                if (!LDS || first) k[j] = order_key(__uint_as_float(k[j]));
+                if (LDS && first && i < part_end) held[i] = k[j];
+                f(k[j], i);
             }
         }
     };
+    // rows of the part to choose from: lo .. lo + width
+    const uint32_t width = (uint32_t)max(min(hi, part_end) - lo, 0);
     uint32_t prefix = 0, left = want, mask = 0;
-#pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const uint32_t top = pass == 2 ? 1023u : 2047u;
         for (int i = tid; i < SEL_BINS; i += SEL_THREADS) hist[i] = 0;
         __syncthreads();
-        each([&](uint32_t k, int i, bool in) {
-            const bool count = in && i >= lo && i < hi && (k & mask) == prefix;
-            const uint32_t d = (k >> shift) & top;
+        each(pass == 0, [&](uint32_t k, int i) {
+            const bool count = (uint32_t)(i - lo) < width && (k & mask) == prefix;
+            const uint32_t d = (k >> shift) & top, d0 = __builtin_amdgcn_readfirstlane(d);
             // one add where the whole wave has one digit (equal masses)
-            const uint64_t all = __ballot(count);
-            if (!all) return;
-            const uint32_t d0 = __builtin_amdgcn_readlane(d, __builtin_ctzll(all));
-            if (__ballot(count && d == d0) == all) {
-                if (lane == 0) atomicAdd(&hist[d0], (uint32_t)__popcll(all));
+            if (__ballot(count && d == d0) == ~0ull) {
+                if (lane == 0) atomicAdd(&hist[d0], 64u);
             } else if (count) {
                 atomicAdd(&hist[d], 1u);
             }
@@ -284,7 +269,8 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
         if (lane == 63) sums[wave] = run;
         __syncthreads();
         uint32_t above = run - h1 - h0;
-        for (int w = 0; w < wave; ++w) above += sums[w];
+#pragma unroll
+        for (int w = 0; w < SEL_WAVES; ++w) above += w < wave ? sums[w] : 0;
         if (above < left && above + h1 >= left) {
             pick[0] = d1;
             pick[1] = left - above;
@@ -297,20 +283,21 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
         prefix |= pick[0] << shift;
         mask |= top << shift;
         left = pick[1];
-        __syncthreads();
     }
     // `left` of the rows whose key is `prefix` are kept, and all above it
     __shared__ uint32_t kept[SEL_WAVES], tied[SEL_WAVES];
+    const uint32_t floor_key = want > 0 ? prefix : 0xffffffffu;
     uint32_t nk = 0, nt = 0;
-    auto is_kept = [&](uint32_t k, int i, bool in) {
-        return in && (i < lo || i >= hi || (want > 0 && k > prefix));
+    auto marks = [&](uint32_t k, int i, uint64_t& a, uint64_t& t) {
+        const bool choose = (uint32_t)(i - lo) < width;
+        a = __ballot(choose ? k > floor_key : i < part_end);
+        t = __ballot(choose && k == prefix);
     };
-    auto is_tie = [&](uint32_t k, int i, bool in) {
-        return in && i >= lo && i < hi && k == prefix;
-    };
-    each([&](uint32_t k, int i, bool in) {
-        nk += (uint32_t)__popcll(__ballot(is_kept(k, i, in)));
-        nt += (uint32_t)__popcll(__ballot(is_tie(k, i, in)));
+    each(false, [&](uint32_t k, int i) {
+        uint64_t a, t;
+        marks(k, i, a, t);
+        nk += (uint32_t)__popcll(a);
+        nt += (uint32_t)__popcll(t);
     });
     if (lane == 0) {
         kept[wave] = nk;
@@ -318,19 +305,19 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
     }
     __syncthreads();
     uint32_t bk = 0, bt = 0;
-    for (int w = 0; w < wave; ++w) {
-        bk += kept[w];
-        bt += tied[w];
+#pragma unroll
+    for (int w = 0; w < SEL_WAVES; ++w) {
+        bk += w < wave ? kept[w] : 0;
+        bt += w < wave ? tied[w] : 0;
     }
-    const uint64_t below = (1ull << lane) - 1;
-    each([&](uint32_t k, int i, bool in) {
-        const bool a = is_kept(k, i, in), t = is_tie(k, i, in);
-        const uint64_t ab = __ballot(a), tb = __ballot(t);
-        const uint32_t ra = bk + (uint32_t)__popcll(ab & below);
-        const uint32_t rt = bt + (uint32_t)__popcll(tb & below);
-        if (a || (t && rt < left)) rows[ra + min(rt, left)] = i;
-        bk += (uint32_t)__popcll(ab);
-        bt += (uint32_t)__popcll(tb);
+    each(false, [&](uint32_t k, int i) {
+        uint64_t a, t;
+        marks(k, i, a, t);
+        const uint32_t ra = bk + __builtin_amdgcn_mbcnt_hi((uint32_t)(a >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)a, 0));
+        const uint32_t rt = bt + __builtin_amdgcn_mbcnt_hi((uint32_t)(t >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)t, 0));
+        if (((a >> lane) & 1) || (((t >> lane) & 1) && rt < left)) rows[ra + min(rt, left)] = i;
+        bk += (uint32_t)__popcll(a);
+        bt += (uint32_t)__popcll(t);
     });
 }
 
@@ -491,8 +478,13 @@ extern "C" int nkv_cache8_evict(void* stream, const nkv_cache8_evict_args* a, vo
                   a->rows, a->out_length, a->length, c.cap, o.cap, c.B, c.H, (int)a->n,
                   (int)a->keep, (int)a->sink, (int)a->recent};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    if (a->n <= SEL_REG) select_kernel<true><<<(unsigned)(c.B * c.H), SEL_THREADS, 0, s>>>(p);
-    else select_kernel<false><<<(unsigned)(c.B * c.H), SEL_THREADS, 0, s>>>(p);
+    if (a->n <= SEL_LDS) {
+        const size_t smem = (size_t)a->n * 4;
+        if ((rc = set_smem(select_kernel<true>, smem))) return rc;
+        select_kernel<true><<<(unsigned)(c.B * c.H), SEL_THREADS, smem, s>>>(p);
+    } else {
+        select_kernel<false><<<(unsigned)(c.B * c.H), SEL_THREADS, 0, s>>>(p);
+    }
     NKV_LAUNCH_CHECK();
     const int64_t blocks = cdiv(std::min(a->keep, a->n), C8_BLOCK);
     if (blocks) {

@@ -697,6 +697,46 @@ struct MassParams {
     int B, H, G, D, Q, n, causal, rows, splits, blocks;
 };
 
+// Sums over lanes of many values at once: each step adds two half-sized sets of
+// partial sums across lanes, a lane keeping the set that one bit of its number
+// names, until lane r of 16 (32) has the sum of v[r].  The exchanges are DPP and
+// permlane moves in the VALU; through LDS (__shfl_xor) they took 10 us of a
+// 25 us call over 8 ragged sequences.
+template <int CTRL>
+__device__ __forceinline__ float dpp_from(float x) {
+    return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+
+template <int H, int CTRL>
+__device__ __forceinline__ void reduce_step(float* v, bool upper) {
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+        const float give = upper ? v[i] : v[i + H], keep = upper ? v[i + H] : v[i];
+        v[i] = keep + dpp_from<CTRL>(give);
+    }
+}
+
+// over the 16 lanes of a row: partners l ^ 8, l ^ 7, l ^ 2, l ^ 1
+__device__ __forceinline__ float reduce16(float* v, int r) {
+    reduce_step<8, 0x128>(v, r & 8);   // row_ror:8
+    reduce_step<4, 0x141>(v, r & 4);   // row_half_mirror
+    reduce_step<2, 0x4e>(v, r & 2);    // quad_perm:[2,3,0,1]
+    reduce_step<1, 0xb1>(v, r & 1);    // quad_perm:[1,0,3,2]
+    return v[0];
+}
+
+// over the 32 lanes of a half wave: the swap leaves one value's two rows in the
+// even row of the pair and the other's in the odd one
+__device__ __forceinline__ float reduce32(float* v, int l32) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]),
+                                                        __float_as_uint(v[i + 16]), false, false);
+        v[i] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    }
+    return reduce16(v, l32 & 15);
+}
+
 // The result of one block's row i: the sum goes to this split's partial sums, or
 // with one split on top of the mass.
 __device__ __forceinline__ void mass_store(const MassParams& p, int bh, int64_t row, int len,
@@ -713,7 +753,8 @@ __device__ __forceinline__ void mass_store(const MassParams& p, int bh, int64_t 
 
 // Few query rows: a wave holds a block of 64 cached rows as operands (four
 // tiles of 16 keys) and takes the groups of 16 query rows in turn; the sums
-// over queries stay in registers until the end.  Bound by the read of K.
+// over queries stay in registers until the end.  Bound by the read of K: all of
+// a wave's loads are issued before the first is used.
 template <typename T, int FMT, int P>
 __global__ void __launch_bounds__(256) mass_kernel(MassParams p) {
     constexpr int STEPS = P / 32, PIECES = P / 64;
@@ -724,62 +765,63 @@ __global__ void __launch_bounds__(256) mass_kernel(MassParams p) {
     if (blk >= p.blocks) return;
     const int len = c8_length(p.length, b, p.n);
     const int64_t key0 = (int64_t)blk * C8_BLOCK;
+    // the row whose sum this lane ends up with, of tile r / 4
+    const int mykey = 16 * (r >> 2) + 4 * g + (r & 3);
+    const int64_t at = (int64_t)bh * p.cap + key0;
+    const float before = p.mass[at + mykey];
     if (key0 >= len) {
-        mass_store(p, bh, key0 + lane, len, 0, 0.0f);
+        if (p.out != p.mass) p.out[at + mykey] = before;
         return;
     }
-    const int64_t at = (int64_t)bh * p.cap + key0;
     u32x4 kr[4][PIECES];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < PIECES; ++i)
             kr[t][i] = *reinterpret_cast<const u32x4*>(p.k + (at + 16 * t + r) * P + 64 * i + 16 * g);
-    const float c = p.scale_log2 * fmaxf(p.ks[(int64_t)bh * (p.cap / C8_BLOCK) + blk], SCALE_MIN);
-    x8 kf[4][STEPS];
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            kf[t][2 * i] = codes_x8<T, FMT>(kr[t][i][0], kr[t][i][1]);
-            kf[t][2 * i + 1] = codes_x8<T, FMT>(kr[t][i][2], kr[t][i][3]);
-        }
-    f32x4 sum[4] = {};
+    const float sk = p.ks[(int64_t)bh * (p.cap / C8_BLOCK) + blk];
     // the first group with a row that sees the block's first key
-    int rg0 = 0;
-    if (p.causal) rg0 = max(0, (int)key0 - (len - p.Q)) * p.G / 16;
+    int rg = 0;
+    if (p.causal)
+        rg = (int)min((int64_t)max(0, (int)key0 - (len - p.Q)) * p.G / 16, (int64_t)p.rows / 16);
     const int groups = (p.rows + 15) / 16;
-    for (int rg = rg0; rg < groups; ++rg) {
+    x8 qf[STEPS];
+    float z;
+    int seen;
+    auto load_group = [&] {
         const RowAt mine = row_at(rg * 16 + r, hk, p.G, p.Q);
-        const int seen = (!mine.there ? 0 : p.causal ? len - p.Q + 1 + mine.t : len) - (int)key0;
-        x8 qf[STEPS];
+        seen = (!mine.there ? 0 : p.causal ? len - p.Q + 1 + mine.t : len) - (int)key0;
         load_q<T, P>(qf, p.q + b * p.q_sb + mine.t * p.q_st + mine.head * p.q_sh, mine.there, g, p.D);
-        float off = INFINITY;
-        if (mine.there) {
-            const float z = p.lse[((int64_t)b * p.H * p.G + mine.head) * p.Q + mine.t];
-            off = z == -INFINITY ? INFINITY : z * LOG2E;
-        }
+        z = mine.there ? p.lse[((int64_t)b * p.H * p.G + mine.head) * p.Q + mine.t] : -INFINITY;
+    };
+    load_group();
+    const float c = p.scale_log2 * fmaxf(sk, SCALE_MIN);
+    f32x4 sum[4] = {};
+    for (;;) {
+        const float off = z == -INFINITY ? INFINITY : z * LOG2E;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             f32x4 s{};
 #pragma unroll
-            for (int i = 0; i < STEPS; ++i) s = T::mfma16(kf[t][i], qf[i], s);
+            for (int i = 0; i < PIECES; ++i) {
+                s = T::mfma16(codes_x8<T, FMT>(kr[t][i][0], kr[t][i][1]), qf[2 * i], s);
+                s = T::mfma16(codes_x8<T, FMT>(kr[t][i][2], kr[t][i][3]), qf[2 * i + 1], s);
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float w = __builtin_amdgcn_exp2f(fmaf(s[e], c, -off));
                 sum[t][e] += 16 * t + 4 * g + e < seen ? w : 0.0f;
             }
         }
+        if (++rg >= groups) break;
+        load_group();
     }
+    float v[16];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float x = sum[t][e];
-#pragma unroll
-            for (int k = 1; k < 16; k <<= 1) x += __shfl_xor(x, k);
-            if (r == 0) mass_store(p, bh, key0 + 16 * t + 4 * g + e, len, 0, x);
-        }
+    for (int i = 0; i < 16; ++i) v[i] = sum[i >> 2][i & 3];
+    const float x = reduce16(v, r);
+    if (key0 + mykey < len) p.out[at + mykey] = before + x;
+    else if (p.out != p.mass) p.out[at + mykey] = before;
 }
 
 // Many query rows: four waves hold a block of 64 cached rows each (two tiles of
@@ -907,16 +949,14 @@ __global__ void __launch_bounds__(256, 2) mass_tile_kernel(MassParams p) {
         }
     }
     if (blk >= p.blocks) return;
+    // value i is sum[i / 16][i % 16], of key 32 (i / 16) + 8 (i % 16 / 4) + 4 hf +
+    // i % 4; lane l32 ends up with value l32
+    float v[32];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            float x = sum[t][e];
-#pragma unroll
-            for (int k = 1; k < 32; k <<= 1) x += __shfl_xor(x, k);
-            if (l32 == 0)
-                mass_store(p, bh, (int64_t)key0 + 32 * t + 8 * (e >> 2) + 4 * hf + (e & 3), len, split, x);
-        }
+    for (int i = 0; i < 32; ++i) v[i] = sum[i >> 4][i & 15];
+    const float x = reduce32(v, l32);
+    const int e = l32 & 15;
+    mass_store(p, bh, (int64_t)key0 + 32 * (l32 >> 4) + 8 * (e >> 2) + 4 * hf + (e & 3), len, split, x);
 }
 
 // Joins the row splits' partial sums, in their order.
@@ -1156,18 +1196,18 @@ struct MassPlan {
     size_t bytes;
 };
 
-// Row splits: where the blocks of keys fill less than two workgroups a CU, as
-// many as do, each with at least four steps.
+// Row splits: only where the blocks of keys fill less than two workgroups a CU,
+// each with at least four steps (1,176 workgroups of 25 steps took 176 us
+// whole, 190 in three splits).
 MassPlan mass_plan(const nkv_cache8_mass_args* a) {
     MassPlan pl{};
     const int64_t rows = a->Q * a->G, heads = (int64_t)a->cache.B * a->cache.H;
     pl.n64 = cdiv(a->n, C8_BLOCK) * C8_BLOCK;
     pl.tile = rows >= MT_ROWS;
     pl.splits = 1;
-    const int64_t base = heads * cdiv(pl.n64, 4 * C8_BLOCK);
+    const int64_t base = heads * cdiv(pl.n64, 4 * C8_BLOCK), steps = cdiv(rows, MT_ROWS);
     if (pl.tile && base > 0 && base < 512)
-        pl.splits = (int)std::max<int64_t>(
-            1, std::min<int64_t>({cdiv(512, base), cdiv(rows, MT_ROWS) / 4, 256}));
+        pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(512, base), steps / 4, 64}));
     if (pl.splits > 1) pl.bytes = (size_t)pl.splits * heads * pl.n64 * sizeof(float);
     return pl;
 }
