@@ -64,6 +64,11 @@ struct Bf16 {
     static constexpr int DTYPE = NKV_ROWS_BF16;
     static __device__ __forceinline__ float load(uint16_t b) { return bf16_bits_to_f32(b); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
+    // e4m3 codes 2 h and 2 h + 1 of a word
+    template <int h>
+    static __device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, h));
+    }
     static __device__ __forceinline__ f32x4 mfma16(x8 a, x8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
@@ -84,6 +89,10 @@ struct Fp16 {
         __builtin_memcpy(&u, &v, 4);
         return u;
     }
+    template <int h>
+    static __device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, h));
+    }
     static __device__ __forceinline__ f32x4 mfma16(x8 a, x8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
@@ -102,6 +111,9 @@ __device__ __forceinline__ X8 as_x8(u32x4 v) {
 // Eight consecutive codes as an MFMA operand of type T.
 template <typename T, int FMT>
 __device__ __forceinline__ typename T::x8 codes_x8(uint32_t lo, uint32_t hi) {
+    if constexpr (FMT == NKV_CACHE8_E4M3)
+        return as_x8<typename T::x8>(u32x4{T::template e4m3_pair<0>(lo), T::template e4m3_pair<1>(lo),
+                                           T::template e4m3_pair<0>(hi), T::template e4m3_pair<1>(hi)});
     const f32x2 a = code_pair<FMT>(lo, 0), b = code_pair<FMT>(lo, 1);
     const f32x2 c = code_pair<FMT>(hi, 0), d = code_pair<FMT>(hi, 1);
     return as_x8<typename T::x8>(

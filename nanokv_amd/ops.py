@@ -1424,9 +1424,10 @@ class Cache8:
             raise ValueError("cache codes must be [B, H, cap, pitch], pitch 64 for head_dim <= 64 "
                              "and 128 above")
         B, H, cap, _ = shape
-        if cap % CACHE8_BLOCK or ks.shape != (B, H, cap // CACHE8_BLOCK) or vs.shape != ks.shape:
+        scales = ks.shape
+        if cap % CACHE8_BLOCK or scales != (B, H, cap // CACHE8_BLOCK) or vs.shape != scales:
             raise ValueError("cache scales must be [B, H, cap / 64] with cap a multiple of 64")
-        if ks.dtype != torch.float32 or vs.dtype != torch.float32:
+        if ks.dtype is not torch.float32 or vs.dtype is not torch.float32:
             raise TypeError("cache scales must be float32")
         if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous()
                 and vs.is_contiguous()):
@@ -1439,48 +1440,50 @@ def _cache8_call(name: str, device: torch.device, *args) -> None:
     """One C call with its tensors' device current (a launch on another device's
     stream would go to the current one)."""
     fn = getattr(lib(), name)
-    if torch.cuda.current_device() == device.index:
-        check(name, fn(_stream(device), *args))
+    if torch._C._cuda_getDevice() == device.index:
+        code = fn(_stream(device), *args)
     else:
         with torch.cuda.device(device):
-            check(name, fn(_stream(device), *args))
+            code = fn(_stream(device), *args)
+    if code:
+        check(name, code)
 
 
 def _cache8_scratch(name: str, args, device: torch.device, workspace: Optional[torch.Tensor]):
     """The workspace of a call: the caller's if given, else one from torch's
     allocator, which orders its reuse behind the launch's stream."""
-    size = getattr(lib(), name + "_workspace_size")
-    need = size(byref(args))
+    need = getattr(lib(), name)(byref(args))
     if need == 0:
         return None, 0
     if workspace is None:
-        workspace = torch.empty(need, device=device, dtype=torch.uint8)
-    elif workspace.device != device or not workspace.is_contiguous():
+        return torch.empty(need, device=device, dtype=torch.uint8), need
+    if workspace.device != device or not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous tensor on the inputs' device")
     return workspace, workspace.numel() * workspace.element_size()
 
 
-def _cache8_lengths(t: Optional[torch.Tensor], B: int, name: str) -> Optional[int]:
+def _cache8_ints(t: Optional[torch.Tensor], B: int, name: str) -> Optional[int]:
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.shape != (B,) or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != (B,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of one entry per sequence")
     return t.data_ptr()
 
 
-def _cache8_bound(cache: Cache8, length, max_length: Optional[int]):
-    """(length tensor or None, the bound n) of a call's length: an int for all
-    sequences, or an int32 tensor [B] with entries in [0, max_length]."""
+def _cache8_bound(cap: int, B: int, length, max_length: Optional[int]):
+    """(pointer or None, the bound n) of a call's length: an int for all
+    sequences, or an int32 tensor [B] whose entries are clamped to [0,
+    max_length]."""
     if isinstance(length, torch.Tensor):
-        n = cache.cap if max_length is None else int(max_length)
-        lengths = length
+        n = cap if max_length is None else int(max_length)
+        at = _cache8_ints(length, B, "length")
     else:
-        n, lengths = int(length), None
+        n, at = int(length), None
         if max_length is not None and n > max_length:
             raise ValueError("length is above max_length")
-    if not 0 <= n <= cache.cap:
-        raise ValueError(f"length must be in [0, {cache.cap}]")
-    return lengths, n
+    if not 0 <= n <= cap:
+        raise ValueError(f"length must be in [0, {cap}]")
+    return at, n
 
 
 def cache8_write(cache: Cache8, k: torch.Tensor, v: torch.Tensor, start,
@@ -1495,44 +1498,37 @@ def cache8_write(cache: Cache8, k: torch.Tensor, v: torch.Tensor, start,
     int32 [B], how many of a sequence's T rows are written (a padded batch)."""
     given = start if isinstance(start, torch.Tensor) else None
     device = _require_gpu(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, given, counts)
-    a = NkvCache8WriteArgs()
-    a.cache = c = cache.struct()
-    if k.dtype not in _ROW_CODES or v.dtype != k.dtype:
+    c = cache.struct()
+    code = _ROW_CODES.get(k.dtype)
+    if code is None or v.dtype != k.dtype:
         raise TypeError("k and v must both be bf16, fp16 or fp32")
-    if k.dim() != 4 or v.shape != k.shape or k.shape[0] != c.B or k.shape[2] != c.H \
-            or k.shape[3] != c.D:
+    shape, B = k.shape, c.B
+    if len(shape) != 4 or v.shape != shape or shape[0] != B or shape[2] != c.H or shape[3] != c.D:
         raise ValueError("k and v must be [B, T, H, head_dim] of the cache's B, H and head_dim")
-    a.T, a.dtype = k.shape[1], _ROW_CODES[k.dtype]
     if k.numel() == 0:
         return
-    a.k, a.v = k.data_ptr(), v.data_ptr()
-    a.k_sb, a.k_st, a.k_sh = _strides_bthd(k, "k")
-    a.v_sb, a.v_st, a.v_sh = _strides_bthd(v, "v")
-    a.counts = _cache8_lengths(counts, c.B, "counts")
-    if given is not None:
-        a.start_dev = _cache8_lengths(given, c.B, "start")
-    else:
-        a.start = int(start)
+    a = NkvCache8WriteArgs(c, k.data_ptr(), *_strides_bthd(k, "k"),
+                           v.data_ptr(), *_strides_bthd(v, "v"), shape[1],
+                           0 if given is not None else int(start),
+                           _cache8_ints(given, B, "start"), _cache8_ints(counts, B, "counts"),
+                           code)
     _cache8_call("nkv_cache8_write", device, byref(a))
 
 
-def _cache8_query(a, q: torch.Tensor, cache: Cache8, length, max_length, softmax_scale, causal):
-    """Fills the query half of attend's and mass's arguments."""
-    a.cache = c = cache.struct()
+def _cache8_query(q: torch.Tensor, cache: Cache8, length, max_length, softmax_scale):
+    """The query half of attend's and mass's arguments: the cache, then (cache,
+    G, dtype, Q, n, length, q, strides) and the softmax scale."""
+    c = cache.struct()
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError("q must be bf16 or fp16")
-    if q.dim() != 4 or q.shape[0] != c.B or q.shape[3] != c.D or q.shape[2] == 0 \
-            or q.shape[2] % c.H:
+    shape, H, D = q.shape, c.H, c.D
+    if len(shape) != 4 or shape[0] != c.B or shape[3] != D or shape[2] == 0 or shape[2] % H:
         raise ValueError("q must be [B, Q, heads, head_dim] with heads a multiple of the cache's")
-    a.G, a.dtype, a.Q = q.shape[2] // c.H, _ROW_CODES[q.dtype], q.shape[1]
-    lengths, a.n = _cache8_bound(cache, length, max_length)
-    a.length = _cache8_lengths(lengths, c.B, "length")
-    a.q = q.data_ptr()
-    if q.numel():
-        a.q_sb, a.q_st, a.q_sh = _strides_bthd(q, "q")
-    a.softmax_scale = c.D ** -0.5 if softmax_scale is None else float(softmax_scale)
-    a.causal = 1 if causal else 0
-    return c
+    at, n = _cache8_bound(c.cap, c.B, length, max_length)
+    strides = _strides_bthd(q, "q") if q.numel() else (0, 0, 0)
+    scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
+    return c, (c, shape[2] // H, _ROW_CODES[q.dtype], shape[1], n, at, q.data_ptr(),
+               *strides), scale
 
 
 def cache8_attend(q: torch.Tensor, cache: Cache8, length, *, max_length: Optional[int] = None,
@@ -1551,20 +1547,18 @@ def cache8_attend(q: torch.Tensor, cache: Cache8, length, *, max_length: Optiona
     uint8 buffer of nkv_cache8_attend_workspace_size bytes."""
     device = _require_gpu(q, cache.k, cache.v, cache.k_scale, cache.v_scale, out,
                           length if isinstance(length, torch.Tensor) else None)
-    a = NkvCache8AttendArgs()
-    c = _cache8_query(a, q, cache, length, max_length, softmax_scale, causal)
+    c, query, scale = _cache8_query(q, cache, length, max_length, softmax_scale)
+    B, Q, heads, D = q.shape
     if out is None:
-        out = torch.empty(q.shape, device=device, dtype=q.dtype)
+        out = torch.empty((B, Q, heads, D), device=device, dtype=q.dtype)
+        strides = (Q * heads * D, heads * D, D)
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError("out must have q's shape and type")
-    a.out = out.data_ptr()
-    if q.numel():
-        a.o_sb, a.o_st, a.o_sh = _strides_bthd(out, "out")
-    lse = None
-    if return_lse:
-        lse = torch.empty((c.B, q.shape[2], q.shape[1]), device=device, dtype=torch.float32)
-        a.lse = lse.data_ptr()
-    scratch, nbytes = _cache8_scratch("nkv_cache8_attend", a, device, workspace)
+    else:
+        strides = _strides_bthd(out, "out") if q.numel() else (0, 0, 0)
+    lse = torch.empty((B, heads, Q), device=device, dtype=torch.float32) if return_lse else None
+    a = NkvCache8AttendArgs(*query, out.data_ptr(), *strides, _ptr(lse), scale, bool(causal))
+    scratch, nbytes = _cache8_scratch("nkv_cache8_attend_workspace_size", a, device, workspace)
     _cache8_call("nkv_cache8_attend", device, byref(a), _ptr(scratch), nbytes)
     return out, lse
 
@@ -1580,8 +1574,7 @@ def cache8_mass(q: torch.Tensor, cache: Cache8, lse: torch.Tensor, mass: torch.T
     out = mass if out is None else out
     device = _require_gpu(q, cache.k, cache.v, cache.k_scale, cache.v_scale, lse, mass, out,
                           length if isinstance(length, torch.Tensor) else None)
-    a = NkvCache8MassArgs()
-    c = _cache8_query(a, q, cache, length, max_length, softmax_scale, causal)
+    c, query, scale = _cache8_query(q, cache, length, max_length, softmax_scale)
     _contig(lse, torch.float32, "lse")
     if lse.shape != (c.B, q.shape[2], q.shape[1]):
         raise ValueError("lse must be [B, heads, Q]")
@@ -1589,8 +1582,9 @@ def cache8_mass(q: torch.Tensor, cache: Cache8, lse: torch.Tensor, mass: torch.T
         _contig(t, torch.float32, name)
         if t.shape != (c.B, c.H, c.cap):
             raise ValueError(f"{name} must be [B, H, cap]")
-    a.lse, a.mass, a.out = lse.data_ptr(), mass.data_ptr(), out.data_ptr()
-    scratch, nbytes = _cache8_scratch("nkv_cache8_mass", a, device, workspace)
+    a = NkvCache8MassArgs(*query, lse.data_ptr(), mass.data_ptr(), out.data_ptr(), scale,
+                          bool(causal))
+    scratch, nbytes = _cache8_scratch("nkv_cache8_mass_workspace_size", a, device, workspace)
     _cache8_call("nkv_cache8_mass", device, byref(a), _ptr(scratch), nbytes)
     return out
 
@@ -1608,21 +1602,19 @@ def cache8_evict(cache: Cache8, mass: torch.Tensor, length, out: Cache8, out_mas
     device = _require_gpu(cache.k, cache.v, cache.k_scale, cache.v_scale, mass, out.k, out.v,
                           out.k_scale, out.v_scale, out_mass,
                           length if isinstance(length, torch.Tensor) else None)
-    a = NkvCache8EvictArgs()
-    a.cache, a.out = c, o = cache.struct(), out.struct()
+    c, o = cache.struct(), out.struct()
     for name, t, cap in (("mass", mass, c.cap), ("out_mass", out_mass, o.cap)):
         _contig(t, torch.float32, name)
         if t.shape != (c.B, c.H, cap):
             raise ValueError(f"{name} must be [B, H, cap] of its cache")
-    lengths, a.n = _cache8_bound(cache, length, max_length)
-    a.length = _cache8_lengths(lengths, c.B, "length")
-    a.keep, a.sink, a.recent = int(keep), int(sink), int(recent)
-    if a.keep < 1:
+    at, n = _cache8_bound(c.cap, c.B, length, max_length)
+    keep = int(keep)
+    if keep < 1:
         raise ValueError("keep must be positive")
-    rows = torch.empty((c.B, c.H, a.keep), device=device, dtype=torch.int32)
+    rows = torch.empty((c.B, c.H, keep), device=device, dtype=torch.int32)
     left = torch.empty((c.B,), device=device, dtype=torch.int32)
-    a.mass, a.out_mass = mass.data_ptr(), out_mass.data_ptr()
-    a.rows, a.out_length = rows.data_ptr(), left.data_ptr()
-    scratch, nbytes = _cache8_scratch("nkv_cache8_evict", a, device, workspace)
+    a = NkvCache8EvictArgs(c, o, mass.data_ptr(), out_mass.data_ptr(), rows.data_ptr(),
+                           left.data_ptr(), at, n, keep, int(sink), int(recent))
+    scratch, nbytes = _cache8_scratch("nkv_cache8_evict_workspace_size", a, device, workspace)
     _cache8_call("nkv_cache8_evict", device, byref(a), _ptr(scratch), nbytes)
     return rows, left
