@@ -57,6 +57,48 @@ __device__ __forceinline__ f32x2 code_pair(uint32_t w, int h) {
     }
 }
 
+// x / s with y = 1 / s rounded to the nearest, itself rounded to the nearest:
+// x y corrected twice by its exact remainder (the second correction of a result
+// within one step rounds as the division does; Markstein, "Computation of
+// elementary functions on the IBM RISC System/6000 processor").  Five
+// instructions, where the compiler's division takes ten.  Quotients below 2^-60,
+// where a remainder may underflow, give the zero code either way.
+__device__ __forceinline__ float div_by(float x, float s, float y) {
+    float q = x * y;
+    q = fmaf(fmaf(-q, s, x), y, q);
+    return fmaf(fmaf(-q, s, x), y, q);
+}
+
+// to_codes of values that are known to be finite and within the largest code.
+template <int FMT>
+__device__ __forceinline__ uint32_t to_codes_fast(float a, float b, float c, float d) {
+    if constexpr (FMT == NKV_CACHE8_INT8) {
+        // 1.5 * 2^23 + x: the sum's rounding is the rounding to a whole number,
+        // and its low byte is the code
+        constexpr float BIG = 12582912.0f;
+        const uint32_t x = __float_as_uint(a + BIG), y = __float_as_uint(b + BIG);
+        const uint32_t z = __float_as_uint(c + BIG), w = __float_as_uint(d + BIG);
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(w, z, 0x0c0c0400u),
+                                     __builtin_amdgcn_perm(y, x, 0x0c0c0400u), 0x05040100u);
+    } else {
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+    }
+}
+
+// max over a wave, in the VALU: the four 16-lane rows first, then lanes l ^ 8,
+// l ^ 7, l ^ 2 and l ^ 1 of a row
+__device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = max(b[0], b[1]);
+    x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp(x, 0x128, 0xf, 0xf, true));
+    x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp(x, 0x141, 0xf, 0xf, true));
+    x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp(x, 0x4e, 0xf, 0xf, true));
+    return max(x, (uint32_t)__builtin_amdgcn_mov_dpp(x, 0xb1, 0xf, 0xf, true));
+}
+
 // The 16-bit types of queries and outputs.  Both hold every code exactly, so
 // products of queries and codes are formed in the queries' own type.
 struct Bf16 {

@@ -48,37 +48,72 @@ struct WriteParams {
     int B, H, D;
 };
 
-// Eight consecutive elements of a row as fp32.
+// Eight consecutive elements of a row as they come.
 template <int DTYPE>
-__device__ __forceinline__ void load8(const void* x, int64_t at, float (&f)[8]) {
-    if constexpr (DTYPE == NKV_ROWS_FP32) {
-        const f32x4* p = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(x) + at);
-        const f32x4 a = p[0], b = p[1];
+struct Piece {
+    static constexpr int W = DTYPE == NKV_ROWS_FP32 ? 8 : 4;
+    // the least bit pattern of a magnitude that is not finite
+    static constexpr uint32_t INF =
+        DTYPE == NKV_ROWS_FP32 ? 0x7f800000u : DTYPE == NKV_ROWS_BF16 ? 0x7f80u : 0x7c00u;
+    uint32_t w[W];
+    __device__ __forceinline__ void load(const void* x, int64_t at) {
+        const u32x4* p = reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(x) +
+                                                        at * (W / 2));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = a[i], f[4 + i] = b[i];
-    } else {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(x) + at);
+        for (int i = 0; i < W / 4; ++i) {
+            const u32x4 v = p[i];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint16_t u = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-            f[i] = DTYPE == NKV_ROWS_BF16 ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
+            for (int k = 0; k < 4; ++k) w[4 * i + k] = v[k];
         }
     }
-}
-
-__device__ __forceinline__ float wave_max(float x) {
+    // magnitudes as integers order as the magnitudes do, NaN above infinity
+    __device__ __forceinline__ void largest(uint32_t& m) const {
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
+        for (int i = 0; i < W; ++i) {
+            if constexpr (DTYPE == NKV_ROWS_FP32) {
+                m = max(m, w[i] & 0x7fffffffu);
+            } else {
+                typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+                m = __builtin_bit_cast(
+                    uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
+                                                        __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu)));
+            }
+        }
+    }
+    static __device__ __forceinline__ float from(uint32_t bits) {
+        if constexpr (DTYPE == NKV_ROWS_FP32) return __uint_as_float(bits);
+        else if constexpr (DTYPE == NKV_ROWS_BF16) return bf16_bits_to_f32((uint16_t)bits);
+        else return f16_bits_to_f32((uint16_t)bits);
+    }
+    __device__ __forceinline__ float operator[](int e) const {
+        if constexpr (DTYPE == NKV_ROWS_FP32) return __uint_as_float(w[e]);
+        else if constexpr (DTYPE == NKV_ROWS_BF16)
+            return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+        else return f16_bits_to_f32((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
+    }
+};
+
+// The largest of a workgroup's values, in every thread.
+__device__ __forceinline__ uint32_t block_umax(uint32_t x) {
+    __shared__ uint32_t part[4];
+    x = wave_umax(x);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = max(max(part[0], part[1]), max(part[2], part[3]));
+    __syncthreads();
     return x;
 }
 
 // One workgroup per (block of 64 rows, head, K or V, item): the block's new
 // rows are read once into registers, eight elements a thread and piece, their
 // amplitude is reduced, and the codes are written.  Bound by HBM: three bytes
-// move per bf16 element.
+// move per bf16 element.  Blocks that hold a value that is not finite take a
+// slower path of the same results.
 template <int DTYPE, int FMT, int P>
 __global__ void __launch_bounds__(256) write_kernel(WriteParams p) {
     constexpr int CH = P / 8, STEP = 256 / CH, N = C8_BLOCK / STEP;
+    constexpr float TOP = Fmt8<FMT>::TOP;
+    using X = Piece<DTYPE>;
     const int kv = blockIdx.z & 1, b = blockIdx.z >> 1, h = blockIdx.y;
     const int64_t start =
         p.start_dev ? min(max((int64_t)p.start_dev[b], (int64_t)0), p.cap) : p.start;
@@ -92,32 +127,35 @@ __global__ void __launch_bounds__(256) write_kernel(WriteParams p) {
     float* scale = p.scale[kv] + bh * (p.cap / C8_BLOCK) + blk;
     const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
     const int lo = (int)max(start - row0, (int64_t)0), hi = (int)min(end - row0, (int64_t)C8_BLOCK);
-    float x[N][8];
-    float top = 0.0f;
+    X x[N];
+    const int64_t src = b * p.sb[kv] + (row0 - start) * p.st[kv] + h * p.sh[kv] + 8 * c;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int r = r0 + STEP * i;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
-        if (r >= lo && r < hi && 8 * c < p.D)
-            load8<DTYPE>(p.x[kv], b * p.sb[kv] + (row0 + r - start) * p.st[kv] + h * p.sh[kv] + 8 * c,
-                         x[i]);
+        x[i] = X{};
+        if (r >= lo && r < hi && 8 * c < p.D) x[i].load(p.x[kv], src + r * p.st[kv]);
     }
+    const float s0 = lo > 0 ? *scale : 0.0f;
+    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int i = 0; i < N; ++i) x[i].largest(m);
+    if constexpr (DTYPE != NKV_ROWS_FP32) m = max(m & 0xffffu, m >> 16);
+    m = block_umax(m);
+    const bool finite = m < X::INF;
+    float top = X::from(m);
+    if (!finite) {  // the largest finite value
+        float t = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float a = fabsf(x[i][e]);
-            top = fmaxf(top, a < INFINITY ? a : 0.0f);  // finite values alone
-        }
-    __shared__ float part[4];
-    top = wave_max(top);
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-    float s = fmaxf(top, C8_TINY) / Fmt8<FMT>::TOP;
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float a = fabsf(x[i][e]);
+                t = fmaxf(t, a < INFINITY ? a : 0.0f);
+            }
+        top = __uint_as_float(block_umax(__float_as_uint(t)));
+    }
+    float s = fmaxf(top, C8_TINY) / TOP;
     if (lo > 0) {
-        const float s0 = *scale;
         if (s0 >= s) {
             s = s0;
         } else {
@@ -134,18 +172,27 @@ __global__ void __launch_bounds__(256) write_kernel(WriteParams p) {
             }
         }
     }
+    const float y = 1.0f / s;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int r = r0 + STEP * i;
         if (r < lo || r >= hi) continue;
-        const float(&f)[8] = x[i];
+        float q[8];
         u32x2 w;
-        w[0] = to_codes<FMT>(f[0] / s, f[1] / s, f[2] / s, f[3] / s);
-        w[1] = to_codes<FMT>(f[4] / s, f[5] / s, f[6] / s, f[7] / s);
+        if (finite) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[e] = div_by(x[i][e], s, y);
+            w[0] = to_codes_fast<FMT>(q[0], q[1], q[2], q[3]);
+            w[1] = to_codes_fast<FMT>(q[4], q[5], q[6], q[7]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[e] = x[i][e] / s;
+            w[0] = to_codes<FMT>(q[0], q[1], q[2], q[3]);
+            w[1] = to_codes<FMT>(q[4], q[5], q[6], q[7]);
+        }
         *reinterpret_cast<u32x2*>(codes + r * P + 8 * c) = w;
     }
-    __syncthreads();  // every thread has read the old scale
-    if (threadIdx.x == 0) *scale = s;
+    if (threadIdx.x == 0) *scale = s;  // read by every thread before block_umax
 }
 
 template <int DTYPE>
@@ -346,7 +393,7 @@ __global__ void __launch_bounds__(256) compact_kernel(EvictParams p) {
         }
         src[r] = at;
         from[r] = s;
-        const float m = wave_max(s);
+        const float m = __uint_as_float(wave_umax(__float_as_uint(s)));  // (not negative)
         if (r == 0) {
             top = m;
             p.out_scale[kv][bh * (p.out_cap / C8_BLOCK) + blockIdx.x] = m;
