@@ -886,7 +886,7 @@ int nkv_cache8_mass(void* stream, const nkv_cache8_mass_args* args, void* worksp
  *   rows        [B, H, keep] int32, the rows kept, -1 past the last
  *   out_length  [B] int32, min(length, keep)
  * Rows of out and out_mass past the kept ones are left as they were.  Nothing
- * of out or out_mass may overlap the cache or mass.
+ * of out or out_mass may overlap the cache or mass.  mass is 16-byte aligned.
  */
 typedef struct nkv_cache8_evict_args {
     nkv_cache8 cache;

@@ -236,10 +236,21 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 // it, rows equal to the last key from the lowest up.  Up to SEL_LDS rows the
 // keys stay in LDS (one read of the masses), longer heads are read again for
 // each digit and for the list.
+// Sums over lanes 0 .. l: within the rows of 16, then from row to row (DPP).
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
+    return x;
+}
+
 constexpr int SEL_WAVES = 16, SEL_THREADS = 64 * SEL_WAVES;
 constexpr int SEL_LDS = 32768;
 constexpr int SEL_BINS = 2048;
-constexpr int SEL_AHEAD = 8;          // keys of a lane in flight
+constexpr int SEL_AHEAD = 4;            // keys of a lane in flight from LDS
 
 template <bool LDS>
 __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
@@ -260,76 +271,99 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
     // this wave's part: rows part .. part_end in steps of 64
     const int steps = (n + SEL_THREADS - 1) / SEL_THREADS;
     const int part = wave * steps * 64, part_end = min(part + steps * 64, n);
-    extern __shared__ uint32_t held[];                  // the keys, in row order (LDS)
-    __shared__ uint32_t hist[SEL_BINS];
-    __shared__ uint32_t sums[SEL_WAVES];
-    __shared__ uint32_t pick[2];                        // digit, rows still wanted in it
-    // f(key, row) over the part in order, SEL_AHEAD loads in flight; rows past
-    // the part's end come with any key
-    auto each = [&](bool first, auto f) {
-        for (int j0 = 0; j0 < steps; j0 += SEL_AHEAD) {
-            uint32_t k[SEL_AHEAD];
+    extern __shared__ __align__(16) uint32_t held[];    // LDS: the keys in row order
+    __shared__ uint32_t hist[3][SEL_BINS];  // one a pass: no wave waits to reuse it
+    // f(key, row) over the part in order, AHEAD keys in flight; rows past the
+    // part's end come with any key
+    constexpr int AHEAD = LDS ? SEL_AHEAD : 8;
+    auto each = [&](auto f) {
+        for (int j0 = 0; j0 < steps; j0 += AHEAD) {
+            uint32_t k[AHEAD];
+            const int i0 = part + 64 * j0 + lane;
 #pragma unroll
-            for (int j = 0; j < SEL_AHEAD; ++j) {
-                const int i = min(part + 64 * (j0 + j) + lane, n - 1);
-                k[j] = LDS && !first ? held[i] : __float_as_uint(mass[i]);
+            for (int j = 0; j < AHEAD; ++j) {
+                if (LDS) k[j] = held[i0 + 64 * j];  // (up to AHEAD steps past the end)
+                else k[j] = __float_as_uint(mass[min(i0 + 64 * j, n - 1)]);
             }
 #pragma unroll
-            for (int j = 0; j < SEL_AHEAD; ++j) {
+            for (int j = 0; j < AHEAD; ++j) {
                 if (j0 + j >= steps) break;
-                const int i = part + 64 * (j0 + j) + lane;
-                if (!LDS || first) k[j] = order_key(__uint_as_float(k[j]));
-                if (LDS && first && i < part_end) held[i] = k[j];
-                f(k[j], i);
+                f(LDS ? k[j] : order_key(__uint_as_float(k[j])), i0 + 64 * j);
             }
         }
     };
     // rows of the part to choose from: lo .. lo + width
     const uint32_t width = (uint32_t)max(min(hi, part_end) - lo, 0);
     uint32_t prefix = 0, left = want, mask = 0;
+    // digit d is counted at 64 (d mod 32) + d / 32: lane d / 32 reads it below,
+    // without bank conflicts
+    auto bin = [](uint32_t d) { return (d & 31) << 6 | d >> 5; };
+    auto count_digit = [&](uint32_t* hist, bool count, uint32_t d) {
+        if (__ballot(count) == ~0ull) {  // one add where the whole wave has one digit (equal masses)
+            const uint32_t d0 = __builtin_amdgcn_readfirstlane(d);
+            if (__ballot(d == d0) == ~0ull) {
+                if (lane == 0) atomicAdd(&hist[bin(d0)], 64u);
+                return;
+            }
+        }
+        if (count) atomicAdd(&hist[bin(d)], 1u);
+    };
+    for (int i = tid; i < 3 * SEL_BINS; i += SEL_THREADS) hist[0][i] = 0;
+    __syncthreads();
+#pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const uint32_t top = pass == 2 ? 1023u : 2047u;
-        for (int i = tid; i < SEL_BINS; i += SEL_THREADS) hist[i] = 0;
-        __syncthreads();
-        each(pass == 0, [&](uint32_t k, int i) {
-            const bool count = (uint32_t)(i - lo) < width && (k & mask) == prefix;
-            const uint32_t d = (k >> shift) & top, d0 = __builtin_amdgcn_readfirstlane(d);
-            // one add where the whole wave has one digit (equal masses)
-            if (__ballot(count && d == d0) == ~0ull) {
-                if (lane == 0) atomicAdd(&hist[d0], 64u);
-            } else if (count) {
-                atomicAdd(&hist[d], 1u);
+        if (LDS && pass == 0) {
+            // four rows a thread and load, every load of the workgroup in flight
+            constexpr int PER = SEL_LDS / (4 * SEL_THREADS);
+            f32x4 x[PER];
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int i = 4 * (tid + SEL_THREADS * j);
+                if (i < n) x[j] = *reinterpret_cast<const f32x4*>(mass + i);
             }
-        });
-        __syncthreads();
-        // the digit at which the count from above reaches `left`: thread t has
-        // the digits 2047 - 2 t and 2046 - 2 t
-        const uint32_t d1 = SEL_BINS - 1 - 2 * tid;
-        const uint32_t h1 = hist[d1], h0 = hist[d1 - 1];
-        uint32_t run = h1 + h0;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t x = __shfl_up(run, o);
-            if (lane >= o) run += x;
-        }
-        if (lane == 63) sums[wave] = run;
-        __syncthreads();
-        uint32_t above = run - h1 - h0;
+            for (int j = 0; j < PER; ++j) {
+                const int i = 4 * (tid + SEL_THREADS * j);
+                if (4 * SEL_THREADS * j >= n) break;
+                u32x4 k;
 #pragma unroll
-        for (int w = 0; w < SEL_WAVES; ++w) above += w < wave ? sums[w] : 0;
-        if (above < left && above + h1 >= left) {
-            pick[0] = d1;
-            pick[1] = left - above;
-        } else if (above + h1 < left && above + h1 + h0 >= left) {
-            pick[0] = d1 - 1;
-            pick[1] = left - above - h1;
+                for (int e = 0; e < 4; ++e) {
+                    k[e] = order_key(x[j][e]);
+                    count_digit(hist[0], i + e >= lo && i + e < hi, k[e] >> 21);
+                }
+                if (i < steps * SEL_THREADS) *reinterpret_cast<u32x4*>(held + i) = k;
+            }
+        } else {
+            each([&](uint32_t k, int i) {
+                count_digit(hist[pass], (uint32_t)(i - lo) < width && (k & mask) == prefix, (k >> shift) & top);
+            });
         }
-        if (tid == 0 && left == 0) pick[0] = top, pick[1] = 0;  // none wanted
         __syncthreads();
-        prefix |= pick[0] << shift;
+        // The digit at which the count from above reaches `left`, found by every
+        // wave for itself: lane l has the 32 digits below 2048 - 32 l.
+        uint32_t h[32], mine = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            h[i] = hist[pass][64 * i + 63 - lane];
+            mine += h[i];
+        }
+        const uint32_t through = wave_scan(mine);
+        const int l0 = __builtin_ctzll(__ballot(through >= left));
+        uint32_t above = through - mine, passed = 32, over = above;
+#pragma unroll
+        for (int i = 31; i >= 0; --i) {
+            above += h[i];
+            if (above < left) {                             // the digit lies below this one
+                passed = i;
+                over = above;
+            }
+        }
+        prefix |= (uint32_t)__builtin_amdgcn_readlane(SEL_BINS - 32 * (lane + 1) + passed - 1, l0)
+                  << shift;
+        left -= (uint32_t)__builtin_amdgcn_readlane(over, l0);
         mask |= top << shift;
-        left = pick[1];
     }
     // `left` of the rows whose key is `prefix` are kept, and all above it
     __shared__ uint32_t kept[SEL_WAVES], tied[SEL_WAVES];
@@ -340,7 +374,7 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
         a = __ballot(choose ? k > floor_key : i < part_end);
         t = __ballot(choose && k == prefix);
     };
-    each(false, [&](uint32_t k, int i) {
+    each([&](uint32_t k, int i) {
         uint64_t a, t;
         marks(k, i, a, t);
         nk += (uint32_t)__popcll(a);
@@ -357,12 +391,18 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
         bk += w < wave ? kept[w] : 0;
         bt += w < wave ? tied[w] : 0;
     }
-    each(false, [&](uint32_t k, int i) {
+    each([&](uint32_t k, int i) {
         uint64_t a, t;
         marks(k, i, a, t);
-        const uint32_t ra = bk + __builtin_amdgcn_mbcnt_hi((uint32_t)(a >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)a, 0));
-        const uint32_t rt = bt + __builtin_amdgcn_mbcnt_hi((uint32_t)(t >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)t, 0));
-        if (((a >> lane) & 1) || (((t >> lane) & 1) && rt < left)) rows[ra + min(rt, left)] = i;
+        const uint32_t ra = bk + __builtin_amdgcn_mbcnt_hi((uint32_t)(a >> 32),
+                                                           __builtin_amdgcn_mbcnt_lo((uint32_t)a, 0));
+        if (t == 0) {
+            if ((a >> lane) & 1) rows[ra + min(bt, left)] = i;
+        } else {
+            const uint32_t rt = bt + __builtin_amdgcn_mbcnt_hi(
+                                         (uint32_t)(t >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)t, 0));
+            if (((a >> lane) & 1) || (((t >> lane) & 1) && rt < left)) rows[ra + min(rt, left)] = i;
+        }
         bk += (uint32_t)__popcll(a);
         bt += (uint32_t)__popcll(t);
     });
@@ -451,6 +491,8 @@ int check_evict(const nkv_cache8_evict_args* a) {
     if (c.B == 0) return NKV_OK;
     NKV_REQUIRE(a->mass && a->out_mass && a->rows && a->out_length, NKV_ERR_INVALID,
                 "mass, out_mass, rows and out_length are required");
+    NKV_REQUIRE(reinterpret_cast<uintptr_t>(a->mass) % 16 == 0, NKV_ERR_INVALID,
+                "mass must be 16-byte aligned");
     const int64_t heads = (int64_t)c.B * c.H, P = c8_pitch(c.D);
     const Range in[5] = {{c.k, heads * c.cap * P}, {c.v, heads * c.cap * P},
                          {c.k_scale, heads * c.cap / 16}, {c.v_scale, heads * c.cap / 16},
@@ -526,7 +568,8 @@ extern "C" int nkv_cache8_evict(void* stream, const nkv_cache8_evict_args* a, vo
                   (int)a->keep, (int)a->sink, (int)a->recent};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     if (a->n <= SEL_LDS) {
-        const size_t smem = (size_t)a->n * 4;
+        // whole steps of every wave, and the reads ahead of the last one
+        const size_t smem = (size_t)(cdiv(a->n, SEL_THREADS) * SEL_THREADS + 64 * SEL_AHEAD) * 4;
         if ((rc = set_smem(select_kernel<true>, smem))) return rc;
         select_kernel<true><<<(unsigned)(c.B * c.H), SEL_THREADS, smem, s>>>(p);
     } else {

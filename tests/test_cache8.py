@@ -159,6 +159,7 @@ def test_mass_refusals(kw, code, text):
     (dict(recent=-1), _lib.NKV_ERR_INVALID, b"sink"),
     (dict(n=129), _lib.NKV_ERR_INVALID, b"n must"),
     (dict(mass=None), _lib.NKV_ERR_INVALID, b"required"),
+    (dict(mass=PTR + (8 << 24) + 4), _lib.NKV_ERR_INVALID, b"mass must be 16"),
 ])
 def test_evict_refusals(kw, code, text):
     refused("nkv_cache8_evict", evict_args(**kw), code, text, None, 0)
