@@ -101,8 +101,43 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
 
 // The 16-bit types of queries and outputs.  Both hold every code exactly, so
 // products of queries and codes are formed in the queries' own type.
+// Partial: eight values of a split's partial result.
+struct Partial16 {
+    u32x4 w;
+    __device__ __forceinline__ void load(const void* p, int64_t at) {
+        w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p) + at);
+    }
+    __device__ __forceinline__ void store(void* p, int64_t at) const {
+        *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(p) + at) = w;
+    }
+    __device__ __forceinline__ void set(const float (&o)[8], float f);
+    __device__ __forceinline__ float operator[](int k) const {
+        return f16_bits_to_f32((uint16_t)(w[k >> 1] >> (16 * (k & 1))));
+    }
+};
+
+struct Partial32 {
+    f32x4 a, b;
+    __device__ __forceinline__ void load(const void* p, int64_t at) {
+        const f32x4* q = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(p) + at);
+        a = q[0];
+        b = q[1];
+    }
+    __device__ __forceinline__ void store(void* p, int64_t at) const {
+        f32x4* q = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p) + at);
+        q[0] = a;
+        q[1] = b;
+    }
+    __device__ __forceinline__ void set(const float (&o)[8], float f) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a[k] = o[k] * f, b[k] = o[4 + k] * f;
+    }
+    __device__ __forceinline__ float operator[](int k) const { return k < 4 ? a[k] : b[k - 4]; }
+};
+
 struct Bf16 {
     using x8 = bf16x8;
+    using Partial = Partial16;
     static constexpr int DTYPE = NKV_ROWS_BF16;
     static __device__ __forceinline__ float load(uint16_t b) { return bf16_bits_to_f32(b); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
@@ -121,6 +156,7 @@ struct Bf16 {
 
 struct Fp16 {
     using x8 = f16x8;
+    using Partial = Partial32;
     static constexpr int DTYPE = NKV_ROWS_FP16;
     static __device__ __forceinline__ float load(uint16_t b) { return f16_bits_to_f32(b); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -142,6 +178,11 @@ struct Fp16 {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     }
 };
+
+__device__ __forceinline__ void Partial16::set(const float (&o)[8], float f) {
+    w = u32x4{Fp16::pack(o[0] * f, o[1] * f), Fp16::pack(o[2] * f, o[3] * f),
+              Fp16::pack(o[4] * f, o[5] * f), Fp16::pack(o[6] * f, o[7] * f)};
+}
 
 template <typename X8>
 __device__ __forceinline__ X8 as_x8(u32x4 v) {

@@ -38,9 +38,8 @@ struct AttendParams {
     uint16_t* out;
     float* lse;
     // partial results of the splits, [B*H][splits][rows]: the output in units of
-    // 2^unit (at most the largest code, so fp16 holds it), the maximum (log2),
-    // the sum and the unit
-    uint16_t* part;               // [..][P] fp16
+    // 2^unit, the maximum (log2), the sum and the unit
+    void* part;                   // [..][P] of T::Partial
     f32x4* part_ml;
     int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;
     int64_t cap, items;
@@ -95,19 +94,21 @@ __device__ __forceinline__ void store_row(const AttendParams& p, int b, int hk, 
 }
 static_assert(LIFT == 12.0f, "store_row's and store_partial's lift");
 
-// The same as one split's partial result: the output over its sum is at most
-// the largest code, and its rounding to fp16 an eighth of bf16's.
-template <int P>
+// The same as one split's partial result, the output over its sum (at most the
+// largest code): in fp16 for bf16 outputs, where its rounding is an eighth of
+// theirs, in fp32 for fp16 ones.
+template <typename T, int P>
 __device__ __forceinline__ void store_partial(const AttendParams& p, int bh, int split, int row,
                                               int d, float M, float L, float U,
                                               const float (&o)[8]) {
     if (row >= p.rows) return;
     const int64_t i = ((int64_t)bh * p.splits + split) * p.rows + row;
     const float f = L > 0.0f ? 1.0f / 4096.0f / L : 0.0f;
-    if (d < P)
-        *reinterpret_cast<u32x4*>(p.part + i * P + d) =
-            u32x4{Fp16::pack(o[0] * f, o[1] * f), Fp16::pack(o[2] * f, o[3] * f),
-                  Fp16::pack(o[4] * f, o[5] * f), Fp16::pack(o[6] * f, o[7] * f)};
+    if (d < P) {
+        typename T::Partial x;
+        x.set(o, f);
+        x.store(p.part, i * P + d);
+    }
     if (d == 0) p.part_ml[i] = f32x4{M, L, U, 0.0f};
 }
 
@@ -119,11 +120,9 @@ __global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
     using x8 = typename T::x8;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t item = blockIdx.x;
-    const int rg = (int)(item % p.groups);
-    const int64_t rest = item / p.groups;
-    const int split = (int)(rest % p.splits);
-    const int bh = (int)(rest / p.splits), b = bh / p.H, hk = bh % p.H;
+    const uint32_t item = blockIdx.x, rest = item / (uint32_t)p.groups;
+    const int rg = (int)(item - rest * p.groups), bh = (int)(rest / (uint32_t)p.splits);
+    const int split = (int)(rest - (uint32_t)bh * p.splits), b = bh / p.H, hk = bh - b * p.H;
     const int len = c8_length(p.length, b, p.n);
     const int row0 = rg * 16;
     const RowAt mine = row_at(row0 + r, hk, p.G, p.Q);
@@ -300,7 +299,7 @@ __global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
             for (int i = 0; i < 8; ++i) acc[i] += f * so[w][mr][d + i];
     }
     const int row = row0 + mr;
-    if (p.splits > 1) store_partial<P>(p, bh, split, row, d, M, L, U, acc);
+    if (p.splits > 1) store_partial<T, P>(p, bh, split, row, d, M, L, U, acc);
     else store_row<T>(p, b, hk, row, d, M, L, U, acc);
 }
 
@@ -393,13 +392,12 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // groups of one head and split run on one XCD in consecutive slots (block
     // i goes to XCD i % 8), so its L2 serves all but the first read of a block
-    const int64_t per = (p.items + 7) >> 3;
-    const int64_t item = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if (item >= p.items) return;
-    const int rg = (int)(item % p.groups);
-    const int64_t rest = item / p.groups;
-    const int64_t BH = (int64_t)p.B * p.H;
-    const int split = (int)(rest / BH), bh = (int)(rest % BH), b = bh / p.H, hk = bh % p.H;
+    const uint32_t items = (uint32_t)p.items, BH = (uint32_t)(p.B * p.H);
+    const uint32_t item = (blockIdx.x & 7) * ((items + 7) >> 3) + (blockIdx.x >> 3);
+    if (item >= items) return;
+    const uint32_t rest = item / (uint32_t)p.groups;
+    const int rg = (int)(item - rest * p.groups), split = (int)(rest / BH);
+    const int bh = (int)(rest - split * BH), b = bh / p.H, hk = bh - b * p.H;
     const int len = c8_length(p.length, b, p.n);
     const int row0 = rg * p.per_group * 32;
     const int rows_end = min(row0 + p.per_group * 32, p.rows);
@@ -470,30 +468,15 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
         const int next = slot == 2 ? 0 : slot + 1;
         const bool work = active && key0 < wlast;
         f32x16 s[2];
-        f16x8 vf[2][2 * DB];
-        auto lds_v = [&](int j) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int i = 0; i < DB; ++i)
-                    vf[j][k * DB + i] = *reinterpret_cast<const f16x8*>(smem + vofs[2 * j + k] + i * 4096);
-        };
         if (work) {
-            x8 kf[2][KS];
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int kk = 0; kk < KS; ++kk)
-                    kf[j][kk] = *reinterpret_cast<const x8*>(smem + kofs[kk] + j * 64 * P);
-            __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                s[j] = T::mfma32(kf[j][0], qf[0], f32x16{});
-#pragma unroll
-                for (int kk = 1; kk < KS; ++kk) s[j] = T::mfma32(kf[j][kk], qf[kk], s[j]);
-            }
+                    s[j] = T::mfma32(*reinterpret_cast<const x8*>(smem + kofs[kk] + j * 64 * P), qf[kk],
+                                     kk ? s[j] : f32x16{});
             __builtin_amdgcn_s_setprio(0);
-            lds_v(0);
         }
         const float c = p.scale_log2 * fmaxf(sk, SCALE_MIN);
         const float lsv = __builtin_amdgcn_logf(fmaxf(sv, SCALE_MIN));
@@ -544,7 +527,6 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
                     pw[j][i >> 1] = Fp16::pack(w0, w1);
                 }
             l = l * alpha + lsum * __builtin_amdgcn_exp2f(unit - lsv - LIFT);
-            lds_v(1);
             __builtin_amdgcn_s_setprio(1);
             if (__any(up)) {
 #pragma unroll
@@ -559,7 +541,9 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
                     const f16x8 pf = as_x8<f16x8>(
                         u32x4{pw[j][4 * k], pw[j][4 * k + 1], pw[j][4 * k + 2], pw[j][4 * k + 3]});
 #pragma unroll
-                    for (int i = 0; i < DB; ++i) o[i] = Fp16::mfma32(vf[j][k * DB + i], pf, o[i]);
+                    for (int i = 0; i < DB; ++i)
+                        o[i] = Fp16::mfma32(
+                            *reinterpret_cast<const f16x8*>(smem + vofs[2 * j + k] + i * 4096), pf, o[i]);
                 }
             __builtin_amdgcn_s_setprio(0);
         }
@@ -588,36 +572,34 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
             float x[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) x[k] = o[i][8 * e + k];
-            if (p.splits > 1) store_partial<P>(p, bh, split, row, d, m, l, unit, x);
+            if (p.splits > 1) store_partial<T, P>(p, bh, split, row, d, m, l, unit, x);
             else store_row<T>(p, b, hk, row, d, m, l, unit, x);
         }
 }
 
-// The merge of the splits' partial results: 16 threads a row and group of
+// The merge of the splits' partial results: P / 8 threads a row and group of
 // splits, eight columns each; out = sum a 2^unit o / sum a with a = 2^(m - M) l.
-// SG groups share a row's splits and are joined in LDS.
-template <typename T, int P, int SG>
+// SG groups share a row's splits and are joined in LDS; a thread has AHEAD
+// splits' loads in flight.
+template <typename T, int P, int SG, int AHEAD>
 __global__ void __launch_bounds__(256) merge_kernel(AttendParams p) {
-    constexpr int ROWS = 16 / SG;
-    const int64_t at = (int64_t)blockIdx.x * ROWS + threadIdx.x / (16 * SG);
-    const int sg = threadIdx.x / 16 % SG, d = (threadIdx.x % 16) * 8;
-    const int64_t bh = at / p.rows;
-    const bool in = bh < (int64_t)p.B * p.H;
-    const int row = in ? (int)(at % p.rows) : 0, b = (int)(bh / p.H), hk = (int)(bh % p.H);
-    const int64_t first = bh * p.splits * p.rows + row;
+    constexpr int PARTS = P / 8, ROWS = 256 / (PARTS * SG);
+    const int row = blockIdx.x * ROWS + threadIdx.x / (PARTS * SG);
+    const int sg = threadIdx.x / PARTS % SG, d = (threadIdx.x % PARTS) * 8;
+    const int b = blockIdx.z, hk = blockIdx.y;
+    const bool in = row < p.rows;
+    const int64_t first = ((int64_t)b * p.H + hk) * p.splits * p.rows + row;
     float M = -INFINITY, U = -INFINITY, L = 0.0f, acc[8] = {};
     if (in) {
-        // AHEAD splits' loads in flight, then folded into the running result
-        constexpr int AHEAD = 8;
         for (int s0 = sg; s0 < p.splits; s0 += SG * AHEAD) {
             f32x4 ml[AHEAD];
-            u32x4 x[AHEAD];
+            typename T::Partial x[AHEAD];
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
                 const int s = min(s0 + SG * j, p.splits - 1);
                 const int64_t i = first + (int64_t)s * p.rows;
                 ml[j] = p.part_ml[i];
-                x[j] = d < P ? *reinterpret_cast<const u32x4*>(p.part + i * P + d) : u32x4{};
+                x[j].load(p.part, i * P + d);
                 if (s0 + SG * j >= p.splits) ml[j][0] = ml[j][2] = -INFINITY;
             }
             float m1 = M, u1 = U;
@@ -641,15 +623,14 @@ __global__ void __launch_bounds__(256) merge_kernel(AttendParams p) {
                 L += a;
                 const float f = a == 0.0f ? 0.0f : a * __builtin_amdgcn_exp2f(ml[j][2] - U);
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    acc[k] += f * f16_bits_to_f32((uint16_t)(x[j][k >> 1] >> (16 * (k & 1))));
+                for (int k = 0; k < 8; ++k) acc[k] += f * x[j][k];
             }
         }
     }
     if constexpr (SG > 1) {
-        __shared__ float sh[ROWS][SG][16][8];
+        __shared__ float sh[ROWS][SG][PARTS][8];
         __shared__ float sml[ROWS][SG][3];
-        const int lr = threadIdx.x / (16 * SG), part = threadIdx.x % 16;
+        const int lr = threadIdx.x / (PARTS * SG), part = threadIdx.x % PARTS;
 #pragma unroll
         for (int k = 0; k < 8; ++k) sh[lr][sg][part][k] = acc[k];
         if (part == 0) {
@@ -989,6 +970,7 @@ int check_query(const nkv_cache8& c, int G, int dtype, int64_t Q, int64_t n, flo
         return bad(NKV_ERR_UNSUPPORTED, "too many query rows");
     if (dtype != NKV_ROWS_BF16 && dtype != NKV_ROWS_FP16)
         return bad(NKV_ERR_INVALID, "queries must be bf16 or fp16");
+    if (c.H > 65535 || c.B > 65535) return bad(NKV_ERR_UNSUPPORTED, "too many heads or items");
     if (n < 0 || n > c.cap) return bad(NKV_ERR_INVALID, "n must be in [0, cap]");
     if (!(scale > 0.0f) || !(scale < INFINITY))
         return bad(NKV_ERR_INVALID, "softmax_scale must be positive and finite");
@@ -1047,7 +1029,7 @@ Plan attend_plan(const nkv_cache8_attend_args* a) {
     if (pl.splits > 1) {
         const size_t rows = (size_t)heads * pl.splits * pl.rows;
         pl.ml = rows * sizeof(f32x4);
-        pl.part = rows * c8_pitch(c.D) * 2;
+        pl.part = rows * c8_pitch(c.D) * (a->dtype == NKV_ROWS_FP16 ? 4 : 2);
     }
     return pl;
 }
@@ -1079,9 +1061,14 @@ int attend_run(const AttendParams& p, bool tile, hipStream_t s) {
 
 template <typename T, int P>
 void merge_run(const AttendParams& p, hipStream_t s) {
-    const int64_t rows = (int64_t)p.B * p.H * p.rows;
-    if (p.splits > 8) merge_kernel<T, P, 16><<<(unsigned)rows, 256, 0, s>>>(p);
-    else merge_kernel<T, P, 1><<<(unsigned)cdiv(rows, 16), 256, 0, s>>>(p);
+    constexpr int PARTS = P / 8;
+    auto grid = [&](int sg) {
+        return dim3((unsigned)cdiv(p.rows, 256 / (PARTS * sg)), (unsigned)p.H, (unsigned)p.B);
+    };
+    if (p.splits > 8) merge_kernel<T, P, 16, 8><<<grid(16), 256, 0, s>>>(p);
+    else if (p.splits > 4) merge_kernel<T, P, 1, 8><<<grid(1), 256, 0, s>>>(p);
+    else if (p.splits > 2) merge_kernel<T, P, 1, 4><<<grid(1), 256, 0, s>>>(p);
+    else merge_kernel<T, P, 1, 2><<<grid(1), 256, 0, s>>>(p);
 }
 
 template <typename T, int FMT, int P>
@@ -1143,7 +1130,7 @@ extern "C" int nkv_cache8_attend(void* stream, const nkv_cache8_attend_args* a, 
     p.out = (uint16_t*)a->out;
     p.lse = a->lse;
     p.part_ml = (f32x4*)workspace;
-    p.part = (uint16_t*)((char*)workspace + pl.ml);
+    p.part = (char*)workspace + pl.ml;
     p.q_sb = a->q_sb, p.q_st = a->q_st, p.q_sh = a->q_sh;
     p.o_sb = a->o_sb, p.o_st = a->o_st, p.o_sh = a->o_sh;
     p.cap = c.cap;
