@@ -112,10 +112,24 @@ __device__ __forceinline__ void store_partial(const AttendParams& p, int bh, int
     if (d == 0) p.part_ml[i] = f32x4{M, L, U, 0.0f};
 }
 
-// Four waves of a workgroup share 16 query rows and a range of 64-row blocks;
-// wave w takes blocks w, w + 4, ... and the waves' results are merged in LDS.
-template <typename T, int FMT, int P>
-__global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
+// W waves of a workgroup share 16 query rows and a range of 64-row blocks; wave
+// w takes blocks w, w + W, ... and the waves' results are merged in LDS.  A
+// block costs a wave about 500 VALU instructions, most of them conversions of
+// codes, so few blocks want all CUs: four waves a workgroup, and eight only
+// where there is a block for each of eight waves on every CU (us with four and
+// eight, 8 key heads of 4 query heads: 1 x 8,192 rows 10.8, 13.6; 8 x 2,048
+// 12.5, 11.6; 32 x 1,024 16.7, 14.0; 32 x 4,096 45.3, 42.2).
+constexpr int64_t ROWS_EIGHT = 2048;  // blocks in all heads
+
+template <int P, int W>
+struct RowsSmem {
+    float o[W][16][P + 4];
+    float ml[W][16][2];
+    float unit[W];
+};
+
+template <typename T, int FMT, int P, int W>
+__global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
     constexpr int STEPS = P / 32, PIECES = P / 64, DB = P / 16;
     using x8 = typename T::x8;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
@@ -146,7 +160,7 @@ __global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
     // m: the row's maximum (log2 units), l: its sum of 2^(z - m) over this
     // lane's keys; o holds sum of 2^(z - m) * sv * code in units of 2^unit
     float m = -INFINITY, l = 0.0f, unit = -INFINITY;
-    for (int blk = b0 + wave; blk < b1; blk += 4) {
+    for (int blk = b0 + wave; blk < b1; blk += W) {
         const int64_t key0 = (int64_t)blk * C8_BLOCK;
         u32x4 kr[4][PIECES];
 #pragma unroll
@@ -263,40 +277,40 @@ __global__ void __launch_bounds__(256) attend_kernel(AttendParams p) {
         }
     }
     l = rows4_sum(l);
-    // merge of the four waves: o[i][e] is column DB (4 g + e) + i of row r
-    __shared__ float so[4][16][P + 4];
-    __shared__ float sml[4][16][2];
-    __shared__ float su[4];
+    // merge of the waves: o[i][e] is column DB (4 g + e) + i of row r
+    extern __shared__ __align__(16) unsigned char rows_smem[];
+    RowsSmem<P, W>& sm = *reinterpret_cast<RowsSmem<P, W>*>(rows_smem);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int i = 0; i < DB; i += 4)
-            *reinterpret_cast<f32x4*>(&so[wave][r][DB * (4 * g + e) + i]) =
+            *reinterpret_cast<f32x4*>(&sm.o[wave][r][DB * (4 * g + e) + i]) =
                 f32x4{o[i][e], o[i + 1][e], o[i + 2][e], o[i + 3][e]};
     if (g == 0) {
-        sml[wave][r][0] = m;
-        sml[wave][r][1] = l;
+        sm.ml[wave][r][0] = m;
+        sm.ml[wave][r][1] = l;
     }
-    if (lane == 0) su[wave] = unit;
+    if (lane == 0) sm.unit[wave] = unit;
     __syncthreads();
+    if (threadIdx.x >= 256) return;
     const int mr = threadIdx.x / 16, d = (threadIdx.x % 16) * 8;
     float M = -INFINITY, U = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        M = fmaxf(M, sml[w][mr][0]);
-        U = fmaxf(U, su[w]);
+    for (int w = 0; w < W; ++w) {
+        M = fmaxf(M, sm.ml[w][mr][0]);
+        U = fmaxf(U, sm.unit[w]);
     }
     float L = 0.0f, acc[8] = {};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const float mw = sml[w][mr][0];
+    for (int w = 0; w < W; ++w) {
+        const float mw = sm.ml[w][mr][0];
         if (mw == -INFINITY) continue;
         const float a = __builtin_amdgcn_exp2f(mw - M);
-        L += a * sml[w][mr][1];
-        const float f = a * __builtin_amdgcn_exp2f(su[w] - U);
+        L += a * sm.ml[w][mr][1];
+        const float f = a * __builtin_amdgcn_exp2f(sm.unit[w] - U);
         if (d < P)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] += f * so[w][mr][d + i];
+            for (int i = 0; i < 8; ++i) acc[i] += f * sm.o[w][mr][d + i];
     }
     const int row = row0 + mr;
     if (p.splits > 1) store_partial<T, P>(p, bh, split, row, d, M, L, U, acc);
@@ -982,7 +996,7 @@ int check_query(const nkv_cache8& c, int G, int dtype, int64_t Q, int64_t n, flo
 }
 
 struct Plan {
-    bool tile;
+    bool tile, eight;             // the tile kernel; eight waves a workgroup of the other
     int groups, splits, per_group;
     int64_t items, rows;
     size_t part, ml;              // bytes
@@ -1018,12 +1032,13 @@ Plan attend_plan(const nkv_cache8_attend_args* a) {
         }
         pl.items = base * pl.splits;
     } else {
-        // enough workgroups to fill the chip, each with at least four blocks
-        // of keys (one a wave)
+        // eight waves a CU in either width, and a block of keys for each
         pl.groups = (int)cdiv(pl.rows, 16);
         const int64_t base = heads * pl.groups;
-        if (base > 0 && base < 512)
-            pl.splits = (int)std::max<int64_t>(1, std::min(cdiv(512, base), blocks / 4));
+        pl.eight = base * blocks >= ROWS_EIGHT;
+        const int64_t slots = pl.eight ? 256 : 512, waves = pl.eight ? 8 : 4;
+        if (base > 0 && base < slots)
+            pl.splits = (int)std::max<int64_t>(1, std::min(cdiv(slots, base), blocks / waves));
         pl.items = base * pl.splits;
     }
     if (pl.splits > 1) {
@@ -1046,17 +1061,25 @@ int check_attend(const nkv_cache8_attend_args* a) {
     return NKV_OK;
 }
 
+template <typename T, int FMT, int P, int W>
+int attend_rows_run(const AttendParams& p, hipStream_t s) {
+    constexpr int SMEM = sizeof(RowsSmem<P, W>);
+    if (SMEM > 65536)
+        if (int rc = set_smem(attend_kernel<T, FMT, P, W>, SMEM)) return rc;
+    attend_kernel<T, FMT, P, W><<<(unsigned)p.items, 64 * W, SMEM, s>>>(p);
+    return NKV_OK;
+}
+
 template <typename T, int FMT, int P>
-int attend_run(const AttendParams& p, bool tile, hipStream_t s) {
-    if (tile) {
+int attend_run(const AttendParams& p, const Plan& pl, hipStream_t s) {
+    if (pl.tile) {
         constexpr int SMEM = TileCodes<T, FMT, P>::SMEM;
         if (int rc = set_smem(attend_tile_kernel<T, FMT, P>, SMEM)) return rc;
         attend_tile_kernel<T, FMT, P>
             <<<(unsigned)(8 * cdiv(p.items, 8)), 64 * TILE_WAVES, SMEM, s>>>(p);
-    } else {
-        attend_kernel<T, FMT, P><<<(unsigned)p.items, 256, 0, s>>>(p);
+        return NKV_OK;
     }
-    return NKV_OK;
+    return pl.eight ? attend_rows_run<T, FMT, P, 8>(p, s) : attend_rows_run<T, FMT, P, 4>(p, s);
 }
 
 template <typename T, int P>
@@ -1144,7 +1167,7 @@ extern "C" int nkv_cache8_attend(void* stream, const nkv_cache8_attend_args* a, 
     p.per_group = pl.per_group;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     dispatch(a->dtype, c.format, c.D, [&](auto t, auto f, auto w) {
-        rc = attend_run<decltype(t), decltype(f)::value, decltype(w)::value>(p, pl.tile, s);
+        rc = attend_run<decltype(t), decltype(f)::value, decltype(w)::value>(p, pl, s);
     });
     if (rc) return rc;
     NKV_LAUNCH_CHECK();
