@@ -757,7 +757,7 @@ int nkv_finish(void* stream, const nkv_finish_args* args);
  * scale.  Row n of head h of item b is k[((b*H + h)*cap + n)*P + d], d < D,
  * with P = 64 for D <= 64 and 128 above (columns D .. P hold zero), and its
  * scale k_scale[(b*H + h)*(cap/64) + n/64]; v likewise.  D % 8 == 0, D <= 128;
- * cap % 64 == 0, cap <= 2^30.  k and v are 16-byte aligned.
+ * cap % 64 == 0, cap <= 2^29; B * H <= 2^21.  k and v are 16-byte aligned.
  * The caller keeps each item's length.  Rows at or past it may hold anything:
  * no call lets them into a result.
  */

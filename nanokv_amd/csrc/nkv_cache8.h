@@ -203,6 +203,34 @@ __device__ __forceinline__ typename T::x8 codes_x8(uint32_t lo, uint32_t hi) {
         u32x4{T::pack(a[0], a[1]), T::pack(b[0], b[1]), T::pack(c[0], c[1]), T::pack(d[0], d[1])});
 }
 
+// Four columns of two rows' codes (one word each) as fp16 pairs (row a, row b) of
+// each column.  int8: a code + 128 in the low byte of the half 0x6400 is 1,152 +
+// code; two byte permutations and one packed subtraction, where converting and
+// packing one code at a time takes half as many instructions again.
+template <int FMT>
+__device__ __forceinline__ void column_pairs(uint32_t a, uint32_t b, uint32_t (&out)[4]) {
+    if constexpr (FMT == NKV_CACHE8_INT8) {
+        a ^= 0x80808080u;
+        b ^= 0x80808080u;
+        const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x05010400u);  // a0 b0 a1 b1
+        const uint32_t hi = __builtin_amdgcn_perm(b, a, 0x07030602u);  // a2 b2 a3 b3
+        const f16x2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const uint32_t x = __builtin_amdgcn_perm(0x64646464u, c < 2 ? lo : hi,
+                                                     c & 1 ? 0x04030402u : 0x04010400u);
+            out[c] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, x) - bias);
+        }
+    } else {
+        const f32x2 a0 = code_pair<FMT>(a, 0), a1 = code_pair<FMT>(a, 1);
+        const f32x2 b0 = code_pair<FMT>(b, 0), b1 = code_pair<FMT>(b, 1);
+        out[0] = Fp16::pack(a0[0], b0[0]);
+        out[1] = Fp16::pack(a0[1], b0[1]);
+        out[2] = Fp16::pack(a1[0], b1[0]);
+        out[3] = Fp16::pack(a1[1], b1[1]);
+    }
+}
+
 // Sequence length of batch item b: its own entry clamped to [0, n], or n.
 __device__ __forceinline__ int c8_length(const int32_t* length, int b, int n) {
     return length ? min(max(length[b], 0), n) : n;

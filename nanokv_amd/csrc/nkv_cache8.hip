@@ -21,9 +21,9 @@ int cache8_check(const nkv_cache8* c, const char* who) {
         return bad(NKV_ERR_UNSUPPORTED, "head width must be a multiple of 8, at most 128");
     if (c->format != NKV_CACHE8_INT8 && c->format != NKV_CACHE8_E4M3)
         return bad(NKV_ERR_INVALID, "unknown cache format");
-    if (c->cap < C8_BLOCK || c->cap % C8_BLOCK || c->cap > (1 << 30))
-        return bad(NKV_ERR_INVALID, "cap must be a positive multiple of 64, at most 2^30");
-    if ((int64_t)c->B * c->H > INT32_MAX / 4) return bad(NKV_ERR_UNSUPPORTED, "too many heads");
+    if (c->cap < C8_BLOCK || c->cap % C8_BLOCK || c->cap > (1 << 29))
+        return bad(NKV_ERR_INVALID, "cap must be a positive multiple of 64, at most 2^29");
+    if ((int64_t)c->B * c->H > 1 << 21) return bad(NKV_ERR_UNSUPPORTED, "too many heads");
     if (c->B == 0) return NKV_OK;
     if (!c->k || !c->v || !c->k_scale || !c->v_scale)
         return bad(NKV_ERR_INVALID, "cache codes and scales are required");

@@ -60,6 +60,31 @@ __device__ __forceinline__ RowAt row_at(int row, int hk, int G, int Q) {
     return {r / G, hk * G + r % G, there};
 }
 
+// The work of a workgroup: a group of query rows of a unit (head and key split).
+// Block i runs on XCD i % 8, and the groups of a unit take consecutive slots of
+// one XCD, whose L2 then serves all but the first read of its codes.  Units go
+// to the XCDs in turn, so that sequences of unlike lengths spread over them
+// (whole runs of sequences to an XCD: 150 us against 137 for 32 of them); with
+// fewer than UNITS units an XCD takes a run of (unit, group) pairs instead.
+constexpr int UNITS = 32;
+
+struct Item {
+    uint32_t unit;
+    int group;
+    bool there;
+};
+
+__device__ __forceinline__ Item item_of(const AttendParams& p) {
+    const uint32_t x = blockIdx.x & 7, k = blockIdx.x >> 3, groups = (uint32_t)p.groups;
+    const uint32_t items = (uint32_t)p.items, units = items / groups;
+    if (units >= UNITS) {
+        const uint32_t u = k / groups * 8 + x;
+        return {u, (int)(k % groups), u < units};
+    }
+    const uint32_t item = x * ((items + 7) >> 3) + k, u = item / groups;
+    return {u, (int)(item - u * groups), item < items && k < (items + 7) >> 3};
+}
+
 // Operand step s of a K or Q row covers d = 64 (s / 2) + 16 g + 8 (s % 2) .. + 8
 // in lane row group g (lane / 16): the same order on both sides, and one
 // 16-byte piece of codes gives two steps.
@@ -83,14 +108,14 @@ __device__ __forceinline__ void store_row(const AttendParams& p, int b, int hk, 
                                           float lift = 1.0f / 4096.0f) {
     const RowAt at = row_at(row, hk, p.G, p.Q);
     if (!at.there) return;
-    const float f = L > 0.0f ? lift / L * __builtin_amdgcn_exp2f(U) : 0.0f;
+    const float f = L == 0.0f ? 0.0f : lift / L * __builtin_amdgcn_exp2f(U);
     if (d < p.D)
         *reinterpret_cast<u32x4*>(p.out + b * p.o_sb + at.t * p.o_st + at.head * p.o_sh + d) =
             u32x4{T::pack(o[0] * f, o[1] * f), T::pack(o[2] * f, o[3] * f),
                   T::pack(o[4] * f, o[5] * f), T::pack(o[6] * f, o[7] * f)};
     if (d == 0 && p.lse)
         p.lse[((int64_t)b * p.H * p.G + at.head) * p.Q + at.t] =
-            L > 0.0f ? M * LN2 + logf(L) : -INFINITY;
+            L == 0.0f ? -INFINITY : M * LN2 + logf(L);  // (NaN for a NaN query)
 }
 static_assert(LIFT == 12.0f, "store_row's and store_partial's lift");
 
@@ -103,7 +128,7 @@ __device__ __forceinline__ void store_partial(const AttendParams& p, int bh, int
                                               const float (&o)[8]) {
     if (row >= p.rows) return;
     const int64_t i = ((int64_t)bh * p.splits + split) * p.rows + row;
-    const float f = L > 0.0f ? 1.0f / 4096.0f / L : 0.0f;
+    const float f = L == 0.0f ? 0.0f : 1.0f / 4096.0f / L;
     if (d < P) {
         typename T::Partial x;
         x.set(o, f);
@@ -121,45 +146,57 @@ __device__ __forceinline__ void store_partial(const AttendParams& p, int bh, int
 // 12.5, 11.6; 32 x 1,024 16.7, 14.0; 32 x 4,096 45.3, 42.2).
 constexpr int64_t ROWS_EIGHT = 2048;  // blocks in all heads
 
-template <int P, int W>
+template <int P, int W, int NQ>
 struct RowsSmem {
-    float o[W][16][P + 4];
-    float ml[W][16][2];
+    float o[W][16 * NQ][P + 4];
+    float ml[W][16 * NQ][2];
     float unit[W];
 };
 
-template <typename T, int FMT, int P, int W>
+// NQ groups of 16 query rows to a wave: with more than 16 rows two, for half the
+// reads and conversions of codes.
+template <typename T, int FMT, int P, int W, int NQ>
 __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
-    constexpr int STEPS = P / 32, PIECES = P / 64, DB = P / 16;
+    constexpr int STEPS = P / 32, PIECES = P / 64, DB = P / 16, ROWS = 16 * NQ;
     using x8 = typename T::x8;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t item = blockIdx.x, rest = item / (uint32_t)p.groups;
-    const int rg = (int)(item - rest * p.groups), bh = (int)(rest / (uint32_t)p.splits);
-    const int split = (int)(rest - (uint32_t)bh * p.splits), b = bh / p.H, hk = bh - b * p.H;
+    const Item it = item_of(p);
+    if (!it.there) return;
+    const int rg = it.group, bh = (int)(it.unit / (uint32_t)p.splits);
+    const int split = (int)(it.unit - (uint32_t)bh * p.splits), b = bh / p.H, hk = bh - b * p.H;
     const int len = c8_length(p.length, b, p.n);
-    const int row0 = rg * 16;
-    const RowAt mine = row_at(row0 + r, hk, p.G, p.Q);
-    const int end = !mine.there ? 0 : p.causal ? len - p.Q + 1 + mine.t : len;
+    const int row0 = rg * ROWS;
     // blocks that the group's last row sees
-    const int last_t = min(row0 + 15, p.G * p.Q - 1) / p.G;
+    const int last_t = min(row0 + ROWS - 1, p.rows - 1) / p.G;
     const int last = max(0, p.causal ? len - p.Q + 1 + last_t : len);
     const int first = p.causal ? len - p.Q + 1 + row0 / p.G : len;  // what its first row sees
     const int nb = (last + C8_BLOCK - 1) / C8_BLOCK;
     const int b0 = (int)((int64_t)split * nb / p.splits);
     const int b1 = (int)((int64_t)(split + 1) * nb / p.splits);
-    x8 qf[STEPS];
-    load_q<T, P>(qf, p.q + b * p.q_sb + mine.t * p.q_st + mine.head * p.q_sh, mine.there, g, p.D);
+    x8 qf[NQ][STEPS];
+    int end[NQ];                              // keys that the lane's row sees
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const RowAt mine = row_at(row0 + 16 * n + r, hk, p.G, p.Q);
+        end[n] = !mine.there ? 0 : p.causal ? len - p.Q + 1 + mine.t : len;
+        load_q<T, P>(qf[n], p.q + b * p.q_sb + mine.t * p.q_st + mine.head * p.q_sh, mine.there, g,
+                     p.D);
+    }
     const uint8_t* kbase = p.k + ((int64_t)bh * p.cap + r) * P + 16 * g;
     const uint8_t* vbase = p.v + ((int64_t)bh * p.cap + 4 * g) * P + DB * r;
     const float* ks = p.ks + (int64_t)bh * (p.cap / C8_BLOCK);
     const float* vs = p.vs + (int64_t)bh * (p.cap / C8_BLOCK);
-    f32x4 o[DB];
+    f32x4 o[NQ][DB];
 #pragma unroll
-    for (int i = 0; i < DB; ++i) o[i] = f32x4{};
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int i = 0; i < DB; ++i) o[n][i] = f32x4{};
     // m: the row's maximum (log2 units), l: its sum of 2^(z - m) over this
-    // lane's keys; o holds sum of 2^(z - m) * sv * code in units of 2^unit
-    float m = -INFINITY, l = 0.0f, unit = -INFINITY;
+    // lane's keys; o holds sum of 2^(z - m + LIFT) * sv * code in units of 2^unit
+    float m[NQ], l[NQ], unit = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) m[n] = -INFINITY, l[n] = 0.0f;
     for (int blk = b0 + wave; blk < b1; blk += W) {
         const int64_t key0 = (int64_t)blk * C8_BLOCK;
         u32x4 kr[4][PIECES];
@@ -168,8 +205,8 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
 #pragma unroll
             for (int i = 0; i < PIECES; ++i)
                 kr[t][i] = *reinterpret_cast<const u32x4*>(kbase + (key0 + 16 * t) * P + 64 * i);
-        // V: lane (r, g) holds columns DB r .. + DB of the keys that its
-        // probabilities are of: 32 c + 16 a + 4 g + j
+        // V: lane (r, g) holds columns DB r .. + DB of the keys that its weights
+        // are of: 32 c + 16 a + 4 g + j
         uint32_t vr[2][8][DB / 4];
 #pragma unroll
         for (int c = 0; c < 2; ++c)
@@ -185,26 +222,35 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
                 }
             }
         const float sk = fmaxf(ks[blk], SCALE_MIN), sv = fmaxf(vs[blk], SCALE_MIN);
-        f32x4 s[4];
+        f32x4 s[NQ][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            s[t] = f32x4{};
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) s[n][t] = f32x4{};
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
-                s[t] = T::mfma16(codes_x8<T, FMT>(kr[t][i][0], kr[t][i][1]), qf[2 * i], s[t]);
-                s[t] = T::mfma16(codes_x8<T, FMT>(kr[t][i][2], kr[t][i][3]), qf[2 * i + 1], s[t]);
+                const x8 a = codes_x8<T, FMT>(kr[t][i][0], kr[t][i][1]);
+                const x8 c = codes_x8<T, FMT>(kr[t][i][2], kr[t][i][3]);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    s[n][t] = T::mfma16(a, qf[n][2 * i], s[n][t]);
+                    s[n][t] = T::mfma16(c, qf[n][2 * i + 1], s[n][t]);
+                }
             }
         }
         if (key0 + C8_BLOCK > first) {
-            // scores of unseen keys; s[t][e] is of key 16 t + 4 g + e
-            const int seen = end - (int)key0;
+            // scores of unseen keys; s[n][t][e] is of key 16 t + 4 g + e
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+            for (int n = 0; n < NQ; ++n) {
+                const int seen = end[n] - (int)key0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (16 * t + 4 * g + e >= seen) s[t][e] = -INFINITY;
-            // rows at or past the length may hold NaN codes, which a zero
-            // probability does not remove
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (16 * t + 4 * g + e >= seen) s[n][t][e] = -INFINITY;
+            }
+            // rows at or past the length may hold NaN codes, which a zero weight
+            // does not remove
             const int valid = len - (int)key0;
             if (FMT == NKV_CACHE8_E4M3 && valid < C8_BLOCK) {
 #pragma unroll
@@ -220,101 +266,111 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
         if (lsv > unit) {
             const float f = __builtin_amdgcn_exp2f(unit - lsv);
 #pragma unroll
-            for (int i = 0; i < DB; ++i)
+            for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[i][e] *= f;
+                for (int i = 0; i < DB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[n][i][e] *= f;
             unit = lsv;
         }
-        float tm = s[0][0];
+        uint32_t pw[NQ][2][4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int n = 0; n < NQ; ++n) {
+            float tm = s[n][0][0];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) tm = fmaxf(tm, s[t][e]);
-        tm = rows4_max(tm) * c;
-        const bool up = tm > m + TAU;
-        const float mn = up ? tm : m;
-        const float alpha = up ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
-        m = mn;
-        const float off = (mn == -INFINITY ? 0.0f : mn) + (unit - lsv) - LIFT;
-        float lsum = 0.0f;
-        uint32_t pw[2][4];
+            for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            float w[4];
+                for (int e = 0; e < 4; ++e) tm = fmaxf(tm, s[n][t][e]);
+            tm = rows4_max(tm) * c;
+            const bool up = tm > m[n] + TAU;
+            const float mn = up ? tm : m[n];
+            const float alpha = up ? __builtin_amdgcn_exp2f(m[n] - mn) : 1.0f;
+            m[n] = mn;
+            const float off = (mn == -INFINITY ? 0.0f : mn) + (unit - lsv) - LIFT;
+            float lsum = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                w[e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, -off));
-                lsum += w[e];
-            }
-            pw[t >> 1][2 * (t & 1)] = Fp16::pack(w[0], w[1]);
-            pw[t >> 1][2 * (t & 1) + 1] = Fp16::pack(w[2], w[3]);
-        }
-        l = l * alpha + lsum * __builtin_amdgcn_exp2f(unit - lsv - LIFT);
-        if (__any(up)) {
+            for (int t = 0; t < 4; ++t) {
+                float w[4];
 #pragma unroll
-            for (int i = 0; i < DB; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[i][e] *= alpha;
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const f16x8 pf = as_x8<f16x8>(u32x4{pw[k][0], pw[k][1], pw[k][2], pw[k][3]});
-#pragma unroll
-            for (int w = 0; w < DB / 4; ++w)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    f32x2 a[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) a[j] = code_pair<FMT>(vr[k][j][w], h);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const f16x8 vf = as_x8<f16x8>(
-                            u32x4{Fp16::pack(a[0][e], a[1][e]), Fp16::pack(a[2][e], a[3][e]),
-                                  Fp16::pack(a[4][e], a[5][e]), Fp16::pack(a[6][e], a[7][e])});
-                        o[4 * w + 2 * h + e] = Fp16::mfma16(vf, pf, o[4 * w + 2 * h + e]);
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    w[e] = __builtin_amdgcn_exp2f(fmaf(s[n][t][e], c, -off));
+                    lsum += w[e];
                 }
+                pw[n][t >> 1][2 * (t & 1)] = Fp16::pack(w[0], w[1]);
+                pw[n][t >> 1][2 * (t & 1) + 1] = Fp16::pack(w[2], w[3]);
+            }
+            l[n] = l[n] * alpha + lsum * __builtin_amdgcn_exp2f(unit - lsv - LIFT);
+            if (__any(up)) {
+#pragma unroll
+                for (int i = 0; i < DB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[n][i][e] *= alpha;
+            }
         }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int w = 0; w < DB / 4; ++w) {
+                uint32_t pairs[4][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    column_pairs<FMT>(vr[k][2 * j][w], vr[k][2 * j + 1][w], pairs[j]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const f16x8 vf =
+                        as_x8<f16x8>(u32x4{pairs[0][e], pairs[1][e], pairs[2][e], pairs[3][e]});
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
+                        o[n][4 * w + e] = Fp16::mfma16(
+                            vf, as_x8<f16x8>(u32x4{pw[n][k][0], pw[n][k][1], pw[n][k][2], pw[n][k][3]}),
+                            o[n][4 * w + e]);
+                }
+            }
     }
-    l = rows4_sum(l);
-    // merge of the waves: o[i][e] is column DB (4 g + e) + i of row r
+    // merge of the waves: o[n][i][e] is column DB (4 g + e) + i of row 16 n + r
     extern __shared__ __align__(16) unsigned char rows_smem[];
-    RowsSmem<P, W>& sm = *reinterpret_cast<RowsSmem<P, W>*>(rows_smem);
+    RowsSmem<P, W, NQ>& sm = *reinterpret_cast<RowsSmem<P, W, NQ>*>(rows_smem);
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-        for (int i = 0; i < DB; i += 4)
-            *reinterpret_cast<f32x4*>(&sm.o[wave][r][DB * (4 * g + e) + i]) =
-                f32x4{o[i][e], o[i + 1][e], o[i + 2][e], o[i + 3][e]};
-    if (g == 0) {
-        sm.ml[wave][r][0] = m;
-        sm.ml[wave][r][1] = l;
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int i = 0; i < DB; i += 4)
+                *reinterpret_cast<f32x4*>(&sm.o[wave][16 * n + r][DB * (4 * g + e) + i]) =
+                    f32x4{o[n][i][e], o[n][i + 1][e], o[n][i + 2][e], o[n][i + 3][e]};
+        const float sum = rows4_sum(l[n]);
+        if (g == 0) {
+            sm.ml[wave][16 * n + r][0] = m[n];
+            sm.ml[wave][16 * n + r][1] = sum;
+        }
     }
     if (lane == 0) sm.unit[wave] = unit;
     __syncthreads();
-    if (threadIdx.x >= 256) return;
-    const int mr = threadIdx.x / 16, d = (threadIdx.x % 16) * 8;
-    float M = -INFINITY, U = -INFINITY;
+    if (threadIdx.x >= 16 * ROWS) return;
+    for (int mr = threadIdx.x / 16; mr < ROWS; mr += 4 * W) {
+        const int d = (threadIdx.x % 16) * 8;
+        float M = -INFINITY, U = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-        M = fmaxf(M, sm.ml[w][mr][0]);
-        U = fmaxf(U, sm.unit[w]);
+        for (int w = 0; w < W; ++w) {
+            M = fmaxf(M, sm.ml[w][mr][0]);
+            U = fmaxf(U, sm.unit[w]);
+        }
+        float L = 0.0f, acc[8] = {};
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            // (a wave that saw no key has zero sums, or with a NaN query NaN ones)
+            const float mw = sm.ml[w][mr][0], uw = sm.unit[w];
+            const float a = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - M);
+            L += a * sm.ml[w][mr][1];
+            const float f = uw == -INFINITY ? 0.0f : a * __builtin_amdgcn_exp2f(uw - U);
+            if (d < P)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[i] += f * sm.o[w][mr][d + i];
+        }
+        const int row = row0 + mr;
+        if (p.splits > 1) store_partial<T, P>(p, bh, split, row, d, M, L, U, acc);
+        else store_row<T>(p, b, hk, row, d, M, L, U, acc);
     }
-    float L = 0.0f, acc[8] = {};
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-        const float mw = sm.ml[w][mr][0];
-        if (mw == -INFINITY) continue;
-        const float a = __builtin_amdgcn_exp2f(mw - M);
-        L += a * sm.ml[w][mr][1];
-        const float f = a * __builtin_amdgcn_exp2f(sm.unit[w] - U);
-        if (d < P)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] += f * sm.o[w][mr][d + i];
-    }
-    const int row = row0 + mr;
-    if (p.splits > 1) store_partial<T, P>(p, bh, split, row, d, M, L, U, acc);
-    else store_row<T>(p, b, hk, row, d, M, L, U, acc);
 }
 
 // ---------------------------------------------------------------- many rows
@@ -381,17 +437,13 @@ struct TileCodes {
                     if (4 * kq + i >= valid) v[i] = 0;
             const int R0 = 4 * ((dq & ~3) | ((dq & 1) << 1) | ((dq >> 1) & 1));
             const int q = kq & 7, chunk = 4 * (kq >> 3) + 2 * (q >> 2) + (q & 1), half = (q >> 1) & 1;
-            f32x2 a[4][2];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) a[i][h] = code_pair<FMT>(v[i], h);
+            uint32_t lo[4], hi[4];
+            column_pairs<FMT>(v[0], v[1], lo);
+            column_pairs<FMT>(v[2], v[3], hi);
 #pragma unroll
             for (int c = 0; c < 4; ++c)
                 *reinterpret_cast<u32x2*>(vd + (R0 + c) * 128 + 16 * (chunk ^ vsw(R0 + c)) +
-                                          8 * half) =
-                    u32x2{Fp16::pack(a[0][c >> 1][c & 1], a[1][c >> 1][c & 1]),
-                          Fp16::pack(a[2][c >> 1][c & 1], a[3][c >> 1][c & 1])};
+                                          8 * half) = u32x2{lo[c], hi[c]};
         }
     }
 };
@@ -404,14 +456,11 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
     extern __shared__ __align__(16) unsigned char smem[];  // TileCodes::SMEM
     const int lane = threadIdx.x & 63, hf = lane >> 5, l32 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // groups of one head and split run on one XCD in consecutive slots (block
-    // i goes to XCD i % 8), so its L2 serves all but the first read of a block
-    const uint32_t items = (uint32_t)p.items, BH = (uint32_t)(p.B * p.H);
-    const uint32_t item = (blockIdx.x & 7) * ((items + 7) >> 3) + (blockIdx.x >> 3);
-    if (item >= items) return;
-    const uint32_t rest = item / (uint32_t)p.groups;
-    const int rg = (int)(item - rest * p.groups), split = (int)(rest / BH);
-    const int bh = (int)(rest - split * BH), b = bh / p.H, hk = bh - b * p.H;
+    const Item it = item_of(p);
+    if (!it.there) return;
+    const uint32_t BH = (uint32_t)(p.B * p.H);
+    const int rg = it.group, split = (int)(it.unit / BH);
+    const int bh = (int)(it.unit - split * BH), b = bh / p.H, hk = bh - b * p.H;
     const int len = c8_length(p.length, b, p.n);
     const int row0 = rg * p.per_group * 32;
     const int rows_end = min(row0 + p.per_group * 32, p.rows);
@@ -614,7 +663,7 @@ __global__ void __launch_bounds__(256) merge_kernel(AttendParams p) {
                 const int64_t i = first + (int64_t)s * p.rows;
                 ml[j] = p.part_ml[i];
                 x[j].load(p.part, i * P + d);
-                if (s0 + SG * j >= p.splits) ml[j][0] = ml[j][2] = -INFINITY;
+                if (s0 + SG * j >= p.splits) ml[j] = f32x4{-INFINITY, 0.0f, -INFINITY, 0.0f};
             }
             float m1 = M, u1 = U;
 #pragma unroll
@@ -622,9 +671,8 @@ __global__ void __launch_bounds__(256) merge_kernel(AttendParams p) {
                 m1 = fmaxf(m1, ml[j][0]);
                 u1 = fmaxf(u1, ml[j][2]);
             }
-            if (m1 == -INFINITY) continue;
             const float b0 = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - m1);
-            const float c0 = M == -INFINITY ? 0.0f : b0 * __builtin_amdgcn_exp2f(U - u1);
+            const float c0 = U == -INFINITY ? 0.0f : b0 * __builtin_amdgcn_exp2f(U - u1);
             L *= b0;
 #pragma unroll
             for (int k = 0; k < 8; ++k) acc[k] *= c0;
@@ -633,9 +681,9 @@ __global__ void __launch_bounds__(256) merge_kernel(AttendParams p) {
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
                 const float a =
-                    ml[j][0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[j][0] - M) * ml[j][1];
+                    (ml[j][0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[j][0] - M)) * ml[j][1];
                 L += a;
-                const float f = a == 0.0f ? 0.0f : a * __builtin_amdgcn_exp2f(ml[j][2] - U);
+                const float f = ml[j][2] == -INFINITY ? 0.0f : a * __builtin_amdgcn_exp2f(ml[j][2] - U);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) acc[k] += f * x[j][k];
             }
@@ -664,11 +712,10 @@ __global__ void __launch_bounds__(256) merge_kernel(AttendParams p) {
         for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
 #pragma unroll
         for (int s = 0; s < SG; ++s) {
-            const float ms = sml[lr][s][0];
-            if (ms == -INFINITY) continue;
-            const float a = __builtin_amdgcn_exp2f(ms - M);
+            const float ms = sml[lr][s][0], us = sml[lr][s][2];
+            const float a = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - M);
             L += a * sml[lr][s][1];
-            const float f = a * __builtin_amdgcn_exp2f(sml[lr][s][2] - U);
+            const float f = us == -INFINITY ? 0.0f : a * __builtin_amdgcn_exp2f(us - U);
 #pragma unroll
             for (int k = 0; k < 8; ++k) acc[k] += f * sh[lr][s][part][k];
         }
@@ -996,14 +1043,20 @@ int check_query(const nkv_cache8& c, int G, int dtype, int64_t Q, int64_t n, flo
 }
 
 struct Plan {
-    bool tile, eight;             // the tile kernel; eight waves a workgroup of the other
+    bool tile, eight, two;        // the tile kernel; of the other, eight waves, two groups of rows
     int groups, splits, per_group;
     int64_t items, rows;
     size_t part, ml;              // bytes
 };
 
-// From this many rows of a key head on, the tile kernel.
+// Up to this many rows of a key head, the kernel of 16-row groups; above it the
+// tile kernel (us with either: 24 x 8 heads of 1,024 rows 27.8, 30.5 at 64 query
+// rows and 40.2, 32.3 at 96; 8 heads of 4,096 rows 12.9, 18.0 and 18.5, 18.9).
 constexpr int64_t TILE_ROWS = 64;
+// Two groups to a wave from this many (group, block) pairs on (us with one and
+// two: 1,024 pairs 11.5, 13.2; 2,048 12.9, 14.7; 8,192 24.0, 21.1; 12,288 30.7,
+// 27.8).
+constexpr int64_t ROWS_TWO = 4096;
 
 Plan attend_plan(const nkv_cache8_attend_args* a) {
     const nkv_cache8& c = a->cache;
@@ -1011,7 +1064,7 @@ Plan attend_plan(const nkv_cache8_attend_args* a) {
     pl.rows = a->Q * a->G;
     const int64_t heads = (int64_t)c.B * c.H, blocks = cdiv(a->n, C8_BLOCK);
     pl.splits = 1;
-    pl.tile = pl.rows >= TILE_ROWS;
+    pl.tile = pl.rows > TILE_ROWS;
     if (pl.tile) {
         // the fewest groups of up to eight 32-row blocks, of even size
         const int64_t qb = cdiv(pl.rows, 32);
@@ -1022,7 +1075,8 @@ Plan attend_plan(const nkv_cache8_attend_args* a) {
         // block's time; a workgroup's start and end cost some blocks, and a
         // merge its partials' traffic
         double best = 0.0;
-        for (int64_t s = 1; s <= 16 && (s == 1 || blocks >= 4 * s); ++s) {
+        const int64_t most = std::max<int64_t>(16, cdiv(256, std::max<int64_t>(base, 1)));
+        for (int64_t s = 1; s <= most && (s == 1 || blocks >= 4 * s); ++s) {
             const double merge = s == 1 ? 0.0 : 4.0 + (double)heads * pl.rows * s * 2e-4;
             const double t = (double)cdiv(base * s, 256) * ((double)blocks / s + 6.0) + merge;
             if (s == 1 || t < best) {
@@ -1032,11 +1086,15 @@ Plan attend_plan(const nkv_cache8_attend_args* a) {
         }
         pl.items = base * pl.splits;
     } else {
-        // eight waves a CU in either width, and a block of keys for each
-        pl.groups = (int)cdiv(pl.rows, 16);
+        // eight waves a CU in either width, and a block of keys for each; twice
+        // the workgroups where sequences have lengths of their own, so that CUs
+        // with short ones take more (32 ragged sequences up to 16,384: 151 us
+        // with 256 workgroups, 137 with 512)
+        pl.two = pl.rows > 16 && heads * cdiv(pl.rows, 16) * blocks >= ROWS_TWO;
+        pl.groups = (int)cdiv(pl.rows, pl.two ? 32 : 16);
         const int64_t base = heads * pl.groups;
         pl.eight = base * blocks >= ROWS_EIGHT;
-        const int64_t slots = pl.eight ? 256 : 512, waves = pl.eight ? 8 : 4;
+        const int64_t slots = pl.eight && !a->length ? 256 : 512, waves = pl.eight ? 8 : 4;
         if (base > 0 && base < slots)
             pl.splits = (int)std::max<int64_t>(1, std::min(cdiv(slots, base), blocks / waves));
         pl.items = base * pl.splits;
@@ -1057,16 +1115,23 @@ int check_attend(const nkv_cache8_attend_args* a) {
     NKV_REQUIRE(a->out, NKV_ERR_INVALID, "out is required");
     NKV_REQUIRE(reinterpret_cast<uintptr_t>(a->out) % 16 == 0 && (a->o_sb | a->o_st | a->o_sh) % 8 == 0,
                 NKV_ERR_INVALID, "out must be 16-byte aligned with strides divisible by 8");
-    NKV_REQUIRE(attend_plan(a).items <= INT32_MAX - 8, NKV_ERR_UNSUPPORTED, "too many query rows");
+    // a launch has fewer than 2^32 threads
+    NKV_REQUIRE(attend_plan(a).items <= 1 << 22, NKV_ERR_UNSUPPORTED, "too many query rows");
     return NKV_OK;
 }
 
-template <typename T, int FMT, int P, int W>
+// Blocks of a launch over p.items workgroups in item_of's order.
+unsigned item_blocks(const AttendParams& p) {
+    const int64_t units = p.items / p.groups;
+    return (unsigned)(units >= UNITS ? 8 * cdiv(units, 8) * p.groups : 8 * cdiv(p.items, 8));
+}
+
+template <typename T, int FMT, int P, int W, int NQ>
 int attend_rows_run(const AttendParams& p, hipStream_t s) {
-    constexpr int SMEM = sizeof(RowsSmem<P, W>);
+    constexpr int SMEM = sizeof(RowsSmem<P, W, NQ>);
     if (SMEM > 65536)
-        if (int rc = set_smem(attend_kernel<T, FMT, P, W>, SMEM)) return rc;
-    attend_kernel<T, FMT, P, W><<<(unsigned)p.items, 64 * W, SMEM, s>>>(p);
+        if (int rc = set_smem(attend_kernel<T, FMT, P, W, NQ>, SMEM)) return rc;
+    attend_kernel<T, FMT, P, W, NQ><<<item_blocks(p), 64 * W, SMEM, s>>>(p);
     return NKV_OK;
 }
 
@@ -1076,10 +1141,12 @@ int attend_run(const AttendParams& p, const Plan& pl, hipStream_t s) {
         constexpr int SMEM = TileCodes<T, FMT, P>::SMEM;
         if (int rc = set_smem(attend_tile_kernel<T, FMT, P>, SMEM)) return rc;
         attend_tile_kernel<T, FMT, P>
-            <<<(unsigned)(8 * cdiv(p.items, 8)), 64 * TILE_WAVES, SMEM, s>>>(p);
+            <<<item_blocks(p), 64 * TILE_WAVES, SMEM, s>>>(p);
         return NKV_OK;
     }
-    return pl.eight ? attend_rows_run<T, FMT, P, 8>(p, s) : attend_rows_run<T, FMT, P, 4>(p, s);
+    if (pl.two)
+        return pl.eight ? attend_rows_run<T, FMT, P, 8, 2>(p, s) : attend_rows_run<T, FMT, P, 4, 2>(p, s);
+    return pl.eight ? attend_rows_run<T, FMT, P, 8, 1>(p, s) : attend_rows_run<T, FMT, P, 4, 1>(p, s);
 }
 
 template <typename T, int P>

@@ -67,7 +67,7 @@ BAD_CACHES = [
     (dict(fmt=2), _lib.NKV_ERR_INVALID, b"format"),
     (dict(cap=0), _lib.NKV_ERR_INVALID, b"multiple of 64"),
     (dict(cap=100), _lib.NKV_ERR_INVALID, b"multiple of 64"),
-    (dict(cap=1 << 31), _lib.NKV_ERR_INVALID, b"at most 2^30"),
+    (dict(cap=1 << 31), _lib.NKV_ERR_INVALID, b"at most 2^29"),
     (dict(at=PTR + 8), _lib.NKV_ERR_INVALID, b"aligned"),
     (dict(B=1 << 16, H=1 << 16), _lib.NKV_ERR_UNSUPPORTED, b"too many heads"),
 ]

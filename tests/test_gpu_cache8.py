@@ -174,7 +174,8 @@ def test_attend(dev, fmt, dtype, H, G, D, Q, lengths, causal):
 
 
 @pytest.mark.parametrize("H,G,Q,N", [(1, 1, 1, 20000), (1, 16, 1, 8191), (2, 2, 3, 5000),
-                                     (1, 1, 40, 4097), (1, 2, 90, 9001)])
+                                     (1, 1, 40, 4097), (1, 2, 90, 9001),
+                                     (8, 1, 33, 16500), (2, 4, 16, 65537)])
 def test_attend_long(dev, H, G, Q, N):
     """Key splits and their merge."""
     cache = make_cache(dev, 1, H, N, 128, "int8", 10, [N])
@@ -383,3 +384,145 @@ def test_streams_and_graph(dev):
         assert torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1])
         step(*warm, *new[i])                   # eager work between replays
     assert torch.equal(s3[2], state[2]) and torch.equal(s3[0].v, state[0].v)
+
+
+# ---------------------------------------------------------------- what callers may do
+@pytest.mark.parametrize("Q,G", [(1, 2), (20, 2), (100, 2)])
+def test_attend_lengths_outside_the_bound(dev, Q, G):
+    """Lengths below zero are none, above max_length the bound."""
+    cache = make_cache(dev, 3, 2, 192, 64, "e4m3", 50, [100, 100, 100])
+    q = torch.randn((3, Q, 2 * G, 64), generator=torch.Generator().manual_seed(51)).bfloat16().to(dev)
+    n = torch.tensor([-5, 10_000, 70], dtype=torch.int32, device=dev)
+    out, lse = ops.cache8_attend(q, cache, n, max_length=100)
+    gl = check_attend(q, cache, "e4m3", [0, 100, 70], False, out, lse)
+    assert np.isneginf(gl[0]).all()
+    m = torch.zeros((3, 2, cache.cap), device=dev)
+    ops.cache8_mass(q, cache, lse, m, n, max_length=100)
+    assert (m[0] == 0).all() and (m[:, :, 100:] == 0).all() and (m[2, :, 70:] == 0).all()
+    # every query gives a weight of one: the sums of fp32 sums, a few steps off
+    want = torch.tensor([0.0, Q * G, Q * G], device=dev)[:, None].expand(3, 2)
+    assert ((m.sum(2) - want).abs() <= 1e-4 * Q * G).all()
+
+
+@pytest.mark.parametrize("Q", [1, 40, 200])
+def test_attend_a_nan_query_spoils_its_own_row_alone(dev, Q):
+    cache = make_cache(dev, 1, 2, 700, 128, "int8", 52, [700])
+    q = torch.randn((1, Q, 4, 128), generator=torch.Generator().manual_seed(53)).bfloat16().to(dev)
+    clean, lse = ops.cache8_attend(q, cache, 700)
+    bad = q.clone()
+    bad[0, Q // 2, 1, 5] = float("nan")
+    out, l2 = ops.cache8_attend(bad, cache, 700)
+    assert torch.isnan(out[0, Q // 2, 1]).all() and torch.isnan(l2[0, 1, Q // 2])
+    keep = torch.ones((Q, 4), dtype=torch.bool, device=dev)
+    keep[Q // 2, 1] = False
+    assert torch.equal(out[0][keep], clean[0][keep])
+    assert torch.equal(l2[0].T[keep], lse[0].T[keep])
+
+
+@pytest.mark.parametrize("Q", [1, 50, 130])
+def test_attend_into_the_queries_and_in_a_given_workspace(dev, Q):
+    cache = make_cache(dev, 1, 1, 9000, 128, "int8", 54, [9000])
+    q = torch.randn((1, Q, 3, 128), generator=torch.Generator().manual_seed(55)).bfloat16().to(dev)
+    want, lse = ops.cache8_attend(q, cache, 9000)
+    same = q.clone()
+    work = torch.full((1 << 24,), 0xFF, dtype=torch.uint8, device=dev)
+    got, l2 = ops.cache8_attend(same, cache, 9000, out=same, workspace=work)
+    assert got is same and torch.equal(got, want) and torch.equal(l2, lse)
+    small = torch.empty(16, dtype=torch.uint8, device=dev)
+    with pytest.raises(RuntimeError, match="workspace"):
+        ops.cache8_attend(q, cache, 9000, workspace=small)
+
+
+def test_mass_row_splits_and_their_join(dev):
+    """Few blocks of keys and many rows, a hostile workspace, another output."""
+    cache = make_cache(dev, 2, 1, 200, 64, "e4m3", 56, [200, 77])
+    q = torch.randn((2, 600, 3, 64), generator=torch.Generator().manual_seed(57)).half().to(dev)
+    n = torch.tensor([200, 77], dtype=torch.int32, device=dev)
+    _, lse = ops.cache8_attend(q, cache, n, causal=True)
+    m0 = torch.rand((2, 1, cache.cap), generator=torch.Generator().manual_seed(58))
+    k, _ = cache_values(cache, "e4m3")
+    rm, tol = ref.mass(q.double().cpu().numpy(), k, lse.double().cpu().numpy(), m0.numpy(),
+                       [200, 77], True, 0.125)
+    work = torch.full((1 << 20,), 0xFF, dtype=torch.uint8, device=dev)
+    m, out = m0.to(dev), torch.full((2, 1, cache.cap), float("nan"), device=dev)
+    ops.cache8_mass(q, cache, lse, m, n, out=out, causal=True, workspace=work)
+    assert torch.equal(m.cpu(), m0)
+    assert (np.abs(out.double().cpu().numpy() - rm) <= tol).all()
+    ops.cache8_mass(q, cache, lse, m, n, causal=True)
+    assert torch.equal(m, out)
+
+
+def test_evict_long_heads(dev):
+    """Heads whose keys do not fit the selection's LDS, equal masses among them."""
+    n, keep, H = 40_000, 9_001, 3
+    cache = make_cache(dev, 1, H, n, 8, "int8", 59, [n])
+    m = torch.rand((1, H, cache.cap), generator=torch.Generator().manual_seed(60))
+    m[0, 1] = 0.25
+    m[0, 2] = (m[0, 2] * 50).floor()
+    out = ops.Cache8.empty(1, H, keep, 8, dev, "int8")
+    out_m = torch.zeros((1, H, out.cap), device=dev)
+    old = raw(out.k).copy(), out.k_scale.cpu().numpy()
+    rows, left = ops.cache8_evict(cache, m.to(dev), n, out, out_m, keep=keep, sink=7, recent=100)
+    want = ref.evict(m.numpy(), [n], keep, 7, 100)
+    assert left.tolist() == [keep] and rows[0].tolist() == want[0]
+    rc, rs = ref.compact(raw(cache.k), cache.k_scale.cpu().numpy(), want, *old, "int8")
+    assert np.array_equal(out.k_scale.cpu().numpy(), rs) and np.array_equal(raw(out.k), rc)
+
+
+def test_calls_of_every_kernel_captured_and_replayed(dev):
+    """Many rows, few rows over many blocks, the weight of many rows with a join
+    and an eviction in one graph, replayed with new inputs and eager calls
+    between, equal the eager calls."""
+    B, H, G, D, N = 2, 4, 2, 128, 16_000
+    g = torch.Generator().manual_seed(61)
+    cache = make_cache(dev, B, H, N, D, "int8", 62, [N, N])
+    small = ops.Cache8.empty(B, H, 512, D, dev, "int8")
+    q = torch.zeros((B, 150, H * G, D), dtype=torch.bfloat16, device=dev)
+    kv = torch.zeros((2, B, 70, H, D), dtype=torch.bfloat16, device=dev)
+    start = torch.tensor([130, 7], dtype=torch.int32, device=dev)
+    n = torch.tensor([N, 901], dtype=torch.int32, device=dev)
+
+    def calls(small):
+        ops.cache8_write(small, kv[0], kv[1], start)
+        a, la = ops.cache8_attend(q, cache, n)
+        b, lb = ops.cache8_attend(q[:, :1].contiguous(), cache, n)
+        c, lc = ops.cache8_attend(q[:, :9].contiguous(), cache, n, causal=True)
+        m = torch.zeros((B, H, cache.cap), device=dev)
+        ops.cache8_mass(q, cache, la, m, n)
+        ops.cache8_mass(q, small, torch.zeros_like(la), m[:, :, :512].contiguous(), 200)
+        out = ops.Cache8.empty(B, H, 300, D, dev, "int8")
+        om = torch.zeros((B, H, out.cap), device=dev)
+        rows, left = ops.cache8_evict(cache, m, n, out, om, keep=300, sink=3, recent=20)
+        return [a, la, b, lb, c, lc, m, rows, left, out.k, out.v, out.k_scale, om, small.k,
+                small.v_scale]
+
+    def fill(i):
+        gi = torch.Generator().manual_seed(70 + i)
+        q.copy_(torch.randn(q.shape, generator=gi))
+        kv.copy_(torch.randn(kv.shape, generator=gi))
+
+    def fresh():
+        return ops.Cache8.empty(B, H, 512, D, dev, "int8")
+
+    fill(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        calls(fresh())
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = calls(small)
+    for i in range(4):
+        fill(i)
+        for t in (small.k, small.v):
+            t.zero_()
+        for t in (small.k_scale, small.v_scale):
+            t.fill_(1.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = calls(fresh())                  # eager work between replays
+        torch.cuda.synchronize()
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
