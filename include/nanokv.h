@@ -838,8 +838,9 @@ typedef struct nkv_cache8_attend_args {
     int causal;
 } nkv_cache8_attend_args;
 
-/* Bytes of workspace nkv_cache8_attend needs for these arguments (0 if none);
- * a smaller one fails with NKV_ERR_WORKSPACE and launches nothing. */
+/* Bytes of workspace nkv_cache8_attend wants for these arguments (0 if none), for
+ * the partial results of its key splits; 16-byte aligned.  In a smaller one, or
+ * none, it takes fewer splits (the same attention within rounding). */
 size_t nkv_cache8_attend_workspace_size(const nkv_cache8_attend_args* args);
 int nkv_cache8_attend(void* stream, const nkv_cache8_attend_args* args, void* workspace,
                       size_t workspace_bytes);
@@ -869,6 +870,7 @@ typedef struct nkv_cache8_mass_args {
     int causal;
 } nkv_cache8_mass_args;
 
+/* Likewise for the partial sums of row splits (the same sums within rounding). */
 size_t nkv_cache8_mass_workspace_size(const nkv_cache8_mass_args* args);
 int nkv_cache8_mass(void* stream, const nkv_cache8_mass_args* args, void* workspace,
                     size_t workspace_bytes);
@@ -902,6 +904,7 @@ typedef struct nkv_cache8_evict_args {
     int64_t recent;
 } nkv_cache8_evict_args;
 
+/* 0: no scratch is used now; callers ask all the same. */
 size_t nkv_cache8_evict_workspace_size(const nkv_cache8_evict_args* args);
 int nkv_cache8_evict(void* stream, const nkv_cache8_evict_args* args, void* workspace,
                      size_t workspace_bytes);

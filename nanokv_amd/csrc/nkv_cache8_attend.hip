@@ -1058,7 +1058,8 @@ constexpr int64_t TILE_ROWS = 64;
 // 27.8).
 constexpr int64_t ROWS_TWO = 4096;
 
-Plan attend_plan(const nkv_cache8_attend_args* a) {
+// limit: bytes of workspace; fewer splits where those wanted do not fit.
+Plan attend_plan(const nkv_cache8_attend_args* a, size_t limit = SIZE_MAX) {
     const nkv_cache8& c = a->cache;
     Plan pl{};
     pl.rows = a->Q * a->G;
@@ -1099,10 +1100,17 @@ Plan attend_plan(const nkv_cache8_attend_args* a) {
             pl.splits = (int)std::max<int64_t>(1, std::min(cdiv(slots, base), blocks / waves));
         pl.items = base * pl.splits;
     }
+    const size_t row = sizeof(f32x4) + c8_pitch(c.D) * (a->dtype == NKV_ROWS_FP16 ? 4 : 2);
+    const size_t split = (size_t)heads * pl.rows * row;
+    if (pl.splits > 1 && limit / split < (size_t)pl.splits) {
+        pl.items /= pl.splits;
+        pl.splits = (int)std::max<size_t>(1, limit / split);
+        pl.items *= pl.splits;
+    }
     if (pl.splits > 1) {
         const size_t rows = (size_t)heads * pl.splits * pl.rows;
         pl.ml = rows * sizeof(f32x4);
-        pl.part = rows * c8_pitch(c.D) * (a->dtype == NKV_ROWS_FP16 ? 4 : 2);
+        pl.part = rows * (row - sizeof(f32x4));
     }
     return pl;
 }
@@ -1205,9 +1213,7 @@ extern "C" int nkv_cache8_attend(void* stream, const nkv_cache8_attend_args* a, 
     int rc = check_attend(a);
     if (rc || a->cache.B == 0 || a->Q == 0) return rc;
     const nkv_cache8& c = a->cache;
-    const Plan pl = attend_plan(a);
-    NKV_REQUIRE(pl.part == 0 || (workspace && workspace_bytes >= pl.part + pl.ml),
-                NKV_ERR_WORKSPACE, "workspace missing or too small");
+    const Plan pl = attend_plan(a, workspace ? workspace_bytes : 0);
     NKV_REQUIRE(pl.part == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, NKV_ERR_INVALID,
                 "workspace must be 16-byte aligned");
     AttendParams p{};
@@ -1276,7 +1282,7 @@ struct MassPlan {
 // Row splits: only where the blocks of keys fill less than two workgroups a CU,
 // each with at least four steps (1,176 workgroups of 25 steps took 176 us
 // whole, 190 in three splits).
-MassPlan mass_plan(const nkv_cache8_mass_args* a) {
+MassPlan mass_plan(const nkv_cache8_mass_args* a, size_t limit = SIZE_MAX) {
     MassPlan pl{};
     const int64_t rows = a->Q * a->G, heads = (int64_t)a->cache.B * a->cache.H;
     pl.n64 = cdiv(a->n, C8_BLOCK) * C8_BLOCK;
@@ -1285,7 +1291,10 @@ MassPlan mass_plan(const nkv_cache8_mass_args* a) {
     const int64_t base = heads * cdiv(pl.n64, 4 * C8_BLOCK), steps = cdiv(rows, MT_ROWS);
     if (pl.tile && base > 0 && base < 512)
         pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(512, base), steps / 4, 64}));
-    if (pl.splits > 1) pl.bytes = (size_t)pl.splits * heads * pl.n64 * sizeof(float);
+    const size_t split = (size_t)heads * pl.n64 * sizeof(float);
+    if (pl.splits > 1 && limit / split < (size_t)pl.splits)
+        pl.splits = (int)std::max<size_t>(1, limit / split);
+    if (pl.splits > 1) pl.bytes = pl.splits * split;
     return pl;
 }
 }  // namespace
@@ -1303,9 +1312,7 @@ extern "C" int nkv_cache8_mass(void* stream, const nkv_cache8_mass_args* a, void
     int rc = check_mass(a);
     if (rc || a->cache.B == 0) return rc;
     const nkv_cache8& c = a->cache;
-    const MassPlan pl = mass_plan(a);
-    NKV_REQUIRE(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes), NKV_ERR_WORKSPACE,
-                "workspace missing or too small");
+    const MassPlan pl = mass_plan(a, workspace ? workspace_bytes : 0);
     NKV_REQUIRE(pl.bytes == 0 || reinterpret_cast<uintptr_t>(workspace) % 4 == 0, NKV_ERR_INVALID,
                 "workspace must be 4-byte aligned");
     MassParams p{};

@@ -1544,7 +1544,8 @@ def cache8_attend(q: torch.Tensor, cache: Cache8, length, *, max_length: Optiona
     divided.  causal: the queries are the last Q tokens, query t sees the first
     length - Q + 1 + t rows.  Returns (out like q, lse [B, heads, Q] fp32 or
     None); a query that sees nothing gets 0 and -inf.  workspace: optional
-    uint8 buffer of nkv_cache8_attend_workspace_size bytes."""
+    uint8 buffer, nkv_cache8_attend_workspace_size bytes or fewer (with fewer,
+    fewer key splits)."""
     device = _require_gpu(q, cache.k, cache.v, cache.k_scale, cache.v_scale, out,
                           length if isinstance(length, torch.Tensor) else None)
     c, query, scale = _cache8_query(q, cache, length, max_length, softmax_scale)

@@ -4,6 +4,7 @@ what cannot be on a GPU."""
 import ctypes
 import shutil
 import subprocess
+import sys
 from pathlib import Path
 
 import numpy as np
@@ -12,6 +13,7 @@ import torch
 
 from tests import _cache8_ref as ref
 from nanokv_amd import _lib, ops
+from tests.test_device_attributes import SHIM
 
 PTR = 1 << 20      # stands for device memory; never read
 
@@ -126,14 +128,70 @@ def test_attend_refusals(kw, code, text):
     assert text in lib.nkv_last_error()
 
 
-def test_attend_workspace_refusals():
+def test_workspace_sizes_and_alignment():
     lib = _lib.lib()
     a = attend_args(cache=cache(B=1, H=1, cap=65536), n=65536)
     need = lib.nkv_cache8_attend_workspace_size(ctypes.byref(a))
-    assert need > 0
-    refused("nkv_cache8_attend", a, _lib.NKV_ERR_WORKSPACE, b"workspace", None, 0)
-    refused("nkv_cache8_attend", a, _lib.NKV_ERR_WORKSPACE, b"workspace", PTR, need - 1)
+    # 64 fp16-wide partial rows of 64 columns and 16 bytes of statistics each
+    assert need > 0 and need % (64 * 2 + 16) == 0
     refused("nkv_cache8_attend", a, _lib.NKV_ERR_INVALID, b"aligned", PTR + 4, need)
+    a.dtype = _lib.NKV_ROWS_FP16
+    assert lib.nkv_cache8_attend_workspace_size(ctypes.byref(a)) == need // 144 * (64 * 4 + 16)
+    m = attend_args(_lib.NkvCache8MassArgs, cache=cache(B=1, H=1, cap=1024), n=1000, Q=4096)
+    need = lib.nkv_cache8_mass_workspace_size(ctypes.byref(m))
+    assert need > 0 and need % (1024 * 4) == 0
+    refused("nkv_cache8_mass", m, _lib.NKV_ERR_INVALID, b"aligned", PTR + 2, need)
+
+
+CALLS = r"""
+import ctypes, sys
+shim = ctypes.CDLL(sys.argv[1], mode=ctypes.RTLD_GLOBAL)   # before the library: its symbols come first
+sys.path.insert(0, ".")
+from nanokv_amd import _lib
+from tests import test_cache8 as t
+lib = _lib.lib()
+
+def attend(H, cap, Q, G, D=128, dtype=0, work=True):
+    a = t.attend_args(cache=t.cache(B=1, H=H, cap=cap, D=D), n=cap, Q=Q, G=G, dtype=dtype)
+    need = lib.nkv_cache8_attend_workspace_size(ctypes.byref(a))
+    return lib.nkv_cache8_attend(None, ctypes.byref(a), t.PTR if work else None, need if work else 0)
+
+def evict(cap, keep):
+    big = 1 << 40
+    a = t.evict_args(cache=t.cache(cap=cap, at=t.PTR), n=cap, keep=keep)
+    a.out = _lib.NkvCache8(big, 2 * big, 3 * big, 4 * big, cap, 2, 2, 64, 0)
+    a.cache.v, a.cache.k_scale, a.cache.v_scale = 5 * big, 6 * big, 7 * big
+    a.mass, a.out_mass, a.rows = 8 * big, 9 * big, 10 * big
+    return lib.nkv_cache8_evict(None, ctypes.byref(a), None, 0)
+
+# (call, launches, whether some take more than 64 KB)
+calls = [(lambda: attend(8, 4096, 1, 4), 2, False), (lambda: attend(512, 1024, 1, 4), 1, True),
+         (lambda: attend(8, 4096, 1, 4, work=False), 1, False),
+         (lambda: attend(8, 4096, 40, 1), 2, False), (lambda: attend(64, 8192, 40, 1), 2, True),
+         (lambda: attend(24, 12480, 1560, 1), 2, True), (lambda: attend(24, 12480, 1560, 1, work=False), 1, True),
+         (lambda: evict(32768, 100), 2, True), (lambda: evict(40000 // 64 * 64, 100), 2, False)]
+for i, (call, n, large) in enumerate(calls):
+    for dev in (0, 1, 0):
+        shim.shim_device(dev)
+        rc = call()
+        assert rc == 0, (i, dev, rc, lib.nkv_last_error())
+        assert shim.shim_launches() == n and (shim.shim_large() > 0) == large, (i, dev, shim.shim_launches(), shim.shim_large())
+        assert shim.shim_missing() == 0, (i, dev, shim.shim_missing())
+print("ok")
+"""
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="needs a C compiler")
+def test_launches_with_and_without_workspace_and_lds_on_every_device(tmp_path):
+    """Over stand-ins for the HIP calls (nothing is launched): without a workspace
+    one launch instead of splits and their merge, and every launch above 64 KB
+    of dynamic LDS has its attribute on the device in use."""
+    src, so = tmp_path / "shim.c", tmp_path / "libshim.so"
+    src.write_text(SHIM)
+    subprocess.run(["gcc", "-shared", "-fPIC", "-O1", str(src), "-o", str(so)], check=True)
+    run = subprocess.run([sys.executable, "-c", CALLS, str(so)], capture_output=True, text=True,
+                         cwd=Path(__file__).resolve().parent.parent, timeout=120)
+    assert run.returncode == 0 and run.stdout.strip() == "ok", run.stdout + run.stderr
 
 
 @pytest.mark.parametrize("kw,code,text", QUERY + [

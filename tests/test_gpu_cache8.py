@@ -428,9 +428,13 @@ def test_attend_into_the_queries_and_in_a_given_workspace(dev, Q):
     work = torch.full((1 << 24,), 0xFF, dtype=torch.uint8, device=dev)
     got, l2 = ops.cache8_attend(same, cache, 9000, out=same, workspace=work)
     assert got is same and torch.equal(got, want) and torch.equal(l2, lse)
-    small = torch.empty(16, dtype=torch.uint8, device=dev)
-    with pytest.raises(RuntimeError, match="workspace"):
-        ops.cache8_attend(q, cache, 9000, workspace=small)
+    # less workspace: fewer splits, the same attention within its bound, and
+    # nothing written past its end
+    for nbytes in (16, 20_000 * Q // 16 * 16):
+        work = torch.full((nbytes + 4096,), 0xAB, dtype=torch.uint8, device=dev)
+        less, l3 = ops.cache8_attend(q, cache, 9000, workspace=work[:nbytes])
+        check_attend(q, cache, "int8", [9000], False, less, l3)
+        assert (work[nbytes:] == 0xAB).all()
 
 
 def test_mass_row_splits_and_their_join(dev):
@@ -450,6 +454,12 @@ def test_mass_row_splits_and_their_join(dev):
     assert (np.abs(out.double().cpu().numpy() - rm) <= tol).all()
     ops.cache8_mass(q, cache, lse, m, n, causal=True)
     assert torch.equal(m, out)
+    # a workspace for two splits, and for none
+    for nbytes in (2 * 2 * cache.cap * 4, 16):
+        work = torch.full((nbytes + 4096,), 0xAB, dtype=torch.uint8, device=dev)
+        ops.cache8_mass(q, cache, lse, m0.to(dev), n, out=out, causal=True, workspace=work[:nbytes])
+        assert (np.abs(out.double().cpu().numpy() - rm) <= tol).all()
+        assert (work[nbytes:] == 0xAB).all()
 
 
 def test_evict_long_heads(dev):
