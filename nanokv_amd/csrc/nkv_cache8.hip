@@ -249,7 +249,7 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 
 constexpr int SEL_WAVES = 16, SEL_THREADS = 64 * SEL_WAVES;
 constexpr int SEL_LDS = 32768;
-constexpr int SEL_BINS = 2048;
+constexpr int SEL_BINS = 2048, SEL_SLOTS = SEL_BINS + SEL_BINS / 32;
 constexpr int SEL_AHEAD = 4;            // keys of a lane in flight from LDS
 
 template <bool LDS>
@@ -268,13 +268,18 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
     const float* mass = p.mass + bh * p.cap;
     const int lo = p.sink, hi = n - p.recent;           // the rows between are chosen from
     const uint32_t want = p.keep - p.sink - p.recent;
-    // this wave's part: rows part .. part_end in steps of 64
+    // this wave's part: `steps` times 64 rows from `part` on
     const int steps = (n + SEL_THREADS - 1) / SEL_THREADS;
-    const int part = wave * steps * 64, part_end = min(part + steps * 64, n);
+    const int part = wave * steps * 64;
     extern __shared__ __align__(16) uint32_t held[];    // LDS: the keys in row order
-    __shared__ uint32_t hist[3][SEL_BINS];  // one a pass: no wave waits to reuse it
-    // f(key, row) over the part in order, AHEAD keys in flight; rows past the
-    // part's end come with any key
+    __shared__ uint32_t hist[3][SEL_SLOTS];  // one a pass: no wave waits to reuse it
+    // A row's key here: its mass's, which is at least that of -infinity, or for a
+    // row kept in any case 0, for one past the end 1
+    constexpr uint32_t FIXED = 0, PAST = 1;
+    auto key_of = [&](float x, int i) {
+        return i >= lo && i < hi ? order_key(x) : i < n ? FIXED : PAST;
+    };
+    // f(key, row) over the part in order, AHEAD keys in flight
     constexpr int AHEAD = LDS ? SEL_AHEAD : 8;
     auto each = [&](auto f) {
         for (int j0 = 0; j0 < steps; j0 += AHEAD) {
@@ -288,16 +293,15 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
                 if (j0 + j >= steps) break;
-                f(LDS ? k[j] : order_key(__uint_as_float(k[j])), i0 + 64 * j);
+                const int i = i0 + 64 * j;
+                f(LDS ? k[j] : key_of(__uint_as_float(k[j]), i), i);
             }
         }
     };
-    // rows of the part to choose from: lo .. lo + width
-    const uint32_t width = (uint32_t)max(min(hi, part_end) - lo, 0);
     uint32_t prefix = 0, left = want, mask = 0;
-    // digit d is counted at 64 (d mod 32) + d / 32: lane d / 32 reads it below,
-    // without bank conflicts
-    auto bin = [](uint32_t d) { return (d & 31) << 6 | d >> 5; };
+    // digit d is counted at d + d / 32: lane l reads the 32 from 33 (63 - l) on
+    // below, without bank conflicts
+    auto bin = [](uint32_t d) { return d + (d >> 5); };
     auto count_digit = [&](uint32_t* hist, bool count, uint32_t d) {
         if (__ballot(count) == ~0ull) {  // one add where the whole wave has one digit (equal masses)
             const uint32_t d0 = __builtin_amdgcn_readfirstlane(d);
@@ -308,7 +312,7 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
         }
         if (count) atomicAdd(&hist[bin(d)], 1u);
     };
-    for (int i = tid; i < 3 * SEL_BINS; i += SEL_THREADS) hist[0][i] = 0;
+    for (int i = tid; i < 3 * SEL_SLOTS; i += SEL_THREADS) hist[0][i] = 0;
     __syncthreads();
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
@@ -330,14 +334,14 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
                 u32x4 k;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    k[e] = order_key(x[j][e]);
-                    count_digit(hist[0], i + e >= lo && i + e < hi, k[e] >> 21);
+                    k[e] = key_of(x[j][e], i + e);
+                    count_digit(hist[0], k[e] > PAST, k[e] >> 21);
                 }
                 if (i < steps * SEL_THREADS) *reinterpret_cast<u32x4*>(held + i) = k;
             }
         } else {
             each([&](uint32_t k, int i) {
-                count_digit(hist[pass], (uint32_t)(i - lo) < width && (k & mask) == prefix, (k >> shift) & top);
+                count_digit(hist[pass], pass == 0 ? k > PAST : (k & mask) == prefix, (k >> shift) & top);
             });
         }
         __syncthreads();
@@ -346,7 +350,7 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
         uint32_t h[32], mine = 0;
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-            h[i] = hist[pass][64 * i + 63 - lane];
+            h[i] = hist[pass][33 * (63 - lane) + i];
             mine += h[i];
         }
         const uint32_t through = wave_scan(mine);
@@ -369,14 +373,13 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
     __shared__ uint32_t kept[SEL_WAVES], tied[SEL_WAVES];
     const uint32_t floor_key = want > 0 ? prefix : 0xffffffffu;
     uint32_t nk = 0, nt = 0;
-    auto marks = [&](uint32_t k, int i, uint64_t& a, uint64_t& t) {
-        const bool choose = (uint32_t)(i - lo) < width;
-        a = __ballot(choose ? k > floor_key : i < part_end);
-        t = __ballot(choose && k == prefix);
+    auto marks = [&](uint32_t k, uint64_t& a, uint64_t& t) {
+        a = __ballot(k > floor_key || k == FIXED);
+        t = __ballot(k == prefix);
     };
     each([&](uint32_t k, int i) {
         uint64_t a, t;
-        marks(k, i, a, t);
+        marks(k, a, t);
         nk += (uint32_t)__popcll(a);
         nt += (uint32_t)__popcll(t);
     });
@@ -393,7 +396,7 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
     }
     each([&](uint32_t k, int i) {
         uint64_t a, t;
-        marks(k, i, a, t);
+        marks(k, a, t);
         const uint32_t ra = bk + __builtin_amdgcn_mbcnt_hi((uint32_t)(a >> 32),
                                                            __builtin_amdgcn_mbcnt_lo((uint32_t)a, 0));
         if (t == 0) {
