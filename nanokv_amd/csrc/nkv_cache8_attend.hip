@@ -736,7 +736,7 @@ struct MassParams {
     int64_t q_sb, q_st, q_sh;
     int64_t cap, n64;             // n64: n in whole blocks
     float scale_log2;
-    int B, H, G, D, Q, n, causal, rows, splits, blocks;
+    int B, H, G, D, Q, n, causal, rows, splits, blocks, per;
 };
 
 // Sums over lanes of many values at once: each step adds two half-sized sets of
@@ -793,77 +793,98 @@ __device__ __forceinline__ void mass_store(const MassParams& p, int bh, int64_t 
     }
 }
 
-// Few query rows: a wave holds a block of 64 cached rows as operands (four
-// tiles of 16 keys) and takes the groups of 16 query rows in turn; the sums
-// over queries stay in registers until the end.  Bound by the read of K: all of
-// a wave's loads are issued before the first is used.
+// Waves from which on a wave takes several blocks (8 ragged sequences of 8 heads
+// up to 8,192 rows: 15.6 us with one block a wave, 14.6, 12.6 and 17.1 with
+// 4,096, 2,048 and 1,024 waves).
+constexpr int64_t MASS_WAVES = 2048;
+
+// Few query rows: a wave holds a block of 64 cached rows (four tiles of 16 keys)
+// and takes the groups of 16 query rows in turn; the sums over queries stay in
+// registers until the block's end.  Bound by the read of K.  A wave has p.per
+// blocks, 4 apart, the next one's codes loaded behind the last use of this one's.
 template <typename T, int FMT, int P>
 __global__ void __launch_bounds__(256) mass_kernel(MassParams p) {
     constexpr int STEPS = P / 32, PIECES = P / 64;
     using x8 = typename T::x8;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int blk = blockIdx.x * 4 + wave, bh = blockIdx.y, b = bh / p.H, hk = bh % p.H;
-    if (blk >= p.blocks) return;
+    const int bh = blockIdx.y, b = bh / p.H, hk = bh - b * p.H;
     const int len = c8_length(p.length, b, p.n);
-    const int64_t key0 = (int64_t)blk * C8_BLOCK;
     // the row whose sum this lane ends up with, of tile r / 4
     const int mykey = 16 * (r >> 2) + 4 * g + (r & 3);
-    const int64_t at = (int64_t)bh * p.cap + key0;
-    const float before = p.mass[at + mykey];
-    if (key0 >= len) {
-        if (p.out != p.mass) p.out[at + mykey] = before;
-        return;
-    }
-    u32x4 kr[4][PIECES];
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i)
-            kr[t][i] = *reinterpret_cast<const u32x4*>(p.k + (at + 16 * t + r) * P + 64 * i + 16 * g);
-    const float sk = p.ks[(int64_t)bh * (p.cap / C8_BLOCK) + blk];
-    // the first group with a row that sees the block's first key
-    int rg = 0;
-    if (p.causal)
-        rg = (int)min((int64_t)max(0, (int)key0 - (len - p.Q)) * p.G / 16, (int64_t)p.rows / 16);
+    const int64_t head = (int64_t)bh * p.cap;
+    const float* ks = p.ks + (int64_t)bh * (p.cap / C8_BLOCK);
     const int groups = (p.rows + 15) / 16;
     x8 qf[STEPS];
     float z;
-    int seen;
-    auto load_group = [&] {
+    int end;
+    auto load_group = [&](int rg) {
         const RowAt mine = row_at(rg * 16 + r, hk, p.G, p.Q);
-        seen = (!mine.there ? 0 : p.causal ? len - p.Q + 1 + mine.t : len) - (int)key0;
+        end = !mine.there ? 0 : p.causal ? len - p.Q + 1 + mine.t : len;
         load_q<T, P>(qf, p.q + b * p.q_sb + mine.t * p.q_st + mine.head * p.q_sh, mine.there, g, p.D);
         z = mine.there ? p.lse[((int64_t)b * p.H * p.G + mine.head) * p.Q + mine.t] : -INFINITY;
     };
-    load_group();
-    const float c = p.scale_log2 * fmaxf(sk, SCALE_MIN);
-    f32x4 sum[4] = {};
-    for (;;) {
-        const float off = z == -INFINITY ? INFINITY : z * LOG2E;
+    int blk = blockIdx.x * 4 * p.per + wave;
+    const int blk1 = min(p.blocks, (int)(blockIdx.x + 1) * 4 * p.per);
+    const int seen = (len + C8_BLOCK - 1) / C8_BLOCK;   // blocks below the length
+    u32x4 kr[4][PIECES];
+    float sk, before;
+    auto load_block = [&](int k) {
+        const int64_t at = head + (int64_t)k * C8_BLOCK;
+        before = p.mass[at + mykey];
+        sk = ks[k];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            f32x4 s{};
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int i = 0; i < PIECES; ++i) {
-                s = T::mfma16(codes_x8<T, FMT>(kr[t][i][0], kr[t][i][1]), qf[2 * i], s);
-                s = T::mfma16(codes_x8<T, FMT>(kr[t][i][2], kr[t][i][3]), qf[2 * i + 1], s);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float w = __builtin_amdgcn_exp2f(fmaf(s[e], c, -off));
-                sum[t][e] += 16 * t + 4 * g + e < seen ? w : 0.0f;
-            }
-        }
-        if (++rg >= groups) break;
-        load_group();
+            for (int i = 0; i < PIECES; ++i)
+                kr[t][i] = *reinterpret_cast<const u32x4*>(p.k + (at + 16 * t + r) * P + 64 * i + 16 * g);
+    };
+    if (blk < min(blk1, seen)) {
+        load_block(blk);
+        if (groups == 1) load_group(0);
     }
-    float v[16];
+    for (; blk < min(blk1, seen); blk += 4) {
+        const int key0 = blk * C8_BLOCK;
+        const float c = p.scale_log2 * fmaxf(sk, SCALE_MIN);
+        // the first group with a row that sees the block's first key
+        int rg = 0;
+        if (p.causal)
+            rg = (int)min((int64_t)max(0, key0 - (len - p.Q)) * p.G / 16, (int64_t)groups - 1);
+        f32x4 sum[4] = {};
+        for (;;) {
+            if (groups > 1) load_group(rg);
+            const float off = z == -INFINITY ? INFINITY : z * LOG2E;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = sum[i >> 2][i & 3];
-    const float x = reduce16(v, r);
-    if (key0 + mykey < len) p.out[at + mykey] = before + x;
-    else if (p.out != p.mass) p.out[at + mykey] = before;
+            for (int t = 0; t < 4; ++t) {
+                f32x4 s{};
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) {
+                    s = T::mfma16(codes_x8<T, FMT>(kr[t][i][0], kr[t][i][1]), qf[2 * i], s);
+                    s = T::mfma16(codes_x8<T, FMT>(kr[t][i][2], kr[t][i][3]), qf[2 * i + 1], s);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float w = __builtin_amdgcn_exp2f(fmaf(s[e], c, -off));
+                    sum[t][e] += key0 + 16 * t + 4 * g + e < end ? w : 0.0f;
+                }
+            }
+            if (++rg >= groups) break;
+        }
+        const float first = before;
+        if (blk + 4 < min(blk1, seen)) load_block(blk + 4);
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = sum[i >> 2][i & 3];
+        const float x = reduce16(v, r);
+        const int64_t at = head + key0 + mykey;
+        if (key0 + mykey < len) p.out[at] = first + x;
+        else if (p.out != p.mass) p.out[at] = first;
+    }
+    if (p.out != p.mass)
+        for (; blk < blk1; blk += 4) {
+            const int64_t at = head + (int64_t)blk * C8_BLOCK + mykey;
+            p.out[at] = p.mass[at];
+        }
 }
 
 // Many query rows: four waves hold a block of 64 cached rows each (two tiles of
@@ -1171,7 +1192,7 @@ void merge_run(const AttendParams& p, hipStream_t s) {
 
 template <typename T, int FMT, int P>
 void mass_run(const MassParams& p, bool tile, hipStream_t s) {
-    const dim3 grid((unsigned)cdiv(p.blocks, 4), (unsigned)(p.B * p.H), (unsigned)p.splits);
+    const dim3 grid((unsigned)cdiv(p.blocks, 4 * p.per), (unsigned)(p.B * p.H), (unsigned)p.splits);
     if (tile) mass_tile_kernel<T, FMT, P><<<grid, 256, 0, s>>>(p);
     else mass_kernel<T, FMT, P><<<grid, 256, 0, s>>>(p);
 }
@@ -1335,6 +1356,7 @@ extern "C" int nkv_cache8_mass(void* stream, const nkv_cache8_mass_args* a, void
     // in place, blocks past n have nothing to do
     p.blocks = (int)(p.out == p.mass ? cdiv(a->n, C8_BLOCK) : c.cap / C8_BLOCK);
     if (p.blocks == 0) return NKV_OK;
+    p.per = pl.tile ? 1 : (int)std::min<int64_t>(8, std::max<int64_t>(1, (int64_t)c.B * c.H * p.blocks / MASS_WAVES));
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     dispatch(a->dtype, c.format, c.D, [&](auto t, auto f, auto w) {
         mass_run<decltype(t), decltype(f)::value, decltype(w)::value>(p, pl.tile, s);

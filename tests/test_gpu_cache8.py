@@ -462,6 +462,27 @@ def test_mass_row_splits_and_their_join(dev):
         assert (work[nbytes:] == 0xAB).all()
 
 
+@pytest.mark.parametrize("Q,causal", [(1, False), (9, True)])
+def test_mass_of_several_blocks_a_wave(dev, Q, causal):
+    """Enough blocks that a wave takes more than one, ragged lengths, both outputs."""
+    B, H, G, N = 6, 24, 2, 4100
+    lengths = [4100, 1, 0, 2049, 64, 3000]
+    cache = make_cache(dev, B, H, N, 64, "int8", 63, lengths)
+    q = torch.randn((B, Q, H * G, 64), generator=torch.Generator().manual_seed(64)).bfloat16().to(dev)
+    n = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    out, lse = ops.cache8_attend(q, cache, n, max_length=N, causal=causal)
+    gl = check_attend(q, cache, "int8", lengths, causal, out, lse)
+    k, _ = cache_values(cache, "int8")
+    m0 = torch.rand((B, H, cache.cap), generator=torch.Generator().manual_seed(65))
+    rm, tol = ref.mass(q.double().cpu().numpy(), k, gl, m0.numpy(), lengths, causal, 0.125)
+    m, other = m0.to(dev), torch.full((B, H, cache.cap), float("nan"), device=dev)
+    ops.cache8_mass(q, cache, lse, m, n, out=other, max_length=N, causal=causal)
+    assert torch.equal(m.cpu(), m0)
+    ops.cache8_mass(q, cache, lse, m, n, max_length=N, causal=causal)
+    assert torch.equal(m, other)
+    assert (np.abs(m.double().cpu().numpy() - rm) <= tol).all()
+
+
 def test_evict_long_heads(dev):
     """Heads whose keys do not fit the selection's LDS, equal masses among them."""
     n, keep, H = 40_000, 9_001, 3
