@@ -107,8 +107,11 @@ __device__ __forceinline__ uint32_t block_umax(uint32_t x) {
 // One workgroup per (block of 64 rows, head, K or V, item): the block's new
 // rows are read once into registers, eight elements a thread and piece, their
 // amplitude is reduced, and the codes are written.  Bound by HBM: three bytes
-// move per bf16 element.  Blocks that hold a value that is not finite take a
-// slower path of the same results.
+// move per bf16 element (four prompts of 8,191 x 8 heads, 201 MB: 32 us where the
+// last call's cache is still on the chip's side, 41 us, 4.9 TB/s, where it is
+// not; a copy moves 5.2 TB/s), small calls by their one chain of load, reduction
+// and store (a frame of 1,560 x 24 heads, 29 MB: 7.5 us).  Blocks that hold a
+// value that is not finite take a slower path of the same results.
 template <int DTYPE, int FMT, int P>
 __global__ void __launch_bounds__(256) write_kernel(WriteParams p) {
     constexpr int CH = P / 8, STEP = 256 / CH, N = C8_BLOCK / STEP;
@@ -235,7 +238,10 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 // rows of its own contiguous part in order, behind those of the waves before
 // it, rows equal to the last key from the lowest up.  Up to SEL_LDS rows the
 // keys stay in LDS (one read of the masses), longer heads are read again for
-// each digit and for the list.
+// each digit and for the list.  One workgroup a head keeps it to one launch; it
+// is bound by its CU's instruction issue: 64 heads of 32,768 rows 26.5 us, of
+// which the first digit with the read takes 10, the others 5 each and the two
+// passes of the list 7; 8 heads of 2,048 rows 9.6 us, a chain of barriers.
 // Sums over lanes 0 .. l: within the rows of 16, then from row to row (DPP).
 __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
     x += (uint32_t)__builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
@@ -412,7 +418,8 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
 }
 
 // One workgroup per (block of 64 kept rows, head, K or V, item): gathers the
-// rows' codes onto the largest of their scales.
+// rows' codes onto the largest of their scales.  Bound by HBM: 64 heads of 8,192
+// kept rows, 236 MB, in 47 us, 5.0 TB/s (a copy moves 5.2).
 template <int FMT, int P>
 __global__ void __launch_bounds__(256) compact_kernel(EvictParams p) {
     constexpr int CH = P / 8, STEP = 256 / CH, N = C8_BLOCK / STEP;

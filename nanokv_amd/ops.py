@@ -1551,7 +1551,7 @@ def cache8_attend(q: torch.Tensor, cache: Cache8, length, *, max_length: Optiona
     c, query, scale = _cache8_query(q, cache, length, max_length, softmax_scale)
     B, Q, heads, D = q.shape
     if out is None:
-        out = torch.empty((B, Q, heads, D), device=device, dtype=q.dtype)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         strides = (Q * heads * D, heads * D, D)
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError("out must have q's shape and type")
