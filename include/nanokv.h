@@ -888,7 +888,8 @@ int nkv_cache8_mass(void* stream, const nkv_cache8_mass_args* args, void* worksp
  *   rows        [B, H, keep] int32, the rows kept, -1 past the last
  *   out_length  [B] int32, min(length, keep)
  * Rows of out and out_mass past the kept ones are left as they were.  Nothing
- * of out or out_mass may overlap the cache or mass.  mass is 16-byte aligned.
+ * of out, out_mass, rows or out_length may overlap another array of the call.
+ * mass is 16-byte aligned.
  */
 typedef struct nkv_cache8_evict_args {
     nkv_cache8 cache;
@@ -904,10 +905,7 @@ typedef struct nkv_cache8_evict_args {
     int64_t recent;
 } nkv_cache8_evict_args;
 
-/* 0: no scratch is used now; callers ask all the same. */
-size_t nkv_cache8_evict_workspace_size(const nkv_cache8_evict_args* args);
-int nkv_cache8_evict(void* stream, const nkv_cache8_evict_args* args, void* workspace,
-                     size_t workspace_bytes);
+int nkv_cache8_evict(void* stream, const nkv_cache8_evict_args* args);
 
 #ifdef __cplusplus
 }

@@ -99,9 +99,7 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
     return max(x, (uint32_t)__builtin_amdgcn_mov_dpp(x, 0xb1, 0xf, 0xf, true));
 }
 
-// The 16-bit types of queries and outputs.  Both hold every code exactly, so
-// products of queries and codes are formed in the queries' own type.
-// Partial: eight values of a split's partial result.
+// Eight values of a key split's partial result, in fp16 or in fp32.
 struct Partial16 {
     u32x4 w;
     __device__ __forceinline__ void load(const void* p, int64_t at) {
@@ -135,11 +133,11 @@ struct Partial32 {
     __device__ __forceinline__ float operator[](int k) const { return k < 4 ? a[k] : b[k - 4]; }
 };
 
+// The 16-bit types of queries and outputs.  Both hold every code exactly, so
+// scores are formed in the queries' own type.
 struct Bf16 {
     using x8 = bf16x8;
     using Partial = Partial16;
-    static constexpr int DTYPE = NKV_ROWS_BF16;
-    static __device__ __forceinline__ float load(uint16_t b) { return bf16_bits_to_f32(b); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
     // e4m3 codes 2 h and 2 h + 1 of a word
     template <int h>
@@ -157,8 +155,6 @@ struct Bf16 {
 struct Fp16 {
     using x8 = f16x8;
     using Partial = Partial32;
-    static constexpr int DTYPE = NKV_ROWS_FP16;
-    static __device__ __forceinline__ float load(uint16_t b) { return f16_bits_to_f32(b); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         f16x2 v;
         v[0] = (_Float16)a;

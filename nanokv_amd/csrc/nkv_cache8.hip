@@ -504,15 +504,17 @@ int check_evict(const nkv_cache8_evict_args* a) {
     NKV_REQUIRE(reinterpret_cast<uintptr_t>(a->mass) % 16 == 0, NKV_ERR_INVALID,
                 "mass must be 16-byte aligned");
     const int64_t heads = (int64_t)c.B * c.H, P = c8_pitch(c.D);
-    const Range in[5] = {{c.k, heads * c.cap * P}, {c.v, heads * c.cap * P},
+    const Range in[6] = {{c.k, heads * c.cap * P}, {c.v, heads * c.cap * P},
                          {c.k_scale, heads * c.cap / 16}, {c.v_scale, heads * c.cap / 16},
-                         {a->mass, heads * c.cap * 4}};
-    const Range out[6] = {{o.k, heads * o.cap * P}, {o.v, heads * o.cap * P},
+                         {a->mass, heads * c.cap * 4}, {a->length, a->length ? c.B * 4 : 0}};
+    const Range out[7] = {{o.k, heads * o.cap * P}, {o.v, heads * o.cap * P},
                           {o.k_scale, heads * o.cap / 16}, {o.v_scale, heads * o.cap / 16},
-                          {a->out_mass, heads * o.cap * 4}, {a->rows, heads * a->keep * 4}};
-    for (int i = 0; i < 6; ++i) {
+                          {a->out_mass, heads * o.cap * 4}, {a->rows, heads * a->keep * 4},
+                          {a->out_length, c.B * 4}};
+    for (int i = 0; i < 7; ++i) {
         for (const Range& r : in)
-            NKV_REQUIRE(!out[i].meets(r), NKV_ERR_INVALID, "the outputs overlap the cache or mass");
+            NKV_REQUIRE(!out[i].meets(r), NKV_ERR_INVALID,
+                        "the outputs overlap the cache, mass or length");
         for (int j = 0; j < i; ++j)
             NKV_REQUIRE(!out[i].meets(out[j]), NKV_ERR_INVALID, "the outputs overlap each other");
     }
@@ -559,14 +561,7 @@ extern "C" int nkv_cache8_write(void* stream, const nkv_cache8_write_args* a) {
     return NKV_OK;
 }
 
-extern "C" size_t nkv_cache8_evict_workspace_size(const nkv_cache8_evict_args* a) {
-    clear_error();
-    check_evict(a);
-    return 0;
-}
-
-extern "C" int nkv_cache8_evict(void* stream, const nkv_cache8_evict_args* a, void* workspace,
-                                size_t workspace_bytes) {
+extern "C" int nkv_cache8_evict(void* stream, const nkv_cache8_evict_args* a) {
     clear_error();
     int rc = check_evict(a);
     if (rc) return rc;

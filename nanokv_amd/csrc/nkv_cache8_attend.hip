@@ -1310,6 +1310,12 @@ int check_mass(const nkv_cache8_mass_args* a) {
     return NKV_OK;
 }
 
+// Up to this many rows of a key head each wave reads its queries itself; above,
+// they pass through LDS (us with either: 24 x 8 heads of 2,048 rows 20.4, 20.8 at
+// 32 query rows and 24.4, 20.8 at 48; 8 heads of 4,096 rows 4.5, 5.7 at 32 and
+// 6.0, 5.8 at 64).
+constexpr int64_t MASS_FEW = 32;
+
 struct MassPlan {
     bool tile;
     int splits;
@@ -1324,7 +1330,7 @@ MassPlan mass_plan(const nkv_cache8_mass_args* a, size_t limit = SIZE_MAX) {
     MassPlan pl{};
     const int64_t rows = a->Q * a->G, heads = (int64_t)a->cache.B * a->cache.H;
     pl.n64 = cdiv(a->n, C8_BLOCK) * C8_BLOCK;
-    pl.tile = rows >= MT_ROWS;
+    pl.tile = rows > MASS_FEW;
     pl.splits = 1;
     const int64_t base = heads * cdiv(pl.n64, 4 * C8_BLOCK), steps = cdiv(rows, MT_ROWS);
     if (pl.tile && base > 0 && base < 512)

@@ -1591,8 +1591,7 @@ def cache8_mass(q: torch.Tensor, cache: Cache8, lse: torch.Tensor, mass: torch.T
 
 
 def cache8_evict(cache: Cache8, mass: torch.Tensor, length, out: Cache8, out_mass: torch.Tensor,
-                 *, keep: int, sink: int = 0, recent: int = 0, max_length: Optional[int] = None,
-                 workspace: Optional[torch.Tensor] = None):
+                 *, keep: int, sink: int = 0, recent: int = 0, max_length: Optional[int] = None):
     """Evicts the tokens of least mass, head by head (see nkv_cache8_evict).
 
     Of a sequence longer than keep, each head keeps its first `sink` rows, its
@@ -1616,6 +1615,5 @@ def cache8_evict(cache: Cache8, mass: torch.Tensor, length, out: Cache8, out_mas
     left = torch.empty((c.B,), device=device, dtype=torch.int32)
     a = NkvCache8EvictArgs(c, o, mass.data_ptr(), out_mass.data_ptr(), rows.data_ptr(),
                            left.data_ptr(), at, n, keep, int(sink), int(recent))
-    scratch, nbytes = _cache8_scratch("nkv_cache8_evict_workspace_size", a, device, workspace)
-    _cache8_call("nkv_cache8_evict", device, byref(a), _ptr(scratch), nbytes)
+    _cache8_call("nkv_cache8_evict", device, byref(a))
     return rows, left

@@ -48,7 +48,7 @@ def evict_args(**kw):
     a = _lib.NkvCache8EvictArgs()
     a.cache, a.out = kw.pop("cache", cache()), kw.pop("out", cache(at=PTR + (4 << 24)))
     a.mass, a.out_mass, a.rows = PTR + (8 << 24), PTR + (9 << 24), PTR + (10 << 24)
-    a.out_length, a.n, a.keep = PTR, 128, 64
+    a.out_length, a.n, a.keep = PTR - 1024, 128, 64
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -81,7 +81,7 @@ def test_bad_caches(kw, code, text):
     refused("nkv_cache8_write", write_args(cache=c), code, text)
     refused("nkv_cache8_attend", attend_args(cache=c), code, text, None, 0)
     refused("nkv_cache8_mass", attend_args(_lib.NkvCache8MassArgs, cache=c), code, text, None, 0)
-    refused("nkv_cache8_evict", evict_args(cache=c), code, text, None, 0)
+    refused("nkv_cache8_evict", evict_args(cache=c), code, text)
 
 
 @pytest.mark.parametrize("kw,code,text", [
@@ -161,8 +161,8 @@ def evict(cap, keep):
     a = t.evict_args(cache=t.cache(cap=cap, at=t.PTR), n=cap, keep=keep)
     a.out = _lib.NkvCache8(big, 2 * big, 3 * big, 4 * big, cap, 2, 2, 64, 0)
     a.cache.v, a.cache.k_scale, a.cache.v_scale = 5 * big, 6 * big, 7 * big
-    a.mass, a.out_mass, a.rows = 8 * big, 9 * big, 10 * big
-    return lib.nkv_cache8_evict(None, ctypes.byref(a), None, 0)
+    a.mass, a.out_mass, a.rows, a.out_length = 8 * big, 9 * big, 10 * big, 11 * big
+    return lib.nkv_cache8_evict(None, ctypes.byref(a))
 
 # (call, launches, whether some take more than 64 KB)
 calls = [(lambda: attend(8, 4096, 1, 4), 2, False), (lambda: attend(512, 1024, 1, 4), 1, True),
@@ -210,6 +210,8 @@ def test_mass_refusals(kw, code, text):
     (dict(out=cache()), _lib.NKV_ERR_INVALID, b"overlap"),
     (dict(out_mass=PTR + (8 << 24)), _lib.NKV_ERR_INVALID, b"overlap"),
     (dict(rows=PTR + (9 << 24)), _lib.NKV_ERR_INVALID, b"overlap"),
+    (dict(length=PTR - 64, out_length=PTR - 60), _lib.NKV_ERR_INVALID, b"overlap"),
+    (dict(out_length=PTR + (9 << 24)), _lib.NKV_ERR_INVALID, b"overlap"),
     (dict(keep=0), _lib.NKV_ERR_INVALID, b"keep"),
     (dict(keep=129), _lib.NKV_ERR_INVALID, b"keep"),
     (dict(sink=40, recent=30), _lib.NKV_ERR_INVALID, b"sink"),
@@ -220,7 +222,7 @@ def test_mass_refusals(kw, code, text):
     (dict(mass=PTR + (8 << 24) + 4), _lib.NKV_ERR_INVALID, b"mass must be 16"),
 ])
 def test_evict_refusals(kw, code, text):
-    refused("nkv_cache8_evict", evict_args(**kw), code, text, None, 0)
+    refused("nkv_cache8_evict", evict_args(**kw), code, text)
 
 
 def test_ctypes_structs_match_the_header_layout(tmp_path):
