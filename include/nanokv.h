@@ -905,7 +905,12 @@ typedef struct nkv_cache8_evict_args {
     int64_t recent;
 } nkv_cache8_evict_args;
 
-int nkv_cache8_evict(void* stream, const nkv_cache8_evict_args* args);
+/* Bytes of workspace nkv_cache8_evict needs for these arguments (0 up to 32,768
+ * rows): the counts of the parts that a longer head is chosen in.  16-byte aligned;
+ * a smaller one is NKV_ERR_WORKSPACE. */
+size_t nkv_cache8_evict_workspace_size(const nkv_cache8_evict_args* args);
+int nkv_cache8_evict(void* stream, const nkv_cache8_evict_args* args, void* workspace,
+                     size_t workspace_bytes);
 
 #ifdef __cplusplus
 }

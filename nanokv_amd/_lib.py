@@ -43,7 +43,8 @@ EXPORTED = (
     "nkv_attend_static", "nkv_lift_lse_combine", "nkv_finish", "nkv_reader_rows",
     "nkv_decode_batch", "nkv_c64_fit_rows", "nkv_encode_workspace_size",
     "nkv_cache8_write", "nkv_cache8_attend_workspace_size", "nkv_cache8_attend",
-    "nkv_cache8_mass_workspace_size", "nkv_cache8_mass", "nkv_cache8_evict",
+    "nkv_cache8_mass_workspace_size", "nkv_cache8_mass",
+    "nkv_cache8_evict_workspace_size", "nkv_cache8_evict",
 )
 NKV_STATIC_SCRATCH_BYTES = 64 << 20
 
@@ -321,9 +322,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.nkv_finish.argtypes = [c_void_p, POINTER(NkvFinishArgs)]
     lib.nkv_cache8_write.restype = c_int
     lib.nkv_cache8_write.argtypes = [c_void_p, POINTER(NkvCache8WriteArgs)]
-    lib.nkv_cache8_evict.restype = c_int
-    lib.nkv_cache8_evict.argtypes = [c_void_p, POINTER(NkvCache8EvictArgs)]
-    for name, args in (("attend", NkvCache8AttendArgs), ("mass", NkvCache8MassArgs)):
+    for name, args in (("attend", NkvCache8AttendArgs), ("mass", NkvCache8MassArgs),
+                       ("evict", NkvCache8EvictArgs)):
         size = getattr(lib, f"nkv_cache8_{name}_workspace_size")
         size.restype = c_size_t
         size.argtypes = [POINTER(args)]

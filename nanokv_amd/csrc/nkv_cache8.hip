@@ -223,6 +223,8 @@ struct EvictParams {
     const int32_t* length;
     int64_t cap, out_cap;
     int B, H, n, keep, sink, recent;
+    void* work;                   // part_kernel: the states, then the counts
+    int parts, part_rows;
 };
 
 // A mass as an integer that orders as the masses do: NaN above all, -0 as +0.
@@ -233,15 +235,35 @@ __device__ __forceinline__ uint32_t order_key(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One workgroup per (item, head).  The key of the last row kept is found digit
-// by digit (11, 11 and 10 bits, counts in LDS); then every wave lists the kept
-// rows of its own contiguous part in order, behind those of the waves before
-// it, rows equal to the last key from the lowest up.  Up to SEL_LDS rows the
-// keys stay in LDS (one read of the masses), longer heads are read again for
-// each digit and for the list.  One workgroup a head keeps it to one launch; it
-// is bound by its CU's instruction issue: 64 heads of 32,768 rows 26.5 us, of
-// which the first digit with the read takes 10, the others 5 each and the two
-// passes of the list 7; 8 heads of 2,048 rows 9.6 us, a chain of barriers.
+// The rows an eviction keeps of a head: the key of the last of them is found
+// digit by digit (11, 11 and 10 bits, counts in LDS); then every wave lists the
+// kept rows of its own contiguous part in order, behind those of the waves
+// before it, rows equal to the last key from the lowest up.
+constexpr int SEL_WAVES = 16, SEL_THREADS = 64 * SEL_WAVES;
+constexpr int SEL_BINS = 2048, SEL_SLOTS = SEL_BINS + SEL_BINS / 32;
+
+__device__ __forceinline__ constexpr int digit_shift(int pass) {
+    return pass == 0 ? 21 : pass == 1 ? 10 : 0;
+}
+__device__ __forceinline__ constexpr uint32_t digit_top(int pass) {
+    return pass == 2 ? 1023u : 2047u;
+}
+
+// digit d is counted at d + d / 32: lane l reads the 32 from 33 (63 - l) on
+// in find_digit, without bank conflicts
+__device__ __forceinline__ constexpr uint32_t bin(uint32_t d) { return d + (d >> 5); }
+
+__device__ __forceinline__ void count_digit(uint32_t* hist, int lane, bool count, uint32_t d) {
+    if (__ballot(count) == ~0ull) {  // one add where the whole wave has one digit (equal masses)
+        const uint32_t d0 = __builtin_amdgcn_readfirstlane(d);
+        if (__ballot(d == d0) == ~0ull) {
+            if (lane == 0) atomicAdd(&hist[bin(d0)], 64u);
+            return;
+        }
+    }
+    if (count) atomicAdd(&hist[bin(d)], 1u);
+}
+
 // Sums over lanes 0 .. l: within the rows of 16, then from row to row (DPP).
 __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
     x += (uint32_t)__builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
@@ -253,129 +275,48 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
     return x;
 }
 
-constexpr int SEL_WAVES = 16, SEL_THREADS = 64 * SEL_WAVES;
-constexpr int SEL_LDS = 32768;
-constexpr int SEL_BINS = 2048, SEL_SLOTS = SEL_BINS + SEL_BINS / 32;
-constexpr int SEL_AHEAD = 4;            // keys of a lane in flight from LDS
+// The digit at which the count from above reaches `left`, found by every wave
+// for itself: lane l has the 32 digits below 2048 - 32 l.  `left` becomes what
+// is left at that digit.
+__device__ __forceinline__ uint32_t find_digit(const uint32_t* hist, int lane, uint32_t& left) {
+    uint32_t h[32], mine = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        h[i] = hist[33 * (63 - lane) + i];
+        mine += h[i];
+    }
+    const uint32_t through = wave_scan(mine);
+    const int l0 = __builtin_ctzll(__ballot(through >= left));
+    uint32_t above = through - mine, passed = 32, over = above;
+#pragma unroll
+    for (int i = 31; i >= 0; --i) {
+        above += h[i];
+        if (above < left) {                             // the digit lies below this one
+            passed = i;
+            over = above;
+        }
+    }
+    left -= (uint32_t)__builtin_amdgcn_readlane(over, l0);
+    return (uint32_t)__builtin_amdgcn_readlane(SEL_BINS - 32 * (lane + 1) + passed - 1, l0);
+}
 
-template <bool LDS>
-__global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
-    const int b = blockIdx.x / p.H;
-    const int64_t bh = blockIdx.x;
-    const int n = c8_length(p.length, b, p.n);
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int32_t* rows = p.rows + bh * p.keep;
-    if (blockIdx.x % p.H == 0 && tid == 0) p.out_length[b] = min(n, p.keep);
-    if (n <= p.keep) {
-        for (int i = tid; i < p.keep; i += SEL_THREADS) rows[i] = i < n ? i : -1;
-        return;
-    }
-    const float* mass = p.mass + bh * p.cap;
-    const int lo = p.sink, hi = n - p.recent;           // the rows between are chosen from
-    const uint32_t want = p.keep - p.sink - p.recent;
-    // this wave's part: `steps` times 64 rows from `part` on
-    const int steps = (n + SEL_THREADS - 1) / SEL_THREADS;
-    const int part = wave * steps * 64;
-    extern __shared__ __align__(16) uint32_t held[];    // LDS: the keys in row order
-    __shared__ uint32_t hist[3][SEL_SLOTS];  // one a pass: no wave waits to reuse it
-    // A row's key here: its mass's, which is at least that of -infinity, or for a
-    // row kept in any case 0, for one past the end 1
-    constexpr uint32_t FIXED = 0, PAST = 1;
-    auto key_of = [&](float x, int i) {
-        return i >= lo && i < hi ? order_key(x) : i < n ? FIXED : PAST;
-    };
-    // f(key, row) over the part in order, AHEAD keys in flight
-    constexpr int AHEAD = LDS ? SEL_AHEAD : 8;
-    auto each = [&](auto f) {
-        for (int j0 = 0; j0 < steps; j0 += AHEAD) {
-            uint32_t k[AHEAD];
-            const int i0 = part + 64 * j0 + lane;
-#pragma unroll
-            for (int j = 0; j < AHEAD; ++j) {
-                if (LDS) k[j] = held[i0 + 64 * j];  // (up to AHEAD steps past the end)
-                else k[j] = __float_as_uint(mass[min(i0 + 64 * j, n - 1)]);
-            }
-#pragma unroll
-            for (int j = 0; j < AHEAD; ++j) {
-                if (j0 + j >= steps) break;
-                const int i = i0 + 64 * j;
-                f(LDS ? k[j] : key_of(__uint_as_float(k[j]), i), i);
-            }
-        }
-    };
-    uint32_t prefix = 0, left = want, mask = 0;
-    // digit d is counted at d + d / 32: lane l reads the 32 from 33 (63 - l) on
-    // below, without bank conflicts
-    auto bin = [](uint32_t d) { return d + (d >> 5); };
-    auto count_digit = [&](uint32_t* hist, bool count, uint32_t d) {
-        if (__ballot(count) == ~0ull) {  // one add where the whole wave has one digit (equal masses)
-            const uint32_t d0 = __builtin_amdgcn_readfirstlane(d);
-            if (__ballot(d == d0) == ~0ull) {
-                if (lane == 0) atomicAdd(&hist[bin(d0)], 64u);
-                return;
-            }
-        }
-        if (count) atomicAdd(&hist[bin(d)], 1u);
-    };
-    for (int i = tid; i < 3 * SEL_SLOTS; i += SEL_THREADS) hist[0][i] = 0;
-    __syncthreads();
-#pragma unroll
-    for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-        const uint32_t top = pass == 2 ? 1023u : 2047u;
-        if (LDS && pass == 0) {
-            // four rows a thread and load, every load of the workgroup in flight
-            constexpr int PER = SEL_LDS / (4 * SEL_THREADS);
-            f32x4 x[PER];
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int i = 4 * (tid + SEL_THREADS * j);
-                if (i < n) x[j] = *reinterpret_cast<const f32x4*>(mass + i);
-            }
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int i = 4 * (tid + SEL_THREADS * j);
-                if (4 * SEL_THREADS * j >= n) break;
-                u32x4 k;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    k[e] = key_of(x[j][e], i + e);
-                    count_digit(hist[0], k[e] > PAST, k[e] >> 21);
-                }
-                if (i < steps * SEL_THREADS) *reinterpret_cast<u32x4*>(held + i) = k;
-            }
-        } else {
-            each([&](uint32_t k, int i) {
-                count_digit(hist[pass], pass == 0 ? k > PAST : (k & mask) == prefix, (k >> shift) & top);
-            });
-        }
-        __syncthreads();
-        // The digit at which the count from above reaches `left`, found by every
-        // wave for itself: lane l has the 32 digits below 2048 - 32 l.
-        uint32_t h[32], mine = 0;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            h[i] = hist[pass][33 * (63 - lane) + i];
-            mine += h[i];
-        }
-        const uint32_t through = wave_scan(mine);
-        const int l0 = __builtin_ctzll(__ballot(through >= left));
-        uint32_t above = through - mine, passed = 32, over = above;
-#pragma unroll
-        for (int i = 31; i >= 0; --i) {
-            above += h[i];
-            if (above < left) {                             // the digit lies below this one
-                passed = i;
-                over = above;
-            }
-        }
-        prefix |= (uint32_t)__builtin_amdgcn_readlane(SEL_BINS - 32 * (lane + 1) + passed - 1, l0)
-                  << shift;
-        left -= (uint32_t)__builtin_amdgcn_readlane(over, l0);
-        mask |= top << shift;
-    }
-    // `left` of the rows whose key is `prefix` are kept, and all above it
+// The key of row i: its mass's, which is at least that of -infinity, or for a
+// row kept in any case 0, for one past the end 1.
+struct Chosen {
+    int lo, hi, n;                // the rows lo .. hi are chosen from
+};
+constexpr uint32_t FIXED = 0, PAST = 1;
+__device__ __forceinline__ uint32_t row_key(const Chosen& r, float x, int i) {
+    return i >= r.lo && i < r.hi ? order_key(x) : i < r.n ? FIXED : PAST;
+}
+
+// Lists the kept rows of a workgroup's part, in order, behind `bk` kept and `bt`
+// tied rows before it: `left` of all rows whose key is `prefix`, and all above
+// it.  each(f) calls f(key, row) for the keys of this wave's part.
+template <typename Each>
+__device__ __forceinline__ void list_rows(Each each, uint32_t prefix, uint32_t left, uint32_t want,
+                                          uint32_t bk, uint32_t bt, int wave, int lane,
+                                          int32_t* rows) {
     __shared__ uint32_t kept[SEL_WAVES], tied[SEL_WAVES];
     const uint32_t floor_key = want > 0 ? prefix : 0xffffffffu;
     uint32_t nk = 0, nt = 0;
@@ -383,7 +324,7 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
         a = __ballot(k > floor_key || k == FIXED);
         t = __ballot(k == prefix);
     };
-    each([&](uint32_t k, int i) {
+    each([&](uint32_t k, int) {
         uint64_t a, t;
         marks(k, a, t);
         nk += (uint32_t)__popcll(a);
@@ -394,7 +335,6 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
         tied[wave] = nt;
     }
     __syncthreads();
-    uint32_t bk = 0, bt = 0;
 #pragma unroll
     for (int w = 0; w < SEL_WAVES; ++w) {
         bk += w < wave ? kept[w] : 0;
@@ -415,6 +355,223 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
         bk += (uint32_t)__popcll(a);
         bt += (uint32_t)__popcll(t);
     });
+}
+
+// Up to SEL_LDS rows: one workgroup a head, whose keys stay in LDS (one read of
+// the masses, one launch).  It is bound by its CU's instruction issue: 64 heads
+// of 32,768 rows 26.5 us, of which the first digit with the read takes 10, the
+// others 5 each and the two passes of the list 7; 8 heads of 2,048 rows 9.6 us,
+// a chain of barriers.
+constexpr int SEL_LDS = 32768;
+constexpr int SEL_AHEAD = 4;            // keys of a lane in flight from LDS
+
+__global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
+    const int b = blockIdx.x / p.H;
+    const int64_t bh = blockIdx.x;
+    const int n = c8_length(p.length, b, p.n);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int32_t* rows = p.rows + bh * p.keep;
+    if (blockIdx.x % p.H == 0 && tid == 0) p.out_length[b] = min(n, p.keep);
+    if (n <= p.keep) {
+        for (int i = tid; i < p.keep; i += SEL_THREADS) rows[i] = i < n ? i : -1;
+        return;
+    }
+    const float* mass = p.mass + bh * p.cap;
+    const Chosen range{p.sink, n - p.recent, n};
+    const uint32_t want = p.keep - p.sink - p.recent;
+    // this wave's part: `steps` times 64 rows from `part` on
+    const int steps = (n + SEL_THREADS - 1) / SEL_THREADS;
+    const int part = wave * steps * 64;
+    extern __shared__ __align__(16) uint32_t held[];    // the keys in row order
+    __shared__ uint32_t hist[3][SEL_SLOTS];  // one a pass: no wave waits to reuse it
+    // f(key, row) over the part in order, SEL_AHEAD keys in flight
+    auto each = [&](auto f) {
+        for (int j0 = 0; j0 < steps; j0 += SEL_AHEAD) {
+            uint32_t k[SEL_AHEAD];
+            const int i0 = part + 64 * j0 + lane;
+#pragma unroll
+            for (int j = 0; j < SEL_AHEAD; ++j)
+                k[j] = held[i0 + 64 * j];  // (up to SEL_AHEAD steps past the end)
+#pragma unroll
+            for (int j = 0; j < SEL_AHEAD; ++j) {
+                if (j0 + j >= steps) break;
+                f(k[j], i0 + 64 * j);
+            }
+        }
+    };
+    uint32_t prefix = 0, left = want, mask = 0;
+    for (int i = tid; i < 3 * SEL_SLOTS; i += SEL_THREADS) hist[0][i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = digit_shift(pass);
+        const uint32_t top = digit_top(pass);
+        if (pass == 0) {
+            // four rows a thread and load, every load of the workgroup in flight
+            constexpr int PER = SEL_LDS / (4 * SEL_THREADS);
+            f32x4 x[PER];
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int i = 4 * (tid + SEL_THREADS * j);
+                if (i < n) x[j] = *reinterpret_cast<const f32x4*>(mass + i);
+            }
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int i = 4 * (tid + SEL_THREADS * j);
+                if (4 * SEL_THREADS * j >= n) break;
+                u32x4 k;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    k[e] = row_key(range, x[j][e], i + e);
+                    count_digit(hist[0], lane, k[e] > PAST, k[e] >> shift);
+                }
+                if (i < steps * SEL_THREADS) *reinterpret_cast<u32x4*>(held + i) = k;
+            }
+        } else {
+            each([&](uint32_t k, int) {
+                count_digit(hist[pass], lane, (k & mask) == prefix, (k >> shift) & top);
+            });
+        }
+        __syncthreads();
+        prefix |= find_digit(hist[pass], lane, left) << shift;
+        mask |= top << shift;
+    }
+    list_rows(each, prefix, left, want, 0, 0, wave, lane, rows);
+}
+
+// Longer heads: parts of PART_ROWS rows or more, at most PARTS of them, each one
+// workgroup's.  A launch counts one digit over every part and stores the counts;
+// the next adds up its head's parts (every workgroup for itself, no atomics in
+// memory, nothing to clear), finds the digit and with it how many rows the parts
+// before its own keep; the fourth lists.  Bound by the chain of four launches (4.9,
+// 7.9, 7.8 and 10.5 us for one head of 131,072 rows; masses loaded ahead of the
+// sums change nothing there and cost 10 % of a full chip's): whole evictions of
+// that head 34.7 us and of 1,000,000 rows 65 us, where one workgroup that read the
+// masses five times took 141 and 1,028; 64 heads of 65,536 rows 118 (146).  At
+// SEL_LDS rows and below the chain costs more than it spreads (8 heads of 32,768
+// rows: 34.7 us against select_kernel's 32.3, 64 heads: 65.6 against 60.8, 8 heads
+// of 16,384: 30.8 against 21.4).  Parts of 4,096 rows add up twice the counts (64
+// heads of 65,536 rows: 143 us), of 16,384 lengthen the chain (one head of
+// 131,072: 39), and 128 parts a head instead of 64 add up more (1,000,000: 78).
+constexpr int PART_ROWS = 8192, PARTS = 64;
+
+int part_rows(int64_t n) {
+    const int64_t rows = std::max<int64_t>(PART_ROWS, (n + PARTS - 1) / PARTS);
+    return (int)((rows + 4 * SEL_THREADS - 1) / (4 * SEL_THREADS) * (4 * SEL_THREADS));
+}
+
+// A part's counts of two passes (a launch reads one and writes the other) and what
+// its workgroup knows after them.
+struct PartState {
+    uint32_t prefix, left, kept, pad;
+};
+constexpr size_t PART_BYTES = 2 * SEL_BINS * sizeof(uint32_t) + sizeof(PartState);
+
+template <int PASS>
+__global__ void __launch_bounds__(SEL_THREADS) part_kernel(EvictParams p) {
+    const int64_t bh = blockIdx.x / p.parts;
+    const int part = blockIdx.x % p.parts, b = (int)(bh / p.H);
+    const int n = c8_length(p.length, b, p.n);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int32_t* rows = p.rows + bh * p.keep;
+    if (PASS == 0 && part == 0 && tid == 0 && bh % p.H == 0) p.out_length[b] = min(n, p.keep);
+    if (n <= p.keep) {
+        if (PASS == 0)
+            for (int i = part * SEL_THREADS + tid; i < p.keep; i += p.parts * SEL_THREADS)
+                rows[i] = i < n ? i : -1;
+        return;
+    }
+    const int first = part * p.part_rows;
+    if (first >= n) return;
+    const int last = min(first + p.part_rows, n), active = (n + p.part_rows - 1) / p.part_rows;
+    const float* mass = p.mass + bh * p.cap;
+    const Chosen range{p.sink, n - p.recent, n};
+    const uint32_t want = p.keep - p.sink - p.recent;
+    const int64_t all = (int64_t)p.B * p.H * p.parts;
+    PartState* state = reinterpret_cast<PartState*>(p.work) + blockIdx.x;
+    uint32_t* counts = reinterpret_cast<uint32_t*>(reinterpret_cast<PartState*>(p.work) + all);
+    auto counts_of = [&](int pass, int w) {
+        return counts + ((pass & 1) * all + bh * p.parts + w) * SEL_BINS;
+    };
+    __shared__ uint32_t hist[SEL_SLOTS], total[SEL_SLOTS], sums[SEL_WAVES], tie;
+    for (int i = tid; i < SEL_SLOTS; i += SEL_THREADS) hist[i] = 0;
+    uint32_t prefix = 0, mask = 0, tied = 0;
+    PartState st{0, want, 0, 0};
+    if constexpr (PASS > 0) {
+        if constexpr (PASS > 1) st = *state;
+        // digits 2 tid and 2 tid + 1 of all parts, and of those before this one
+        u32x2 s{}, e{};
+#pragma unroll 8
+        for (int w = 0; w < active; ++w) {
+            const u32x2 x = reinterpret_cast<const u32x2*>(counts_of(PASS - 1, w))[tid];
+            s += x;
+            if (w < part) e += x;
+        }
+        total[bin(2 * tid)] = s[0];
+        total[bin(2 * tid + 1)] = s[1];
+        __syncthreads();
+        const uint32_t d = find_digit(total, lane, st.left);
+        const uint32_t over = (2u * tid > d ? e[0] : 0) + (2u * tid + 1 > d ? e[1] : 0);
+        if (tid == (int)(d >> 1)) tie = e[d & 1];
+        const uint32_t sum = wave_scan(over);
+        if (lane == 63) sums[wave] = sum;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < SEL_WAVES; ++w) st.kept += sums[w];
+        tied = tie;
+        prefix = st.prefix |= d << digit_shift(PASS - 1);
+        if (PASS < 3 && tid == 0) *state = st;
+        mask = PASS == 1 ? 0xffe00000u : 0xfffffc00u;
+    } else {
+        __syncthreads();
+    }
+    if constexpr (PASS < 3) {
+        for (int i0 = first + 4 * tid; i0 < first + p.part_rows; i0 += PART_ROWS) {
+            f32x4 x[PART_ROWS / (4 * SEL_THREADS)];
+#pragma unroll
+            for (int j = 0; j < PART_ROWS / (4 * SEL_THREADS); ++j) {
+                const int i = i0 + 4 * SEL_THREADS * j;
+                x[j] = f32x4{};
+                if (i < last) x[j] = *reinterpret_cast<const f32x4*>(mass + i);
+            }
+#pragma unroll
+            for (int j = 0; j < PART_ROWS / (4 * SEL_THREADS); ++j) {
+                const int i = i0 + 4 * SEL_THREADS * j;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    // (rows of the next part, where this one's end inside the step, do not count)
+                    const uint32_t k = i < last ? row_key(range, x[j][e], i + e) : PAST;
+                    count_digit(hist, lane, PASS == 0 ? k > PAST : (k & mask) == prefix,
+                                (k >> digit_shift(PASS)) & digit_top(PASS));
+                }
+            }
+        }
+        __syncthreads();
+        const u32x2 mine{hist[bin(2 * tid)], hist[bin(2 * tid + 1)]};
+        reinterpret_cast<u32x2*>(counts_of(PASS, part))[tid] = mine;
+    } else {
+        const int steps = (last - first + SEL_THREADS - 1) / SEL_THREADS;
+        const int begin = first + wave * steps * 64;
+        constexpr int AHEAD = 8;
+        auto each = [&](auto f) {
+            for (int j0 = 0; j0 < steps; j0 += AHEAD) {
+                float x[AHEAD];
+                const int i0 = begin + 64 * j0 + lane;
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) x[j] = mass[min(i0 + 64 * j, n - 1)];
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) {
+                    if (j0 + j >= steps) break;
+                    const int i = i0 + 64 * j;
+                    f(i < last ? row_key(range, x[j], i) : PAST, i);
+                }
+            }
+        };
+        const uint32_t fixed = min(first, range.lo) + max(first - range.hi, 0);
+        list_rows(each, prefix, st.left, want, fixed + st.kept, tied, wave, lane, rows);
+    }
 }
 
 // One workgroup per (block of 64 kept rows, head, K or V, item): gathers the
@@ -484,6 +641,8 @@ struct Range {
     bool meets(const Range& o) const { return lo < o.hi && o.lo < hi; }
 };
 
+int evict_parts(int64_t n) { return (int)cdiv(n, part_rows(n)); }
+
 int check_evict(const nkv_cache8_evict_args* a) {
     NKV_REQUIRE(a, NKV_ERR_INVALID, "args is null");
     int rc = cache8_check(&a->cache, __func__);
@@ -518,7 +677,14 @@ int check_evict(const nkv_cache8_evict_args* a) {
         for (int j = 0; j < i; ++j)
             NKV_REQUIRE(!out[i].meets(out[j]), NKV_ERR_INVALID, "the outputs overlap each other");
     }
+    NKV_REQUIRE(a->n <= SEL_LDS || heads * evict_parts(a->n) < 1 << 22, NKV_ERR_UNSUPPORTED,
+                "too many heads of this length");
     return NKV_OK;
+}
+
+size_t evict_bytes(const nkv_cache8_evict_args* a) {
+    if (a->n <= SEL_LDS) return 0;
+    return (size_t)a->cache.B * a->cache.H * evict_parts(a->n) * PART_BYTES;
 }
 
 }  // namespace
@@ -561,24 +727,41 @@ extern "C" int nkv_cache8_write(void* stream, const nkv_cache8_write_args* a) {
     return NKV_OK;
 }
 
-extern "C" int nkv_cache8_evict(void* stream, const nkv_cache8_evict_args* a) {
+extern "C" size_t nkv_cache8_evict_workspace_size(const nkv_cache8_evict_args* a) {
+    clear_error();
+    return check_evict(a) == NKV_OK ? evict_bytes(a) : 0;
+}
+
+extern "C" int nkv_cache8_evict(void* stream, const nkv_cache8_evict_args* a, void* workspace,
+                                size_t workspace_bytes) {
     clear_error();
     int rc = check_evict(a);
     if (rc) return rc;
     const nkv_cache8 &c = a->cache, &o = a->out;
     if (c.B == 0) return NKV_OK;
+    const size_t need = evict_bytes(a);
+    NKV_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), NKV_ERR_WORKSPACE,
+                "workspace is smaller than nkv_cache8_evict_workspace_size");
+    NKV_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, NKV_ERR_INVALID,
+                "workspace must be 16-byte aligned");
     EvictParams p{{(const uint8_t*)c.k, (const uint8_t*)c.v}, {c.k_scale, c.v_scale},
                   {(uint8_t*)o.k, (uint8_t*)o.v}, {o.k_scale, o.v_scale}, a->mass, a->out_mass,
                   a->rows, a->out_length, a->length, c.cap, o.cap, c.B, c.H, (int)a->n,
-                  (int)a->keep, (int)a->sink, (int)a->recent};
+                  (int)a->keep, (int)a->sink, (int)a->recent, workspace, 0, 0};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    if (a->n <= SEL_LDS) {
+    if (need == 0) {
         // whole steps of every wave, and the reads ahead of the last one
         const size_t smem = (size_t)(cdiv(a->n, SEL_THREADS) * SEL_THREADS + 64 * SEL_AHEAD) * 4;
-        if ((rc = set_smem(select_kernel<true>, smem))) return rc;
-        select_kernel<true><<<(unsigned)(c.B * c.H), SEL_THREADS, smem, s>>>(p);
+        if ((rc = set_smem(select_kernel, smem))) return rc;
+        select_kernel<<<(unsigned)(c.B * c.H), SEL_THREADS, smem, s>>>(p);
     } else {
-        select_kernel<false><<<(unsigned)(c.B * c.H), SEL_THREADS, 0, s>>>(p);
+        p.part_rows = part_rows(a->n);
+        p.parts = evict_parts(a->n);
+        const unsigned grid = (unsigned)(c.B * c.H * p.parts);
+        part_kernel<0><<<grid, SEL_THREADS, 0, s>>>(p);
+        part_kernel<1><<<grid, SEL_THREADS, 0, s>>>(p);
+        part_kernel<2><<<grid, SEL_THREADS, 0, s>>>(p);
+        part_kernel<3><<<grid, SEL_THREADS, 0, s>>>(p);
     }
     NKV_LAUNCH_CHECK();
     const int64_t blocks = cdiv(std::min(a->keep, a->n), C8_BLOCK);

@@ -1591,14 +1591,16 @@ def cache8_mass(q: torch.Tensor, cache: Cache8, lse: torch.Tensor, mass: torch.T
 
 
 def cache8_evict(cache: Cache8, mass: torch.Tensor, length, out: Cache8, out_mass: torch.Tensor,
-                 *, keep: int, sink: int = 0, recent: int = 0, max_length: Optional[int] = None):
+                 *, keep: int, sink: int = 0, recent: int = 0, max_length: Optional[int] = None,
+                 workspace: Optional[torch.Tensor] = None):
     """Evicts the tokens of least mass, head by head (see nkv_cache8_evict).
 
     Of a sequence longer than keep, each head keeps its first `sink` rows, its
     last `recent` and those of the largest mass [B, H, cap] between, in order;
     they go to the front of `out` (another cache, cap >= keep) and their masses
     to out_mass [B, H, out.cap].  Returns (rows [B, H, keep] int32: the rows
-    kept, -1 past the last; lengths [B] int32)."""
+    kept, -1 past the last; lengths [B] int32).  workspace: optional uint8 buffer
+    of nkv_cache8_evict_workspace_size bytes (none up to 32,768 rows)."""
     device = _require_gpu(cache.k, cache.v, cache.k_scale, cache.v_scale, mass, out.k, out.v,
                           out.k_scale, out.v_scale, out_mass,
                           length if isinstance(length, torch.Tensor) else None)
@@ -1615,5 +1617,6 @@ def cache8_evict(cache: Cache8, mass: torch.Tensor, length, out: Cache8, out_mas
     left = torch.empty((c.B,), device=device, dtype=torch.int32)
     a = NkvCache8EvictArgs(c, o, mass.data_ptr(), out_mass.data_ptr(), rows.data_ptr(),
                            left.data_ptr(), at, n, keep, int(sink), int(recent))
-    _cache8_call("nkv_cache8_evict", device, byref(a))
+    scratch, nbytes = _cache8_scratch("nkv_cache8_evict_workspace_size", a, device, workspace)
+    _cache8_call("nkv_cache8_evict", device, byref(a), _ptr(scratch), nbytes)
     return rows, left

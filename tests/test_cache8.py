@@ -81,7 +81,7 @@ def test_bad_caches(kw, code, text):
     refused("nkv_cache8_write", write_args(cache=c), code, text)
     refused("nkv_cache8_attend", attend_args(cache=c), code, text, None, 0)
     refused("nkv_cache8_mass", attend_args(_lib.NkvCache8MassArgs, cache=c), code, text, None, 0)
-    refused("nkv_cache8_evict", evict_args(cache=c), code, text)
+    refused("nkv_cache8_evict", evict_args(cache=c), code, text, None, 0)
 
 
 @pytest.mark.parametrize("kw,code,text", [
@@ -141,6 +141,16 @@ def test_workspace_sizes_and_alignment():
     need = lib.nkv_cache8_mass_workspace_size(ctypes.byref(m))
     assert need > 0 and need % (1024 * 4) == 0
     refused("nkv_cache8_mass", m, _lib.NKV_ERR_INVALID, b"aligned", PTR + 2, need)
+    for n, parts in ((32768, 0), (32832, 5), (1 << 20, 64), (1 << 29, 64)):
+        e = evict_args(cache=cache(B=1, H=1, cap=n, at=1 << 44), n=n, keep=64)
+        e.cache.v, e.cache.k_scale, e.cache.v_scale, e.mass = 2 << 44, 3 << 44, 4 << 44, 5 << 44
+        e.out, e.out_mass = cache(B=1, H=1, cap=64), PTR + (9 << 24)
+        need = lib.nkv_cache8_evict_workspace_size(ctypes.byref(e))
+        assert need == parts * (2 * 2048 * 4 + 16), lib.nkv_last_error()
+        if need:
+            refused("nkv_cache8_evict", e, _lib.NKV_ERR_INVALID, b"aligned", PTR + 8, need)
+            refused("nkv_cache8_evict", e, _lib.NKV_ERR_WORKSPACE, b"smaller", PTR, need - 1)
+            refused("nkv_cache8_evict", e, _lib.NKV_ERR_WORKSPACE, b"smaller", None, need)
 
 
 CALLS = r"""
@@ -162,14 +172,15 @@ def evict(cap, keep):
     a.out = _lib.NkvCache8(big, 2 * big, 3 * big, 4 * big, cap, 2, 2, 64, 0)
     a.cache.v, a.cache.k_scale, a.cache.v_scale = 5 * big, 6 * big, 7 * big
     a.mass, a.out_mass, a.rows, a.out_length = 8 * big, 9 * big, 10 * big, 11 * big
-    return lib.nkv_cache8_evict(None, ctypes.byref(a))
+    need = lib.nkv_cache8_evict_workspace_size(ctypes.byref(a))
+    return lib.nkv_cache8_evict(None, ctypes.byref(a), t.PTR, need)
 
 # (call, launches, whether some take more than 64 KB)
 calls = [(lambda: attend(8, 4096, 1, 4), 2, False), (lambda: attend(512, 1024, 1, 4), 1, True),
          (lambda: attend(8, 4096, 1, 4, work=False), 1, False),
          (lambda: attend(8, 4096, 40, 1), 2, False), (lambda: attend(64, 8192, 40, 1), 2, True),
          (lambda: attend(24, 12480, 1560, 1), 2, True), (lambda: attend(24, 12480, 1560, 1, work=False), 1, True),
-         (lambda: evict(32768, 100), 2, True), (lambda: evict(40000 // 64 * 64, 100), 2, False)]
+         (lambda: evict(32768, 100), 2, True), (lambda: evict(40000 // 64 * 64, 100), 5, False)]
 for i, (call, n, large) in enumerate(calls):
     for dev in (0, 1, 0):
         shim.shim_device(dev)
@@ -222,7 +233,7 @@ def test_mass_refusals(kw, code, text):
     (dict(mass=PTR + (8 << 24) + 4), _lib.NKV_ERR_INVALID, b"mass must be 16"),
 ])
 def test_evict_refusals(kw, code, text):
-    refused("nkv_cache8_evict", evict_args(**kw), code, text)
+    refused("nkv_cache8_evict", evict_args(**kw), code, text, None, 0)
 
 
 def test_ctypes_structs_match_the_header_layout(tmp_path):

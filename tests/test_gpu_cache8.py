@@ -500,6 +500,65 @@ def test_evict_long_heads(dev):
     assert np.array_equal(out.k_scale.cpu().numpy(), rs) and np.array_equal(raw(out.k), rc)
 
 
+@pytest.mark.parametrize("n,lengths,keep,sink,recent", [
+    (33_000, [33_000, 32_769, 8_193, 100, 0], 100, 3, 20),       # parts that end inside, or never start
+    (40_000, [40_000, 24_576, 9_000], 9_000, 8_193, 300),        # the first rows pass a part
+    (70_000, [70_000, 65_537], 30_000, 10, 20_000),              # so do the last ones
+    (70_000, [70_000], 500, 200, 300),                           # none to choose
+    (70_000, [70_000, 69_999], 69_998, 0, 0),                    # one or two go
+    (600_001, [600_001], 150_000, 1, 1),                         # parts of more than one step
+])
+def test_evict_in_parts(dev, n, lengths, keep, sink, recent):
+    """Heads longer than one workgroup takes: rows, lengths and masses equal the
+    plain form's, nothing behind the workspace is written, and a captured call
+    replayed with new masses gives what an eager one gives."""
+    B, H = len(lengths), 4
+    cache = ops.Cache8.empty(B, H, n, 8, dev, "e4m3")
+    g = torch.Generator().manual_seed(81)
+    m = torch.rand((B, H, cache.cap), generator=g)
+    m[:, 1] = (m[:, 1] * 7).floor() - 3             # equal masses in every part, zero of both signs
+    m[:, 1, ::2] = -m[:, 1, ::2]
+    m[:, 2] = 0.25
+    m[:, 2, 5::4096] = float("nan")
+    m[:, 2, 9::1000] = float("-inf")
+    m[:, 3, 11::777] = float("inf")
+    device_n = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    out = ops.Cache8.empty(B, H, keep, 8, dev, "e4m3")
+    out_m = torch.full((B, H, out.cap), -7.0, device=dev)
+    parts = -(-n // (8192 if n < 64 * 8192 else -(-n // 64 // 4096) * 4096))
+    need = B * H * parts * (2 * 2048 * 4 + 16)
+    work = torch.full((need + 4096,), 0x5a, dtype=torch.uint8, device=dev)
+    md = m.to(dev)
+
+    def call(**kw):
+        return ops.cache8_evict(cache, md, device_n, out, out_m, keep=keep, sink=sink,
+                                recent=recent, max_length=n, **kw)
+
+    with pytest.raises(RuntimeError, match="workspace"):
+        call(workspace=work[:need - 16])
+    rows, left = call(workspace=work[:need])
+    want = ref.evict(m.numpy(), lengths, keep, sink, recent)
+    assert left.tolist() == [min(x, keep) for x in lengths]
+    rows, kept = rows.cpu().numpy(), out_m.cpu().numpy()
+    for b in range(B):
+        for h in range(H):
+            w = np.asarray(want[b][h], np.int64)
+            assert np.array_equal(rows[b, h, :len(w)], w), (b, h)
+            assert (rows[b, h, len(w):] == -1).all()
+            assert np.array_equal(kept[b, h, :len(w)], m[b, h].numpy()[w], equal_nan=True)
+            assert (kept[b, h, len(w):] == -7.0).all()
+    assert (work[need:] == 0x5a).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for i in range(3):
+        md.copy_(m.roll(1000 * i + 1, 2))
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = call()
+        assert torch.equal(got[0], eager[0]) and torch.equal(got[1], eager[1])
+
+
 def test_calls_of_every_kernel_captured_and_replayed(dev):
     """Many rows, few rows over many blocks, the weight of many rows with a join
     and an eviction in one graph, replayed with new inputs and eager calls
