@@ -819,8 +819,9 @@ int nkv_cache8_write(void* stream, const nkv_cache8_write_args* args);
  *   lse  [B, H*G, Q] fp32 natural-log row log-sum-exp, or NULL
  * length: device [B], clamped to [0, n] (NULL: n for every item); n <= cap is
  * also what the work is divided by.  Scores, softmax and sums are fp32; the
- * probabilities are rounded to q's type for their product with the codes.
- * q and out are 16-byte aligned with strides divisible by 8.
+ * probabilities are rounded to fp16 for their product with the codes.
+ * q and out are 16-byte aligned with strides divisible by 8; out's rows do not
+ * overlap.
  */
 typedef struct nkv_cache8_attend_args {
     nkv_cache8 cache;

@@ -18,6 +18,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <utility>
 
 namespace nkv {
 namespace {
@@ -1163,6 +1164,16 @@ int check_attend(const nkv_cache8_attend_args* a) {
                 NKV_ERR_INVALID, "out must be 16-byte aligned with strides divisible by 8");
     // a launch has fewer than 2^32 threads
     NKV_REQUIRE(attend_plan(a).items <= 1 << 22, NKV_ERR_UNSUPPORTED, "too many query rows");
+    // every row of out lies past the end of those of the smaller strides
+    std::pair<int64_t, int64_t> dims[3] = {
+        {a->o_sb, a->cache.B}, {a->o_st, a->Q}, {a->o_sh, (int64_t)a->cache.H * a->G}};
+    std::sort(dims, dims + 3);
+    __int128 end = a->cache.D;
+    for (const auto& [stride, count] : dims) {
+        if (count == 1) continue;
+        NKV_REQUIRE(stride >= end, NKV_ERR_INVALID, "out's rows overlap");
+        end += (__int128)stride * (count - 1);
+    }
     return NKV_OK;
 }
 

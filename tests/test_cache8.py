@@ -41,6 +41,11 @@ def attend_args(cls=_lib.NkvCache8AttendArgs, **kw):
         a.lse, a.mass = PTR, PTR + (8 << 24)
     for k, v in kw.items():
         setattr(a, k, v)
+    if cls is _lib.NkvCache8AttendArgs:        # contiguous, where not given
+        c, heads = a.cache, a.cache.H * a.G
+        given = {k: kw[k] for k in ("o_sb", "o_st", "o_sh") if k in kw}
+        for k, v in {**dict(o_sb=a.Q * heads * c.D, o_st=heads * c.D, o_sh=c.D), **given}.items():
+            setattr(a, k, v)
     return a
 
 
@@ -126,6 +131,30 @@ def test_attend_refusals(kw, code, text):
     lib = _lib.lib()
     assert lib.nkv_cache8_attend_workspace_size(ctypes.byref(attend_args(**kw))) == 0
     assert text in lib.nkv_last_error()
+
+
+@pytest.mark.parametrize("strides,fits", [
+    ((64 * 6, 128, 64), True),               # [B, Q, H, D]
+    ((64 * 6, 64, 64 * 3), True),            # [B, H, Q, D]
+    ((64, 128, 64 * 6), True),               # [H, Q, B, D]
+    ((64 * 18, 64 * 6, 72), True),           # rows with columns between them
+    ((64 * 6, 0, 64), False), ((0, 128, 64), False), ((64 * 6, 128, 0), False),
+    ((64 * 6, 128, 56), False),              # a head's last columns are the next one's first
+    ((64 * 5, 128, 64), False),              # the last token is the next item's first
+    ((-64 * 6, 128, 64), False),
+])
+def test_attend_refuses_an_out_whose_rows_overlap(strides, fits):
+    """Several workgroups would write one row."""
+    kw = dict(zip(("o_sb", "o_st", "o_sh"), strides))
+    a = attend_args(Q=3, **kw)
+    lib = _lib.lib()
+    lib.nkv_cache8_attend_workspace_size(ctypes.byref(a))
+    assert (lib.nkv_last_error() == b"") == fits
+    if not fits:
+        refused("nkv_cache8_attend", a, _lib.NKV_ERR_INVALID, b"overlap", None, 0)
+    one = attend_args(cache=cache(B=1, H=1), Q=1, o_sb=0, o_st=0, o_sh=0)   # strides of one row
+    lib.nkv_cache8_attend_workspace_size(ctypes.byref(one))
+    assert lib.nkv_last_error() == b""
 
 
 def test_workspace_sizes_and_alignment():
