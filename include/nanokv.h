@@ -791,7 +791,8 @@ typedef struct nkv_cache8 {
  * cap]; counts (device, [B]; NULL: T for every item) says how many of an
  * item's rows are written.  Rows past cap are dropped where start or counts
  * are in device memory, and refused where start is not.
- * k and v are 16-byte aligned with strides divisible by 8.
+ * k and v are 16-byte aligned with strides divisible by 8; the cache's codes and
+ * scales do not overlap each other.
  */
 typedef struct nkv_cache8_write_args {
     nkv_cache8 cache;

@@ -34,6 +34,13 @@ int cache8_check(const nkv_cache8* c, const char* who) {
 
 namespace {
 
+struct Range {
+    uintptr_t lo, hi;
+    Range(const void* p, int64_t bytes)
+        : lo(reinterpret_cast<uintptr_t>(p)), hi(reinterpret_cast<uintptr_t>(p) + (uintptr_t)bytes) {}
+    bool meets(const Range& o) const { return lo < o.hi && o.lo < hi; }
+};
+
 // ---------------------------------------------------------------- write
 struct WriteParams {
     uint8_t* codes[2];            // K, V
@@ -634,13 +641,6 @@ __global__ void __launch_bounds__(256) compact_kernel(EvictParams p) {
     }
 }
 
-struct Range {
-    uintptr_t lo, hi;
-    Range(const void* p, int64_t bytes)
-        : lo(reinterpret_cast<uintptr_t>(p)), hi(reinterpret_cast<uintptr_t>(p) + (uintptr_t)bytes) {}
-    bool meets(const Range& o) const { return lo < o.hi && o.lo < hi; }
-};
-
 int evict_parts(int64_t n) { return (int)cdiv(n, part_rows(n)); }
 
 int check_evict(const nkv_cache8_evict_args* a) {
@@ -710,6 +710,13 @@ extern "C" int nkv_cache8_write(void* stream, const nkv_cache8_write_args* a) {
     NKV_REQUIRE((reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v)) % 16 == 0 &&
                     (a->k_sb | a->k_st | a->k_sh | a->v_sb | a->v_st | a->v_sh) % 8 == 0,
                 NKV_ERR_INVALID, "k and v must be 16-byte aligned with strides divisible by 8");
+    const int64_t heads = (int64_t)c.B * c.H, bytes = heads * c.cap * c8_pitch(c.D);
+    const Range out[4] = {{c.k, bytes}, {c.v, bytes}, {c.k_scale, heads * c.cap / 16},
+                          {c.v_scale, heads * c.cap / 16}};
+    for (int i = 1; i < 4; ++i)
+        for (int j = 0; j < i; ++j)
+            NKV_REQUIRE(!out[i].meets(out[j]), NKV_ERR_INVALID,
+                        "the cache's codes and scales overlap each other");
     WriteParams p{{(uint8_t*)c.k, (uint8_t*)c.v}, {c.k_scale, c.v_scale}, {a->k, a->v},
                   {a->k_sb, a->v_sb}, {a->k_st, a->v_st}, {a->k_sh, a->v_sh},
                   a->start_dev, a->counts, c.cap, a->start, a->T, c.B, c.H, c.D};

@@ -99,6 +99,10 @@ def test_bad_caches(kw, code, text):
     (dict(v=PTR + 4), _lib.NKV_ERR_INVALID, b"aligned"),
     (dict(v_st=100), _lib.NKV_ERR_INVALID, b"strides"),
     (dict(cache=cache(H=70000, B=1)), _lib.NKV_ERR_UNSUPPORTED, b"too many heads"),
+    (dict(cache=_lib.NkvCache8(PTR, PTR, PTR + (2 << 24), PTR + (3 << 24), 128, 2, 2, 64, 0)),
+     _lib.NKV_ERR_INVALID, b"overlap each other"),
+    (dict(cache=_lib.NkvCache8(PTR, PTR + (1 << 24), PTR + (2 << 24), PTR + (2 << 24) + 28, 128, 2, 2,
+                               64, 0)), _lib.NKV_ERR_INVALID, b"overlap each other"),
 ])
 def test_write_refusals(kw, code, text):
     refused("nkv_cache8_write", write_args(**kw), code, text)
