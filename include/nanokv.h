@@ -854,7 +854,7 @@ int nkv_cache8_attend(void* stream, const nkv_cache8_attend_args* args, void* wo
  * with lse of nkv_cache8_attend on the same arguments (a row with lse = -inf
  * adds nothing).  mass and out are [B, H, cap] fp32 and may be the same
  * array, whose entries past the length are then not touched (otherwise they
- * are copied).  Deterministic: no atomics.
+ * are copied).  Q = 0 adds nothing (lse may be NULL).  Deterministic: no atomics.
  */
 typedef struct nkv_cache8_mass_args {
     nkv_cache8 cache;             /* v and v_scale are not read */

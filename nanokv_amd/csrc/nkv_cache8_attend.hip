@@ -1040,7 +1040,8 @@ __global__ void __launch_bounds__(256, 2) mass_tile_kernel(MassParams p) {
     mass_store(p, bh, (int64_t)key0 + 32 * (l32 >> 4) + 8 * (e >> 2) + 4 * hf + (e & 3), len, split, x);
 }
 
-// Joins the row splits' partial sums, in their order.
+// Joins the row splits' partial sums, in their order.  (With n = 0 it copies mass to
+// out: the weight of no queries.)
 __global__ void __launch_bounds__(256) mass_join_kernel(MassParams p) {
     const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int bh = blockIdx.y;
@@ -1390,6 +1391,15 @@ extern "C" int nkv_cache8_mass(void* stream, const nkv_cache8_mass_args* a, void
     // in place, blocks past n have nothing to do
     p.blocks = (int)(p.out == p.mass ? cdiv(a->n, C8_BLOCK) : c.cap / C8_BLOCK);
     if (p.blocks == 0) return NKV_OK;
+    const dim3 join((unsigned)cdiv((int64_t)p.blocks * C8_BLOCK, 256), (unsigned)(c.B * c.H));
+    if (a->Q == 0) {  // the kernels take a row at least
+        if (p.out == p.mass) return NKV_OK;
+        p.n = 0;
+        p.length = nullptr;
+        mass_join_kernel<<<join, 256, 0, reinterpret_cast<hipStream_t>(stream)>>>(p);
+        NKV_LAUNCH_CHECK();
+        return NKV_OK;
+    }
     p.per = pl.tile ? 1 : (int)std::min<int64_t>(8, std::max<int64_t>(1, (int64_t)c.B * c.H * p.blocks / MASS_WAVES));
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     dispatch(a->dtype, c.format, c.D, [&](auto t, auto f, auto w) {
@@ -1397,8 +1407,7 @@ extern "C" int nkv_cache8_mass(void* stream, const nkv_cache8_mass_args* a, void
     });
     NKV_LAUNCH_CHECK();
     if (pl.splits > 1) {
-        const dim3 grid((unsigned)cdiv((int64_t)p.blocks * C8_BLOCK, 256), (unsigned)(c.B * c.H));
-        mass_join_kernel<<<grid, 256, 0, s>>>(p);
+        mass_join_kernel<<<join, 256, 0, s>>>(p);
         NKV_LAUNCH_CHECK();
     }
     return NKV_OK;

@@ -1,0 +1,54 @@
+"""Calls of the 8-bit cache at the edges of what is allowed, without a GPU: the
+library runs over stand-ins for the HIP calls, which count its launches."""
+import ctypes
+import shutil
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+
+from tests.test_device_attributes import SHIM
+
+ROOT = Path(__file__).resolve().parent.parent
+
+HEAD = r"""
+import ctypes, sys
+shim = ctypes.CDLL(sys.argv[1], mode=ctypes.RTLD_GLOBAL)   # before the library: its symbols come first
+sys.path.insert(0, ".")
+from nanokv_amd import _lib
+from tests import test_cache8 as t
+lib = _lib.lib()
+
+def launches(name, args, *more):
+    shim.shim_device(0)
+    rc = getattr(lib, name)(None, ctypes.byref(args), *more)
+    assert rc == 0, (rc, lib.nkv_last_error())
+    return shim.shim_launches()
+"""
+
+
+def over_stand_ins(tmp_path, code):
+    if shutil.which("gcc") is None:
+        pytest.skip("needs a C compiler")
+    src, so = tmp_path / "shim.c", tmp_path / "libshim.so"
+    src.write_text(SHIM)
+    subprocess.run(["gcc", "-shared", "-fPIC", "-O1", str(src), "-o", str(so)], check=True)
+    run = subprocess.run([sys.executable, "-c", HEAD + code + "\nprint('ok')", str(so)],
+                         capture_output=True, text=True, cwd=ROOT, timeout=120)
+    assert run.returncode == 0 and run.stdout.strip() == "ok", run.stdout + run.stderr
+
+
+def test_no_query_rows_launch_no_attention(tmp_path):
+    """The weight of no queries: nothing in place, one copy into another array."""
+    over_stand_ins(tmp_path, r"""
+for causal in (0, 1):
+    a = t.attend_args(_lib.NkvCache8MassArgs, Q=0, q=None, lse=None, causal=causal)
+    assert lib.nkv_cache8_mass_workspace_size(ctypes.byref(a)) == 0
+    a.out = a.mass
+    assert launches("nkv_cache8_mass", a, None, 0) == 0
+    a.out = t.PTR + (12 << 24)
+    assert launches("nkv_cache8_mass", a, None, 0) == 1
+    assert launches("nkv_cache8_attend", t.attend_args(Q=0, q=None, out=None, causal=causal),
+                    None, 0) == 0
+""")
