@@ -61,6 +61,15 @@ __device__ __forceinline__ RowAt row_at(int row, int hk, int G, int Q) {
     return {r / G, hk * G + r % G, there};
 }
 
+// log2 of a block's value scale in a wave whose unit is `unit`.  The sum of the
+// softmax is taken from the weights, which carry 2^(lsv - unit): it is at most
+// 2^-QUIET, so that they stay normal numbers down to 2^(z - m) = 2^-78 and the sum
+// does not depend on the values.  Weights of quieter blocks are zero in fp16 anyway.
+constexpr float QUIET = 60.0f;
+__device__ __forceinline__ float value_log2(float sv, float unit) {
+    return fmaxf(__builtin_amdgcn_logf(sv), unit - QUIET);
+}
+
 // The work of a workgroup: a group of query rows of a unit (head and key split).
 // Block i runs on XCD i % 8, and the groups of a unit take consecutive slots of
 // one XCD, whose L2 then serves all but the first read of its codes.  Units go
@@ -267,7 +276,8 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
                             for (int w = 0; w < DB / 4; ++w) vr[c][j][w] = 0;
             }
         }
-        const float c = p.scale_log2 * sk, lsv = __builtin_amdgcn_logf(sv);
+        const float c = p.scale_log2 * sk;
+        const float lsv = value_log2(sv, unit);
         if (lsv > unit) {
             const float f = __builtin_amdgcn_exp2f(unit - lsv);
 #pragma unroll
@@ -556,7 +566,7 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
             __builtin_amdgcn_s_setprio(0);
         }
         const float c = p.scale_log2 * fmaxf(sk, SCALE_MIN);
-        const float lsv = __builtin_amdgcn_logf(fmaxf(sv, SCALE_MIN));
+        const float lsv = value_log2(fmaxf(sv, SCALE_MIN), unit);
         // block blk + 1 (behind the last, the last again, for no one)
         codes.store(smem + (kslot ^ 1) * Codes::K_BYTES,
                     smem + 2 * Codes::K_BYTES + next * Codes::V_BYTES,

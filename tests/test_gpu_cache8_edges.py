@@ -28,3 +28,32 @@ def test_mass_of_no_queries_is_the_mass(dev, fmt, causal):
     assert ops.cache8_mass(q, cache, lse, m, n, causal=causal) is m
     for t in (m, other):
         assert np.array_equal(t.cpu().numpy().view(np.uint32), was)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Q,N", [(1, 700), (9, 700), (100, 700), (1, 8000), (100, 8000)])
+@pytest.mark.parametrize("loud", [2.0 ** 40, 2.0 ** 76, 2.0 ** 100, 1e38])
+def test_log_sums_do_not_depend_on_the_values(dev, dtype, loud, Q, N):
+    """Values of any finite size beside blocks of zeros, as the write takes them:
+    the log sums are those of the keys, the outputs finite numbers."""
+    g = torch.Generator().manual_seed(102)
+    k, v = torch.randn((2, 1, N, 2, 64), generator=g).to(dev)
+    v[:, :64] *= loud / v[:, :64].abs().max()
+    v[:, 128:192] = 0
+    v[:, 256:320] = 0                         # (the first block's wave, where it has two)
+    v[:, -65:] = 0
+    cache = ops.Cache8.empty(1, 2, N, 64, dev, "int8")
+    ops.cache8_write(cache, k, v, 0)
+    q = torch.randn((1, Q, 4, 64), generator=g).to(dtype).to(dev)
+    out, lse = ops.cache8_attend(q, cache, N)
+    if dtype == torch.bfloat16:
+        check_attend(q, cache, "int8", [N], False, out, lse)
+    else:                                     # (outputs beyond the type's range are infinite)
+        assert not torch.isnan(out).any()
+    cv = cache_values(cache, "int8")
+    _, rl, _, ltol = ref.attend(q.double().cpu().numpy(), cv[0], cv[1] / loud, [N], False, 0.125, 2.0 ** -8)
+    assert (np.abs(lse.double().cpu().numpy() - rl) <= ltol).all()
+    # as those beside even values are
+    quiet = ops.Cache8(cache.k, cache.v, cache.k_scale, torch.ones_like(cache.v_scale), 64)
+    _, l2 = ops.cache8_attend(q, quiet, N)
+    assert (np.abs(l2.double().cpu().numpy() - rl) <= ltol).all()
