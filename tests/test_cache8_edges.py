@@ -8,6 +8,7 @@ from pathlib import Path
 
 import pytest
 
+from nanokv_amd import build
 from tests.test_device_attributes import SHIM
 
 ROOT = Path(__file__).resolve().parent.parent
@@ -52,3 +53,9 @@ for causal in (0, 1):
     assert launches("nkv_cache8_attend", t.attend_args(Q=0, q=None, out=None, causal=causal),
                     None, 0) == 0
 """)
+
+
+def test_the_attention_is_compiled_with_nans():
+    """What a NaN query does to its own row is documented, so no flag may let the
+    compiler take NaN for impossible there."""
+    assert not [f for f in build.SOURCES["nkv_cache8_attend.hip"] if "nan" in f or "fast" in f]

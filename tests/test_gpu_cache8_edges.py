@@ -57,3 +57,22 @@ def test_log_sums_do_not_depend_on_the_values(dev, dtype, loud, Q, N):
     quiet = ops.Cache8(cache.k, cache.v, cache.k_scale, torch.ones_like(cache.v_scale), 64)
     _, l2 = ops.cache8_attend(q, quiet, N)
     assert (np.abs(l2.double().cpu().numpy() - rl) <= ltol).all()
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("fmt,D,Q,N,H", [("int8", 128, 1, 700, 2), ("e4m3", 64, 7, 20_000, 1),
+                                         ("e4m3", 128, 5, 4096, 40), ("int8", 64, 20, 16_384, 8),
+                                         ("e4m3", 64, 90, 300, 1), ("int8", 128, 90, 9000, 1)])
+def test_queries_that_are_not_finite_stay_in_their_rows(dev, fmt, D, Q, N, H, value):
+    """In every kernel, with key splits and without: the row is NaN, and no other."""
+    cache = make_cache(dev, 1, H, N, D, fmt, 105, [N])
+    q = torch.randn((1, Q, 2 * H, D), generator=torch.Generator().manual_seed(106)).bfloat16().to(dev)
+    bad = q.clone()
+    bad[0, Q // 2, 1, 5] = value
+    keep = torch.ones((Q, 2 * H), dtype=torch.bool, device=dev)
+    keep[Q // 2, 1] = False
+    for work in (None, torch.zeros(16, dtype=torch.uint8, device=dev)):
+        clean, lse = ops.cache8_attend(q, cache, N, workspace=work)
+        out, l2 = ops.cache8_attend(bad, cache, N, workspace=work)
+        assert torch.isnan(out[0, Q // 2, 1]).all() and torch.isnan(l2[0, 1, Q // 2])
+        assert torch.equal(out[0][keep], clean[0][keep]) and torch.equal(l2[0].T[keep], lse[0].T[keep])
