@@ -819,8 +819,11 @@ int nkv_cache8_write(void* stream, const nkv_cache8_write_args* args);
  *   out  [B, Q, H*G, D] of q's type (o_sb/o_st/o_sh)
  *   lse  [B, H*G, Q] fp32 natural-log row log-sum-exp, or NULL
  * length: device [B], clamped to [0, n] (NULL: n for every item); n <= cap is
- * also what the work is divided by.  Scores, softmax and sums are fp32; the
- * probabilities are rounded to fp16 for their product with the codes.
+ * also what the work is divided by.  Scores, softmax and sums are fp32; for
+ * their product with the codes the weights p * v_scale are rounded to fp16,
+ * relative to the row's largest one (11 bits down to 2^-26 of it, multiples of
+ * 2^-36 of it below): values that a row does not see, or gives no weight to,
+ * do not change its result beyond the order of its sums.
  * q and out are 16-byte aligned with strides divisible by 8; out's rows do not
  * overlap.
  */

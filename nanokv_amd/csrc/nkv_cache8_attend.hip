@@ -9,10 +9,14 @@
 // The weights p * sv of the second product are rounded to fp16 whatever the
 // queries' type: with bf16 their rounding is as large as the output's own (2^-9
 // relative; over 262,144 keys the output was 0.0026 off in norm where its own
-// rounding makes 0.0017).  fp16's range is enough because they are held in
-// units: w = 2^(z - m + LIFT) * sv / 2^unit, where unit is the log2 of the
-// largest sv so far and m is at most TAU below the row's maximum, is at most
-// 2^(LIFT + TAU) and keeps all 11 bits down to p = 2^-(14 + LIFT).
+// rounding makes 0.0017).  fp16's range is enough because a row's weights are held
+// relative to its own largest one: with m the row's running maximum of z and wm
+// that of z + log2 sv, over the keys it sees, and both at most TAU behind,
+//   w = 2^(z + log2 sv - wm + LIFT) <= 2^(LIFT + TAU)
+// keeps all 11 bits down to 2^-(14 + LIFT) of the largest weight and is a multiple
+// of 2^-(24 + LIFT) of it below.  A loud block that a row does not see, or gives no
+// weight to, costs the row nothing.  The softmax's sum is 2^(z - m)'s: the same
+// exponentials, multiplied back by what separates the two units.
 #include "nkv_cache8.h"
 
 #include <math.h>
@@ -27,7 +31,20 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr float TAU = 3.0f;           // a row's maximum is moved when it is off by 2^TAU
 constexpr float LIFT = 12.0f;         // 2^(LIFT + TAU) < 65504
+constexpr float FLOOR = -0x1p126f;    // a maximum before the first key (finite: no inf - inf)
+// A block's weights that lie more than this below the row's largest are taken as
+// 2^-QUIET of their 2^(z - m): they are zero in fp16 (2^(LIFT + TAU - QUIET) = 2^-25)
+// either way, and stay normal numbers for the sum.
+constexpr float QUIET = 40.0f;
 constexpr float SCALE_MIN = 0x1p-100f;  // keeps an unwritten block's scale out of log2(0)
+
+// A row's running statistics (log2 units): the maximum of z and the sum of 2^(z -
+// m); the maximum of z + log2 sv and the sum of 2^(z + log2 sv - wm + LIFT), in which
+// units the row's output is.
+struct alignas(16) Stat {
+    float m, l, wm, lw;
+};
+constexpr Stat NO_KEYS{FLOOR, 0.0f, FLOOR, 0.0f};
 
 struct AttendParams {
     const uint8_t* k;
@@ -38,10 +55,10 @@ struct AttendParams {
     const uint16_t* q;
     uint16_t* out;
     float* lse;
-    // partial results of the splits, [B*H][splits][rows]: the output in units of
-    // 2^unit, the maximum (log2), the sum and the unit
+    // partial results of the splits, [B*H][splits][rows]: the output over its sum of
+    // weights, and a Stat
     void* part;                   // [..][P] of T::Partial
-    f32x4* part_ml;
+    Stat* part_st;
     int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;
     int64_t cap, items;
     float scale_log2;
@@ -61,13 +78,21 @@ __device__ __forceinline__ RowAt row_at(int row, int hk, int G, int Q) {
     return {r / G, hk * G + r % G, there};
 }
 
-// log2 of a block's value scale in a wave whose unit is `unit`.  The sum of the
-// softmax is taken from the weights, which carry 2^(lsv - unit): it is at most
-// 2^-QUIET, so that they stay normal numbers down to 2^(z - m) = 2^-78 and the sum
-// does not depend on the values.  Weights of quieter blocks are zero in fp16 anyway.
-constexpr float QUIET = 60.0f;
-__device__ __forceinline__ float value_log2(float sv, float unit) {
-    return fmaxf(__builtin_amdgcn_logf(sv), unit - QUIET);
+// Whether a row's maxima are more than TAU behind a block's, tm and tm + lsv; where
+// they are (up), catch_up moves them there and gives what the output is multiplied
+// by.  (The tile kernel does it without a branch and scales its output behind the
+// exponentials: with both in a branch before them 70 us instead of 63 at width 64.)
+__device__ __forceinline__ bool behind(const Stat& st, float tm, float lsv) {
+    return tm > st.m + TAU || tm + lsv > st.wm + TAU;
+}
+__device__ __forceinline__ float catch_up(Stat& st, bool up, float tm, float lsv) {
+    const float m = up ? fmaxf(st.m, tm) : st.m, wm = up ? fmaxf(st.wm, tm + lsv) : st.wm;
+    const float alpha = __builtin_amdgcn_exp2f(st.wm - wm);
+    st.l *= __builtin_amdgcn_exp2f(st.m - m);
+    st.lw *= alpha;
+    st.m = m;
+    st.wm = wm;
+    return alpha;
 }
 
 // The work of a workgroup: a group of query rows of a unit (head and key split).
@@ -110,41 +135,41 @@ __device__ __forceinline__ void load_q(typename T::x8 (&qf)[P / 32], const uint1
     }
 }
 
-// Eight columns of a row's result: o is in units of 2^(U + LIFT) (a merge's:
-// 2^U, with `lift` 1), l its sum.
+// Eight columns of a row's result, o in units of 2^(wm - LIFT).
 template <typename T>
 __device__ __forceinline__ void store_row(const AttendParams& p, int b, int hk, int row, int d,
-                                          float M, float L, float U, const float (&o)[8],
-                                          float lift = 1.0f / 4096.0f) {
+                                          const Stat& st, const float (&o)[8]) {
     const RowAt at = row_at(row, hk, p.G, p.Q);
     if (!at.there) return;
-    const float f = L == 0.0f ? 0.0f : lift / L * __builtin_amdgcn_exp2f(U);
+    const float f = st.l == 0.0f ? 0.0f : 1.0f / 4096.0f / st.l;
+    const float u = __builtin_amdgcn_exp2f(st.wm - st.m);
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = o[k] * f * u;
     if (d < p.D)
         *reinterpret_cast<u32x4*>(p.out + b * p.o_sb + at.t * p.o_st + at.head * p.o_sh + d) =
-            u32x4{T::pack(o[0] * f, o[1] * f), T::pack(o[2] * f, o[3] * f),
-                  T::pack(o[4] * f, o[5] * f), T::pack(o[6] * f, o[7] * f)};
+            u32x4{T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(x[4], x[5]), T::pack(x[6], x[7])};
     if (d == 0 && p.lse)
         p.lse[((int64_t)b * p.H * p.G + at.head) * p.Q + at.t] =
-            L == 0.0f ? -INFINITY : M * LN2 + logf(L);  // (NaN for a NaN query)
+            st.l == 0.0f ? -INFINITY : st.m * LN2 + logf(st.l);  // (NaN for a NaN query)
 }
-static_assert(LIFT == 12.0f, "store_row's and store_partial's lift");
+static_assert(LIFT == 12.0f, "store_row's 4,096");
 
-// The same as one split's partial result, the output over its sum (at most the
-// largest code): in fp16 for bf16 outputs, where its rounding is an eighth of
-// theirs, in fp32 for fp16 ones.
+// The same as one split's partial result, the output over its sum of weights (at
+// most the largest code): in fp16 for bf16 outputs, where its rounding is an eighth
+// of theirs, in fp32 for fp16 ones.
 template <typename T, int P>
 __device__ __forceinline__ void store_partial(const AttendParams& p, int bh, int split, int row,
-                                              int d, float M, float L, float U,
-                                              const float (&o)[8]) {
+                                              int d, const Stat& st, const float (&o)[8]) {
     if (row >= p.rows) return;
     const int64_t i = ((int64_t)bh * p.splits + split) * p.rows + row;
-    const float f = L == 0.0f ? 0.0f : 1.0f / 4096.0f / L;
+    const float f = st.lw == 0.0f ? 0.0f : 1.0f / st.lw;
     if (d < P) {
         typename T::Partial x;
         x.set(o, f);
         x.store(p.part, i * P + d);
     }
-    if (d == 0) p.part_ml[i] = f32x4{M, L, U, 0.0f};
+    if (d == 0) p.part_st[i] = st;
 }
 
 // W waves of a workgroup share 16 query rows and a range of 64-row blocks; wave
@@ -163,8 +188,7 @@ constexpr int64_t ROWS_EIGHT = 2048;  // blocks in all heads
 template <int P, int W, int NQ>
 struct RowsSmem {
     float o[W][16 * NQ][P + 4];
-    float ml[W][16 * NQ][2];
-    float unit[W];
+    Stat st[W][16 * NQ];
 };
 
 // NQ groups of 16 query rows to a wave: with more than 16 rows two, for half the
@@ -206,11 +230,11 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
         for (int i = 0; i < DB; ++i) o[n][i] = f32x4{};
-    // m: the row's maximum (log2 units), l: its sum of 2^(z - m) over this
-    // lane's keys; o holds sum of 2^(z - m + LIFT) * sv * code in units of 2^unit
-    float m[NQ], l[NQ], unit = -INFINITY;
+    // the maxima of the lane's row, the sums over its own keys; o holds the sum of
+    // the weights times the codes
+    Stat st[NQ];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) m[n] = -INFINITY, l[n] = 0.0f;
+    for (int n = 0; n < NQ; ++n) st[n] = NO_KEYS;
     for (int blk = b0 + wave; blk < b1; blk += W) {
         const int64_t key0 = (int64_t)blk * C8_BLOCK;
         u32x4 kr[4][PIECES];
@@ -219,6 +243,9 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
 #pragma unroll
             for (int i = 0; i < PIECES; ++i)
                 kr[t][i] = *reinterpret_cast<const u32x4*>(kbase + (key0 + 16 * t) * P + 64 * i);
+        // (K's loads before V's: the scores wait for them alone; 30.4 us without the
+        // fence for the long call, 29.6 with it)
+        __builtin_amdgcn_sched_barrier(0);
         // V: lane (r, g) holds columns DB r .. + DB of the keys that its weights
         // are of: 32 c + 16 a + 4 g + j
         uint32_t vr[2][8][DB / 4];
@@ -276,18 +303,7 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
                             for (int w = 0; w < DB / 4; ++w) vr[c][j][w] = 0;
             }
         }
-        const float c = p.scale_log2 * sk;
-        const float lsv = value_log2(sv, unit);
-        if (lsv > unit) {
-            const float f = __builtin_amdgcn_exp2f(unit - lsv);
-#pragma unroll
-            for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                for (int i = 0; i < DB; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[n][i][e] *= f;
-            unit = lsv;
-        }
+        const float c = p.scale_log2 * sk, lsv = __builtin_amdgcn_logf(sv);
         uint32_t pw[NQ][2][4];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
@@ -297,11 +313,16 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) tm = fmaxf(tm, s[n][t][e]);
             tm = rows4_max(tm) * c;
-            const bool up = tm > m[n] + TAU;
-            const float mn = up ? tm : m[n];
-            const float alpha = up ? __builtin_amdgcn_exp2f(m[n] - mn) : 1.0f;
-            m[n] = mn;
-            const float off = (mn == -INFINITY ? 0.0f : mn) + (unit - lsv) - LIFT;
+            const bool up = behind(st[n], tm, lsv);
+            if (__any(up)) {
+                const float alpha = catch_up(st[n], up, tm, lsv);
+#pragma unroll
+                for (int i = 0; i < DB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[n][i][e] *= alpha;
+            }
+            const float apart = fminf(st[n].wm - lsv - st[n].m, QUIET) - LIFT;
+            const float off = st[n].m + apart;
             float lsum = 0.0f;
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -314,13 +335,8 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
                 pw[n][t >> 1][2 * (t & 1)] = Fp16::pack(w[0], w[1]);
                 pw[n][t >> 1][2 * (t & 1) + 1] = Fp16::pack(w[2], w[3]);
             }
-            l[n] = l[n] * alpha + lsum * __builtin_amdgcn_exp2f(unit - lsv - LIFT);
-            if (__any(up)) {
-#pragma unroll
-                for (int i = 0; i < DB; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[n][i][e] *= alpha;
-            }
+            st[n].l += lsum * __builtin_amdgcn_exp2f(apart);
+            st[n].lw += lsum;
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k)
@@ -353,38 +369,34 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
             for (int i = 0; i < DB; i += 4)
                 *reinterpret_cast<f32x4*>(&sm.o[wave][16 * n + r][DB * (4 * g + e) + i]) =
                     f32x4{o[n][i][e], o[n][i + 1][e], o[n][i + 2][e], o[n][i + 3][e]};
-        const float sum = rows4_sum(l[n]);
-        if (g == 0) {
-            sm.ml[wave][16 * n + r][0] = m[n];
-            sm.ml[wave][16 * n + r][1] = sum;
-        }
+        st[n].l = rows4_sum(st[n].l);
+        st[n].lw = rows4_sum(st[n].lw);
+        if (g == 0) sm.st[wave][16 * n + r] = st[n];
     }
-    if (lane == 0) sm.unit[wave] = unit;
     __syncthreads();
     if (threadIdx.x >= 16 * ROWS) return;
     for (int mr = threadIdx.x / 16; mr < ROWS; mr += 4 * W) {
         const int d = (threadIdx.x % 16) * 8;
-        float M = -INFINITY, U = -INFINITY;
+        Stat all = NO_KEYS;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            M = fmaxf(M, sm.ml[w][mr][0]);
-            U = fmaxf(U, sm.unit[w]);
+            all.m = fmaxf(all.m, sm.st[w][mr].m);
+            all.wm = fmaxf(all.wm, sm.st[w][mr].wm);
         }
-        float L = 0.0f, acc[8] = {};
+        float acc[8] = {};
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            // (a wave that saw no key has zero sums, or with a NaN query NaN ones)
-            const float mw = sm.ml[w][mr][0], uw = sm.unit[w];
-            const float a = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - M);
-            L += a * sm.ml[w][mr][1];
-            const float f = uw == -INFINITY ? 0.0f : a * __builtin_amdgcn_exp2f(uw - U);
+            const Stat one = sm.st[w][mr];
+            all.l += __builtin_amdgcn_exp2f(one.m - all.m) * one.l;
+            const float f = __builtin_amdgcn_exp2f(one.wm - all.wm);
+            all.lw += f * one.lw;
             if (d < P)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) acc[i] += f * sm.o[w][mr][d + i];
         }
         const int row = row0 + mr;
-        if (p.splits > 1) store_partial<T, P>(p, bh, split, row, d, M, L, U, acc);
-        else store_row<T>(p, b, hk, row, d, M, L, U, acc);
+        if (p.splits > 1) store_partial<T, P>(p, bh, split, row, d, all, acc);
+        else store_row<T>(p, b, hk, row, d, all, acc);
     }
 }
 
@@ -517,7 +529,7 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
     f32x16 o[DB];
 #pragma unroll
     for (int i = 0; i < DB; ++i) o[i] = f32x16{};
-    float m = -INFINITY, l = 0.0f, unit = -INFINITY;
+    Stat st = NO_KEYS;
     Codes codes;
     float sk = 1.0f, sv = 1.0f;  // scales of the current block
     if (b0 < b1) {
@@ -566,7 +578,7 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
             __builtin_amdgcn_s_setprio(0);
         }
         const float c = p.scale_log2 * fmaxf(sk, SCALE_MIN);
-        const float lsv = value_log2(fmaxf(sv, SCALE_MIN), unit);
+        const float lsv = __builtin_amdgcn_logf(fmaxf(sv, SCALE_MIN));
         // block blk + 1 (behind the last, the last again, for no one)
         codes.store(smem + (kslot ^ 1) * Codes::K_BYTES,
                     smem + 2 * Codes::K_BYTES + next * Codes::V_BYTES,
@@ -583,25 +595,16 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
                     for (int i = 0; i < 16; ++i)
                         if (32 * j + 8 * (i >> 2) + 4 * hf + (i & 3) >= seen) s[j][i] = -INFINITY;
             }
-            if (lsv > unit) {
-                const float f = __builtin_amdgcn_exp2f(unit - lsv);
-#pragma unroll
-                for (int i = 0; i < DB; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[i][e] *= f;
-                unit = lsv;
-            }
             float tm = s[0][0];
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) tm = fmaxf(tm, s[j][i]);
             tm = halfwave_max(tm) * c;
-            const bool up = tm > m + TAU;
-            const float mn = up ? tm : m;
-            const float alpha = up ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
-            m = mn;
-            const float off = (mn == -INFINITY ? 0.0f : mn) + (unit - lsv) - LIFT;
+            const bool up = behind(st, tm, lsv);
+            const float alpha = catch_up(st, up, tm, lsv);
+            const float apart = fminf(st.wm - lsv - st.m, QUIET) - LIFT;
+            const float off = st.m + apart;
             float lsum = 0.0f;
             uint32_t pw[2][8];
 #pragma unroll
@@ -613,7 +616,8 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
                     lsum += w0 + w1;
                     pw[j][i >> 1] = Fp16::pack(w0, w1);
                 }
-            l = l * alpha + lsum * __builtin_amdgcn_exp2f(unit - lsv - LIFT);
+            st.l += lsum * __builtin_amdgcn_exp2f(apart);
+            st.lw += lsum;
             __builtin_amdgcn_s_setprio(1);
             if (__any(up)) {
 #pragma unroll
@@ -649,7 +653,8 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
         slot = next;
         if (!lag) lds_barrier();
     }
-    l = halfwave_sum(l);
+    st.l = halfwave_sum(st.l);
+    st.lw = halfwave_sum(st.lw);
     if (!active) return;
 #pragma unroll
     for (int i = 0; i < DB; ++i)
@@ -659,13 +664,14 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
             float x[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) x[k] = o[i][8 * e + k];
-            if (p.splits > 1) store_partial<T, P>(p, bh, split, row, d, m, l, unit, x);
-            else store_row<T>(p, b, hk, row, d, m, l, unit, x);
+            if (p.splits > 1) store_partial<T, P>(p, bh, split, row, d, st, x);
+            else store_row<T>(p, b, hk, row, d, st, x);
         }
 }
 
 // The merge of the splits' partial results: P / 8 threads a row and group of
-// splits, eight columns each; out = sum a 2^unit o / sum a with a = 2^(m - M) l.
+// splits, eight columns each; with M and W the largest m and wm, out = 2^(W - M - LIFT)
+// sum(2^(wm - W) lw o) / sum(2^(m - M) l).
 // SG groups share a row's splits and are joined in LDS; a thread has AHEAD
 // splits' loads in flight.  37,440 rows of 3 splits (30 MB) 7.8 us, 16 rows of 256
 // 4.5 us (309 us with one thread walking all of a row's splits).
@@ -677,38 +683,40 @@ __global__ void __launch_bounds__(256) merge_kernel(AttendParams p) {
     const int b = blockIdx.z, hk = blockIdx.y;
     const bool in = row < p.rows;
     const int64_t first = ((int64_t)b * p.H + hk) * p.splits * p.rows + row;
-    float M = -INFINITY, U = -INFINITY, L = 0.0f, acc[8] = {};
+    Stat all = NO_KEYS;
+    float acc[8] = {};
+    // (a thread without splits, or with those of no keys, adds zeros)
+    auto grow = [&](float m, float wm) {
+        const float f = __builtin_amdgcn_exp2f(all.wm - wm);
+        all.l *= __builtin_amdgcn_exp2f(all.m - m);
+        all.m = m;
+        all.wm = wm;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] *= f;
+    };
     if (in) {
         for (int s0 = sg; s0 < p.splits; s0 += SG * AHEAD) {
-            f32x4 ml[AHEAD];
+            Stat st[AHEAD];
             typename T::Partial x[AHEAD];
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
                 const int s = min(s0 + SG * j, p.splits - 1);
                 const int64_t i = first + (int64_t)s * p.rows;
-                ml[j] = p.part_ml[i];
+                st[j] = p.part_st[i];
                 x[j].load(p.part, i * P + d);
-                if (s0 + SG * j >= p.splits) ml[j] = f32x4{-INFINITY, 0.0f, -INFINITY, 0.0f};
+                if (s0 + SG * j >= p.splits) st[j] = NO_KEYS;
             }
-            float m1 = M, u1 = U;
+            float m1 = all.m, w1 = all.wm;
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
-                m1 = fmaxf(m1, ml[j][0]);
-                u1 = fmaxf(u1, ml[j][2]);
+                m1 = fmaxf(m1, st[j].m);
+                w1 = fmaxf(w1, st[j].wm);
             }
-            const float b0 = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - m1);
-            const float c0 = U == -INFINITY ? 0.0f : b0 * __builtin_amdgcn_exp2f(U - u1);
-            L *= b0;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) acc[k] *= c0;
-            M = m1;
-            U = u1;
+            grow(m1, w1);
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
-                const float a =
-                    (ml[j][0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[j][0] - M)) * ml[j][1];
-                L += a;
-                const float f = ml[j][2] == -INFINITY ? 0.0f : a * __builtin_amdgcn_exp2f(ml[j][2] - U);
+                all.l += __builtin_amdgcn_exp2f(st[j].m - all.m) * st[j].l;
+                const float f = __builtin_amdgcn_exp2f(st[j].wm - all.wm) * st[j].lw;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) acc[k] += f * x[j][k];
             }
@@ -721,31 +729,29 @@ __global__ void __launch_bounds__(256) merge_kernel(AttendParams p) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) sh[lr][sg][part][k] = acc[k];
         if (part == 0) {
-            sml[lr][sg][0] = M;
-            sml[lr][sg][1] = L;
-            sml[lr][sg][2] = U;
+            sml[lr][sg][0] = all.m;
+            sml[lr][sg][1] = all.l;
+            sml[lr][sg][2] = all.wm;
         }
         __syncthreads();
         if (sg) return;
 #pragma unroll
         for (int s = 0; s < SG; ++s) {
-            M = fmaxf(M, sml[lr][s][0]);
-            U = fmaxf(U, sml[lr][s][2]);
+            all.m = fmaxf(all.m, sml[lr][s][0]);
+            all.wm = fmaxf(all.wm, sml[lr][s][2]);
         }
-        L = 0.0f;
+        all.l = 0.0f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
 #pragma unroll
         for (int s = 0; s < SG; ++s) {
-            const float ms = sml[lr][s][0], us = sml[lr][s][2];
-            const float a = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - M);
-            L += a * sml[lr][s][1];
-            const float f = us == -INFINITY ? 0.0f : a * __builtin_amdgcn_exp2f(us - U);
+            all.l += __builtin_amdgcn_exp2f(sml[lr][s][0] - all.m) * sml[lr][s][1];
+            const float f = __builtin_amdgcn_exp2f(sml[lr][s][2] - all.wm);
 #pragma unroll
             for (int k = 0; k < 8; ++k) acc[k] += f * sh[lr][s][part][k];
         }
     }
-    if (in) store_row<T>(p, b, hk, row, d, M, L, U, acc, 1.0f);
+    if (in) store_row<T>(p, b, hk, row, d, all, acc);
 }
 
 // ---------------------------------------------------------------- mass
@@ -1150,7 +1156,7 @@ Plan attend_plan(const nkv_cache8_attend_args* a, size_t limit = SIZE_MAX) {
             pl.splits = (int)std::max<int64_t>(1, std::min(cdiv(slots, base), blocks / waves));
         pl.items = base * pl.splits;
     }
-    const size_t row = sizeof(f32x4) + c8_pitch(c.D) * (a->dtype == NKV_ROWS_FP16 ? 4 : 2);
+    const size_t row = sizeof(Stat) + c8_pitch(c.D) * (a->dtype == NKV_ROWS_FP16 ? 4 : 2);
     const size_t split = (size_t)heads * pl.rows * row;
     if (pl.splits > 1 && limit / split < (size_t)pl.splits) {
         pl.items /= pl.splits;
@@ -1159,8 +1165,8 @@ Plan attend_plan(const nkv_cache8_attend_args* a, size_t limit = SIZE_MAX) {
     }
     if (pl.splits > 1) {
         const size_t rows = (size_t)heads * pl.splits * pl.rows;
-        pl.ml = rows * sizeof(f32x4);
-        pl.part = rows * (row - sizeof(f32x4));
+        pl.ml = rows * sizeof(Stat);
+        pl.part = rows * (row - sizeof(Stat));
     }
     return pl;
 }
@@ -1253,7 +1259,7 @@ void dispatch(int dtype, int format, int D, F f) {
     }
 }
 static_assert(NKV_CACHE8_INT8 == 0 && NKV_CACHE8_E4M3 == 1, "dispatch");
-static_assert(sizeof(f32x4) == 16, "partials");
+static_assert(sizeof(Stat) == 16 && alignof(Stat) == 16, "partials");
 
 }  // namespace
 }  // namespace nkv
@@ -1285,7 +1291,7 @@ extern "C" int nkv_cache8_attend(void* stream, const nkv_cache8_attend_args* a, 
     p.q = (const uint16_t*)a->q;
     p.out = (uint16_t*)a->out;
     p.lse = a->lse;
-    p.part_ml = (f32x4*)workspace;
+    p.part_st = (Stat*)workspace;
     p.part = (char*)workspace + pl.ml;
     p.q_sb = a->q_sb, p.q_st = a->q_st, p.q_sh = a->q_sh;
     p.o_sb = a->o_sb, p.o_st = a->o_st, p.o_sh = a->o_sh;

@@ -76,3 +76,84 @@ def test_queries_that_are_not_finite_stay_in_their_rows(dev, fmt, D, Q, N, H, va
         out, l2 = ops.cache8_attend(bad, cache, N, workspace=work)
         assert torch.isnan(out[0, Q // 2, 1]).all() and torch.isnan(l2[0, 1, Q // 2])
         assert torch.equal(out[0][keep], clean[0][keep]) and torch.equal(l2[0].T[keep], lse[0].T[keep])
+def check_rows(q, cache, fmt, lengths, causal, out, lse):
+    """check_attend with a bound of the row's own: what a weight below fp16's normal
+    range is off by (2^-25, where the row's largest is at least 2^12) counts against
+    the largest weight that the row gives, not against the loudest value there is."""
+    D, B, Q = q.shape[3], q.shape[0], q.shape[1]
+    k, v = cache_values(cache, fmt)
+    half = 2.0 ** -8 if q.dtype == torch.bfloat16 else 2.0 ** -11
+    qd = q.double().cpu().numpy()
+    ro, rl, otol, ltol = ref.attend(qd, k, v, lengths, causal, D ** -0.5, half)
+    end = ref.visible(B, Q, lengths, causal)
+    top = np.repeat(np.nan_to_num(cache.v_scale.double().cpu().numpy()), 64, 2) * float(ref.TOP[fmt])
+    G = q.shape[2] // k.shape[1]
+    for b in range(B):
+        for h in range(q.shape[2]):
+            n = int(end[b].max())
+            hidden = np.arange(n)[None] >= end[b][:, None]
+            z = np.where(hidden, -np.inf, qd[b, :, h] @ k[b, h // G, :n].T * D ** -0.5)
+            w = np.exp(z - rl[b, h][:, None]) * top[b, h // G, :n]
+            mag = np.where(hidden, 0, np.abs(qd[b, :, h]) @ np.abs(k[b, h // G, :n]).T * D ** -0.5)
+            ez = (D + 4) * 2.0 ** -24 * mag + 2.0 ** -21
+            a = (w / top[b, h // G, :n])[:, :, None] * np.abs(v[b, h // G, :n])[None]
+            # the weight's two roundings, the score's, the output's, and a partial result's
+            # below fp16's normal range
+            otol[b, :, h] = (a * (2.0 ** -10 + 4 * ez)[:, :, None]).sum(1) * 1.01 \
+                + half * np.abs(ro[b, :, h]) + (n * 2.0 ** -37 * w.max(1) + 2.0 ** -25 * w.sum(1))[:, None] \
+                + (2.0 ** -25 if half == 2.0 ** -11 else 1e-30)
+            ltol[b, h] = 2 * (np.exp(z - rl[b, h][:, None]) * ez).sum(1) \
+                + 2.0 ** -22 * (np.abs(rl[b, h]) + 16)
+    got = out.double().cpu().numpy()
+    assert (np.abs(got - ro) <= otol).all(), np.max(np.abs(got - ro) / otol)
+    assert (np.abs(lse.double().cpu().numpy() - rl) <= ltol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Q,N", [(1, 700), (9, 700), (100, 700), (1, 8000), (9, 8000), (100, 8000)])
+@pytest.mark.parametrize("loud", [2.0 ** 20, 2.0 ** 28, 2.0 ** 40, 2.0 ** 90])
+def test_loud_values_without_weight_cost_nothing(dev, dtype, loud, Q, N):
+    """Blocks of very large values whose keys have next to no weight: outputs as
+    near as the values that count allow, with key splits and without."""
+    g = torch.Generator().manual_seed(103)
+    k, v = torch.randn((2, 1, N, 2, 64), generator=g).to(dev)
+    for first in (0, 256, N - 65):
+        v[:, first:first + 64] *= loud
+        k[:, first:first + 64] = 0
+        k[:, first:first + 64, :, 0] = -200.0              # a score of -200 below
+    cache = ops.Cache8.empty(1, 2, N, 64, dev, "int8")
+    ops.cache8_write(cache, k, v, 0)
+    q = torch.randn((1, Q, 4, 64), generator=g)
+    q[..., 0] = 8.0
+    q[..., 1:] *= 3                                        # weight on few keys
+    q = q.to(dtype).to(dev)
+    # (the last block holds loud and other values: its own scale is what it is)
+    cache.v_scale[:, :, (N - 65) // 64] = cache.v_scale[:, :, 1]
+    out, lse = ops.cache8_attend(q, cache, N)
+    check_rows(q, cache, "int8", [N], False, out, lse)
+    none = torch.zeros(16, dtype=torch.uint8, device=dev)  # no room for splits
+    out, lse = ops.cache8_attend(q, cache, N, workspace=none)
+    check_rows(q, cache, "int8", [N], False, out, lse)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("Q,G", [(60, 1), (150, 1), (150, 4)])
+def test_causal_rows_do_not_depend_on_later_values(dev, dtype, fmt, Q, G):
+    """Queries before a run of very large values: as near as if it were not there."""
+    g = torch.Generator().manual_seed(104)
+    N = 2018 + Q
+    k, v = torch.randn((2, 2, N, 1, 128), generator=g).to(dev)
+    k *= 3
+    v[:, N - Q // 2:] *= 2.0 ** 45
+    cache = ops.Cache8.empty(2, 1, N, 128, dev, fmt)
+    at = torch.tensor([0, 0], dtype=torch.int32, device=dev)
+    for first in range(0, N, 64):                          # (a block's scale is its own)
+        ops.cache8_write(cache, k[:, first:first + 64], v[:, first:first + 64], at)
+        at += 64
+    q = torch.randn((2, Q, G, 128), generator=g).to(dtype).to(dev)
+    out, lse = ops.cache8_attend(q, cache, N, causal=True)
+    seen = 2048 - 2018                                     # queries that see whole quiet blocks only
+    few = ops.cache8_attend(q[:, :seen], cache, N - Q + seen, causal=True)
+    check_rows(q[:, :seen], cache, fmt, [N - Q + seen] * 2, True, out[:, :seen], lse[:, :, :seen])
+    check_rows(q[:, :seen], cache, fmt, [N - Q + seen] * 2, True, *few)
