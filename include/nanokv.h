@@ -64,7 +64,7 @@
 extern "C" {
 #endif
 
-#define NKV_ABI_VERSION 9
+#define NKV_ABI_VERSION 10
 
 enum nkv_status {
     NKV_OK = 0,
@@ -815,7 +815,12 @@ int nkv_cache8_write(void* stream, const nkv_cache8_write_args* args);
  * over a cache: query head h reads key head h / G, softmax(q k^T *
  * softmax_scale) v over the item's first `length` rows; with causal, query t
  * sees the first length - Q + 1 + t of them (the queries are the last Q
- * tokens).  A query that sees no key gets out = 0 and lse = -inf.
+ * tokens).  counts (device [B], clamped to [0, Q]; NULL: Q for every item) is
+ * how many of an item's Q rows are queries, the first ones, as the rows that
+ * nkv_cache8_write takes (a batch padded on the right): with causal, query t
+ * then sees the first length - counts + 1 + t rows, and a row at or past counts
+ * sees none, whatever it holds.  A query that sees no key gets out = 0 and lse =
+ * -inf.
  *   out  [B, Q, H*G, D] of q's type (o_sb/o_st/o_sh)
  *   lse  [B, H*G, Q] fp32 natural-log row log-sum-exp, or NULL
  * length: device [B], clamped to [0, n] (NULL: n for every item); n <= cap is
@@ -841,6 +846,7 @@ typedef struct nkv_cache8_attend_args {
     float* lse;
     float softmax_scale;
     int causal;
+    const int32_t* counts;        /* device [B], or NULL */
 } nkv_cache8_attend_args;
 
 /* Bytes of workspace nkv_cache8_attend wants for these arguments (0 if none), for
@@ -873,6 +879,7 @@ typedef struct nkv_cache8_mass_args {
     float* out;
     float softmax_scale;
     int causal;
+    const int32_t* counts;        /* as nkv_cache8_attend's */
 } nkv_cache8_mass_args;
 
 /* Likewise for the partial sums of row splits (the same sums within rounding). */

@@ -13,7 +13,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libnanokv_hip.so"
 
-NKV_ABI_VERSION = 9
+NKV_ABI_VERSION = 10
 NKV_OK = 0
 NKV_ERR_INVALID = -1
 NKV_ERR_UNSUPPORTED = -2
@@ -231,6 +231,7 @@ class NkvCache8AttendArgs(Structure):
         ("q", c_void_p), ("q_sb", c_int64), ("q_st", c_int64), ("q_sh", c_int64),
         ("out", c_void_p), ("o_sb", c_int64), ("o_st", c_int64), ("o_sh", c_int64),
         ("lse", c_void_p), ("softmax_scale", c_float), ("causal", c_int),
+        ("counts", c_void_p),
     ]
 
 
@@ -240,7 +241,7 @@ class NkvCache8MassArgs(Structure):
         ("length", c_void_p),
         ("q", c_void_p), ("q_sb", c_int64), ("q_st", c_int64), ("q_sh", c_int64),
         ("lse", c_void_p), ("mass", c_void_p), ("out", c_void_p),
-        ("softmax_scale", c_float), ("causal", c_int),
+        ("softmax_scale", c_float), ("causal", c_int), ("counts", c_void_p),
     ]
 
 

@@ -52,6 +52,7 @@ struct AttendParams {
     const float* ks;
     const float* vs;
     const int32_t* length;
+    const int32_t* counts;
     const uint16_t* q;
     uint16_t* out;
     float* lse;
@@ -93,6 +94,21 @@ __device__ __forceinline__ float catch_up(Stat& st, bool up, float tm, float lsv
     st.m = m;
     st.wm = wm;
     return alpha;
+}
+
+// The queries of an item: `nq` of its Q rows, the last tokens of `len`.
+struct Queries {
+    int len, nq, causal;
+    // keys that query t < nq sees, and any row t
+    __device__ __forceinline__ int sees(int t) const { return causal ? len - nq + 1 + t : len; }
+    __device__ __forceinline__ int end(int t) const { return t >= nq ? 0 : sees(t); }
+    // the least and the most that any of the queries t0 .. t1 sees
+    __device__ __forceinline__ int least(int t0, int t1) const { return t1 >= nq ? 0 : sees(t0); }
+    __device__ __forceinline__ int most(int t0, int t1) const { return t0 >= nq ? 0 : sees(min(t1, nq - 1)); }
+};
+template <typename Params>
+__device__ __forceinline__ Queries queries_of(const Params& p, int b) {
+    return {c8_length(p.length, b, p.n), c8_length(p.counts, b, p.Q), p.causal};
 }
 
 // The work of a workgroup: a group of query rows of a unit (head and key split).
@@ -203,12 +219,12 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
     if (!it.there) return;
     const int rg = it.group, bh = (int)(it.unit / (uint32_t)p.splits);
     const int split = (int)(it.unit - (uint32_t)bh * p.splits), b = bh / p.H, hk = bh - b * p.H;
-    const int len = c8_length(p.length, b, p.n);
+    const Queries qs = queries_of(p, b);
+    const int len = qs.len;
     const int row0 = rg * ROWS;
-    // blocks that the group's last row sees
-    const int last_t = min(row0 + ROWS - 1, p.rows - 1) / p.G;
-    const int last = max(0, p.causal ? len - p.Q + 1 + last_t : len);
-    const int first = p.causal ? len - p.Q + 1 + row0 / p.G : len;  // what its first row sees
+    // blocks that some row of the group sees, and keys that every row does
+    const int t0 = row0 / p.G, t1 = min(row0 + ROWS - 1, p.rows - 1) / p.G;
+    const int last = max(0, qs.most(t0, t1)), first = qs.least(t0, t1);
     const int nb = (last + C8_BLOCK - 1) / C8_BLOCK;
     const int b0 = (int)((int64_t)split * nb / p.splits);
     const int b1 = (int)((int64_t)(split + 1) * nb / p.splits);
@@ -217,7 +233,7 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         const RowAt mine = row_at(row0 + 16 * n + r, hk, p.G, p.Q);
-        end[n] = !mine.there ? 0 : p.causal ? len - p.Q + 1 + mine.t : len;
+        end[n] = mine.there ? qs.end(mine.t) : 0;
         load_q<T, P>(qf[n], p.q + b * p.q_sb + mine.t * p.q_st + mine.head * p.q_sh, mine.there, g,
                      p.D);
     }
@@ -497,20 +513,21 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
     const uint32_t BH = (uint32_t)(p.B * p.H);
     const int rg = it.group, split = (int)(it.unit / BH);
     const int bh = (int)(it.unit - split * BH), b = bh / p.H, hk = bh - b * p.H;
-    const int len = c8_length(p.length, b, p.n);
+    const Queries qs = queries_of(p, b);
+    const int len = qs.len;
     const int row0 = rg * p.per_group * 32;
     const int rows_end = min(row0 + p.per_group * 32, p.rows);
-    // keys that the group's last row sees
-    const int last = max(0, p.causal ? len - p.Q + 1 + (rows_end - 1) / p.G : len);
+    // keys that some row of the group sees
+    const int last = max(0, qs.most(row0 / p.G, (rows_end - 1) / p.G));
     const int nb = (last + C8_BLOCK - 1) / C8_BLOCK;
     const int b0 = (int)((int64_t)split * nb / p.splits);
     const int b1 = (int)((int64_t)(split + 1) * nb / p.splits);
     const int wrow = row0 + 32 * wave, row = wrow + l32;
     const bool active = wrow < rows_end;
     const RowAt mine = row_at(row, hk, p.G, p.Q);
-    const int end = !mine.there ? 0 : p.causal ? len - p.Q + 1 + mine.t : len;
-    const int first = p.causal ? len - p.Q + 1 + wrow / p.G : len;  // what the wave's first row sees
-    const int wlast = p.causal ? len - p.Q + 1 + (min(wrow + 32, p.rows) - 1) / p.G : len;
+    const int end = mine.there ? qs.end(mine.t) : 0;
+    const int t0 = wrow / p.G, t1 = (min(wrow + 32, p.rows) - 1) / p.G;
+    const int first = qs.least(t0, t1), wlast = qs.most(t0, t1);  // of the wave
     x8 qf[KS];
     {
         const uint16_t* q = p.q + b * p.q_sb + mine.t * p.q_st + mine.head * p.q_sh;
@@ -759,6 +776,7 @@ struct MassParams {
     const uint8_t* k;
     const float* ks;
     const int32_t* length;
+    const int32_t* counts;
     const uint16_t* q;
     const float* lse;
     const float* mass;
@@ -840,18 +858,19 @@ __global__ void __launch_bounds__(256) mass_kernel(MassParams p) {
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int bh = blockIdx.y, b = bh / p.H, hk = bh - b * p.H;
-    const int len = c8_length(p.length, b, p.n);
+    const Queries qs = queries_of(p, b);
+    const int len = qs.len;
     // the row whose sum this lane ends up with, of tile r / 4
     const int mykey = 16 * (r >> 2) + 4 * g + (r & 3);
     const int64_t head = (int64_t)bh * p.cap;
     const float* ks = p.ks + (int64_t)bh * (p.cap / C8_BLOCK);
-    const int groups = (p.rows + 15) / 16;
+    const int groups = max(1, (qs.nq * p.G + 15) / 16);
     x8 qf[STEPS];
     float z;
     int end;
     auto load_group = [&](int rg) {
-        const RowAt mine = row_at(rg * 16 + r, hk, p.G, p.Q);
-        end = !mine.there ? 0 : p.causal ? len - p.Q + 1 + mine.t : len;
+        const RowAt mine = row_at(rg * 16 + r, hk, p.G, qs.nq);
+        end = mine.there ? qs.sees(mine.t) : 0;
         load_q<T, P>(qf, p.q + b * p.q_sb + mine.t * p.q_st + mine.head * p.q_sh, mine.there, g, p.D);
         z = mine.there ? p.lse[((int64_t)b * p.H * p.G + mine.head) * p.Q + mine.t] : -INFINITY;
     };
@@ -880,7 +899,7 @@ __global__ void __launch_bounds__(256) mass_kernel(MassParams p) {
         // the first group with a row that sees the block's first key
         int rg = 0;
         if (p.causal)
-            rg = (int)min((int64_t)max(0, key0 - (len - p.Q)) * p.G / 16, (int64_t)groups - 1);
+            rg = (int)min((int64_t)max(0, key0 - (len - qs.nq)) * p.G / 16, (int64_t)groups - 1);
         f32x4 sum[4] = {};
         for (;;) {
             if (groups > 1) load_group(rg);
@@ -935,9 +954,9 @@ struct MassRows {
     float off;
     int end;
     // rows row0 .. + 64: thread t brings chunks t % 4 + 4 i of row t / 4
-    __device__ __forceinline__ void load(const MassParams& p, int b, int hk, int len, int row0) {
+    __device__ __forceinline__ void load(const MassParams& p, const Queries& qs, int b, int hk, int row0) {
         const int part = threadIdx.x & 3;
-        const RowAt at = row_at(row0 + (threadIdx.x >> 2), hk, p.G, p.Q);
+        const RowAt at = row_at(row0 + (threadIdx.x >> 2), hk, p.G, qs.nq);
         const uint16_t* src = p.q + b * p.q_sb + at.t * p.q_st + at.head * p.q_sh;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
@@ -946,7 +965,7 @@ struct MassRows {
             if (at.there && d < p.D) q[i] = *reinterpret_cast<const u32x4*>(src + d);
         }
         off = at.there ? p.lse[((int64_t)b * p.H * p.G + at.head) * p.Q + at.t] : -INFINITY;
-        end = p.causal ? len - p.Q + 1 + at.t : len;
+        end = qs.sees(at.t);
     }
     __device__ __forceinline__ void store(unsigned char* buf, float* offs, int* ends) const {
         const int row = threadIdx.x >> 2, part = threadIdx.x & 3;
@@ -970,7 +989,8 @@ __global__ void __launch_bounds__(256, 2) mass_tile_kernel(MassParams p) {
     const int lane = threadIdx.x & 63, hf = lane >> 5, l32 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int bh = blockIdx.y, b = bh / p.H, hk = bh % p.H, split = blockIdx.z;
-    const int len = c8_length(p.length, b, p.n);
+    const Queries qs = queries_of(p, b);
+    const int len = qs.len;
     const int first_key = blockIdx.x * 4 * C8_BLOCK;    // of the workgroup
     const int blk = blockIdx.x * 4 + wave, key0 = blk * C8_BLOCK;
     if (first_key >= len) {
@@ -993,16 +1013,16 @@ __global__ void __launch_bounds__(256, 2) mass_tile_kernel(MassParams p) {
     const float c = p.scale_log2 * fmaxf(p.ks[(int64_t)bh * (p.cap / C8_BLOCK) + kblk], SCALE_MIN);
     f32x16 sum[2] = {};
     // steps with a row that sees the workgroup's first key, this split's share
-    const int steps = (p.rows + MT_ROWS - 1) / MT_ROWS;
+    const int steps = (qs.nq * p.G + MT_ROWS - 1) / MT_ROWS;
     int s0 = 0;
-    if (p.causal) s0 = min((int64_t)steps, (int64_t)max(0, first_key - (len - p.Q)) * p.G / MT_ROWS);
+    if (p.causal) s0 = min((int64_t)steps, (int64_t)max(0, first_key - (len - qs.nq)) * p.G / MT_ROWS);
     const int st0 = s0 + (int)((int64_t)split * (steps - s0) / p.splits);
     const int st1 = s0 + (int)((int64_t)(split + 1) * (steps - s0) / p.splits);
     if (st0 < st1) {
         MassRows<T, P> rows;
-        rows.load(p, b, hk, len, st0 * MT_ROWS);
+        rows.load(p, qs, b, hk, st0 * MT_ROWS);
         rows.store(smem[0], offs[0], ends[0]);
-        rows.load(p, b, hk, len, min(st0 + 1, st1 - 1) * MT_ROWS);
+        rows.load(p, qs, b, hk, min(st0 + 1, st1 - 1) * MT_ROWS);
         uint32_t qofs[KS];
 #pragma unroll
         for (int s = 0; s < KS; ++s)
@@ -1011,7 +1031,7 @@ __global__ void __launch_bounds__(256, 2) mass_tile_kernel(MassParams p) {
         for (int st = st0; st < st1; ++st) {
             const int cur = (st - st0) & 1;
             // what the step's first row sees
-            const int first = p.causal ? len - p.Q + 1 + st * MT_ROWS / p.G : len;
+            const int first = qs.sees(st * MT_ROWS / p.G);
             const bool masked = key0 + C8_BLOCK > first;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -1041,7 +1061,7 @@ __global__ void __launch_bounds__(256, 2) mass_tile_kernel(MassParams p) {
                 }
             }
             rows.store(smem[cur ^ 1], offs[cur ^ 1], ends[cur ^ 1]);
-            rows.load(p, b, hk, len, min(st + 2, st1 - 1) * MT_ROWS);
+            rows.load(p, qs, b, hk, min(st + 2, st1 - 1) * MT_ROWS);
             lds_barrier();
         }
     }
@@ -1288,6 +1308,7 @@ extern "C" int nkv_cache8_attend(void* stream, const nkv_cache8_attend_args* a, 
     p.ks = c.k_scale;
     p.vs = c.v_scale;
     p.length = a->length;
+    p.counts = a->counts;
     p.q = (const uint16_t*)a->q;
     p.out = (uint16_t*)a->out;
     p.lse = a->lse;
@@ -1391,6 +1412,7 @@ extern "C" int nkv_cache8_mass(void* stream, const nkv_cache8_mass_args* a, void
     p.k = (const uint8_t*)c.k;
     p.ks = c.k_scale;
     p.length = a->length;
+    p.counts = a->counts;
     p.q = (const uint16_t*)a->q;
     p.lse = a->lse;
     p.mass = a->mass;

@@ -1533,6 +1533,7 @@ def _cache8_query(q: torch.Tensor, cache: Cache8, length, max_length, softmax_sc
 
 def cache8_attend(q: torch.Tensor, cache: Cache8, length, *, max_length: Optional[int] = None,
                   softmax_scale: Optional[float] = None, causal: bool = False,
+                  counts: Optional[torch.Tensor] = None,
                   return_lse: bool = True, out: Optional[torch.Tensor] = None,
                   workspace: Optional[torch.Tensor] = None):
     """Attention over an 8-bit cache (see nkv_cache8_attend).
@@ -1542,11 +1543,14 @@ def cache8_attend(q: torch.Tensor, cache: Cache8, length, *, max_length: Optiona
     rows visible, an int for every sequence or an int32 tensor [B] on the
     device, clamped to [0, max_length] (default: cap), by which the work is
     divided.  causal: the queries are the last Q tokens, query t sees the first
-    length - Q + 1 + t rows.  Returns (out like q, lse [B, heads, Q] fp32 or
+    length - Q + 1 + t rows.  counts: int32 [B], how many of a sequence's Q rows are
+    queries, the first ones, as cache8_write's (a padded batch): causal query t
+    then sees length - counts + 1 + t rows, and a row past them none, whatever it
+    holds.  Returns (out like q, lse [B, heads, Q] fp32 or
     None); a query that sees nothing gets 0 and -inf.  workspace: optional
     uint8 buffer, nkv_cache8_attend_workspace_size bytes or fewer (with fewer,
     fewer key splits)."""
-    device = _require_gpu(q, cache.k, cache.v, cache.k_scale, cache.v_scale, out,
+    device = _require_gpu(q, cache.k, cache.v, cache.k_scale, cache.v_scale, out, counts,
                           length if isinstance(length, torch.Tensor) else None)
     c, query, scale = _cache8_query(q, cache, length, max_length, softmax_scale)
     B, Q, heads, D = q.shape
@@ -1558,7 +1562,8 @@ def cache8_attend(q: torch.Tensor, cache: Cache8, length, *, max_length: Optiona
     else:
         strides = _strides_bthd(out, "out") if q.numel() else (0, 0, 0)
     lse = torch.empty((B, heads, Q), device=device, dtype=torch.float32) if return_lse else None
-    a = NkvCache8AttendArgs(*query, out.data_ptr(), *strides, _ptr(lse), scale, bool(causal))
+    a = NkvCache8AttendArgs(*query, out.data_ptr(), *strides, _ptr(lse), scale, bool(causal),
+                            _cache8_ints(counts, B, "counts"))
     scratch, nbytes = _cache8_scratch("nkv_cache8_attend_workspace_size", a, device, workspace)
     _cache8_call("nkv_cache8_attend", device, byref(a), _ptr(scratch), nbytes)
     return out, lse
@@ -1567,13 +1572,14 @@ def cache8_attend(q: torch.Tensor, cache: Cache8, length, *, max_length: Optiona
 def cache8_mass(q: torch.Tensor, cache: Cache8, lse: torch.Tensor, mass: torch.Tensor, length, *,
                 out: Optional[torch.Tensor] = None, max_length: Optional[int] = None,
                 softmax_scale: Optional[float] = None, causal: bool = False,
+                counts: Optional[torch.Tensor] = None,
                 workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Adds to mass [B, H, cap] fp32 the attention weight that each cached row
     receives from q, summed over the queries and the heads of its group (see
     nkv_cache8_mass).  lse: cache8_attend's, on the same arguments.  out: where
     the sums go (default: mass itself); returned."""
     out = mass if out is None else out
-    device = _require_gpu(q, cache.k, cache.v, cache.k_scale, cache.v_scale, lse, mass, out,
+    device = _require_gpu(q, cache.k, cache.v, cache.k_scale, cache.v_scale, lse, mass, out, counts,
                           length if isinstance(length, torch.Tensor) else None)
     c, query, scale = _cache8_query(q, cache, length, max_length, softmax_scale)
     _contig(lse, torch.float32, "lse")
@@ -1584,7 +1590,7 @@ def cache8_mass(q: torch.Tensor, cache: Cache8, lse: torch.Tensor, mass: torch.T
         if t.shape != (c.B, c.H, c.cap):
             raise ValueError(f"{name} must be [B, H, cap]")
     a = NkvCache8MassArgs(*query, lse.data_ptr(), mass.data_ptr(), out.data_ptr(), scale,
-                          bool(causal))
+                          bool(causal), _cache8_ints(counts, c.B, "counts"))
     scratch, nbytes = _cache8_scratch("nkv_cache8_mass_workspace_size", a, device, workspace)
     _cache8_call("nkv_cache8_mass", device, byref(a), _ptr(scratch), nbytes)
     return out

@@ -7,8 +7,9 @@ import sys
 from pathlib import Path
 
 import pytest
+import torch
 
-from nanokv_amd import build
+from nanokv_amd import build, ops
 from tests.test_device_attributes import SHIM
 
 ROOT = Path(__file__).resolve().parent.parent
@@ -59,3 +60,10 @@ def test_the_attention_is_compiled_with_nans():
     """What a NaN query does to its own row is documented, so no flag may let the
     compiler take NaN for impossible there."""
     assert not [f for f in build.SOURCES["nkv_cache8_attend.hip"] if "nan" in f or "fast" in f]
+
+
+def test_the_wrappers_refuse_counts_of_another_kind():
+    ints = torch.zeros(2, dtype=torch.int32)
+    for bad in (ints.long(), ints[:1], torch.zeros(4, dtype=torch.int32)[::2]):
+        with pytest.raises(ValueError, match="counts"):
+            ops._cache8_ints(bad, 2, "counts")

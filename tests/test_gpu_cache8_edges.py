@@ -157,3 +157,60 @@ def test_causal_rows_do_not_depend_on_later_values(dev, dtype, fmt, Q, G):
     few = ops.cache8_attend(q[:, :seen], cache, N - Q + seen, causal=True)
     check_rows(q[:, :seen], cache, fmt, [N - Q + seen] * 2, True, out[:, :seen], lse[:, :, :seen])
     check_rows(q[:, :seen], cache, fmt, [N - Q + seen] * 2, True, *few)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("fmt,dtype,H,G,D,T,start", [
+    ("int8", torch.bfloat16, 2, 1, 64, 5, [0, 7, 100, 3, 0]),
+    ("e4m3", torch.float16, 1, 4, 128, 9, [0, 7, 100, 3, 0]),
+    ("e4m3", torch.bfloat16, 2, 2, 80, 70, [0, 64, 100, 3, 1]),
+    ("int8", torch.float16, 1, 2, 64, 300, [0, 64, 1000, 3, 1]),
+    ("e4m3", torch.bfloat16, 1, 3, 128, 100, [0, 64, 9000, 3, 1]),      # key splits
+])
+def test_a_batch_padded_on_the_right(dev, fmt, dtype, H, G, D, T, start, causal):
+    """Write, attention and weight with one tensor of counts: each sequence as if it
+    were alone, whatever the padding holds."""
+    B, counts = len(start), [T, T - 2, 1, 0, T // 2]
+    g = torch.Generator().manual_seed(107)
+    cache = make_cache(dev, B, H, max(start) + T, D, fmt, 108, start)
+    kv = torch.randn((2, B, T, H, D), generator=g)
+    q = torch.randn((B, T, H * G, D), generator=g)
+    for b, c in enumerate(counts):
+        kv[:, b, c:] = float("nan")
+        q[b, c:] = float("nan")
+    kv, q = kv.to(dtype).to(dev), q.to(dtype).to(dev)
+    ints = dict(dtype=torch.int32, device=dev)
+    dc, ds = torch.tensor(counts, **ints), torch.tensor(start, **ints)
+    ops.cache8_write(cache, kv[0], kv[1], ds, dc)
+    lengths = [a + b for a, b in zip(start, counts)]
+    n = torch.tensor(lengths, **ints)
+    m0 = torch.rand((B, H, cache.cap), generator=g)
+    m, other = m0.to(dev), torch.full((B, H, cache.cap), float("nan"), device=dev)
+    for work in (None, torch.zeros(16, dtype=torch.uint8, device=dev)):
+        out, lse = ops.cache8_attend(q, cache, n, causal=causal, counts=dc, workspace=work)
+        bad = lse.clone()                     # (nor is the padding's lse read)
+        for b, c in enumerate(counts):
+            assert (out[b, c:] == 0).all() and torch.isneginf(lse[b, :, c:]).all()
+            bad[b, :, c:] = 0.0
+            if c:
+                one = ops.Cache8(*(t[b:b + 1].contiguous() for t in (cache.k, cache.v, cache.k_scale,
+                                                                     cache.v_scale)), D)
+                check_rows(q[b:b + 1, :c], one, fmt, lengths[b:b + 1], causal, out[b:b + 1, :c],
+                           lse[b:b + 1, :, :c])
+        m.copy_(m0)
+        ops.cache8_mass(q, cache, bad, m, n, out=other, causal=causal, counts=dc, workspace=work)
+        ops.cache8_mass(q, cache, bad, m, n, causal=causal, counts=dc, workspace=work)
+        assert torch.equal(m, other)
+        k, _ = cache_values(cache, fmt)
+        for b, c in enumerate(counts):
+            if c:
+                rm, tol = ref.mass(q[b:b + 1, :c].double().cpu().numpy(), k[b:b + 1],
+                                   lse[b:b + 1, :, :c].double().cpu().numpy(), m0[b:b + 1].numpy(),
+                                   lengths[b:b + 1], causal, D ** -0.5)
+                assert (np.abs(m[b:b + 1].double().cpu().numpy() - rm) <= tol).all()
+            else:
+                assert torch.equal(m[b].cpu(), m0[b])
+    # counts outside [0, Q] are those
+    wide = torch.tensor([T + 5 if c == T else -3 if c == 0 else c for c in counts], **ints)
+    again, l2 = ops.cache8_attend(q, cache, n, causal=causal, counts=wide, workspace=work)
+    assert torch.equal(again, out) and torch.equal(l2, lse)
