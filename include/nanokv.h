@@ -860,10 +860,12 @@ int nkv_cache8_attend(void* stream, const nkv_cache8_attend_args* args, void* wo
  * The attention weight each cached row receives:
  *   out[b, h, n] = mass[b, h, n] + sum over the queries that see row n, and
  *                  the G query heads of h, of exp(q.k_n * softmax_scale - lse)
- * with lse of nkv_cache8_attend on the same arguments (a row with lse = -inf
- * adds nothing).  mass and out are [B, H, cap] fp32 and may be the same
- * array, whose entries past the length are then not touched (otherwise they
- * are copied).  Q = 0 adds nothing (lse may be NULL).  Deterministic: no atomics.
+ * with lse of nkv_cache8_attend on the same arguments.  A row whose lse is not
+ * finite adds nothing: one that sees no key, or whose query holds NaN or
+ * infinities (its weights would stay in mass for good).  mass and out are [B, H,
+ * cap] fp32 and may be the same array, whose entries past the length are then not
+ * touched (otherwise they are copied).  Q = 0 adds nothing (lse may be NULL).
+ * Deterministic: no atomics.
  */
 typedef struct nkv_cache8_mass_args {
     nkv_cache8 cache;             /* v and v_scale are not read */

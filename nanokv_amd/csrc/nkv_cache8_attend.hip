@@ -903,7 +903,9 @@ __global__ void __launch_bounds__(256) mass_kernel(MassParams p) {
         f32x4 sum[4] = {};
         for (;;) {
             if (groups > 1) load_group(rg);
-            const float off = z == -INFINITY ? INFINITY : z * LOG2E;
+            const bool adds = fabsf(z) < INFINITY;      // (a NaN query's lse is NaN)
+            const float off = adds ? z * LOG2E : 0.0f;
+            const int seen_to = adds ? end : 0;
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 f32x4 s{};
@@ -915,7 +917,7 @@ __global__ void __launch_bounds__(256) mass_kernel(MassParams p) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float w = __builtin_amdgcn_exp2f(fmaf(s[e], c, -off));
-                    sum[t][e] += key0 + 16 * t + 4 * g + e < end ? w : 0.0f;
+                    sum[t][e] += key0 + 16 * t + 4 * g + e < seen_to ? w : 0.0f;
                 }
             }
             if (++rg >= groups) break;
@@ -967,13 +969,18 @@ struct MassRows {
         off = at.there ? p.lse[((int64_t)b * p.H * p.G + at.head) * p.Q + at.t] : -INFINITY;
         end = qs.sees(at.t);
     }
-    __device__ __forceinline__ void store(unsigned char* buf, float* offs, int* ends) const {
+    // a row whose lse is not finite becomes zeros with weight 2^-inf
+    __device__ __forceinline__ void store(unsigned char* buf, float* offs, int* ends) {
         const int row = threadIdx.x >> 2, part = threadIdx.x & 3;
+        const bool adds = fabsf(off) < INFINITY;
+        if (!adds)
+#pragma unroll
+            for (int i = 0; i < PER; ++i) q[i] = u32x4{};
 #pragma unroll
         for (int i = 0; i < PER; ++i)
             *reinterpret_cast<u32x4*>(buf + row * 2 * P + 16 * ((part + 4 * i) ^ (row & (CH - 1)))) = q[i];
         if (part == 0) {
-            offs[row] = off == -INFINITY ? INFINITY : off * LOG2E;
+            offs[row] = adds ? off * LOG2E : INFINITY;
             ends[row] = end;
         }
     }

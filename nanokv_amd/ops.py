@@ -1576,8 +1576,9 @@ def cache8_mass(q: torch.Tensor, cache: Cache8, lse: torch.Tensor, mass: torch.T
                 workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Adds to mass [B, H, cap] fp32 the attention weight that each cached row
     receives from q, summed over the queries and the heads of its group (see
-    nkv_cache8_mass).  lse: cache8_attend's, on the same arguments.  out: where
-    the sums go (default: mass itself); returned."""
+    nkv_cache8_mass).  lse: cache8_attend's, on the same arguments (counts among
+    them); a row whose lse is not finite adds nothing.  out: where the sums go
+    (default: mass itself); returned."""
     out = mass if out is None else out
     device = _require_gpu(q, cache.k, cache.v, cache.k_scale, cache.v_scale, lse, mass, out, counts,
                           length if isinstance(length, torch.Tensor) else None)

@@ -214,3 +214,30 @@ def test_a_batch_padded_on_the_right(dev, fmt, dtype, H, G, D, T, start, causal)
     wide = torch.tensor([T + 5 if c == T else -3 if c == 0 else c for c in counts], **ints)
     again, l2 = ops.cache8_attend(q, cache, n, causal=causal, counts=wide, workspace=work)
     assert torch.equal(again, out) and torch.equal(l2, lse)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("fmt,dtype,Q,G,N,causal", [
+    ("int8", torch.bfloat16, 1, 4, 700, False), ("e4m3", torch.float16, 9, 2, 130, True),
+    ("e4m3", torch.bfloat16, 40, 2, 1000, True), ("int8", torch.bfloat16, 600, 2, 900, False),
+])
+def test_queries_that_are_not_finite_add_no_weight(dev, fmt, dtype, Q, G, N, causal, value):
+    """The masses equal those of the other rows alone, to the last bit."""
+    cache = make_cache(dev, 2, 1, N, 64, fmt, 109, [N, N - 64])
+    n = torch.tensor([N, N - 64], dtype=torch.int32, device=dev)
+    q = torch.randn((2, Q, G, 64), generator=torch.Generator().manual_seed(110)).to(dtype).to(dev)
+    _, lse = ops.cache8_attend(q, cache, n, causal=causal)
+    bad = q.clone()
+    bad[0, Q // 2, 1, 5] = value
+    _, l2 = ops.cache8_attend(bad, cache, n, causal=causal)
+    assert torch.isnan(l2[0, 1, Q // 2])
+    lse[0, 1, Q // 2] = float("-inf")
+    m0 = torch.rand((2, 1, cache.cap), generator=torch.Generator().manual_seed(111)).to(dev)
+    for work in (None, torch.zeros(16, dtype=torch.uint8, device=dev)):
+        want = ops.cache8_mass(q, cache, lse, m0.clone(), n, causal=causal, workspace=work)
+        got = ops.cache8_mass(bad, cache, l2, m0.clone(), n, causal=causal, workspace=work)
+        assert torch.equal(got, want) and torch.isfinite(got).all()
+        for other in (float("inf"), float("nan")):
+            l2[0, 1, Q // 2] = other
+            got = ops.cache8_mass(q, cache, l2, m0.clone(), n, causal=causal, workspace=work)
+            assert torch.equal(got, want)
