@@ -62,7 +62,7 @@ __device__ __forceinline__ f32x2 code_pair(uint32_t w, int h) {
 // within one step rounds as the division does; Markstein, "Computation of
 // elementary functions on the IBM RISC System/6000 processor").  Five
 // instructions, where the compiler's division takes ten.  Quotients below 2^-60,
-// where a remainder may underflow, give the zero code either way.
+// where a remainder may underflow, give the zero code either way; -0 gives +0.
 __device__ __forceinline__ float div_by(float x, float s, float y) {
     float q = x * y;
     q = fmaf(fmaf(-q, s, x), y, q);

@@ -191,7 +191,11 @@ __global__ void __launch_bounds__(256) write_kernel(WriteParams p) {
         u32x2 w;
         if (finite) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) q[e] = div_by(x[i][e], s, y);
+            for (int e = 0; e < 8; ++e) {
+                q[e] = div_by(x[i][e], s, y);
+                // (-0, whose remainder is +0; e4m3 keeps its sign)
+                if constexpr (FMT == NKV_CACHE8_E4M3) q[e] = copysignf(q[e], x[i][e]);
+            }
             w[0] = to_codes_fast<FMT>(q[0], q[1], q[2], q[3]);
             w[1] = to_codes_fast<FMT>(q[4], q[5], q[6], q[7]);
         } else {

@@ -241,3 +241,25 @@ def test_queries_that_are_not_finite_add_no_weight(dev, fmt, dtype, Q, G, N, cau
             l2[0, 1, Q // 2] = other
             got = ops.cache8_mass(q, cache, l2, m0.clone(), n, causal=causal, workspace=work)
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_zeros_keep_their_sign(dev, fmt, dtype):
+    """-0 and quotients that round to it, in finite blocks and beside infinities and
+    NaN, and under a scale that grows: the codes of the division, to the last bit."""
+    cache = ops.Cache8.empty(1, 1, 192, 64, dev, fmt)
+    x = torch.randn((1, 150, 1, 64), generator=torch.Generator().manual_seed(112))
+    x[:, :, :, ::3] = -0.0
+    x[:, :, :, 1::6] *= -1e-6
+    x[0, 70, 0, 5], x[0, 71, 0, 8] = float("inf"), float("nan")
+    x[0, 135:] *= 3
+    x = x.to(dtype).to(dev)
+    want = raw(cache.k).copy(), cache.k_scale.cpu().numpy()
+    for first, last in ((0, 130), (130, 135), (135, 150)):
+        part = x[:, first:last].contiguous()
+        ops.cache8_write(cache, part, part, first)
+        want = ref.write(*want, part.float().cpu().numpy(), [first], [last - first], fmt)
+    for codes, scale in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        assert np.array_equal(scale.cpu().numpy(), want[1])
+        assert np.array_equal(raw(codes).view(np.uint8), want[0].view(np.uint8))
