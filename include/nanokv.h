@@ -785,8 +785,10 @@ typedef struct nkv_cache8 {
  * rounded once (IEEE fp32 division); a block that holds rows before `start`
  * keeps its scale s0 if that is larger, and its codes become round(code *
  * (s0 / s)) if it is not.  New codes are round(x / s) to the nearest, ties to
- * even; infinities give the largest code, NaN zero.  Rows past those written
- * are left as they were (a block's scale may have grown over them).
+ * even; infinities give the largest code, NaN zero.  The codes of rows past those
+ * written are left as they were, but not their values: a block's scale may have
+ * grown over them, or, where the write starts on the block's first row, be that
+ * of the new rows alone, larger or smaller.
  * start_dev (device, [B]; NULL: `start` for every item) is clamped to [0,
  * cap]; counts (device, [B]; NULL: T for every item) says how many of an
  * item's rows are written.  Rows past cap are dropped where start or counts

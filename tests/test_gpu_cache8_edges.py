@@ -263,3 +263,20 @@ def test_zeros_keep_their_sign(dev, fmt, dtype):
     for codes, scale in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
         assert np.array_equal(scale.cpu().numpy(), want[1])
         assert np.array_equal(raw(codes).view(np.uint8), want[0].view(np.uint8))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_a_write_over_old_rows(dev, fmt):
+    """Rows behind those written keep their codes; a write that starts on a block's
+    first row sets its scale anew, also below the old one, one that starts inside
+    the block does not lower it."""
+    cache = make_cache(dev, 1, 2, 192, 64, fmt, 113)
+    x = torch.randn((1, 20, 2, 64), generator=torch.Generator().manual_seed(114)).to(dev) * 2.0 ** -20
+    for start in (64, 130):
+        before = raw(cache.k).copy(), cache.k_scale.cpu().numpy()
+        ops.cache8_write(cache, x, x, start)
+        rc, rs = ref.write(*before, x.cpu().numpy(), [start], [20], fmt)
+        assert np.array_equal(raw(cache.k), rc) and np.array_equal(cache.k_scale.cpu().numpy(), rs)
+        assert np.array_equal(rc[:, :, start + 20:], before[0][:, :, start + 20:])
+        lower = rs[:, :, start // 64] < before[1][:, :, start // 64]
+        assert lower.all() if start % 64 == 0 else not lower.any()
