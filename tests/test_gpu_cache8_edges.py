@@ -280,3 +280,48 @@ def test_a_write_over_old_rows(dev, fmt):
         assert np.array_equal(rc[:, :, start + 20:], before[0][:, :, start + 20:])
         lower = rs[:, :, start // 64] < before[1][:, :, start // 64]
         assert lower.all() if start % 64 == 0 else not lower.any()
+
+
+def test_mass_over_a_cache_written_in_the_same_graph(dev):
+    """A captured write and the weight over what it wrote: every replay with new
+    tokens against the plain form and against eager calls between."""
+    B, H, G, D, T = 2, 2, 2, 64, 70
+    start, lengths = [130, 7], [200, 77]
+    ints = dict(dtype=torch.int32, device=dev)
+    ds, n = torch.tensor(start, **ints), torch.tensor(lengths, **ints)
+    cache = ops.Cache8.empty(B, H, 256, D, dev, "int8")
+    q = torch.zeros((B, 40, H * G, D), dtype=torch.bfloat16, device=dev)
+    kv = torch.zeros((2, B, T, H, D), dtype=torch.bfloat16, device=dev)
+    m0 = torch.rand((B, H, cache.cap), generator=torch.Generator().manual_seed(115)).to(dev)
+
+    def calls(c):
+        ops.cache8_write(c, kv[0], kv[1], ds)
+        _, lse = ops.cache8_attend(q, c, n, causal=True)
+        out = torch.empty_like(m0)
+        return lse, ops.cache8_mass(q, c, lse, m0, n, out=out, causal=True)
+
+    def empty(c):
+        for t in (c.k, c.v):
+            t.zero_()
+        for t in (c.k_scale, c.v_scale):
+            t.fill_(1.0)
+
+    calls(ops.Cache8.empty(B, H, 256, D, dev, "int8"))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lse, got = calls(cache)
+    for i in range(3):
+        g = torch.Generator().manual_seed(116 + i)
+        q.copy_(torch.randn(q.shape, generator=g))
+        kv.copy_(torch.randn(kv.shape, generator=g))
+        empty(cache)
+        graph.replay()
+        torch.cuda.synchronize()
+        k, _ = cache_values(cache, "int8")
+        rm, tol = ref.mass(q.double().cpu().numpy(), k, lse.double().cpu().numpy(), m0.cpu().numpy(),
+                           lengths, True, D ** -0.5)
+        assert (np.abs(got.double().cpu().numpy() - rm) <= tol).all()
+        other = ops.Cache8.empty(B, H, 256, D, dev, "int8")
+        l2, want = calls(other)
+        assert torch.equal(got, want) and torch.equal(lse, l2) and torch.equal(cache.k, other.k)
