@@ -1141,8 +1141,7 @@ constexpr int64_t TILE_ROWS = 64;
 // 27.8).
 constexpr int64_t ROWS_TWO = 4096;
 
-// limit: bytes of workspace; fewer splits where those wanted do not fit.
-Plan attend_plan(const nkv_cache8_attend_args* a, size_t limit = SIZE_MAX) {
+Plan attend_plan(const nkv_cache8_attend_args* a) {
     const nkv_cache8& c = a->cache;
     Plan pl{};
     pl.rows = a->Q * a->G;
@@ -1183,22 +1182,28 @@ Plan attend_plan(const nkv_cache8_attend_args* a, size_t limit = SIZE_MAX) {
             pl.splits = (int)std::max<int64_t>(1, std::min(cdiv(slots, base), blocks / waves));
         pl.items = base * pl.splits;
     }
-    const size_t row = sizeof(Stat) + c8_pitch(c.D) * (a->dtype == NKV_ROWS_FP16 ? 4 : 2);
-    const size_t split = (size_t)heads * pl.rows * row;
-    if (pl.splits > 1 && limit / split < (size_t)pl.splits) {
-        pl.items /= pl.splits;
-        pl.splits = (int)std::max<size_t>(1, limit / split);
-        pl.items *= pl.splits;
-    }
-    if (pl.splits > 1) {
-        const size_t rows = (size_t)heads * pl.splits * pl.rows;
-        pl.ml = rows * sizeof(Stat);
-        pl.part = rows * (row - sizeof(Stat));
-    }
     return pl;
 }
 
-int check_attend(const nkv_cache8_attend_args* a) {
+// The plan's workspace; in fewer than `limit` bytes fewer splits where those wanted do
+// not fit.
+void attend_fit(const nkv_cache8_attend_args* a, Plan& pl, size_t limit) {
+    if (pl.splits == 1) return;
+    const size_t part = c8_pitch(a->cache.D) * (a->dtype == NKV_ROWS_FP16 ? 4 : 2);
+    const size_t rows = (size_t)a->cache.B * a->cache.H * pl.rows;
+    const size_t most = limit / (rows * (sizeof(Stat) + part));
+    if (most < (size_t)pl.splits) {
+        pl.items /= pl.splits;
+        pl.splits = (int)std::max<size_t>(1, most);
+        pl.items *= pl.splits;
+        if (pl.splits == 1) return;
+    }
+    pl.ml = rows * pl.splits * sizeof(Stat);
+    pl.part = rows * pl.splits * part;
+}
+
+// Also plans the call where there is something to do (pl.items > 0).
+int check_attend(const nkv_cache8_attend_args* a, Plan& pl) {
     NKV_REQUIRE(a, NKV_ERR_INVALID, "args is null");
     int rc = check_query(a->cache, a->G, a->dtype, a->Q, a->n, a->softmax_scale, a->q, a->q_sb,
                          a->q_st, a->q_sh, __func__);
@@ -1207,7 +1212,8 @@ int check_attend(const nkv_cache8_attend_args* a) {
     NKV_REQUIRE(reinterpret_cast<uintptr_t>(a->out) % 16 == 0 && (a->o_sb | a->o_st | a->o_sh) % 8 == 0,
                 NKV_ERR_INVALID, "out must be 16-byte aligned with strides divisible by 8");
     // a launch has fewer than 2^32 threads
-    NKV_REQUIRE(attend_plan(a).items <= 1 << 22, NKV_ERR_UNSUPPORTED, "too many query rows");
+    pl = attend_plan(a);
+    NKV_REQUIRE(pl.items <= 1 << 22, NKV_ERR_UNSUPPORTED, "too many query rows");
     // every row of out lies past the end of those of the smaller strides
     std::pair<int64_t, int64_t> dims[3] = {
         {a->o_sb, a->cache.B}, {a->o_st, a->Q}, {a->o_sh, (int64_t)a->cache.H * a->G}};
@@ -1295,18 +1301,20 @@ using namespace nkv;
 
 extern "C" size_t nkv_cache8_attend_workspace_size(const nkv_cache8_attend_args* a) {
     clear_error();
-    if (check_attend(a) || a->cache.B == 0 || a->Q == 0) return 0;
-    const Plan pl = attend_plan(a);
+    Plan pl{};
+    if (check_attend(a, pl) || pl.items == 0) return 0;
+    attend_fit(a, pl, SIZE_MAX);
     return pl.part + pl.ml;
 }
 
 extern "C" int nkv_cache8_attend(void* stream, const nkv_cache8_attend_args* a, void* workspace,
                                  size_t workspace_bytes) {
     clear_error();
-    int rc = check_attend(a);
-    if (rc || a->cache.B == 0 || a->Q == 0) return rc;
+    Plan pl{};
+    int rc = check_attend(a, pl);
+    if (rc || pl.items == 0) return rc;
     const nkv_cache8& c = a->cache;
-    const Plan pl = attend_plan(a, workspace ? workspace_bytes : 0);
+    attend_fit(a, pl, workspace ? workspace_bytes : 0);
     NKV_REQUIRE(pl.part == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, NKV_ERR_INVALID,
                 "workspace must be 16-byte aligned");
     AttendParams p{};
