@@ -36,6 +36,11 @@ constexpr float FLOOR = -0x1p126f;    // a maximum before the first key (finite:
 // 2^-QUIET of their 2^(z - m): they are zero in fp16 (2^(LIFT + TAU - QUIET) = 2^-25)
 // either way, and stay normal numbers for the sum.
 constexpr float QUIET = 40.0f;
+// A score's factor softmax_scale * log2 e * sk, kept from 0 and infinity: a hidden
+// score of -inf times 0 and a score of 0 times infinity would be NaN.
+__device__ __forceinline__ float score_factor(float scale_log2, float sk) {
+    return __builtin_amdgcn_fmed3f(scale_log2 * sk, 0x1p-126f, 0x1.fffffep127f);
+}
 constexpr float SCALE_MIN = 0x1p-100f;  // keeps an unwritten block's scale out of log2(0)
 
 // A row's running statistics (log2 units): the maximum of z and the sum of 2^(z -
@@ -319,7 +324,7 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
                             for (int w = 0; w < DB / 4; ++w) vr[c][j][w] = 0;
             }
         }
-        const float c = p.scale_log2 * sk, lsv = __builtin_amdgcn_logf(sv);
+        const float c = score_factor(p.scale_log2, sk), lsv = __builtin_amdgcn_logf(sv);
         uint32_t pw[NQ][2][4];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
@@ -594,7 +599,7 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
                                      kk ? s[j] : f32x16{});
             __builtin_amdgcn_s_setprio(0);
         }
-        const float c = p.scale_log2 * fmaxf(sk, SCALE_MIN);
+        const float c = score_factor(p.scale_log2, fmaxf(sk, SCALE_MIN));
         const float lsv = __builtin_amdgcn_logf(fmaxf(sv, SCALE_MIN));
         // block blk + 1 (behind the last, the last again, for no one)
         codes.store(smem + (kslot ^ 1) * Codes::K_BYTES,
@@ -895,7 +900,7 @@ __global__ void __launch_bounds__(256) mass_kernel(MassParams p) {
     }
     for (; blk < min(blk1, seen); blk += 4) {
         const int key0 = blk * C8_BLOCK;
-        const float c = p.scale_log2 * fmaxf(sk, SCALE_MIN);
+        const float c = score_factor(p.scale_log2, fmaxf(sk, SCALE_MIN));
         // the first group with a row that sees the block's first key
         int rg = 0;
         if (p.causal)
@@ -1017,7 +1022,8 @@ __global__ void __launch_bounds__(256, 2) mass_tile_kernel(MassParams p) {
                 kf[t][2 * i + 1] = codes_x8<T, FMT>(w[2], w[3]);
             }
     }
-    const float c = p.scale_log2 * fmaxf(p.ks[(int64_t)bh * (p.cap / C8_BLOCK) + kblk], SCALE_MIN);
+    const float c =
+        score_factor(p.scale_log2, fmaxf(p.ks[(int64_t)bh * (p.cap / C8_BLOCK) + kblk], SCALE_MIN));
     f32x16 sum[2] = {};
     // steps with a row that sees the workgroup's first key, this split's share
     const int steps = (qs.nq * p.G + MT_ROWS - 1) / MT_ROWS;
@@ -1333,7 +1339,7 @@ extern "C" int nkv_cache8_attend(void* stream, const nkv_cache8_attend_args* a, 
     p.o_sb = a->o_sb, p.o_st = a->o_st, p.o_sh = a->o_sh;
     p.cap = c.cap;
     p.items = pl.items;
-    p.scale_log2 = a->softmax_scale * LOG2E;
+    p.scale_log2 = std::min(a->softmax_scale * LOG2E, 0x1.fffffep127f);
     p.B = c.B, p.H = c.H, p.G = a->G, p.D = c.D, p.Q = (int)a->Q, p.n = (int)a->n;
     p.causal = a->causal != 0;
     p.splits = pl.splits;
@@ -1434,7 +1440,7 @@ extern "C" int nkv_cache8_mass(void* stream, const nkv_cache8_mass_args* a, void
     p.out = a->out;
     p.q_sb = a->q_sb, p.q_st = a->q_st, p.q_sh = a->q_sh;
     p.cap = c.cap;
-    p.scale_log2 = a->softmax_scale * LOG2E;
+    p.scale_log2 = std::min(a->softmax_scale * LOG2E, 0x1.fffffep127f);
     p.B = c.B, p.H = c.H, p.G = a->G, p.D = c.D, p.Q = (int)a->Q, p.n = (int)a->n;
     p.causal = a->causal != 0;
     p.rows = (int)(a->Q * a->G);

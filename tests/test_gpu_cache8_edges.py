@@ -325,3 +325,23 @@ def test_mass_over_a_cache_written_in_the_same_graph(dev):
         other = ops.Cache8.empty(B, H, 256, D, dev, "int8")
         l2, want = calls(other)
         assert torch.equal(got, want) and torch.equal(lse, l2) and torch.equal(cache.k, other.k)
+
+
+@pytest.mark.parametrize("softmax_scale", [1e-40, 1e-25, 1e30, 3e38])
+@pytest.mark.parametrize("Q,G,causal", [(1, 2, False), (9, 2, True), (100, 1, True)])
+def test_softmax_scales_of_any_size(dev, Q, G, causal, softmax_scale):
+    """Beside keys of zeros, whose scale is the least there is: hidden keys stay
+    hidden, and where every visible score is zero the weights are equal."""
+    cache = make_cache(dev, 1, 1, 192, 64, "int8", 120, [170])
+    for first, s in ((0, float(ref.TINY) / 127), (64, float(ref.TINY) / 127), (128, 1e12)):
+        cache.k_scale[:, :, first // 64] = s
+    cache.k.zero_()
+    q = torch.randn((1, Q, G, 64), generator=torch.Generator().manual_seed(121)).bfloat16().to(dev)
+    n = torch.tensor([170], dtype=torch.int32, device=dev)
+    out, lse = ops.cache8_attend(q, cache, n, causal=causal, softmax_scale=softmax_scale)
+    check_attend(q, cache, "int8", [170], causal, out, lse, softmax_scale)
+    m = torch.zeros((1, 1, cache.cap), device=dev)
+    ops.cache8_mass(q, cache, lse, m, n, causal=causal, softmax_scale=softmax_scale)
+    rm, tol = ref.mass(q.double().cpu().numpy(), cache_values(cache, "int8")[0],
+                       lse.double().cpu().numpy(), np.zeros((1, 1, 192)), [170], causal, softmax_scale)
+    assert (np.abs(m.double().cpu().numpy() - rm) <= tol).all()
