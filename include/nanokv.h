@@ -792,9 +792,9 @@ typedef struct nkv_cache8 {
  * start_dev (device, [B]; NULL: `start` for every item) is clamped to [0,
  * cap]; counts (device, [B]; NULL: T for every item) says how many of an
  * item's rows are written.  Rows past cap are dropped where start or counts
- * are in device memory, and refused where start is not.
+ * are in device memory, and refused where neither is.
  * k and v are 16-byte aligned with strides divisible by 8; the cache's codes and
- * scales do not overlap each other.
+ * scales overlap neither each other nor anything else of the call.
  */
 typedef struct nkv_cache8_write_args {
     nkv_cache8 cache;
@@ -832,7 +832,8 @@ int nkv_cache8_write(void* stream, const nkv_cache8_write_args* args);
  * 2^-36 of it below): values that a row does not see, or gives no weight to,
  * do not change its result beyond the order of its sums.
  * q and out are 16-byte aligned with strides divisible by 8; out's rows do not
- * overlap.
+ * overlap.  out may be q itself; otherwise out, lse and the workspace overlap
+ * nothing of the call.
  */
 typedef struct nkv_cache8_attend_args {
     nkv_cache8 cache;
@@ -866,7 +867,8 @@ int nkv_cache8_attend(void* stream, const nkv_cache8_attend_args* args, void* wo
  * finite adds nothing: one that sees no key, or whose query holds NaN or
  * infinities (its weights would stay in mass for good).  mass and out are [B, H,
  * cap] fp32 and may be the same array, whose entries past the length are then not
- * touched (otherwise they are copied).  Q = 0 adds nothing (lse may be NULL).
+ * touched (otherwise they are copied); out and the workspace overlap nothing else
+ * of the call.  Q = 0 adds nothing (lse may be NULL).
  * Deterministic: no atomics.
  */
 typedef struct nkv_cache8_mass_args {

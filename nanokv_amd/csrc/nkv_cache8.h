@@ -247,6 +247,14 @@ __device__ __forceinline__ float rows4_sum(float x) {
     return halfwave_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// Bytes of an array of a call, for tests of overlap (host; none where `bytes` is 0).
+struct Range {
+    uintptr_t lo, hi;
+    Range(const void* p, int64_t bytes)
+        : lo(reinterpret_cast<uintptr_t>(p)), hi(reinterpret_cast<uintptr_t>(p) + (uintptr_t)bytes) {}
+    bool meets(const Range& o) const { return lo < o.hi && o.lo < hi; }
+};
+
 // Validates a cache and its shapes (host).
 int cache8_check(const nkv_cache8* c, const char* who);
 

@@ -34,13 +34,6 @@ int cache8_check(const nkv_cache8* c, const char* who) {
 
 namespace {
 
-struct Range {
-    uintptr_t lo, hi;
-    Range(const void* p, int64_t bytes)
-        : lo(reinterpret_cast<uintptr_t>(p)), hi(reinterpret_cast<uintptr_t>(p) + (uintptr_t)bytes) {}
-    bool meets(const Range& o) const { return lo < o.hi && o.lo < hi; }
-};
-
 // ---------------------------------------------------------------- write
 struct WriteParams {
     uint8_t* codes[2];            // K, V
@@ -721,6 +714,10 @@ extern "C" int nkv_cache8_write(void* stream, const nkv_cache8_write_args* a) {
         for (int j = 0; j < i; ++j)
             NKV_REQUIRE(!out[i].meets(out[j]), NKV_ERR_INVALID,
                         "the cache's codes and scales overlap each other");
+    for (const Range& r : out)
+        NKV_REQUIRE(!r.meets({a->start_dev, a->start_dev ? c.B * 4 : 0}) &&
+                        !r.meets({a->counts, a->counts ? c.B * 4 : 0}),
+                    NKV_ERR_INVALID, "the cache overlaps start_dev or counts");
     WriteParams p{{(uint8_t*)c.k, (uint8_t*)c.v}, {c.k_scale, c.v_scale}, {a->k, a->v},
                   {a->k_sb, a->v_sb}, {a->k_st, a->v_st}, {a->k_sh, a->v_sh},
                   a->start_dev, a->counts, c.cap, a->start, a->T, c.B, c.H, c.D};

@@ -1230,6 +1230,18 @@ int check_attend(const nkv_cache8_attend_args* a, Plan& pl) {
         NKV_REQUIRE(stride >= end, NKV_ERR_INVALID, "out's rows overlap");
         end += (__int128)stride * (count - 1);
     }
+    // what is written and what is read; an out with gaps may have anything in them
+    const nkv_cache8& c = a->cache;
+    const int64_t heads = (int64_t)c.B * c.H, codes = heads * c.cap * c8_pitch(c.D);
+    const int64_t rows = heads * a->G * a->Q;
+    const Range in[6] = {{c.k, codes}, {c.v, codes}, {c.k_scale, heads * c.cap / 16},
+                         {c.v_scale, heads * c.cap / 16}, {a->length, a->length ? c.B * 4 : 0},
+                         {a->counts, a->counts ? c.B * 4 : 0}};
+    const Range lse(a->lse, a->lse ? rows * 4 : 0), out(a->out, end == rows * c.D ? rows * c.D * 2 : 0);
+    for (const Range& r : in)
+        NKV_REQUIRE(!r.meets(lse) && !r.meets(out), NKV_ERR_INVALID,
+                    "out or lse overlaps the cache, length or counts");
+    NKV_REQUIRE(!lse.meets(out), NKV_ERR_INVALID, "lse overlaps out");
     return NKV_OK;
 }
 
@@ -1376,7 +1388,15 @@ int check_mass(const nkv_cache8_mass_args* a) {
     const uintptr_t m = reinterpret_cast<uintptr_t>(a->mass), o = reinterpret_cast<uintptr_t>(a->out);
     NKV_REQUIRE(m == o || m >= o + bytes || o >= m + bytes, NKV_ERR_INVALID,
                 "out must be mass itself or not overlap it");
-    NKV_REQUIRE((int64_t)a->cache.B * a->cache.H <= 65535, NKV_ERR_UNSUPPORTED, "too many heads");
+    const nkv_cache8& c = a->cache;
+    const int64_t heads = (int64_t)c.B * c.H;
+    NKV_REQUIRE(heads <= 65535, NKV_ERR_UNSUPPORTED, "too many heads");
+    const Range in[5] = {{c.k, heads * c.cap * c8_pitch(c.D)}, {c.k_scale, heads * c.cap / 16},
+                         {a->lse, heads * a->G * a->Q * 4}, {a->length, a->length ? c.B * 4 : 0},
+                         {a->counts, a->counts ? c.B * 4 : 0}};
+    for (const Range& r : in)
+        NKV_REQUIRE(!r.meets({a->out, bytes}), NKV_ERR_INVALID,
+                    "out overlaps the cache's keys, lse, length or counts");
     return NKV_OK;
 }
 

@@ -1396,7 +1396,8 @@ class Cache8:
     def empty(cls, B: int, H: int, cap: int, head_dim: int, device: torch.device,
               format: str = "int8") -> "Cache8":
         """A cache of no rows with room for cap of them (rounded up to whole
-        blocks); format "int8" or "e4m3"."""
+        blocks); format "int8" or "e4m3".  Codes are 0 and scales 1, so rows that a
+        first write leaves out before its start are zeros of that scale."""
         if format not in _CACHE8_FORMATS:
             raise ValueError(f"format must be one of {sorted(_CACHE8_FORMATS)}")
         if head_dim < 1 or head_dim % 8 or head_dim > 128:
@@ -1493,9 +1494,9 @@ def cache8_write(cache: Cache8, k: torch.Tensor, v: torch.Tensor, start,
     k, v: [B, T, H, head_dim] bf16, fp16 or fp32 (any strides divisible by 8,
     contiguous columns).  start: the row of each sequence's first new token, an
     int for all or an int32 tensor [B] on the device (so that a captured graph
-    can move on); a tensor's entries are clamped to [0, cap] and rows past cap
-    dropped, an int that does not leave room for T rows is refused.  counts:
-    int32 [B], how many of a sequence's T rows are written (a padded batch)."""
+    can move on); a tensor's entries are clamped to [0, cap].  counts: int32 [B],
+    how many of a sequence's T rows are written, the first ones (a padded batch).
+    Rows past cap are dropped with either tensor, and refused with neither."""
     given = start if isinstance(start, torch.Tensor) else None
     device = _require_gpu(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, given, counts)
     c = cache.struct()

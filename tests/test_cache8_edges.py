@@ -9,7 +9,8 @@ from pathlib import Path
 import pytest
 import torch
 
-from nanokv_amd import build, ops
+from nanokv_amd import _lib, build, ops
+from tests import test_cache8 as t
 from tests.test_device_attributes import SHIM
 
 ROOT = Path(__file__).resolve().parent.parent
@@ -67,3 +68,43 @@ def test_the_wrappers_refuse_counts_of_another_kind():
     for bad in (ints.long(), ints[:1], torch.zeros(4, dtype=torch.int32)[::2]):
         with pytest.raises(ValueError, match="counts"):
             ops._cache8_ints(bad, 2, "counts")
+
+
+@pytest.mark.parametrize("what", ["k", "v", "k_scale", "v_scale", "length", "counts", "lse"])
+def test_attend_refuses_outputs_over_what_it_reads(what):
+    """Workgroups would read what others have written."""
+    base = t.PTR + (16 << 24)
+    a = t.attend_args(Q=3, length=base, counts=base + 4096, lse=base + 8192)
+    lib = _lib.lib()
+    lib.nkv_cache8_attend_workspace_size(ctypes.byref(a))
+    assert lib.nkv_last_error() == b""
+    at = getattr(a.cache, what) if hasattr(a.cache, what) else getattr(a, what)
+    a.out = at
+    t.refused("nkv_cache8_attend", a, _lib.NKV_ERR_INVALID, b"overlap", None, 0)
+    a.o_st *= 2                               # gaps, which may hold anything
+    a.o_sb *= 2
+    lib.nkv_cache8_attend_workspace_size(ctypes.byref(a))
+    assert lib.nkv_last_error() == b""
+    if what != "lse":
+        a = t.attend_args(Q=3, length=base, counts=base + 4096, lse=at)
+        t.refused("nkv_cache8_attend", a, _lib.NKV_ERR_INVALID, b"overlap", None, 0)
+
+
+@pytest.mark.parametrize("what", ["k", "k_scale", "length", "counts", "lse"])
+def test_mass_refuses_outputs_over_what_it_reads(what):
+    base = t.PTR + (16 << 24)
+    a = t.attend_args(_lib.NkvCache8MassArgs, Q=3, length=base, counts=base + 4096, lse=base + 8192)
+    lib = _lib.lib()
+    lib.nkv_cache8_mass_workspace_size(ctypes.byref(a))
+    assert lib.nkv_last_error() == b""
+    a.out = getattr(a.cache, what) if hasattr(a.cache, what) else getattr(a, what)
+    t.refused("nkv_cache8_mass", a, _lib.NKV_ERR_INVALID, b"overlap", None, 0)
+    a.mass = a.out                            # in place no less
+    t.refused("nkv_cache8_mass", a, _lib.NKV_ERR_INVALID, b"overlap", None, 0)
+
+
+@pytest.mark.parametrize("name", ["start_dev", "counts"])
+def test_write_refuses_a_cache_over_its_starts_or_counts(name):
+    c = t.cache()
+    for at in (c.k + 64, c.v, c.k_scale + 4, c.v_scale):
+        t.refused("nkv_cache8_write", t.write_args(**{name: at}), _lib.NKV_ERR_INVALID, b"overlaps")
