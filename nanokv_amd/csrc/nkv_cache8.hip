@@ -450,14 +450,16 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(EvictParams p) {
 // memory, nothing to clear), finds the digit and with it how many rows the parts
 // before its own keep; the fourth lists.  Bound by the chain of four launches (4.9,
 // 7.9, 7.8 and 10.5 us for one head of 131,072 rows; masses loaded ahead of the
-// sums change nothing there and cost 10 % of a full chip's): whole evictions of
-// that head 34.7 us and of 1,000,000 rows 65 us, where one workgroup that read the
-// masses five times took 141 and 1,028; 64 heads of 65,536 rows 118 (146).  At
-// SEL_LDS rows and below the chain costs more than it spreads (8 heads of 32,768
+// sums change nothing there and cost 10 % of a full chip's).  Whole evictions of
+// width 64, a quarter kept: that head 34 us, where one workgroup that read the
+// masses five times took 141; one of 1,000,000 rows 73; 64 heads of 65,536 rows 118
+// (146 with one workgroup a head; at width 128, with twice the codes to move, 157).
+// At SEL_LDS rows and below the chain costs more than it spreads (8 heads of 32,768
 // rows: 34.7 us against select_kernel's 32.3, 64 heads: 65.6 against 60.8, 8 heads
 // of 16,384: 30.8 against 21.4).  Parts of 4,096 rows add up twice the counts (64
-// heads of 65,536 rows: 143 us), of 16,384 lengthen the chain (one head of
-// 131,072: 39), and 128 parts a head instead of 64 add up more (1,000,000: 78).
+// heads of 65,536 rows: 143 us), of 16,384 lengthen the chain (one head of 131,072:
+// 39), and 128 parts a head instead of 64 add up more (one head of 1,000,000 rows, an
+// earlier measure: 78 us against 65).
 constexpr int PART_ROWS = 8192, PARTS = 64;
 
 int part_rows(int64_t n) {

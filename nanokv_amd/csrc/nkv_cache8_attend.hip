@@ -201,9 +201,10 @@ __device__ __forceinline__ void store_partial(const AttendParams& p, int bh, int
 // eight, 8 key heads of 4 query heads: 1 x 8,192 rows 10.8, 13.6; 8 x 2,048
 // 12.5, 11.6; 32 x 1,024 16.7, 14.0; 32 x 4,096 45.3, 42.2).  Long calls are
 // bound by the read of the codes: 32 ragged sequences up to 16,384 rows, 736 MB,
-// 124 us, 5.9 TB/s (a copy moves 5.2); one query over 2 heads of 262,144 rows,
-// 134 MB, 25 us.  Loads issued a block ahead changed neither (a wave's 24 loads
-// of 16 KB are in flight together, and two waves a SIMD cover the rest).
+// 125 us, 5.9 TB/s (a kernel that only reads moves 6.5, a copy 5.1); one query over
+// 2 heads of 262,144 rows, 134 MB, 25 us.  Loads issued a block ahead changed
+// neither, all 24 of a block before its first product cost 4 % (K's eight are in
+// flight together, V's behind them).
 constexpr int64_t ROWS_EIGHT = 2048;  // blocks in all heads
 
 template <int P, int W, int NQ>
@@ -435,14 +436,16 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
 // product s, lane half h) at chunk ^ vsw(R): reads of eight consecutive rows,
 // and writes of every fourth row, meet eight different chunks.
 //
-// 1,560 queries over 12,480 rows of 24 heads: 239 GFLOP in 269 us, 890 TFLOP/s (a
-// large bf16 product reaches 1,337 here).  The bound is the chip's power more than
-// any unit: MFMAs alone, on random data, run at 20.7 ns each where the clock
-// allows 13, and orders of the same work (scores a block ahead, operands read
+// 1,560 queries over 12,480 rows of 24 heads: 239 GFLOP in 268 - 286 us over several
+// cards, 840 - 890 TFLOP/s (a large bf16 product reaches 1,337).  MFMAs are busy for
+// 36 % of the SIMDs' cycles and the other VALU instructions (softmax, conversions,
+// addresses) for 53 %, at 2.3 of 2.4 GHz: the two waves a SIMD run them beside each
+// other too little.  Orders of the same work (scores a block ahead, operands read
 // ahead, one or two chains of products, priorities or none) took 290 - 294 us all;
-// without LDS operand reads 15 % less, without the exponentials nothing.  Width
-// 64 has half the products for the same softmax and is bound by its VALU work and
-// by one workgroup a CU (31 GFLOP in 59 us; 128 registers, for two, spill).
+// without LDS operand reads 15 % less.  Width 64 has half the products for the same
+// softmax (31 GFLOP in 62 us: MFMA 19 %, VALU 41 %; sequences of unlike lengths
+// leave part of the chip idle) and one workgroup a CU (128 registers, for two,
+// spill).
 constexpr int TILE_WAVES = 8;
 
 __device__ __forceinline__ int vsw(int R) { return ((R >> 2) ^ ((R & 3) << 1)) & 7; }
@@ -696,7 +699,7 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
 // sum(2^(wm - W) lw o) / sum(2^(m - M) l).
 // SG groups share a row's splits and are joined in LDS; a thread has AHEAD
 // splits' loads in flight.  37,440 rows of 3 splits (30 MB) 7.8 us, 16 rows of 256
-// 4.5 us (309 us with one thread walking all of a row's splits).
+// 4.6 us (309 us with one thread walking all of a row's splits).
 template <typename T, int P, int SG, int AHEAD>
 __global__ void __launch_bounds__(256) merge_kernel(AttendParams p) {
     constexpr int PARTS = P / 8, ROWS = 256 / (PARTS * SG);
@@ -949,9 +952,9 @@ __global__ void __launch_bounds__(256) mass_kernel(MassParams p) {
 // loaded into registers a step ahead, one barrier a step): read by every wave
 // from the cache, they would take all of its bandwidth.  Rows are split over
 // workgroups where there are few blocks of keys.  1,560 queries over 12,480 rows
-// of 24 heads: 120 GFLOP in 149 us, 805 TFLOP/s; per 32 rows a wave has 512 cycles
-// of MFMA and as many of exponentials and sums, two waves a SIMD (scores held a
-// step ahead to run the two together spill: 258 us).
+// of 24 heads: 120 GFLOP in 150 us, 800 TFLOP/s, with MFMAs busy for 33 % of the
+// SIMDs' cycles and the other VALU instructions (exponentials and sums) for 50 %, two
+// waves a SIMD (scores held a step ahead to run the two together spill: 258 us).
 constexpr int MT_ROWS = 64;
 
 template <typename T, int P>
