@@ -345,3 +345,41 @@ def test_softmax_scales_of_any_size(dev, Q, G, causal, softmax_scale):
     rm, tol = ref.mass(q.double().cpu().numpy(), cache_values(cache, "int8")[0],
                        lse.double().cpu().numpy(), np.zeros((1, 1, 192)), [170], causal, softmax_scale)
     assert (np.abs(m.double().cpu().numpy() - rm) <= tol).all()
+
+
+@pytest.mark.parametrize("T,N", [(3, 5000), (90, 5000)])
+def test_counts_of_a_captured_call_may_change(dev, T, N):
+    """One graph of a write, attention and weight, replayed with other counts and
+    lengths, equals eager calls between the replays; so it does on a stream of its own."""
+    B, H, G, D = 3, 2, 2, 128
+    ints = dict(dtype=torch.int32, device=dev)
+    base = make_cache(dev, B, H, N + T, D, "e4m3", 122)
+    x = torch.randn((3, B, T, H * G, D), generator=torch.Generator().manual_seed(123)).half().to(dev)
+    start, counts = torch.zeros(B, **ints), torch.zeros(B, **ints)
+    m0 = torch.zeros((B, H, base.cap), device=dev)
+
+    def calls():
+        c = ops.Cache8(*(t.clone() for t in (base.k, base.v, base.k_scale, base.v_scale)), D)
+        ops.cache8_write(c, x[0, :, :, :H], x[1, :, :, :H], start, counts)
+        n = start + counts
+        out, lse = ops.cache8_attend(x[2], c, n, causal=True, counts=counts)
+        return out, lse, ops.cache8_mass(x[2], c, lse, m0, n, out=torch.empty_like(m0), causal=True,
+                                         counts=counts), c.k, c.v_scale
+
+    calls()
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        got = calls()
+    for st, ct in (([0, 70, N], [T, 1, T]), ([N, 0, 5], [T - 1, 0, T]), ([1, 2, 3], [0, 0, 0]),
+                   ([N, N, N], [T, T, T])):
+        start.copy_(torch.tensor(st))
+        counts.copy_(torch.tensor(ct))
+        graph.replay()
+        torch.cuda.synchronize()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = calls()
+        torch.cuda.current_stream().wait_stream(side)
+        for a, b, c in zip(got, calls(), other):
+            assert torch.equal(a, b) and torch.equal(a, c)
