@@ -64,7 +64,7 @@
 extern "C" {
 #endif
 
-#define NKV_ABI_VERSION 10
+#define NKV_ABI_VERSION 11
 
 enum nkv_status {
     NKV_OK = 0,
@@ -929,6 +929,170 @@ typedef struct nkv_cache8_evict_args {
 size_t nkv_cache8_evict_workspace_size(const nkv_cache8_evict_args* args);
 int nkv_cache8_evict(void* stream, const nkv_cache8_evict_args* args, void* workspace,
                      size_t workspace_bytes);
+
+/*
+ * A paged key/value cache (no counterpart in the reference): pools of pages that
+ * many sequences share, `page` rows of all H key heads each, in bf16 or fp16.  Row r
+ * of head h of page p is k[((p*H + h)*page + r)*D + d]; v likewise.  page is a
+ * power of two in [16, 1024]; D % 8 == 0, D <= 128; 1 <= pages < 2^31; H * page * D
+ * <= 2^29; k and v are 16-byte aligned.
+ * A page table [B, table_w] (int32, device; item b's entries from table +
+ * b*table_sb on) names the pages of B sequences: row n of sequence b is row n %
+ * page of page table[b*table_sb + n / page].  Pages may lie in any order and be
+ * shared by sequences that only read them.  An entry outside [0, pages) names no
+ * page: its rows are seen by no query and written by no call.  The caller keeps
+ * the tables and each sequence's length; rows at or past it may hold anything, NaN
+ * included, as may rows that a query does not see: no call lets them into a result.
+ */
+typedef struct nkv_paged_cache {
+    void* k;                      /* [pages, H, page, D] */
+    void* v;
+    int64_t pages;
+    int H;
+    int page;
+    int D;
+    int dtype;                    /* NKV_ROWS_BF16 or NKV_ROWS_FP16 */
+} nkv_paged_cache;
+
+/*
+ * Writes T new rows of each of B sequences behind the `start` rows it has: row t of k
+ * and v ([B, T, H, D], addressed as k[b*k_sb + t*k_st + h*k_sh + d], of the cache's
+ * type or fp32, rounded once) goes to row start + t.  With freqs (fp32, device,
+ * rot / 2 of them) keys are rotated on the way, and the queries q [B, T, Hq, D], if
+ * given, into q_out (of the cache's type): pair i of a row's first rot columns turns
+ * by the angle position * freqs[i], (a, b) to (a cos - b sin, b cos + a sin).  Pair i
+ * is columns i and i + rot / 2 (rot % 16 == 0) or, with interleaved, columns 2 i and
+ * 2 i + 1 (rot % 8 == 0); the columns from rot on keep their values.  Angles are
+ * formed in 64 bits, products and sums in fp32.  positions (device, item b's from
+ * positions + b*pos_sb on; NULL: row t's is start + t) may be any int32.
+ * start_dev (device, [B]; NULL: `start` for every item) is clamped to [0, table_w *
+ * page]; counts (device, [B]; NULL: T) says how many of an item's rows there are:
+ * the rest are not written, neither in the cache nor in q_out.  Rows past the table
+ * are dropped where start or counts are in device memory, and refused where neither
+ * is.
+ * Rows are 16-byte aligned with strides divisible by 8.  q_out may be q itself and
+ * overlaps nothing else of the call, nor do its rows each other; the pools overlap
+ * neither each other nor anything else of the call, and no row is written twice:
+ * no two sequences write into the same page.
+ */
+typedef struct nkv_paged_append_args {
+    nkv_paged_cache cache;
+    const int32_t* table;
+    int64_t table_sb;
+    int64_t table_w;
+    const void* k;
+    int64_t k_sb, k_st, k_sh;
+    const void* v;
+    int64_t v_sb, v_st, v_sh;
+    const void* q;                /* or NULL */
+    int64_t q_sb, q_st, q_sh;
+    void* q_out;
+    int64_t o_sb, o_st, o_sh;
+    const float* freqs;           /* or NULL: nothing is rotated */
+    const int32_t* positions;     /* or NULL */
+    int64_t pos_sb;
+    int64_t T;
+    int64_t start;
+    const int32_t* start_dev;     /* or NULL */
+    const int32_t* counts;        /* or NULL */
+    int B;
+    int Hq;
+    int rot;
+    int interleaved;
+    int dtype;                    /* of k, v and q: the cache's, or NKV_ROWS_FP32 */
+    int _pad;
+} nkv_paged_append_args;
+
+int nkv_paged_append(void* stream, const nkv_paged_append_args* args);
+
+/*
+ * Attention of q [B, Q, H*G, D] (of the cache's type; q[b*q_sb + t*q_st + h*q_sh +
+ * d]) over a paged cache: query head h reads key head h / G, softmax(q k^T *
+ * softmax_scale) v over the sequence's first `length` rows.
+ *   length   device [B], clamped to [0, n] (NULL: n for every item); n <= table_w *
+ *            page is also what the work is divided by
+ *   counts   device [B], clamped to [0, Q] (NULL: Q): how many of an item's Q rows
+ *            are queries, the first ones; a row past them sees no key
+ *   causal   query t sees the first length - counts + 1 + t rows (the queries are
+ *            the sequence's last tokens)
+ *   parents  device int32 (item b's Q entries from parents + b*parents_sb on;
+ *            parents_sb may be 0), or NULL: the queries are a tree of drafted tokens
+ *            whose rows are the sequence's last counts ones, in the queries' order.
+ *            Query t sees the rows before them, its own and those of parents[t], of
+ *            that one's parent and so on; an entry outside [0, t) ends the way.  Q <=
+ *            NKV_PAGED_TREE; not with causal.
+ * A query that sees no key gets out = 0 and lse = -inf.
+ *   out  [B, Q, H*G, D] of q's type (o_sb/o_st/o_sh)
+ *   lse  [B, H*G, Q] fp32 natural-log row log-sum-exp, or NULL
+ * Scores, softmax and sums are fp32; for their product with the values the weights,
+ * relative to the row's largest one, are rounded to the cache's type (bf16 caches
+ * in calls of few rows: to twice its bits).
+ * q and out are 16-byte aligned with strides divisible by 8; out's rows do not
+ * overlap.  out may be q itself; otherwise out, lse and the workspace overlap
+ * nothing of the call.
+ */
+#define NKV_PAGED_TREE 256
+typedef struct nkv_paged_attend_args {
+    nkv_paged_cache cache;
+    const int32_t* table;
+    int64_t table_sb;
+    int64_t table_w;
+    int B;
+    int G;
+    int64_t Q;
+    int64_t n;
+    const int32_t* length;        /* or NULL */
+    const int32_t* counts;        /* or NULL */
+    const int32_t* parents;       /* or NULL */
+    int64_t parents_sb;
+    const void* q;
+    int64_t q_sb, q_st, q_sh;
+    void* out;
+    int64_t o_sb, o_st, o_sh;
+    float* lse;                   /* or NULL */
+    float softmax_scale;
+    int causal;
+} nkv_paged_attend_args;
+
+/* Bytes of workspace nkv_paged_attend wants for these arguments (0 if none), for
+ * the partial results of its key splits; 16-byte aligned.  In a smaller one, or
+ * none, it takes fewer splits (the same attention within rounding). */
+size_t nkv_paged_attend_workspace_size(const nkv_paged_attend_args* args);
+int nkv_paged_attend(void* stream, const nkv_paged_attend_args* args, void* workspace,
+                     size_t workspace_bytes);
+
+/*
+ * Keeps the accepted tokens of a draft: in each of n_caches caches of one geometry (a
+ * model's layers), row start + rows[b*rows_sb + j] of sequence b moves to row start +
+ * j, j < counts.  Every row is read before any is written, so rows may name them in
+ * any order, the same one twice among them.  A row that comes from or goes to no
+ * page, or comes from a negative row, is not written.
+ *   rows        int32, device, M entries an item, M <= NKV_PAGED_COMMIT
+ *   start_dev, counts: as nkv_paged_append's (NULL: start; M)
+ *   out_length  [B] int32, start + counts (both as clamped), or NULL
+ * caches is an array in host memory, of at most NKV_PAGED_CACHES.  The pools overlap neither each other nor
+ * anything else of the call; no two sequences write into the same page, and none
+ * into one that another reads here.
+ */
+#define NKV_PAGED_COMMIT 256
+#define NKV_PAGED_CACHES 64
+typedef struct nkv_paged_commit_args {
+    const nkv_paged_cache* caches;
+    int64_t n_caches;
+    const int32_t* table;
+    int64_t table_sb;
+    int64_t table_w;
+    const int32_t* rows;
+    int64_t rows_sb;
+    int64_t start;
+    const int32_t* start_dev;     /* or NULL */
+    const int32_t* counts;        /* or NULL */
+    int32_t* out_length;          /* or NULL */
+    int B;
+    int M;
+} nkv_paged_commit_args;
+
+int nkv_paged_commit(void* stream, const nkv_paged_commit_args* args);
 
 #ifdef __cplusplus
 }

@@ -13,7 +13,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libnanokv_hip.so"
 
-NKV_ABI_VERSION = 10
+NKV_ABI_VERSION = 11
 NKV_OK = 0
 NKV_ERR_INVALID = -1
 NKV_ERR_UNSUPPORTED = -2
@@ -33,6 +33,9 @@ NKV_CACHE8_E4M3 = 1
 NKV_ROWS_BF16 = 0
 NKV_ROWS_FP16 = 1
 NKV_ROWS_FP32 = 2
+NKV_PAGED_TREE = 256
+NKV_PAGED_COMMIT = 256
+NKV_PAGED_CACHES = 64
 
 # Every symbol include/nanokv.h declares (checked by tests/test_abi.py).
 EXPORTED = (
@@ -45,6 +48,8 @@ EXPORTED = (
     "nkv_cache8_write", "nkv_cache8_attend_workspace_size", "nkv_cache8_attend",
     "nkv_cache8_mass_workspace_size", "nkv_cache8_mass",
     "nkv_cache8_evict_workspace_size", "nkv_cache8_evict",
+    "nkv_paged_append", "nkv_paged_attend_workspace_size", "nkv_paged_attend",
+    "nkv_paged_commit",
 )
 NKV_STATIC_SCRATCH_BYTES = 64 << 20
 
@@ -254,6 +259,51 @@ class NkvCache8EvictArgs(Structure):
     ]
 
 
+class NkvPagedCache(Structure):
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("pages", c_int64), ("H", c_int), ("page", c_int),
+        ("D", c_int), ("dtype", c_int),
+    ]
+
+
+class NkvPagedAppendArgs(Structure):
+    _fields_ = [
+        ("cache", NkvPagedCache),
+        ("table", c_void_p), ("table_sb", c_int64), ("table_w", c_int64),
+        ("k", c_void_p), ("k_sb", c_int64), ("k_st", c_int64), ("k_sh", c_int64),
+        ("v", c_void_p), ("v_sb", c_int64), ("v_st", c_int64), ("v_sh", c_int64),
+        ("q", c_void_p), ("q_sb", c_int64), ("q_st", c_int64), ("q_sh", c_int64),
+        ("q_out", c_void_p), ("o_sb", c_int64), ("o_st", c_int64), ("o_sh", c_int64),
+        ("freqs", c_void_p), ("positions", c_void_p), ("pos_sb", c_int64),
+        ("T", c_int64), ("start", c_int64), ("start_dev", c_void_p), ("counts", c_void_p),
+        ("B", c_int), ("Hq", c_int), ("rot", c_int), ("interleaved", c_int), ("dtype", c_int),
+        ("_pad", c_int),
+    ]
+
+
+class NkvPagedAttendArgs(Structure):
+    _fields_ = [
+        ("cache", NkvPagedCache),
+        ("table", c_void_p), ("table_sb", c_int64), ("table_w", c_int64),
+        ("B", c_int), ("G", c_int), ("Q", c_int64), ("n", c_int64),
+        ("length", c_void_p), ("counts", c_void_p), ("parents", c_void_p),
+        ("parents_sb", c_int64),
+        ("q", c_void_p), ("q_sb", c_int64), ("q_st", c_int64), ("q_sh", c_int64),
+        ("out", c_void_p), ("o_sb", c_int64), ("o_st", c_int64), ("o_sh", c_int64),
+        ("lse", c_void_p), ("softmax_scale", c_float), ("causal", c_int),
+    ]
+
+
+class NkvPagedCommitArgs(Structure):
+    _fields_ = [
+        ("caches", POINTER(NkvPagedCache)), ("n_caches", c_int64),
+        ("table", c_void_p), ("table_sb", c_int64), ("table_w", c_int64),
+        ("rows", c_void_p), ("rows_sb", c_int64), ("start", c_int64),
+        ("start_dev", c_void_p), ("counts", c_void_p), ("out_length", c_void_p),
+        ("B", c_int), ("M", c_int),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -331,6 +381,14 @@ def _declare(lib: ctypes.CDLL) -> None:
         run = getattr(lib, f"nkv_cache8_{name}")
         run.restype = c_int
         run.argtypes = [c_void_p, POINTER(args), c_void_p, c_size_t]
+    lib.nkv_paged_append.restype = c_int
+    lib.nkv_paged_append.argtypes = [c_void_p, POINTER(NkvPagedAppendArgs)]
+    lib.nkv_paged_attend_workspace_size.restype = c_size_t
+    lib.nkv_paged_attend_workspace_size.argtypes = [POINTER(NkvPagedAttendArgs)]
+    lib.nkv_paged_attend.restype = c_int
+    lib.nkv_paged_attend.argtypes = [c_void_p, POINTER(NkvPagedAttendArgs), c_void_p, c_size_t]
+    lib.nkv_paged_commit.restype = c_int
+    lib.nkv_paged_commit.argtypes = [c_void_p, POINTER(NkvPagedCommitArgs)]
 
 
 def lib() -> ctypes.CDLL:

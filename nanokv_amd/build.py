@@ -41,6 +41,8 @@ SOURCES = {
     "nkv_cache8.hip": ["-ffp-contract=off"],
     # (NaN kept: a NaN query's row is NaN, and no other)
     "nkv_cache8_attend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "nkv_paged.hip": [],
+    "nkv_paged_attend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 COMMON = [

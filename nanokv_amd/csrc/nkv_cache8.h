@@ -138,6 +138,7 @@ struct Partial32 {
 struct Bf16 {
     using x8 = bf16x8;
     using Partial = Partial16;
+    static __device__ __forceinline__ float to_f32(uint16_t b) { return bf16_bits_to_f32(b); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
     // e4m3 codes 2 h and 2 h + 1 of a word
     template <int h>
@@ -155,6 +156,7 @@ struct Bf16 {
 struct Fp16 {
     using x8 = f16x8;
     using Partial = Partial32;
+    static __device__ __forceinline__ float to_f32(uint16_t b) { return f16_bits_to_f32(b); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         f16x2 v;
         v[0] = (_Float16)a;

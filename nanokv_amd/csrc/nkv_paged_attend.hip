@@ -1,0 +1,778 @@
+// nkv_paged_attend.hip -- attention over the paged key/value cache
+// (nkv_paged_attend): tokens, causal chunks, frames and trees of drafted tokens.
+//
+// out = sum_j p_j v_j / sum_j p_j with p_j = 2^(z_j - m), z = softmax_scale log2(e)
+// q.k, over the keys a query sees, with the running maximum m of a row at most TAU
+// behind; l = sum p in fp32.  The scores' products are exact and added in fp32.
+//
+// What a query does not see does not reach its result, whatever it holds: a masked
+// score becomes -inf before the softmax, and values that are not finite (which a zero
+// weight would not remove) leave the product and are added apart to the rows that
+// see them.
+#include "nkv_paged.h"
+
+#include <math.h>
+
+#include <algorithm>
+#include <utility>
+
+namespace nkv {
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr float TAU = 3.0f;           // a row's maximum is moved when it is off by 2^TAU
+
+// The 16-bit types as weights and values.  LIFT: fp16 weights are held 2^12 higher
+// (2^(12 + TAU) < 65504), so that they keep all 11 bits down to 2^-26 of the row's
+// largest.
+template <typename T>
+struct Value;
+template <>
+struct Value<Bf16> {
+    static constexpr float LIFT = 0.0f;
+    static constexpr uint32_t EXP = 0x7f807f80u, STEP = 0x00800080u, FRAC = 0x007fu;
+    static constexpr uint32_t ONE = 0x3f80u, N128 = 0x4300u, N129 = 0x4301u;
+};
+template <>
+struct Value<Fp16> {
+    static constexpr float LIFT = 12.0f;
+    static constexpr uint32_t EXP = 0x7c007c00u, STEP = 0x04000400u, FRAC = 0x03ffu;
+    static constexpr uint32_t ONE = 0x3c00u, N128 = 0x5800u, N129 = 0x5808u;
+};
+
+// The high bit of each half of a word that is not finite.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    return ((w & Value<T>::EXP) + Value<T>::STEP) & 0x80008000u;
+}
+
+// A word's two values in two parts: the finite ones (0 in place of the others), and
+// what the others are, as numbers whose sums tell them apart: +inf 1, -inf 128, NaN
+// 129 (exact in either type).
+template <typename T>
+__device__ __forceinline__ void part_word(uint32_t w, uint32_t& finite, uint32_t& kind) {
+    finite = kind = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t x = (w >> (16 * h)) & 0xffffu;
+        const bool bad = (x & Value<T>::EXP & 0xffffu) == (Value<T>::EXP & 0xffffu);
+        const uint32_t k = x & Value<T>::FRAC ? Value<T>::N129 : x & 0x8000u ? Value<T>::N128 : Value<T>::ONE;
+        if (bad) kind |= k << (16 * h);
+        else finite |= x << (16 * h);
+    }
+}
+// What a sum of such numbers (up to 32 of them) adds to a result.
+__device__ __forceinline__ float parted(float o, float sum) {
+    if (sum == 0.0f) return o;
+    const int n = (int)sum;
+    const float up = n & 127 ? INFINITY : 0.0f, down = n >= 128 ? -INFINITY : 0.0f;
+    return o + up + down;
+}
+
+struct AttendParams {
+    PageTable table;
+    const uint16_t* k;
+    const uint16_t* v;
+    const int32_t* length;
+    const int32_t* counts;
+    const int32_t* parents;
+    int64_t parents_sb;
+    const uint16_t* q;
+    uint16_t* out;
+    float* lse;
+    // partial results of the splits, [B*H][splits][rows]: the output's D sums (in units
+    // of 2^(m - LIFT)), and (m, l)
+    float* part;
+    f32x2* part_ml;
+    int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;
+    int64_t items;
+    float scale_log2;
+    int B, H, G, D, Q, n, causal, splits, groups, rows;
+    int page_d;
+};
+
+// Query row r of key head hk is query t = r / G of query head hk * G + r % G.
+struct RowAt {
+    int t, head;
+    bool there;
+};
+__device__ __forceinline__ RowAt row_at(int row, int hk, int G, int Q) {
+    const bool there = row < G * Q;
+    const int r = there ? row : 0;
+    return {r / G, hk * G + r % G, there};
+}
+
+// The queries of an item: `nq` of its Q rows, the last tokens of `len`.
+struct Queries {
+    int len, nq, causal, tree;
+    // keys that query t < nq sees without a gap from the first on, and any row t
+    __device__ __forceinline__ int sees(int t) const {
+        return causal ? len - nq + 1 + t : tree ? len - nq : len;
+    }
+    __device__ __forceinline__ int end(int t) const { return t >= nq ? 0 : sees(t); }
+    // the least that any of the queries t0 .. t1 sees so, and the end of all they see
+    __device__ __forceinline__ int least(int t0, int t1) const { return t1 >= nq ? 0 : sees(t0); }
+    __device__ __forceinline__ int most(int t0, int t1) const {
+        return t0 >= nq ? 0 : tree ? len : sees(min(t1, nq - 1));
+    }
+};
+__device__ __forceinline__ Queries queries_of(const AttendParams& p, int b) {
+    return {c8_length(p.length, b, p.n), c8_length(p.counts, b, p.Q), p.causal, p.parents != nullptr};
+}
+
+// ---------------------------------------------------------------- trees
+// For each of a workgroup's tokens one bit for every token of the draft that it sees:
+// its own and those on the way to the root.
+constexpr int TREE_WORDS = NKV_PAGED_TREE / 32;
+
+template <int TOKENS>
+struct TreeSmem {
+    int32_t parents[NKV_PAGED_TREE];
+    uint32_t bits[TOKENS][TREE_WORDS];
+};
+
+// Tokens t0 .. t0 + count, by all threads of the workgroup.  A way goes to lower tokens
+// only, so it ends.
+template <int TOKENS>
+__device__ __forceinline__ void tree_bits(TreeSmem<TOKENS>& sm, const AttendParams& p, int b, int nq,
+                                          int t0, int count) {
+    for (int i = threadIdx.x; i < p.Q; i += blockDim.x) sm.parents[i] = p.parents[b * p.parents_sb + i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < count; i += blockDim.x) {
+        uint32_t* bits = sm.bits[i];
+#pragma unroll
+        for (int w = 0; w < TREE_WORDS; ++w) bits[w] = 0;
+        for (int a = t0 + i < nq ? t0 + i : -1; a >= 0;) {
+            bits[a >> 5] |= 1u << (a & 31);
+            const int up = sm.parents[a];
+            a = up < a ? up : -1;
+        }
+    }
+    __syncthreads();
+}
+
+// 32 bits from bit `at` on, at > -32; bits below 0 are set (rows before the draft),
+// bits past the last are not.
+__device__ __forceinline__ uint32_t tree_word(const uint32_t* bits, int at) {
+    if (at < 0) return (bits[0] << -at) | ((1u << -at) - 1);
+    const int i = at >> 5;
+    const uint32_t lo = i < TREE_WORDS ? bits[i] : 0, hi = i + 1 < TREE_WORDS ? bits[i + 1] : 0;
+    return (uint32_t)((((uint64_t)hi << 32) | lo) >> (at & 31));
+}
+
+// The first n bits.
+__device__ __forceinline__ uint32_t low_bits(int n) {
+    return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1;
+}
+
+// ---------------------------------------------------------------- results
+// A row's running maximum (log2 units, -inf before the first key) and sum.
+struct Stat {
+    float m, l;
+};
+constexpr float NONE = -INFINITY;
+
+// 2^(m - M) of a part whose maximum is m (a part without keys has weight 0).
+__device__ __forceinline__ float weight(float m, float M) {
+    return m == NONE ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+}
+
+// Eight columns of a row's result, o in units of 2^(m - LIFT).
+template <typename T>
+__device__ __forceinline__ void store_row(const AttendParams& p, int b, int hk, int row, int d,
+                                          const Stat& st, const float (&o)[8]) {
+    const RowAt at = row_at(row, hk, p.G, p.Q);
+    if (!at.there || d >= p.D) return;
+    constexpr float DOWN = Value<T>::LIFT == 0.0f ? 1.0f : 1.0f / 4096.0f;
+    const float f = st.l == 0.0f ? 0.0f : DOWN / st.l;
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = o[k] * f;
+    *reinterpret_cast<u32x4*>(p.out + b * p.o_sb + at.t * p.o_st + at.head * p.o_sh + d) =
+        u32x4{T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(x[4], x[5]), T::pack(x[6], x[7])};
+    if (d == 0 && p.lse)
+        p.lse[((int64_t)b * p.H * p.G + at.head) * p.Q + at.t] =
+            st.l == 0.0f ? -INFINITY : st.m * LN2 + logf(st.l);  // (NaN for a NaN query)
+}
+static_assert(Value<Fp16>::LIFT == 12.0f, "store_row's 4,096");
+
+// The same as one split's partial result.
+__device__ __forceinline__ void store_partial(const AttendParams& p, int bh, int split, int row, int d,
+                                              const Stat& st, const float (&o)[8]) {
+    if (row >= p.rows || d >= p.D) return;
+    const int64_t i = ((int64_t)bh * p.splits + split) * p.rows + row;
+    f32x4* to = reinterpret_cast<f32x4*>(p.part + i * p.D + d);
+    to[0] = f32x4{o[0], o[1], o[2], o[3]};
+    to[1] = f32x4{o[4], o[5], o[6], o[7]};
+    if (d == 0) p.part_ml[i] = f32x2{st.m, st.l};
+}
+
+// The work of a workgroup: a group of query rows of a unit (head and key split).
+// Block i runs on XCD i % 8, and the groups of a unit take consecutive slots of one
+// XCD, whose L2 then serves all but the first read of its rows.  Units go to the XCDs
+// in turn, so that sequences of unlike lengths spread over them; with fewer than
+// UNITS units an XCD takes a run of (unit, group) pairs instead.
+constexpr int UNITS = 32;
+
+struct Item {
+    uint32_t unit;
+    int group;
+    bool there;
+};
+
+__device__ __forceinline__ Item item_of(const AttendParams& p) {
+    const uint32_t x = blockIdx.x & 7, k = blockIdx.x >> 3, groups = (uint32_t)p.groups;
+    const uint32_t items = (uint32_t)p.items, units = items / groups;
+    if (units >= UNITS) {
+        const uint32_t u = k / groups * 8 + x;
+        return {u, (int)(k % groups), u < units};
+    }
+    const uint32_t item = x * ((items + 7) >> 3) + k, u = item / groups;
+    return {u, (int)(item - u * groups), item < items && k < (items + 7) >> 3};
+}
+
+// ---------------------------------------------------------------- few rows
+// W waves of a workgroup share NQ groups of 16 query rows and a range of 32-key tiles;
+// each wave walks a run of tiles of its own, straight from memory into registers, and
+// the waves' results are merged in LDS.  S^T = K Q^T on 16x16x32 MFMAs leaves lane (r,
+// g) = (lane % 16, lane / 16) the scores of row r and keys 16 t + 4 g + e, whose
+// weights are then the operand of O^T += V^T P^T without leaving the registers.  V's
+// columns 8 r .. 8 r + 7 are a lane's (4 r .. of narrow heads), so its transposition is
+// a choice of halves of eight rows' words.
+constexpr int TILE = 32;
+
+// Page numbers of a run of tiles, 64 at a time, a lane each.
+struct Pages {
+    const int32_t* at;
+    int w, first, ids;
+    __device__ __forceinline__ void load(int entry) {
+        first = entry;
+        ids = w ? at[min(entry + (int)(threadIdx.x & 63), w - 1)] : -1;
+    }
+    // entry `entry` (uniform; never below that of the last call by more than it has)
+    __device__ __forceinline__ uint32_t get(int entry) {
+        if (entry >= w) return ~0u;
+        if (entry - first >= 64) load(entry);
+        return (uint32_t)__builtin_amdgcn_readlane(ids, entry - first);
+    }
+};
+
+template <int D, int W, int NQ>
+struct RowsSmem {
+    union {
+        float o[W][16 * NQ][D + 4];
+        TreeSmem<16 * NQ> tree;
+    };
+    Stat st[W][16 * NQ];
+};
+
+template <int KS>
+constexpr int width_of() { return KS == 2 ? 64 : 128; }
+
+template <typename T, int KS, int W, int NQ>
+__global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
+    constexpr int DB = KS == 2 ? 4 : 8, WORDS = DB / 2, ROWS = 16 * NQ, P = width_of<KS>();
+    constexpr bool SPLIT = std::is_same_v<T, Bf16>;
+    using x8 = typename T::x8;
+    using V = Value<T>;
+    extern __shared__ __align__(16) unsigned char rows_smem[];
+    RowsSmem<P, W, NQ>& sm = *reinterpret_cast<RowsSmem<P, W, NQ>*>(rows_smem);
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Item it = item_of(p);
+    if (!it.there) return;
+    const int rg = it.group, bh = (int)(it.unit / (uint32_t)p.splits);
+    const int split = (int)(it.unit - (uint32_t)bh * p.splits), b = bh / p.H, hk = bh - b * p.H;
+    const Queries qs = queries_of(p, b);
+    const int row0 = rg * ROWS;
+    // tiles that some row of the group sees, and keys that every row does
+    const int t0 = row0 / p.G, t1 = min(row0 + ROWS - 1, p.rows - 1) / p.G;
+    const int last = max(0, qs.most(t0, t1)), first = qs.least(t0, t1);
+    const int nt = (last + TILE - 1) / TILE;
+    const int b0 = (int)((int64_t)split * nt / p.splits);
+    const int b1 = (int)((int64_t)(split + 1) * nt / p.splits);
+    x8 qf[NQ][KS];
+    int end[NQ];                              // keys that the lane's row sees
+    const uint32_t* bits[NQ];                 // and the draft's tokens
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const RowAt mine = row_at(row0 + 16 * n + r, hk, p.G, p.Q);
+        end[n] = mine.there ? qs.end(mine.t) : 0;
+        bits[n] = sm.tree.bits[mine.there ? mine.t - t0 : 0];
+        const uint16_t* q = p.q + b * p.q_sb + mine.t * p.q_st + mine.head * p.q_sh;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = 32 * s + 8 * g;
+            u32x4 w{};
+            if (mine.there && d < p.D) w = *reinterpret_cast<const u32x4*>(q + d);
+            qf[n][s] = as_x8<x8>(w);
+        }
+    }
+    if (qs.tree && b1 * TILE > first) tree_bits(sm.tree, p, b, qs.nq, t0, t1 - t0 + 1);
+    // this wave's tiles
+    const int w0 = b0 + (int)((int64_t)wave * (b1 - b0) / W), w1 = b0 + (int)((int64_t)(wave + 1) * (b1 - b0) / W);
+    const int shift = p.table.shift, page_rows = 1 << shift;
+    Pages pages{p.table.at + b * p.table.sb, (int)p.table.w, 0, 0};
+    // lane offsets into a page's rows of the head (elements)
+    uint32_t koff[KS], voff[4];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) koff[s] = r * p.D + (32 * s + 8 * g < p.D ? 32 * s + 8 * g : 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) voff[j] = (4 * g + j) * p.D + min(DB * r, p.D - DB);
+    const int64_t head = (int64_t)hk * p.page_d;
+    // the 16 keys from key on: their element in the pools (page 0's where there is no
+    // page, and `there` false)
+    auto at16 = [&](int key, bool& there) -> int64_t {
+        uint32_t id = pages.get(key >> shift);
+        there = id < p.table.pages;
+        id = there ? id : 0;
+        return (int64_t)id * p.table.page_elems + head + (int64_t)(key & (page_rows - 1)) * p.D;
+    };
+    u32x4 kr[2][KS];
+    uint32_t vr[8][WORDS];
+    int64_t at[2];
+    bool there[2], next_there[2];
+    auto load_k = [&](int tile) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            at[t] = at16(tile * TILE + 16 * t, next_there[t]);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) kr[t][s] = *reinterpret_cast<const u32x4*>(p.k + at[t] + koff[s]);
+        }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint16_t* from = p.v + at[t] + voff[j];
+                if constexpr (DB == 8) {
+                    const u32x4 w = *reinterpret_cast<const u32x4*>(from);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) vr[4 * t + j][i] = w[i];
+                } else {
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(from);
+                    vr[4 * t + j][0] = w[0];
+                    vr[4 * t + j][1] = w[1];
+                }
+            }
+    };
+    f32x4 o[NQ][DB];
+    // the largest score before its scale (a difference of scores is exact where it counts,
+    // however large they are), and l over the lane's own keys
+    Stat st[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        st[n] = {NONE, 0.0f};
+#pragma unroll
+        for (int i = 0; i < DB; ++i) o[n][i] = f32x4{};
+    }
+    if (w0 < w1) {
+        pages.load(w0 * TILE >> shift);
+        load_k(w0);
+        load_v();
+    }
+    for (int tile = w0; tile < w1; ++tile) {
+        const int key0 = tile * TILE;
+        there[0] = next_there[0], there[1] = next_there[1];
+        if (p.D != 32 * KS) {                 // (q is zero there, but not what was loaded)
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+                if (32 * s + 8 * g >= p.D) kr[0][s] = kr[1][s] = u32x4{};
+        }
+        f32x4 s[NQ][2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                s[n][t] = f32x4{};
+#pragma unroll
+                for (int i = 0; i < KS; ++i) s[n][t] = T::mfma16(as_x8<x8>(kr[t][i]), qf[n][i], s[n][t]);
+            }
+        // the next tile's keys go where this one's were
+        if (tile + 1 < w1) load_k(tile + 1);
+        if (key0 + TILE > first || !there[0] || !there[1]) {
+            const uint32_t paged = (there[0] ? 0xffffu : 0u) | (there[1] ? 0xffff0000u : 0u);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                uint32_t seen = low_bits(end[n] - key0);
+                if (qs.tree && end[n] - key0 < 32) seen = tree_word(bits[n], key0 - end[n]);
+                seen = (seen & paged) >> (4 * g);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!(seen >> (16 * t + e) & 1)) s[n][t][e] = -INFINITY;
+            }
+        }
+        // values that are not finite are kept apart, also from rows that see them all: half
+        // a weight may be zero or below it
+        uint32_t bad = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) bad |= not_finite<T>(vr[j][i]);
+        const bool apart = __any(bad != 0);
+        uint32_t ph[NQ][4], pl[NQ][4], ones[NQ][4];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            float tm = s[n][0][0];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) tm = fmaxf(tm, s[n][t][e]);
+            tm = rows4_max(tm);
+            if (apart) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    ones[n][i] = (s[n][i >> 1][2 * (i & 1)] == -INFINITY ? 0u : V::ONE) |
+                                 (s[n][i >> 1][2 * (i & 1) + 1] == -INFINITY ? 0u : V::ONE << 16);
+            }
+            const bool up = (tm - st[n].m) * p.scale_log2 > TAU;
+            if (__any(up)) {
+                const float m = up ? tm : st[n].m;
+                const float alpha = up ? __builtin_amdgcn_exp2f((st[n].m - m) * p.scale_log2) : 1.0f;
+                st[n].m = m;
+                st[n].l *= alpha;
+#pragma unroll
+                for (int i = 0; i < DB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[n][i][e] *= alpha;
+            }
+            // (nothing seen yet: all scores are -inf, all weights 0)
+            const float off = st[n].m == NONE ? 0.0f : st[n].m;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float a = __builtin_amdgcn_exp2f(fmaf(s[n][i >> 1][2 * (i & 1)] - off, p.scale_log2, V::LIFT));
+                const float c =
+                    __builtin_amdgcn_exp2f(fmaf(s[n][i >> 1][2 * (i & 1) + 1] - off, p.scale_log2, V::LIFT));
+                sum += a + c;
+                ph[n][i] = T::pack(a, c);
+                // bf16's 8 bits would be as far off as the output's own: what they leave
+                // of a weight is a second operand (the products cost nothing beside the
+                // read)
+                if constexpr (SPLIT)
+                    pl[n][i] = T::pack(a - __uint_as_float(ph[n][i] << 16),
+                                       c - __uint_as_float(ph[n][i] & 0xffff0000u));
+            }
+            st[n].l += sum;
+        }
+#pragma unroll
+        for (int i = 0; i < DB; ++i) {
+            uint32_t w[4], kind[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                w[j] = __builtin_amdgcn_perm(vr[2 * j + 1][i >> 1], vr[2 * j][i >> 1],
+                                             i & 1 ? 0x07060302u : 0x05040100u);
+            if (apart) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) part_word<T>(w[j], w[j], kind[j]);
+            }
+            const x8 vf = as_x8<x8>(u32x4{w[0], w[1], w[2], w[3]});
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                o[n][i] = T::mfma16(vf, as_x8<x8>(u32x4{ph[n][0], ph[n][1], ph[n][2], ph[n][3]}), o[n][i]);
+                if constexpr (SPLIT)
+                    o[n][i] = T::mfma16(vf, as_x8<x8>(u32x4{pl[n][0], pl[n][1], pl[n][2], pl[n][3]}), o[n][i]);
+                if (apart) {
+                    const f32x4 sum =
+                        T::mfma16(as_x8<x8>(u32x4{kind[0], kind[1], kind[2], kind[3]}),
+                                  as_x8<x8>(u32x4{ones[n][0], ones[n][1], ones[n][2], ones[n][3]}), f32x4{});
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[n][i][e] = parted(o[n][i][e], sum[e]);
+                }
+            }
+        }
+        if (tile + 1 < w1) load_v();
+    }
+    // merge of the waves: o[n][i][e] is column DB (4 g + e) + i of row 16 n + r
+    __syncthreads();  // (the tree's bits are done with)
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int i = 0; i < DB; i += 4)
+                *reinterpret_cast<f32x4*>(&sm.o[wave][16 * n + r][DB * (4 * g + e) + i]) =
+                    f32x4{o[n][i][e], o[n][i + 1][e], o[n][i + 2][e], o[n][i + 3][e]};
+        st[n].l = rows4_sum(st[n].l);
+        st[n].m *= p.scale_log2;
+        if (g == 0) sm.st[wave][16 * n + r] = st[n];
+    }
+    __syncthreads();
+    for (int mr = threadIdx.x / 16; mr < ROWS; mr += 4 * W) {
+        const int d = (threadIdx.x % 16) * 8;
+        if (d >= P) break;
+        Stat all{NONE, 0.0f};
+#pragma unroll
+        for (int w = 0; w < W; ++w) all.m = fmaxf(all.m, sm.st[w][mr].m);
+        float acc[8] = {};
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const Stat one = sm.st[w][mr];
+            const float f = weight(one.m, all.m);
+            all.l += f * one.l;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] += f * sm.o[w][mr][d + i];
+        }
+        // (l is in the weights' units: 2^LIFT too large)
+        if constexpr (V::LIFT != 0.0f) all.l *= 1.0f / 4096.0f;
+        if (p.splits > 1) store_partial(p, bh, split, row0 + mr, d, all, acc);
+        else store_row<T>(p, b, hk, row0 + mr, d, all, acc);
+    }
+}
+
+// ---------------------------------------------------------------- splits
+// The merge of the splits' partial results: a thread eight columns, SG groups of
+// threads share a row's splits and are joined in LDS, and a thread has AHEAD splits'
+// loads in flight.  With M the largest m, out = sum(2^(m - M) o) / sum(2^(m - M) l).
+template <typename T, int SG, int AHEAD>
+__global__ void __launch_bounds__(256) merge_kernel(AttendParams p) {
+    constexpr int PARTS = 16, ROWS = 256 / (PARTS * SG);
+    const int row = blockIdx.x * ROWS + threadIdx.x / (PARTS * SG);
+    const int sg = threadIdx.x / PARTS % SG, part = threadIdx.x % PARTS, d = part * 8;
+    const int b = blockIdx.z, hk = blockIdx.y;
+    const bool in = row < p.rows && d < p.D;
+    const int64_t first = ((int64_t)b * p.H + hk) * p.splits * p.rows + row;
+    Stat all{NONE, 0.0f};
+    float acc[8] = {};
+    if (in) {
+        for (int s0 = sg; s0 < p.splits; s0 += SG * AHEAD) {
+            f32x2 ml[AHEAD];
+            f32x4 x[AHEAD][2];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const int64_t i = first + (int64_t)min(s0 + SG * j, p.splits - 1) * p.rows;
+                ml[j] = p.part_ml[i];
+                const f32x4* from = reinterpret_cast<const f32x4*>(p.part + i * p.D + d);
+                x[j][0] = from[0];
+                x[j][1] = from[1];
+            }
+            float m = all.m;
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j)
+                if (s0 + SG * j < p.splits) m = fmaxf(m, ml[j][0]);
+            const float f = weight(all.m, m);
+            all.m = m;
+            all.l *= f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[k] *= f;
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                if (s0 + SG * j >= p.splits) break;
+                const float w = weight(ml[j][0], m);
+                all.l += w * ml[j][1];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) acc[k] += w * x[j][k >> 2][k & 3];
+            }
+        }
+    }
+    if constexpr (SG > 1) {
+        __shared__ float sh[ROWS][SG][PARTS][8];
+        __shared__ Stat sst[ROWS][SG];
+        const int lr = threadIdx.x / (PARTS * SG);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sh[lr][sg][part][k] = acc[k];
+        if (part == 0) sst[lr][sg] = all;
+        __syncthreads();
+        if (sg) return;
+        all = {NONE, 0.0f};
+#pragma unroll
+        for (int s = 0; s < SG; ++s) all.m = fmaxf(all.m, sst[lr][s].m);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < SG; ++s) {
+            const float f = weight(sst[lr][s].m, all.m);
+            all.l += f * sst[lr][s].l;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[k] += f * sh[lr][s][part][k];
+        }
+    }
+    if (in) store_row<T>(p, b, hk, row, d, all, acc);
+}
+
+// ---------------------------------------------------------------- host
+struct Plan {
+    bool eight, two;              // eight waves; two groups of 16 rows
+    int groups, splits;
+    int64_t items, rows;
+    size_t part, ml;              // bytes
+};
+
+Plan attend_plan(const nkv_paged_attend_args* a) {
+    const nkv_paged_cache& c = a->cache;
+    Plan pl{};
+    pl.rows = a->Q * a->G;
+    const int64_t heads = (int64_t)a->B * c.H, tiles = cdiv(a->n, TILE);
+    pl.splits = 1;
+    pl.two = pl.rows > 16;
+    pl.groups = (int)cdiv(pl.rows, pl.two ? 32 : 16);
+    const int64_t base = heads * pl.groups;
+    pl.eight = base * tiles >= 4096;
+    const int64_t slots = pl.eight && !a->length ? 256 : 512, waves = pl.eight ? 8 : 4;
+    if (base > 0 && base < slots)
+        pl.splits = (int)std::max<int64_t>(1, std::min(cdiv(slots, base), tiles / waves));
+    pl.items = base * pl.splits;
+    return pl;
+}
+
+// The plan's workspace; in fewer than `limit` bytes fewer splits where those wanted do
+// not fit.
+void attend_fit(const nkv_paged_attend_args* a, Plan& pl, size_t limit) {
+    if (pl.splits == 1) return;
+    const size_t rows = (size_t)a->B * a->cache.H * pl.rows;
+    const size_t most = limit / (rows * (sizeof(f32x2) + 4 * a->cache.D));
+    if (most < (size_t)pl.splits) {
+        pl.items /= pl.splits;
+        pl.splits = (int)std::max<size_t>(1, most);
+        pl.items *= pl.splits;
+        if (pl.splits == 1) return;
+    }
+    pl.part = rows * pl.splits * 4 * a->cache.D;
+    pl.ml = rows * pl.splits * sizeof(f32x2);
+}
+
+// Also plans the call where there is something to do (pl.items > 0).
+int check_attend(const nkv_paged_attend_args* a, Plan& pl) {
+    NKV_REQUIRE(a, NKV_ERR_INVALID, "args is null");
+    const nkv_paged_cache& c = a->cache;
+    int rc = paged_check(c, __func__);
+    if (rc) return rc;
+    if ((rc = paged_table_check(c, a->table, a->table_sb, a->table_w, a->B, __func__))) return rc;
+    const PageTable table = page_table(c, a->table, a->table_sb, a->table_w);
+    NKV_REQUIRE(a->G >= 1 && a->Q >= 0, NKV_ERR_INVALID, "G must be positive and Q not negative");
+    NKV_REQUIRE(a->Q <= INT32_MAX / 2 && (__int128)a->Q * a->G <= INT32_MAX / 2 &&
+                    (int64_t)c.H * a->G <= INT32_MAX,
+                NKV_ERR_UNSUPPORTED, "too many query rows");
+    NKV_REQUIRE(a->n >= 0 && a->n <= std::min<int64_t>(table.cap(), 1 << 30), NKV_ERR_INVALID,
+                "n must be in [0, table_w * page] and at most 2^30");
+    NKV_REQUIRE(a->softmax_scale > 0.0f && a->softmax_scale < INFINITY, NKV_ERR_INVALID,
+                "softmax_scale must be positive and finite");
+    NKV_REQUIRE(!a->parents || !a->causal, NKV_ERR_INVALID, "causal and parents exclude each other");
+    NKV_REQUIRE(!a->parents || a->Q <= NKV_PAGED_TREE, NKV_ERR_UNSUPPORTED,
+                "a tree has at most 256 tokens");
+    NKV_REQUIRE(!a->parents || a->parents_sb >= 0, NKV_ERR_INVALID, "parents_sb must not be negative");
+    if (a->B == 0 || a->Q == 0) return NKV_OK;
+    NKV_REQUIRE(a->q && a->out, NKV_ERR_INVALID, "q and out are required");
+    NKV_REQUIRE((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) % 16 == 0 &&
+                    (a->q_sb | a->q_st | a->q_sh | a->o_sb | a->o_st | a->o_sh) % 8 == 0,
+                NKV_ERR_INVALID, "q and out must be 16-byte aligned with strides divisible by 8");
+    pl = attend_plan(a);
+    NKV_REQUIRE(pl.items <= 1 << 22, NKV_ERR_UNSUPPORTED, "too many query rows");
+    const int64_t span = rows_span(a->o_sb, a->B, a->o_st, a->Q, a->o_sh, (int64_t)c.H * a->G, c.D);
+    NKV_REQUIRE(span > 0, NKV_ERR_INVALID, "out's rows overlap");
+    // what is written and what is read; an out with gaps may have anything in them
+    const int64_t rows = (int64_t)a->B * c.H * a->G * a->Q;
+    const Range in[6] = {{c.k, pool_bytes(c)}, {c.v, pool_bytes(c)},
+                         {a->table, table_bytes(a->B, a->table_sb, a->table_w)},
+                         {a->length, a->length ? a->B * 4 : 0}, {a->counts, a->counts ? a->B * 4 : 0},
+                         {a->parents, a->parents ? table_bytes(a->B, a->parents_sb, a->Q) : 0}};
+    const Range lse(a->lse, a->lse ? rows * 4 : 0), out(a->out, span == rows * c.D ? rows * c.D * 2 : 0);
+    for (const Range& r : in)
+        NKV_REQUIRE(!r.meets(lse) && !r.meets(out), NKV_ERR_INVALID,
+                    "out or lse overlaps the cache, table, length, counts or parents");
+    NKV_REQUIRE(!lse.meets(out), NKV_ERR_INVALID, "lse overlaps out");
+    if (a->out == a->q)
+        NKV_REQUIRE(a->q_sb == a->o_sb && a->q_st == a->o_st && a->q_sh == a->o_sh, NKV_ERR_INVALID,
+                    "out over q must have its strides");
+    return NKV_OK;
+}
+
+// Blocks of a launch over p.items workgroups in item_of's order.
+unsigned item_blocks(const AttendParams& p) {
+    const int64_t units = p.items / p.groups;
+    return (unsigned)(units >= UNITS ? 8 * cdiv(units, 8) * p.groups : 8 * cdiv(p.items, 8));
+}
+
+template <typename T, int KS, int W, int NQ>
+int rows_run(const AttendParams& p, hipStream_t s) {
+    constexpr int SMEM = sizeof(RowsSmem<width_of<KS>(), W, NQ>);
+    if (SMEM > 65536)
+        if (int rc = set_smem(attend_kernel<T, KS, W, NQ>, SMEM)) return rc;
+    attend_kernel<T, KS, W, NQ><<<item_blocks(p), 64 * W, SMEM, s>>>(p);
+    return NKV_OK;
+}
+
+template <typename T, int KS>
+int attend_run(const AttendParams& p, const Plan& pl, hipStream_t s) {
+    if (pl.two) return pl.eight ? rows_run<T, KS, 8, 2>(p, s) : rows_run<T, KS, 4, 2>(p, s);
+    return pl.eight ? rows_run<T, KS, 8, 1>(p, s) : rows_run<T, KS, 4, 1>(p, s);
+}
+
+template <typename T>
+int attend_width(const AttendParams& p, const Plan& pl, hipStream_t s) {
+    return p.D <= 64 ? attend_run<T, 2>(p, pl, s)
+                     : p.D <= 96 ? attend_run<T, 3>(p, pl, s) : attend_run<T, 4>(p, pl, s);
+}
+
+template <typename T>
+void merge_run(const AttendParams& p, hipStream_t s) {
+    auto grid = [&](int sg) {
+        return dim3((unsigned)cdiv(p.rows, 16 / sg), (unsigned)p.H, (unsigned)p.B);
+    };
+    if (p.splits > 8) merge_kernel<T, 16, 4><<<grid(16), 256, 0, s>>>(p);
+    else if (p.splits > 4) merge_kernel<T, 1, 8><<<grid(1), 256, 0, s>>>(p);
+    else merge_kernel<T, 1, 4><<<grid(1), 256, 0, s>>>(p);
+}
+
+}  // namespace
+}  // namespace nkv
+
+using namespace nkv;
+
+extern "C" size_t nkv_paged_attend_workspace_size(const nkv_paged_attend_args* a) {
+    clear_error();
+    Plan pl{};
+    if (check_attend(a, pl) || pl.items == 0) return 0;
+    attend_fit(a, pl, SIZE_MAX);
+    return pl.part + pl.ml;
+}
+
+extern "C" int nkv_paged_attend(void* stream, const nkv_paged_attend_args* a, void* workspace,
+                                size_t workspace_bytes) {
+    clear_error();
+    Plan pl{};
+    int rc = check_attend(a, pl);
+    if (rc || pl.items == 0) return rc;
+    const nkv_paged_cache& c = a->cache;
+    attend_fit(a, pl, workspace ? workspace_bytes : 0);
+    NKV_REQUIRE(pl.part == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, NKV_ERR_INVALID,
+                "workspace must be 16-byte aligned");
+    AttendParams p{};
+    p.table = page_table(c, a->table, a->table_sb, a->table_w);
+    p.k = (const uint16_t*)c.k;
+    p.v = (const uint16_t*)c.v;
+    p.length = a->length;
+    p.counts = a->counts;
+    p.parents = a->parents;
+    p.parents_sb = a->parents_sb;
+    p.q = (const uint16_t*)a->q;
+    p.out = (uint16_t*)a->out;
+    p.lse = a->lse;
+    p.part = (float*)workspace;
+    p.part_ml = (f32x2*)((char*)workspace + pl.part);
+    p.q_sb = a->q_sb, p.q_st = a->q_st, p.q_sh = a->q_sh;
+    p.o_sb = a->o_sb, p.o_st = a->o_st, p.o_sh = a->o_sh;
+    p.items = pl.items;
+    // (kept from 0 and infinity: a hidden score of -inf times 0 would be NaN)
+    p.scale_log2 = std::clamp(a->softmax_scale * LOG2E, 0x1p-126f, 0x1.fffffep127f);
+    p.B = a->B, p.H = c.H, p.G = a->G, p.D = c.D, p.Q = (int)a->Q, p.n = (int)a->n;
+    p.causal = a->causal != 0;
+    p.splits = pl.splits;
+    p.groups = pl.groups;
+    p.rows = (int)pl.rows;
+    p.page_d = c.page * c.D;
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    rc = c.dtype == NKV_ROWS_BF16 ? attend_width<Bf16>(p, pl, s) : attend_width<Fp16>(p, pl, s);
+    if (rc) return rc;
+    NKV_LAUNCH_CHECK();
+    if (pl.splits > 1) {
+        if (c.dtype == NKV_ROWS_BF16) merge_run<Bf16>(p, s);
+        else merge_run<Fp16>(p, s);
+        NKV_LAUNCH_CHECK();
+    }
+    return NKV_OK;
+}

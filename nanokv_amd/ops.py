@@ -21,7 +21,8 @@ from ._lib import (NKV_DTYPE_BF16, NKV_DTYPE_FP16, NKV_QUANT_BF16, NKV_QUANT_FP3
                    NkvAttendArgs, NkvCodec, NkvDecodeArgs, NkvEncodeArgs, NkvFastArgs,
                    NkvCamera, NkvFinishArgs, NkvLiftCombineArgs, NkvReaderGroup, NkvC64FitArgs,
                    NkvReaderRowsArgs, NkvRope, NkvCache8, NkvCache8AttendArgs,
-                   NkvCache8EvictArgs, NkvCache8MassArgs, NkvCache8WriteArgs,
+                   NkvCache8EvictArgs, NkvCache8MassArgs, NkvCache8WriteArgs, NkvPagedAppendArgs,
+                   NkvPagedAttendArgs, NkvPagedCache, NkvPagedCommitArgs,
                    NkvSegment, check, lib)
 
 _SCALE_CODES = {torch.bfloat16: NKV_DTYPE_BF16, torch.float16: NKV_DTYPE_FP16}
@@ -1437,7 +1438,7 @@ class Cache8:
                          code)
 
 
-def _cache8_call(name: str, device: torch.device, *args) -> None:
+def _device_call(name: str, device: torch.device, *args) -> None:
     """One C call with its tensors' device current (a launch on another device's
     stream would go to the current one)."""
     fn = getattr(lib(), name)
@@ -1450,7 +1451,7 @@ def _cache8_call(name: str, device: torch.device, *args) -> None:
         check(name, code)
 
 
-def _cache8_scratch(name: str, args, device: torch.device, workspace: Optional[torch.Tensor]):
+def _scratch(name: str, args, device: torch.device, workspace: Optional[torch.Tensor]):
     """The workspace of a call: the caller's if given, else one from torch's
     allocator, which orders its reuse behind the launch's stream."""
     need = getattr(lib(), name)(byref(args))
@@ -1513,7 +1514,7 @@ def cache8_write(cache: Cache8, k: torch.Tensor, v: torch.Tensor, start,
                            0 if given is not None else int(start),
                            _cache8_ints(given, B, "start"), _cache8_ints(counts, B, "counts"),
                            code)
-    _cache8_call("nkv_cache8_write", device, byref(a))
+    _device_call("nkv_cache8_write", device, byref(a))
 
 
 def _cache8_query(q: torch.Tensor, cache: Cache8, length, max_length, softmax_scale):
@@ -1565,8 +1566,8 @@ def cache8_attend(q: torch.Tensor, cache: Cache8, length, *, max_length: Optiona
     lse = torch.empty((B, heads, Q), device=device, dtype=torch.float32) if return_lse else None
     a = NkvCache8AttendArgs(*query, out.data_ptr(), *strides, _ptr(lse), scale, bool(causal),
                             _cache8_ints(counts, B, "counts"))
-    scratch, nbytes = _cache8_scratch("nkv_cache8_attend_workspace_size", a, device, workspace)
-    _cache8_call("nkv_cache8_attend", device, byref(a), _ptr(scratch), nbytes)
+    scratch, nbytes = _scratch("nkv_cache8_attend_workspace_size", a, device, workspace)
+    _device_call("nkv_cache8_attend", device, byref(a), _ptr(scratch), nbytes)
     return out, lse
 
 
@@ -1593,8 +1594,8 @@ def cache8_mass(q: torch.Tensor, cache: Cache8, lse: torch.Tensor, mass: torch.T
             raise ValueError(f"{name} must be [B, H, cap]")
     a = NkvCache8MassArgs(*query, lse.data_ptr(), mass.data_ptr(), out.data_ptr(), scale,
                           bool(causal), _cache8_ints(counts, c.B, "counts"))
-    scratch, nbytes = _cache8_scratch("nkv_cache8_mass_workspace_size", a, device, workspace)
-    _cache8_call("nkv_cache8_mass", device, byref(a), _ptr(scratch), nbytes)
+    scratch, nbytes = _scratch("nkv_cache8_mass_workspace_size", a, device, workspace)
+    _device_call("nkv_cache8_mass", device, byref(a), _ptr(scratch), nbytes)
     return out
 
 
@@ -1625,6 +1626,243 @@ def cache8_evict(cache: Cache8, mass: torch.Tensor, length, out: Cache8, out_mas
     left = torch.empty((c.B,), device=device, dtype=torch.int32)
     a = NkvCache8EvictArgs(c, o, mass.data_ptr(), out_mass.data_ptr(), rows.data_ptr(),
                            left.data_ptr(), at, n, keep, int(sink), int(recent))
-    scratch, nbytes = _cache8_scratch("nkv_cache8_evict_workspace_size", a, device, workspace)
-    _cache8_call("nkv_cache8_evict", device, byref(a), _ptr(scratch), nbytes)
+    scratch, nbytes = _scratch("nkv_cache8_evict_workspace_size", a, device, workspace)
+    _device_call("nkv_cache8_evict", device, byref(a), _ptr(scratch), nbytes)
     return rows, left
+
+
+# ---------------------------------------------------------------- paged cache
+@dataclass
+class PagedCache:
+    """Keys and values in pages (nkv_paged_cache): k and v [pages, H, page, head_dim]
+    bf16 or fp16, contiguous, page a power of two from 16 to 1,024, head_dim a multiple
+    of 8, at most 128.  The caller keeps the sequences' page tables (int32 [B, width],
+    each sequence's pages in order) and lengths; rows that no query sees may hold
+    anything."""
+    k: torch.Tensor
+    v: torch.Tensor
+
+    @classmethod
+    def empty(cls, pages: int, page: int, H: int, head_dim: int, device: torch.device,
+              dtype: torch.dtype = torch.bfloat16) -> "PagedCache":
+        """A pool of `pages` pages of `page` rows, zeros."""
+        shape = (int(pages), int(H), int(page), int(head_dim))
+        cache = cls(*(torch.zeros(shape, device=device, dtype=dtype) for _ in range(2)))
+        cache.struct()
+        return cache
+
+    @property
+    def page(self) -> int:
+        return int(self.k.shape[2])
+
+    def struct(self) -> NkvPagedCache:
+        k, v = self.k, self.v
+        code = _PAGED_CODES.get(k.dtype)
+        if code is None or v.dtype != k.dtype:
+            raise TypeError("cache pages must be bf16 or fp16, k and v alike")
+        shape = k.shape
+        if len(shape) != 4 or v.shape != shape:
+            raise ValueError("cache pages must be [pages, H, page, head_dim], k and v alike")
+        pages, H, page, D = shape
+        if page < 16 or page > 1024 or page & (page - 1):
+            raise ValueError("page must be a power of two from 16 to 1,024")
+        if D < 8 or D % 8 or D > 128 or pages < 1 or H < 1:
+            raise ValueError("head_dim must be a multiple of 8, at most 128, with a page and a head")
+        if not (k.is_contiguous() and v.is_contiguous()):
+            raise ValueError("cache pages must be contiguous")
+        return NkvPagedCache(k.data_ptr(), v.data_ptr(), pages, H, page, D, code)
+
+
+_PAGED_CODES = {torch.bfloat16: _lib.NKV_ROWS_BF16, torch.float16: _lib.NKV_ROWS_FP16}
+
+
+def _int_rows(t: Optional[torch.Tensor], B: int, n: Optional[int], name: str):
+    """(pointer, entries between items) of an int32 [B, n] tensor (or [n], for all
+    items alike) with contiguous columns."""
+    if t is None:
+        return None, 0
+    shape = t.shape
+    if t.dtype is not torch.int32 or len(shape) not in (1, 2) or (n is not None and shape[-1] != n):
+        raise ValueError(f"{name} must be an int32 tensor of {'[B, width]' if n is None else f'[B, {n}]'}")
+    if shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must have contiguous columns")
+    if len(shape) == 1:
+        return t.data_ptr(), 0
+    if shape[0] != B:
+        raise ValueError(f"{name} must have a row for each sequence")
+    return t.data_ptr(), t.stride(0) if B > 1 else 0
+
+
+def _page_table(table: torch.Tensor):
+    """(pointer, entries between items, width, B) of a page table."""
+    if len(table.shape) != 2:
+        raise ValueError("table must be an int32 tensor of [B, width]")
+    B, width = table.shape
+    at, sb = _int_rows(table, B, None, "table")
+    return at, sb, width, B
+
+
+def _paged_rows(t: torch.Tensor, B: int, T: int, D: int, name: str):
+    shape = t.shape
+    if len(shape) != 4 or shape[0] != B or shape[1] != T or shape[3] != D:
+        raise ValueError(f"{name} must be [B, T, heads, head_dim] of the table's B and k's T")
+    return _strides_bthd(t, name) if t.numel() else (0, 0, 0)
+
+
+def paged_append(cache: PagedCache, table: torch.Tensor, k: torch.Tensor, v: torch.Tensor, start, *,
+                 counts: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
+                 q_out: Optional[torch.Tensor] = None, freqs: Optional[torch.Tensor] = None,
+                 positions: Optional[torch.Tensor] = None,
+                 interleaved: bool = False) -> Optional[torch.Tensor]:
+    """Write new rows into a paged cache, in place, rotating keys and queries on the way
+    (see nkv_paged_append).
+
+    k, v: [B, T, H, head_dim] of the cache's type or fp32 (any strides divisible by 8,
+    contiguous columns).  table: int32 [B, width], each sequence's pages in order; an
+    entry that names no page drops its rows.  start: the row of each sequence's first
+    new token, an int for all or an int32 tensor [B] on the device (so that a captured
+    graph can move on; its entries are clamped to the table).  counts: int32 [B], how
+    many of a sequence's T rows there are, the first ones (a padded batch).  Rows past
+    the table are dropped with either tensor, and refused with neither.
+    freqs: fp32 [rot / 2], the angle of each pair per position; keys are rotated by
+    position * freqs, and q [B, T, heads, head_dim] with them: the rotated queries, in
+    the cache's type, are returned (q_out: where they go, q itself allowed; rows past
+    counts are left as they were there, and 0 in a new tensor).  Pairs are columns i and
+    i + rot / 2, or 2 i and 2 i + 1 (interleaved).  positions: int32 [B, T] (or [T]),
+    default start + t."""
+    given = start if isinstance(start, torch.Tensor) else None
+    device = _require_gpu(cache.k, cache.v, table, k, v, given, counts, q, q_out, freqs, positions)
+    c = cache.struct()
+    at, sb, width, B = _page_table(table)
+    if k.dtype not in (cache.k.dtype, torch.float32) or v.dtype != k.dtype:
+        raise TypeError("k and v must both have the cache's type or be fp32")
+    if len(k.shape) != 4 or k.shape[2] != c.H or v.shape != k.shape:
+        raise ValueError("k and v must be [B, T, H, head_dim] of the cache's H and head_dim")
+    T = k.shape[1]
+    ks, vs = _paged_rows(k, B, T, c.D, "k"), _paged_rows(v, B, T, c.D, "v")
+    rot = heads = 0
+    qs = qos = (0, 0, 0)
+    if freqs is not None:
+        _contig(freqs, torch.float32, "freqs")
+        if len(freqs.shape) != 1 or not 1 <= freqs.shape[0] <= c.D // 2:
+            raise ValueError("freqs must be [rot / 2], rot at most head_dim")
+        rot = 2 * freqs.shape[0]
+        if rot % (8 if interleaved else 16):
+            raise ValueError("rot must be a multiple of 16, of 8 where interleaved")
+    elif q is not None or positions is not None:
+        raise ValueError("q and positions need freqs")
+    if q is not None:
+        if q.dtype != k.dtype:
+            raise TypeError("q must have k's type")
+        qs = _paged_rows(q, B, T, c.D, "q")
+        heads = q.shape[2]
+        if heads < 1:
+            raise ValueError("q must have a head")
+        if q_out is None:
+            make = torch.empty if counts is None else torch.zeros
+            q_out = make(q.shape, device=device, dtype=cache.k.dtype)
+            qos = (T * heads * c.D, heads * c.D, c.D)
+        elif q_out.shape != q.shape or q_out.dtype != cache.k.dtype:
+            raise ValueError("q_out must have q's shape and the cache's type")
+        else:
+            qos = _paged_rows(q_out, B, T, c.D, "q_out")
+    elif q_out is not None:
+        raise ValueError("q_out needs q")
+    pos, pos_sb = _int_rows(positions, B, T, "positions")
+    a = NkvPagedAppendArgs(c, at, sb, width, k.data_ptr(), *ks, v.data_ptr(), *vs, _ptr(q), *qs,
+                           _ptr(q_out), *qos, _ptr(freqs), pos, pos_sb, T,
+                           0 if given is not None else int(start), _cache8_ints(given, B, "start"),
+                           _cache8_ints(counts, B, "counts"), B, heads, rot, bool(interleaved),
+                           _ROW_CODES[k.dtype])
+    if k.numel():
+        _device_call("nkv_paged_append", device, byref(a))
+    return q_out
+
+
+def paged_attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, length, *,
+                 max_length: Optional[int] = None, softmax_scale: Optional[float] = None,
+                 causal: bool = False, parents: Optional[torch.Tensor] = None,
+                 counts: Optional[torch.Tensor] = None, return_lse: bool = True,
+                 out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None):
+    """Attention over a paged cache (see nkv_paged_attend).
+
+    q [B, Q, heads, head_dim] of the cache's type, heads a multiple of the cache's
+    (grouped heads: query head h reads key head h // (heads / H)).  table: int32 [B,
+    width].  length: the rows visible, an int for every sequence or an int32 tensor [B]
+    on the device, clamped to [0, max_length] (default: the table's rows), by which the
+    work is divided.  counts: int32 [B], how many of a sequence's Q rows are queries, the
+    first ones (a padded batch); a row past them sees nothing.
+    causal: the queries are the sequence's last counts tokens, query t sees the first
+    length - counts + 1 + t rows.  parents: int32 [B, Q] (or [Q]), the queries are a
+    tree of up to 256 drafted tokens, the sequence's last counts rows in their order:
+    query t sees the rows before the draft, its own and those of its ancestors
+    (parents[t] < t; anything else ends the way, -1 by custom).  A chain, parents[t] =
+    t - 1, is the causal mask.
+    Returns (out like q, lse [B, heads, Q] fp32 or None); a query that sees nothing gets
+    0 and -inf.  workspace: optional uint8 buffer, nkv_paged_attend_workspace_size bytes
+    or fewer (with fewer, fewer key splits)."""
+    device = _require_gpu(q, cache.k, cache.v, table, parents, counts, out,
+                          length if isinstance(length, torch.Tensor) else None)
+    c = cache.struct()
+    at, sb, width, B = _page_table(table)
+    if q.dtype != cache.k.dtype:
+        raise TypeError("q must have the cache's type")
+    shape, H, D = q.shape, c.H, c.D
+    if len(shape) != 4 or shape[0] != B or shape[3] != D or shape[2] == 0 or shape[2] % H:
+        raise ValueError("q must be [B, Q, heads, head_dim] with heads a multiple of the cache's")
+    if causal and parents is not None:
+        raise ValueError("causal and parents exclude each other")
+    _, Q, heads, _ = shape
+    lengths, n = _cache8_bound(width * c.page, B, length, max_length)
+    strides = _strides_bthd(q, "q") if q.numel() else (0, 0, 0)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        os = (Q * heads * D, heads * D, D)
+    elif out.shape != shape or out.dtype != q.dtype:
+        raise ValueError("out must have q's shape and type")
+    else:
+        os = _strides_bthd(out, "out") if q.numel() else (0, 0, 0)
+    lse = torch.empty((B, heads, Q), device=device, dtype=torch.float32) if return_lse else None
+    tree, tree_sb = _int_rows(parents, B, Q, "parents")
+    scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
+    a = NkvPagedAttendArgs(c, at, sb, width, B, heads // H, Q, n, lengths,
+                           _cache8_ints(counts, B, "counts"), tree, tree_sb, q.data_ptr(), *strides,
+                           out.data_ptr(), *os, _ptr(lse), scale, bool(causal))
+    scratch, nbytes = _scratch("nkv_paged_attend_workspace_size", a, device, workspace)
+    _device_call("nkv_paged_attend", device, byref(a), _ptr(scratch), nbytes)
+    return out, lse
+
+
+def paged_commit(caches, table: torch.Tensor, start, rows: torch.Tensor,
+                 counts: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Keep the accepted tokens of a draft, in place (see nkv_paged_commit).
+
+    In each cache (one, or a sequence of a model's layers that share the table), row
+    start + rows[b, j] of sequence b moves to row start + j for j < counts[b].  rows:
+    int32 [B, M], M at most 256, in any order; counts: int32 [B] (default: all M);
+    start: an int or an int32 tensor [B], as paged_append's.  Returns the new lengths,
+    start + counts, int32 [B]."""
+    caches = [caches] if isinstance(caches, PagedCache) else list(caches)
+    if not caches:
+        raise ValueError("a cache is required")
+    given = start if isinstance(start, torch.Tensor) else None
+    device = _require_gpu(*(t for c in caches for t in (c.k, c.v)), table, rows, counts, given)
+    structs = [c.struct() for c in caches]
+    if any(c.k.shape != caches[0].k.shape or c.k.dtype != caches[0].k.dtype for c in caches):
+        raise ValueError("caches must have one shape and type")
+    at, sb, width, B = _page_table(table)
+    if len(rows.shape) != 2:
+        raise ValueError("rows must be an int32 tensor of [B, M]")
+    M = rows.shape[1]
+    if M > _lib.NKV_PAGED_COMMIT:
+        raise ValueError(f"at most {_lib.NKV_PAGED_COMMIT} rows a sequence")
+    path, path_sb = _int_rows(rows, B, M, "rows")
+    first, n = _cache8_ints(given, B, "start"), _cache8_ints(counts, B, "counts")
+    length = torch.empty((B,), device=device, dtype=torch.int32)
+    for i in range(0, len(structs), _lib.NKV_PAGED_CACHES):
+        part = structs[i:i + _lib.NKV_PAGED_CACHES]
+        a = NkvPagedCommitArgs((NkvPagedCache * len(part))(*part), len(part), at, sb, width, path,
+                               path_sb, 0 if given is not None else int(start), first, n,
+                               length.data_ptr(), B, M)
+        _device_call("nkv_paged_commit", device, byref(a))
+    return length
