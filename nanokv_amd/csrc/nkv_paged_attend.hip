@@ -50,24 +50,21 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
 // A word's two values in two parts: the finite ones (0 in place of the others), and
 // what the others are, as numbers whose sums tell them apart: +inf 1, -inf 128, NaN
 // 129 (exact in either type).
+struct Parts {
+    uint32_t finite, kind;
+};
 template <typename T>
-__device__ __forceinline__ void part_word(uint32_t w, uint32_t& finite, uint32_t& kind) {
-    finite = kind = 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const uint32_t x = (w >> (16 * h)) & 0xffffu;
-        const bool bad = (x & Value<T>::EXP & 0xffffu) == (Value<T>::EXP & 0xffffu);
-        const uint32_t k = x & Value<T>::FRAC ? Value<T>::N129 : x & 0x8000u ? Value<T>::N128 : Value<T>::ONE;
-        if (bad) kind |= k << (16 * h);
-        else finite |= x << (16 * h);
-    }
+__device__ __forceinline__ Parts part_word(uint32_t w) {
+    using V = Value<T>;
+    const uint32_t bad = (not_finite<T>(w) >> 15) * 0xffffu;               // whole halves
+    const uint32_t nan = (((w & V::FRAC * 0x10001u) + 0x7fff7fffu) >> 15) & 0x10001u;
+    const uint32_t down = ((w >> 15) & 0x10001u) | nan;
+    return {w & ~bad, (V::ONE * 0x10001u + down * (V::N128 - V::ONE) + nan * (V::N129 - V::N128)) & bad};
 }
 // What a sum of such numbers (up to 32 of them) adds to a result.
 __device__ __forceinline__ float parted(float o, float sum) {
-    if (sum == 0.0f) return o;
     const int n = (int)sum;
-    const float up = n & 127 ? INFINITY : 0.0f, down = n >= 128 ? -INFINITY : 0.0f;
-    return o + up + down;
+    return o + (n & 127 ? INFINITY : 0.0f) + (n >= 128 ? -INFINITY : 0.0f);
 }
 
 struct AttendParams {
@@ -90,6 +87,7 @@ struct AttendParams {
     float scale_log2;
     int B, H, G, D, Q, n, causal, splits, groups, rows;
     int page_d;
+    int per_group;                // tile kernel: 32-row blocks of a group
 };
 
 // Query row r of key head hk is query t = r / G of query head hk * G + r % G.
@@ -468,7 +466,10 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
                                              i & 1 ? 0x07060302u : 0x05040100u);
             if (apart) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) part_word<T>(w[j], w[j], kind[j]);
+                for (int j = 0; j < 4; ++j) {
+                    const Parts x = part_word<T>(w[j]);
+                    w[j] = x.finite, kind[j] = x.kind;
+                }
             }
             const x8 vf = as_x8<x8>(u32x4{w[0], w[1], w[2], w[3]});
 #pragma unroll
@@ -522,6 +523,359 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
         if (p.splits > 1) store_partial(p, bh, split, row0 + mr, d, all, acc);
         else store_row<T>(p, b, hk, row0 + mr, d, all, acc);
     }
+}
+
+// ---------------------------------------------------------------- many rows
+// Eight waves of 32 query rows each share every tile of 128 keys.  K and V rows go from
+// their pages into LDS as they are, by 1 KB copies of the memory system (wave w those of
+// keys 16 w .. 16 w + 15, which lie in one page), into the other of two buffers a
+// tile ahead, one barrier a tile.  S^T = K Q^T on 32x32x16 MFMAs puts a query in a lane's
+// column (16 of the scores of each 32 keys, the other 16 in lane ^ 32), and its weights
+// are then the operand of O^T += V^T P^T without leaving the registers; V^T's operand
+// is read from V's rows by the LDS's transposing reads (four keys of a column each).
+//
+// LDS: row k of a tile at PITCH k; K's 16-byte chunk c at c ^ (k mod chunks), V's 64-byte
+// chunk c at c ^ (k mod 4) (narrow rows: c ^ (k / 2 mod 2)), so that neither kind of
+// read meets a bank twice; the copies' lanes take their chunks from where that is.
+// Columns past D are zero from the start on.
+constexpr int TILE_WAVES = 8, TILE_KEYS = 128;
+
+template <int P>
+struct TileLds {
+    static constexpr int PITCH = P == 64 ? 128 : 256, CH = PITCH / 16, ROWS = 1024 / PITCH;  // rows of a copy
+    static constexpr int BUF = TILE_KEYS * PITCH, SMEM = 4 * BUF;                              // K0 K1 V0 V1
+    static constexpr int COPIES = 16 / ROWS;                                                   // of 16 keys
+    static __device__ __forceinline__ int vswz(int row) { return P == 64 ? (row >> 1 & 1) << 2 : (row & 3) << 2; }
+};
+
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x2 lds_columns(const unsigned char* p) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                         (__attribute__((address_space(3))) i16x4*)p));
+}
+
+template <typename T, int P>
+__global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendParams p) {
+    constexpr int KS = P / 16, DB = P / 32;
+    using x8 = typename T::x8;
+    using V = Value<T>;
+    using L = TileLds<P>;
+    extern __shared__ __align__(16) unsigned char smem[];  // TileLds::SMEM, and the tree's
+    TreeSmem<32 * TILE_WAVES>& tree = *reinterpret_cast<TreeSmem<32 * TILE_WAVES>*>(smem + L::SMEM);
+    const int lane = threadIdx.x & 63, hf = lane >> 5, l32 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Item it = item_of(p);
+    if (!it.there) return;
+    const uint32_t BH = (uint32_t)(p.B * p.H);
+    const int rg = it.group, split = (int)(it.unit / BH);
+    const int bh = (int)(it.unit - split * BH), b = bh / p.H, hk = bh - b * p.H;
+    const Queries qs = queries_of(p, b);
+    const int row0 = rg * p.per_group * 32;
+    const int rows_end = min(row0 + p.per_group * 32, p.rows);
+    // tiles that some row of the group sees
+    const int g0 = row0 / p.G, g1 = (rows_end - 1) / p.G;
+    const int last = max(0, qs.most(g0, g1));
+    const int nt = (last + TILE_KEYS - 1) / TILE_KEYS;
+    const int b0 = (int)((int64_t)split * nt / p.splits);
+    const int b1 = (int)((int64_t)(split + 1) * nt / p.splits);
+    const int wrow = row0 + 32 * wave, row = wrow + l32;
+    const bool active = wrow < rows_end;
+    const RowAt mine = row_at(row, hk, p.G, p.Q);
+    const int end = mine.there ? qs.end(mine.t) : 0;
+    const int t0 = wrow / p.G, t1 = (min(wrow + 32, p.rows) - 1) / p.G;
+    const int first = qs.least(t0, t1), wlast = active ? qs.most(t0, t1) : 0;  // of the wave
+    x8 qf[KS];
+    {
+        const uint16_t* q = p.q + b * p.q_sb + mine.t * p.q_st + mine.head * p.q_sh;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = 16 * s + 8 * hf;
+            u32x4 w{};
+            if (active && mine.there && d < p.D) w = *reinterpret_cast<const u32x4*>(q + d);
+            qf[s] = as_x8<x8>(w);
+        }
+    }
+    if (qs.tree && b1 * TILE_KEYS > qs.least(g0, g1)) tree_bits(tree, p, b, qs.nq, g0, g1 - g0 + 1);
+    const uint32_t* bits = tree.bits[active && mine.there ? mine.t - g0 : 0];
+    if (p.D < P) {
+        for (int i = threadIdx.x; i < L::SMEM / 16; i += 64 * TILE_WAVES)
+            reinterpret_cast<u32x4*>(smem)[i] = u32x4{};
+        __syncthreads();
+    }
+    // a tile's pages: lane l < 8 that of keys 16 l .. 16 l + 15
+    const int32_t* table = p.table.at + b * p.table.sb;
+    const int shift = p.table.shift, w = (int)p.table.w;
+    auto load_ids = [&](int tile) -> uint32_t {
+        const int entry = (tile * TILE_KEYS + 16 * (lane & 7)) >> shift;
+        return entry < w ? (uint32_t)table[entry] : ~0u;
+    };
+    // this lane's part of the wave's copies: row lr of each, 16-byte slot `slot`
+    const int lr = lane / L::CH, slot = lane % L::CH;
+    uint32_t koff[L::COPIES], voff;
+    bool kin[L::COPIES], vin;
+#pragma unroll
+    for (int e = 0; e < L::COPIES; ++e) {
+        const int r = L::ROWS * e + lr, c = slot ^ (r & (L::CH - 1));
+        kin[e] = 8 * c < p.D;
+        koff[e] = r * p.D + 8 * c;
+    }
+    {
+        const int c = slot ^ L::vswz(lr);
+        vin = 8 * c < p.D;
+        voff = lr * p.D + 8 * c;
+    }
+    const int64_t head = (int64_t)hk * p.page_d;
+    const int page_rows = 1 << shift;
+    auto issue = [&](int tile, int buf, uint32_t ids) {
+        uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)ids, wave);
+        id = id < p.table.pages ? id : 0;
+        const int key = tile * TILE_KEYS + 16 * wave;
+        const int64_t at = (int64_t)id * p.table.page_elems + head + (int64_t)(key & (page_rows - 1)) * p.D;
+        uint32_t vo = voff, ko[L::COPIES];
+#pragma unroll
+        for (int e = 0; e < L::COPIES; ++e) { ko[e] = koff[e]; asm volatile("" : "+v"(ko[e])); }
+        asm volatile("" : "+v"(vo));
+        unsigned char* kd = smem + buf * L::BUF + 16 * wave * L::PITCH;
+        unsigned char* vd = kd + 2 * L::BUF;
+#pragma unroll
+        for (int e = 0; e < L::COPIES; ++e)
+            if (kin[e]) dma16(p.k + at + ko[e], kd + 1024 * e);
+#pragma unroll
+        for (int e = 0; e < L::COPIES; ++e)
+            if (vin) dma16(p.v + at + L::ROWS * e * p.D + vo, vd + 1024 * e);
+    };
+    // operand offsets in buffer 0: K row l32 (+ 32 j), chunk 2 kk + hf; V rows 4 hf +
+    // lane % 16 / 4 (+ 32 j + 16 k, and 8 on), 32 columns i: column 16 (l32 / 16) on.  A
+    // group of 16 lanes gets column 4 a + e in lane 4 a' + e, a' = a with its bits
+    // swapped: a lane's results are then eight consecutive columns.
+    uint32_t kofs[KS], vofs[DB];
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) {
+        kofs[kk] = l32 * L::PITCH + 16 * ((2 * kk + hf) ^ (l32 & (L::CH - 1)));
+        asm volatile("" : "+v"(kofs[kk]));
+    }
+#pragma unroll
+    for (int i = 0; i < DB; ++i) {
+        const int x = lane & 15, k = 4 * hf + (x >> 2), a = ((x & 1) << 1) | (x >> 1 & 1);
+        const int chunk = 4 * i + 2 * (l32 >> 4) + (a >> 1);
+        vofs[i] = 2 * L::BUF + k * L::PITCH + 16 * (chunk ^ L::vswz(k)) + 8 * (a & 1);
+        asm volatile("" : "+v"(vofs[i]));
+    }
+    f32x16 o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; ++i) o[i] = f32x16{};
+    Stat st{NONE, 0.0f};
+    uint32_t ids = 0, paged = 0, next_paged = 0;
+    if (b0 < b1) {
+        ids = load_ids(b0);
+        next_paged = (uint32_t)__ballot(lane < 8 && ids < p.table.pages);
+        issue(b0, 0, ids);
+        ids = load_ids(b0 + 1);
+    }
+    // Whether some row of the wave does not see some of the 32 keys from k0 on (there: their
+    // halves' pages, a bit each), and which of them the lane's row sees.
+    auto masked = [&](int k0, uint32_t there) { return k0 + 32 > first || (there & 3) != 3; };
+    auto seen_word = [&](int k0, uint32_t there) {
+        const uint32_t seen = qs.tree && end - k0 < 32 ? tree_word(bits, k0 - end) : low_bits(end - k0);
+        return seen & ((there & 1 ? 0xffffu : 0u) | (there & 2 ? 0xffff0000u : 0u));
+    };
+    // One 32-key step's softmax and products with the V^T operands vf.
+    auto softmax_pv = [&](f32x16& s, const u32x4 (&vf)[2][DB]) {
+        float tm = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) tm = fmaxf(tm, s[i]);
+        tm = halfwave_max(tm) * p.scale_log2;
+        const bool up = tm > st.m + TAU;
+        const float m = up ? tm : st.m;
+        const float alpha = up ? __builtin_amdgcn_exp2f(st.m - m) : 1.0f;
+        st.m = m;
+        float c = p.scale_log2, off = (m == NONE ? 0.0f : m) - V::LIFT;
+        if (__any(fabsf(off) > 0x1p20f)) {
+            // a maximum so large that its own rounding counts: differences of rounded
+            // products instead of the product's remainder
+            const float ref = m == NONE ? 0.0f : m;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float z = s[i] * c;
+                asm("" : "+v"(z));
+                s[i] = z - ref;
+            }
+            c = 1.0f, off = -V::LIFT;
+        }
+        uint32_t pw[8];
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * i], c, -off));
+            const float y = __builtin_amdgcn_exp2f(fmaf(s[2 * i + 1], c, -off));
+            sum += x + y;
+            pw[i] = T::pack(x, y);
+        }
+        st.l = st.l * alpha + sum;
+        __builtin_amdgcn_s_setprio(1);
+        if (__any(up)) {
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const x8 pf = as_x8<x8>(u32x4{pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]});
+#pragma unroll
+            for (int i = 0; i < DB; ++i) o[i] = T::mfma32(as_x8<x8>(vf[k][i]), pf, o[i]);
+        }
+        __builtin_amdgcn_s_setprio(0);
+    };
+    // Waves w and w + 4 share a SIMD.  Waves 4-7 run half a step behind waves 0-3: each
+    // carries its tile's last step (masked scores in s, V^T operands in vf) across the
+    // barrier and finishes it first in the next tile, so that one's softmax runs beside
+    // the other's products.
+    const bool lag = wave >= TILE_WAVES / 2;
+    bool pend = false;
+    bool apart = false;                       // values that are not finite were taken out
+    f32x16 s;
+    x8 kf[KS];
+    u32x4 vf[2][DB];
+    auto load_k = [&](int j) {
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk)
+            kf[kk] = *reinterpret_cast<const x8*>(smem + kofs[kk] + j * 32 * L::PITCH);
+    };
+    auto load_v = [&](int j) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < DB; ++i) {
+                const u32x2 a = lds_columns(smem + vofs[i] + (32 * j + 16 * k) * L::PITCH);
+                const u32x2 c = lds_columns(smem + vofs[i] + (32 * j + 16 * k + 8) * L::PITCH);
+                vf[k][i] = u32x4{a[0], a[1], c[0], c[1]};
+            }
+    };
+    auto scores = [&]() {
+        __builtin_amdgcn_s_setprio(1);
+        s = T::mfma32(kf[0], qf[0], f32x16{});
+#pragma unroll
+        for (int kk = 1; kk < KS; ++kk) s = T::mfma32(kf[kk], qf[kk], s);
+        __builtin_amdgcn_s_setprio(0);
+    };
+    constexpr int STEPS = TILE_KEYS / 32;
+    // (one more turn than tiles, for what the lagging waves carry out of the last)
+    for (int tile = b0; tile <= b1; ++tile) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        paged = next_paged;
+        if (tile + 1 < b1) {
+            next_paged = (uint32_t)__ballot(lane < 8 && ids < p.table.pages);
+            issue(tile + 1, (tile + 1 - b0) & 1, ids);
+            ids = load_ids(tile + 2);
+        }
+        const int key0 = tile * TILE_KEYS;
+        const int nsub = tile == b1 ? 0 : min(max(wlast - key0 + 31, 0) >> 5, STEPS);
+        // (an idle wave's reads of the first step stay inside the buffer)
+        load_k(0);
+        if (pend) {
+            softmax_pv(s, vf);
+            // the new tile's V^T reads wait for the carried products, so that both sets
+            // are never live at once
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        pend = false;
+        load_v(0);
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) {
+            if (j >= nsub) break;
+            scores();
+            if (j + 1 < nsub) load_k(j + 1);
+            const int k0 = key0 + 32 * j;
+            if (masked(k0, paged >> (2 * j))) {
+                const uint32_t seen = seen_word(k0, paged >> (2 * j)) >> (4 * hf);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!(seen >> (8 * (i >> 2) + (i & 3)) & 1)) s[i] = -INFINITY;
+                uint32_t bad = 0;
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int i = 0; i < DB; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) bad |= not_finite<T>(vf[k][i][e]);
+                if (__any(bad != 0)) {
+                    apart = true;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int i = 0; i < DB; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) vf[k][i][e] = part_word<T>(vf[k][i][e]).finite;
+                }
+            }
+            if (lag && j + 1 == nsub) {
+                pend = true;
+                break;
+            }
+            softmax_pv(s, vf);
+            if (j + 1 < nsub) load_v(j + 1);
+        }
+        const int step = (tile - b0) & 1 ? -L::BUF : L::BUF;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+            kofs[kk] += step;
+            asm volatile("" : "+v"(kofs[kk]));
+        }
+#pragma unroll
+        for (int i = 0; i < DB; ++i) {
+            vofs[i] += step;
+            asm volatile("" : "+v"(vofs[i]));
+        }
+    }
+    // What was taken out of masked steps goes to the rows that see it, from memory.
+    if (apart)
+#pragma unroll 1
+        for (int k0 = b0 * TILE_KEYS; k0 < min(b1 * TILE_KEYS, wlast); k0 += 32) {
+            uint32_t id[2], there = 0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int entry = (k0 + 16 * h) >> shift;
+                id[h] = entry < w ? (uint32_t)table[entry] : ~0u;
+                if (id[h] < p.table.pages) there |= 1u << h;
+                else id[h] = 0;
+            }
+            if (!masked(k0, there)) continue;
+            const uint32_t seen = seen_word(k0, there);
+#pragma unroll 1
+            for (int k = 0; k < 32; ++k) {
+                const int64_t at = (int64_t)id[k >> 4] * p.table.page_elems + head +
+                                   (int64_t)((k0 + k) & (page_rows - 1)) * p.D;
+#pragma unroll
+                for (int i = 0; i < DB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int d = 32 * i + 16 * e + 8 * hf;
+                        u32x4 x{};
+                        if (d < p.D && seen >> k & 1) x = *reinterpret_cast<const u32x4*>(p.v + at + d);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float y = T::to_f32((uint16_t)(x[j >> 1] >> (16 * (j & 1))));
+                            if (!(fabsf(y) < INFINITY)) o[i][8 * e + j] += y;
+                        }
+                    }
+            }
+        }
+    st.l = halfwave_sum(st.l);
+    if constexpr (V::LIFT != 0.0f) st.l *= 1.0f / 4096.0f;
+    if (!active) return;
+#pragma unroll
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int d = 32 * i + 16 * e + 8 * hf;
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = o[i][8 * e + k];
+            if (p.splits > 1) store_partial(p, bh, split, row, d, st, x);
+            else store_row<T>(p, b, hk, row, d, st, x);
+        }
 }
 
 // ---------------------------------------------------------------- splits
@@ -596,11 +950,15 @@ __global__ void __launch_bounds__(256) merge_kernel(AttendParams p) {
 
 // ---------------------------------------------------------------- host
 struct Plan {
-    bool eight, two;              // eight waves; two groups of 16 rows
-    int groups, splits;
+    bool tile, eight, two;        // the tile kernel; of the other, eight waves, two groups of rows
+    int groups, splits, per_group;
     int64_t items, rows;
     size_t part, ml;              // bytes
 };
+
+// Up to this many rows of a key head, the kernel of 16-row groups; above it the tile
+// kernel.
+constexpr int64_t TILE_ROWS = 64;
 
 Plan attend_plan(const nkv_paged_attend_args* a) {
     const nkv_paged_cache& c = a->cache;
@@ -608,6 +966,28 @@ Plan attend_plan(const nkv_paged_attend_args* a) {
     pl.rows = a->Q * a->G;
     const int64_t heads = (int64_t)a->B * c.H, tiles = cdiv(a->n, TILE);
     pl.splits = 1;
+    pl.tile = pl.rows > TILE_ROWS;
+    if (pl.tile) {
+        // the fewest groups of up to eight 32-row blocks, of even size
+        const int64_t qb = cdiv(pl.rows, 32), blocks = cdiv(a->n, 64);
+        pl.groups = (int)cdiv(qb, TILE_WAVES);
+        pl.per_group = (int)cdiv(qb, pl.groups);
+        const int64_t base = heads * pl.groups;
+        // splits whose rounds of 256 workgroups take least, in units of the time of 64
+        // keys; a workgroup's start and end cost some, and a merge its partials' traffic
+        double best = 0.0;
+        const int64_t most = std::max<int64_t>(16, cdiv(256, std::max<int64_t>(base, 1)));
+        for (int64_t s = 1; s <= most && (s == 1 || blocks >= 4 * s); ++s) {
+            const double merge = s == 1 ? 0.0 : 4.0 + (double)heads * pl.rows * s * 4e-4;
+            const double t = (double)cdiv(base * s, 256) * ((double)blocks / s + 6.0) + merge;
+            if (s == 1 || t < best) {
+                best = t;
+                pl.splits = (int)s;
+            }
+        }
+        pl.items = base * pl.splits;
+        return pl;
+    }
     pl.two = pl.rows > 16;
     pl.groups = (int)cdiv(pl.rows, pl.two ? 32 : 16);
     const int64_t base = heads * pl.groups;
@@ -696,6 +1076,14 @@ int rows_run(const AttendParams& p, hipStream_t s) {
     return NKV_OK;
 }
 
+template <typename T, int P>
+int tile_run(const AttendParams& p, hipStream_t s) {
+    const int smem = TileLds<P>::SMEM + (p.parents ? (int)sizeof(TreeSmem<32 * TILE_WAVES>) : 0);
+    if (int rc = set_smem(attend_tile_kernel<T, P>, smem)) return rc;
+    attend_tile_kernel<T, P><<<item_blocks(p), 64 * TILE_WAVES, smem, s>>>(p);
+    return NKV_OK;
+}
+
 template <typename T, int KS>
 int attend_run(const AttendParams& p, const Plan& pl, hipStream_t s) {
     if (pl.two) return pl.eight ? rows_run<T, KS, 8, 2>(p, s) : rows_run<T, KS, 4, 2>(p, s);
@@ -704,6 +1092,8 @@ int attend_run(const AttendParams& p, const Plan& pl, hipStream_t s) {
 
 template <typename T>
 int attend_width(const AttendParams& p, const Plan& pl, hipStream_t s) {
+    if (pl.tile)
+        return p.D <= 64 ? tile_run<T, 64>(p, s) : p.D <= 96 ? tile_run<T, 96>(p, s) : tile_run<T, 128>(p, s);
     return p.D <= 64 ? attend_run<T, 2>(p, pl, s)
                      : p.D <= 96 ? attend_run<T, 3>(p, pl, s) : attend_run<T, 4>(p, pl, s);
 }
@@ -765,6 +1155,7 @@ extern "C" int nkv_paged_attend(void* stream, const nkv_paged_attend_args* a, vo
     p.groups = pl.groups;
     p.rows = (int)pl.rows;
     p.page_d = c.page * c.D;
+    p.per_group = pl.per_group;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     rc = c.dtype == NKV_ROWS_BF16 ? attend_width<Bf16>(p, pl, s) : attend_width<Fp16>(p, pl, s);
     if (rc) return rc;
