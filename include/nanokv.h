@@ -1070,14 +1070,15 @@ int nkv_paged_attend(void* stream, const nkv_paged_attend_args* args, void* work
  *   rows        int32, device, M entries an item, M <= NKV_PAGED_COMMIT
  *   start_dev, counts: as nkv_paged_append's (NULL: start; M)
  *   out_length  [B] int32, start + counts (both as clamped), or NULL
- * caches is an array in host memory, of at most NKV_PAGED_CACHES.  The pools overlap neither each other nor
+ * pools is an array in host memory, of at most NKV_PAGED_CACHES caches.  The pools overlap neither each other nor
  * anything else of the call; no two sequences write into the same page, and none
  * into one that another reads here.
  */
 #define NKV_PAGED_COMMIT 256
 #define NKV_PAGED_CACHES 64
 typedef struct nkv_paged_commit_args {
-    const nkv_paged_cache* caches;
+    nkv_paged_cache cache;        /* its shape and type; k and v are not read */
+    void* const* pools;           /* k and v of each cache in turn, 2 * n_caches */
     int64_t n_caches;
     const int32_t* table;
     int64_t table_sb;

@@ -296,7 +296,7 @@ class NkvPagedAttendArgs(Structure):
 
 class NkvPagedCommitArgs(Structure):
     _fields_ = [
-        ("caches", POINTER(NkvPagedCache)), ("n_caches", c_int64),
+        ("cache", NkvPagedCache), ("pools", POINTER(c_void_p)), ("n_caches", c_int64),
         ("table", c_void_p), ("table_sb", c_int64), ("table_w", c_int64),
         ("rows", c_void_p), ("rows_sb", c_int64), ("start", c_int64),
         ("start_dev", c_void_p), ("counts", c_void_p), ("out_length", c_void_p),

@@ -376,15 +376,14 @@ extern "C" int nkv_paged_append(void* stream, const nkv_paged_append_args* a) {
 extern "C" int nkv_paged_commit(void* stream, const nkv_paged_commit_args* a) {
     clear_error();
     NKV_REQUIRE(a, NKV_ERR_INVALID, "args is null");
-    NKV_REQUIRE(a->caches && a->n_caches >= 1, NKV_ERR_INVALID, "a cache is required");
+    NKV_REQUIRE(a->pools && a->n_caches >= 1, NKV_ERR_INVALID, "a cache is required");
     NKV_REQUIRE(a->n_caches <= NKV_PAGED_CACHES, NKV_ERR_UNSUPPORTED, "at most 64 caches a call");
-    const nkv_paged_cache& c = a->caches[0];
+    const int n = (int)a->n_caches;
+    nkv_paged_cache c = a->cache;
     int rc = NKV_OK;
-    for (int64_t i = 0; i < a->n_caches; ++i) {
-        const nkv_paged_cache& x = a->caches[i];
-        if ((rc = paged_check(x, __func__))) return rc;
-        NKV_REQUIRE(x.pages == c.pages && x.H == c.H && x.page == c.page && x.D == c.D && x.dtype == c.dtype,
-                    NKV_ERR_INVALID, "caches must have one geometry and type");
+    for (int i = 0; i < n; ++i) {
+        c.k = a->pools[2 * i], c.v = a->pools[2 * i + 1];
+        if ((rc = paged_check(c, __func__))) return rc;
     }
     if ((rc = paged_table_check(c, a->table, a->table_sb, a->table_w, a->B, __func__))) return rc;
     const PageTable table = page_table(c, a->table, a->table_sb, a->table_w);
@@ -395,16 +394,12 @@ extern "C" int nkv_paged_commit(void* stream, const nkv_paged_commit_args* a) {
     if ((rc = check_start(a->start, a->start_dev, a->counts, a->M, table.cap(), __func__))) return rc;
     if (a->B == 0 || (a->M == 0 && !a->out_length)) return NKV_OK;
     // every pool against every other: sorted, neighbours must not meet
-    std::pair<uintptr_t, int> sorted[2 * NKV_PAGED_CACHES];
-    const int n = (int)a->n_caches;
-    for (int i = 0; i < n; ++i) {
-        sorted[2 * i] = {reinterpret_cast<uintptr_t>(a->caches[i].k), i};
-        sorted[2 * i + 1] = {reinterpret_cast<uintptr_t>(a->caches[i].v), i};
-    }
+    uintptr_t sorted[2 * NKV_PAGED_CACHES];
+    for (int i = 0; i < 2 * n; ++i) sorted[i] = reinterpret_cast<uintptr_t>(a->pools[i]);
     std::sort(sorted, sorted + 2 * n);
     const uintptr_t bytes = (uintptr_t)pool_bytes(c);
     for (int i = 1; i < 2 * n; ++i)
-        NKV_REQUIRE(sorted[i].first - sorted[i - 1].first >= bytes, NKV_ERR_INVALID, "pools overlap");
+        NKV_REQUIRE(sorted[i] - sorted[i - 1] >= bytes, NKV_ERR_INVALID, "pools overlap");
     const Range small[5] = {{a->table, table_bytes(a->B, a->table_sb, a->table_w)},
                             {a->rows, a->M ? table_bytes(a->B, a->rows_sb, a->M) : 0},
                             {a->start_dev, a->start_dev ? a->B * 4 : 0},
@@ -412,7 +407,7 @@ extern "C" int nkv_paged_commit(void* stream, const nkv_paged_commit_args* a) {
                             {a->out_length, a->out_length ? a->B * 4 : 0}};
     for (int i = 0; i < 2 * n; ++i)
         for (const Range& r : small)
-            NKV_REQUIRE(!r.meets({reinterpret_cast<const void*>(sorted[i].first), (int64_t)bytes}),
+            NKV_REQUIRE(!r.meets({reinterpret_cast<const void*>(sorted[i]), (int64_t)bytes}),
                         NKV_ERR_INVALID, "the pools overlap the table, rows, start_dev, counts or out_length");
     for (int i = 0; i < 4; ++i)
         NKV_REQUIRE(!small[4].meets(small[i]), NKV_ERR_INVALID,
@@ -427,7 +422,7 @@ extern "C" int nkv_paged_commit(void* stream, const nkv_paged_commit_args* a) {
     p.out_length = a->out_length;
     p.H = c.H, p.D = c.D, p.M = a->M, p.B = a->B;
     p.page_d = c.page * c.D;
-    for (int i = 0; i < n; ++i) p.pool[i][0] = (uint16_t*)a->caches[i].k, p.pool[i][1] = (uint16_t*)a->caches[i].v;
+    for (int i = 0; i < n; ++i) p.pool[i][0] = (uint16_t*)a->pools[2 * i], p.pool[i][1] = (uint16_t*)a->pools[2 * i + 1];
     const dim3 grid((unsigned)c.H, (unsigned)a->B, (unsigned)n);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     if (a->M <= 16) commit_kernel<1><<<grid, 256, 0, s>>>(p);

@@ -67,6 +67,19 @@ __device__ __forceinline__ float parted(float o, float sum) {
     return o + (n & 127 ? INFINITY : 0.0f) + (n >= 128 ? -INFINITY : 0.0f);
 }
 
+// Division by a number known on the host, of numbers below 2^31: with 2^(s - 1) < d <=
+// 2^s and mul = floor(2^(31 + s) / d) + 1 the error e = mul d - 2^(31 + s) <= d <= 2^s,
+// so that n e < 2^(31 + s) and the product's high bits are the quotient.
+struct Divisor {
+    uint32_t d, mul, shift;
+    __device__ __forceinline__ uint32_t of(uint32_t n) const { return d == 1 ? n : __umulhi(n, mul) >> shift; }
+};
+Divisor divisor(int64_t d) {
+    int s = 0;
+    while (((int64_t)1 << s) < d) ++s;
+    return {(uint32_t)d, s ? (uint32_t)((((unsigned __int128)1 << (31 + s)) / d) + 1) : 0, s ? (uint32_t)s - 1 : 0};
+}
+
 struct AttendParams {
     PageTable table;
     const uint16_t* k;
@@ -84,6 +97,7 @@ struct AttendParams {
     f32x2* part_ml;
     int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;
     int64_t items;
+    Divisor by_G, by_H, by_BH, by_splits, by_groups;
     float scale_log2;
     int B, H, G, D, Q, n, causal, splits, groups, rows;
     int page_d;
@@ -95,10 +109,10 @@ struct RowAt {
     int t, head;
     bool there;
 };
-__device__ __forceinline__ RowAt row_at(int row, int hk, int G, int Q) {
-    const bool there = row < G * Q;
-    const int r = there ? row : 0;
-    return {r / G, hk * G + r % G, there};
+__device__ __forceinline__ RowAt row_at(const AttendParams& p, int row, int hk) {
+    const bool there = row < p.rows;
+    const int r = there ? row : 0, t = (int)p.by_G.of(r);
+    return {t, hk * p.G + r - t * p.G, there};
 }
 
 // The queries of an item: `nq` of its Q rows, the last tokens of `len`.
@@ -130,20 +144,27 @@ struct TreeSmem {
     uint32_t bits[TOKENS][TREE_WORDS];
 };
 
+// A workgroup's thread's part of the parents (workgroups have at least as many threads
+// as a tree tokens): loaded ahead of all else, and stored where it is needed.
+static_assert(NKV_PAGED_TREE <= 256, "a thread for each token");
+__device__ __forceinline__ int32_t tree_parent(const AttendParams& p, int b) {
+    return p.parents && (int)threadIdx.x < p.Q ? p.parents[b * p.parents_sb + threadIdx.x] : -1;
+}
+
 // Tokens t0 .. t0 + count, by all threads of the workgroup.  A way goes to lower tokens
 // only, so it ends.
 template <int TOKENS>
-__device__ __forceinline__ void tree_bits(TreeSmem<TOKENS>& sm, const AttendParams& p, int b, int nq,
-                                          int t0, int count) {
-    for (int i = threadIdx.x; i < p.Q; i += blockDim.x) sm.parents[i] = p.parents[b * p.parents_sb + i];
+__device__ __forceinline__ void tree_bits(TreeSmem<TOKENS>& sm, int32_t parent, int nq, int t0, int count) {
+    if (threadIdx.x < NKV_PAGED_TREE) sm.parents[threadIdx.x] = parent;
     __syncthreads();
-    for (int i = threadIdx.x; i < count; i += blockDim.x) {
-        uint32_t* bits = sm.bits[i];
+    if ((int)threadIdx.x < count) {
+        uint32_t* bits = sm.bits[threadIdx.x];
 #pragma unroll
         for (int w = 0; w < TREE_WORDS; ++w) bits[w] = 0;
-        for (int a = t0 + i < nq ? t0 + i : -1; a >= 0;) {
-            bits[a >> 5] |= 1u << (a & 31);
+        const int own = t0 + (int)threadIdx.x;
+        for (int a = own < nq ? own : -1; a >= 0;) {
             const int up = sm.parents[a];
+            bits[a >> 5] |= 1u << (a & 31);
             a = up < a ? up : -1;
         }
     }
@@ -180,7 +201,7 @@ __device__ __forceinline__ float weight(float m, float M) {
 template <typename T>
 __device__ __forceinline__ void store_row(const AttendParams& p, int b, int hk, int row, int d,
                                           const Stat& st, const float (&o)[8]) {
-    const RowAt at = row_at(row, hk, p.G, p.Q);
+    const RowAt at = row_at(p, row, hk);
     if (!at.there || d >= p.D) return;
     constexpr float DOWN = Value<T>::LIFT == 0.0f ? 1.0f : 1.0f / 4096.0f;
     const float f = st.l == 0.0f ? 0.0f : DOWN / st.l;
@@ -219,14 +240,21 @@ struct Item {
     bool there;
 };
 
+// Part `split` of n tiles: an even share, the first ones a tile more.
+__device__ __forceinline__ void share_of(const AttendParams& p, int split, int n, int& from, int& to) {
+    const int each = (int)p.by_splits.of(n), more = n - each * p.splits;
+    from = split * each + min(split, more);
+    to = from + each + (split < more);
+}
+
 __device__ __forceinline__ Item item_of(const AttendParams& p) {
     const uint32_t x = blockIdx.x & 7, k = blockIdx.x >> 3, groups = (uint32_t)p.groups;
-    const uint32_t items = (uint32_t)p.items, units = items / groups;
+    const uint32_t items = (uint32_t)p.items, units = p.by_groups.of(items);
     if (units >= UNITS) {
-        const uint32_t u = k / groups * 8 + x;
-        return {u, (int)(k % groups), u < units};
+        const uint32_t u = p.by_groups.of(k), unit = u * 8 + x;
+        return {unit, (int)(k - u * groups), unit < units};
     }
-    const uint32_t item = x * ((items + 7) >> 3) + k, u = item / groups;
+    const uint32_t item = x * ((items + 7) >> 3) + k, u = p.by_groups.of(item);
     return {u, (int)(item - u * groups), item < items && k < (items + 7) >> 3};
 }
 
@@ -280,22 +308,23 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Item it = item_of(p);
     if (!it.there) return;
-    const int rg = it.group, bh = (int)(it.unit / (uint32_t)p.splits);
-    const int split = (int)(it.unit - (uint32_t)bh * p.splits), b = bh / p.H, hk = bh - b * p.H;
+    const int rg = it.group, bh = (int)p.by_splits.of(it.unit);
+    const int split = (int)it.unit - bh * p.splits, b = (int)p.by_H.of(bh), hk = bh - b * p.H;
     const Queries qs = queries_of(p, b);
+    const int32_t parent = tree_parent(p, b);
     const int row0 = rg * ROWS;
     // tiles that some row of the group sees, and keys that every row does
-    const int t0 = row0 / p.G, t1 = min(row0 + ROWS - 1, p.rows - 1) / p.G;
+    const int t0 = (int)p.by_G.of(row0), t1 = (int)p.by_G.of(min(row0 + ROWS, p.rows) - 1);
     const int last = max(0, qs.most(t0, t1)), first = qs.least(t0, t1);
     const int nt = (last + TILE - 1) / TILE;
-    const int b0 = (int)((int64_t)split * nt / p.splits);
-    const int b1 = (int)((int64_t)(split + 1) * nt / p.splits);
+    int b0, b1;
+    share_of(p, split, nt, b0, b1);
     x8 qf[NQ][KS];
     int end[NQ];                              // keys that the lane's row sees
     const uint32_t* bits[NQ];                 // and the draft's tokens
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-        const RowAt mine = row_at(row0 + 16 * n + r, hk, p.G, p.Q);
+        const RowAt mine = row_at(p, row0 + 16 * n + r, hk);
         end[n] = mine.there ? qs.end(mine.t) : 0;
         bits[n] = sm.tree.bits[mine.there ? mine.t - t0 : 0];
         const uint16_t* q = p.q + b * p.q_sb + mine.t * p.q_st + mine.head * p.q_sh;
@@ -307,9 +336,8 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
             qf[n][s] = as_x8<x8>(w);
         }
     }
-    if (qs.tree && b1 * TILE > first) tree_bits(sm.tree, p, b, qs.nq, t0, t1 - t0 + 1);
     // this wave's tiles
-    const int w0 = b0 + (int)((int64_t)wave * (b1 - b0) / W), w1 = b0 + (int)((int64_t)(wave + 1) * (b1 - b0) / W);
+    const int w0 = b0 + (int)((uint32_t)(wave * (b1 - b0)) / W), w1 = b0 + (int)((uint32_t)((wave + 1) * (b1 - b0)) / W);
     const int shift = p.table.shift, page_rows = 1 << shift;
     Pages pages{p.table.at + b * p.table.sb, (int)p.table.w, 0, 0};
     // lane offsets into a page's rows of the head (elements)
@@ -371,6 +399,8 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
         load_k(w0);
         load_v();
     }
+    // (behind the first loads, which it does not wait for)
+    if (qs.tree && b1 * TILE > first) tree_bits(sm.tree, parent, qs.nq, t0, t1 - t0 + 1);
     for (int tile = w0; tile < w1; ++tile) {
         const int key0 = tile * TILE;
         there[0] = next_there[0], there[1] = next_there[1];
@@ -566,23 +596,23 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Item it = item_of(p);
     if (!it.there) return;
-    const uint32_t BH = (uint32_t)(p.B * p.H);
-    const int rg = it.group, split = (int)(it.unit / BH);
-    const int bh = (int)(it.unit - split * BH), b = bh / p.H, hk = bh - b * p.H;
+    const int rg = it.group, split = (int)p.by_BH.of(it.unit);
+    const int bh = (int)it.unit - split * p.B * p.H, b = (int)p.by_H.of(bh), hk = bh - b * p.H;
     const Queries qs = queries_of(p, b);
+    const int32_t parent = tree_parent(p, b);
     const int row0 = rg * p.per_group * 32;
     const int rows_end = min(row0 + p.per_group * 32, p.rows);
     // tiles that some row of the group sees
-    const int g0 = row0 / p.G, g1 = (rows_end - 1) / p.G;
+    const int g0 = (int)p.by_G.of(row0), g1 = (int)p.by_G.of(rows_end - 1);
     const int last = max(0, qs.most(g0, g1));
     const int nt = (last + TILE_KEYS - 1) / TILE_KEYS;
-    const int b0 = (int)((int64_t)split * nt / p.splits);
-    const int b1 = (int)((int64_t)(split + 1) * nt / p.splits);
+    int b0, b1;
+    share_of(p, split, nt, b0, b1);
     const int wrow = row0 + 32 * wave, row = wrow + l32;
     const bool active = wrow < rows_end;
-    const RowAt mine = row_at(row, hk, p.G, p.Q);
+    const RowAt mine = row_at(p, row, hk);
     const int end = mine.there ? qs.end(mine.t) : 0;
-    const int t0 = wrow / p.G, t1 = (min(wrow + 32, p.rows) - 1) / p.G;
+    const int t0 = (int)p.by_G.of(wrow), t1 = (int)p.by_G.of(min(wrow + 32, p.rows) - 1);
     const int first = qs.least(t0, t1), wlast = active ? qs.most(t0, t1) : 0;  // of the wave
     x8 qf[KS];
     {
@@ -595,7 +625,6 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
             qf[s] = as_x8<x8>(w);
         }
     }
-    if (qs.tree && b1 * TILE_KEYS > qs.least(g0, g1)) tree_bits(tree, p, b, qs.nq, g0, g1 - g0 + 1);
     const uint32_t* bits = tree.bits[active && mine.there ? mine.t - g0 : 0];
     if (p.D < P) {
         for (int i = threadIdx.x; i < L::SMEM / 16; i += 64 * TILE_WAVES)
@@ -672,6 +701,7 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
         issue(b0, 0, ids);
         ids = load_ids(b0 + 1);
     }
+    if (qs.tree && b1 * TILE_KEYS > qs.least(g0, g1)) tree_bits(tree, parent, qs.nq, g0, g1 - g0 + 1);
     // Whether some row of the wave does not see some of the 32 keys from k0 on (there: their
     // halves' pages, a bit each), and which of them the lane's row sees.
     auto masked = [&](int k0, uint32_t there) { return k0 + 32 > first || (there & 3) != 3; };
@@ -956,9 +986,12 @@ struct Plan {
     size_t part, ml;              // bytes
 };
 
-// Up to this many rows of a key head, the kernel of 16-row groups; above it the tile
-// kernel.
-constexpr int64_t TILE_ROWS = 64;
+// The tile kernel takes calls of more than TILE_ROWS rows of a key head and more than
+// TILE_WORK (row, key) pairs in all heads: a workgroup's start costs it about 10 us (us
+// with either, rows first; 8 heads of 4,096 keys: 128 rows 19.7, 23.4, 256 rows 25.4,
+// 32.2; 16 heads: 128 rows 24.8, 28.0; 32 heads: 128 rows 32.9, 32.0, 256 rows 51, 40; 64
+// heads: 64 rows 34, 41, 96 rows 51, 43; 64 heads of 8,192 keys, 128 rows: 99, 79).
+constexpr int64_t TILE_ROWS = 64, TILE_WORK = 1 << 24;
 
 Plan attend_plan(const nkv_paged_attend_args* a) {
     const nkv_paged_cache& c = a->cache;
@@ -966,20 +999,23 @@ Plan attend_plan(const nkv_paged_attend_args* a) {
     pl.rows = a->Q * a->G;
     const int64_t heads = (int64_t)a->B * c.H, tiles = cdiv(a->n, TILE);
     pl.splits = 1;
-    pl.tile = pl.rows > TILE_ROWS;
+    pl.tile = pl.rows > TILE_ROWS && heads * pl.rows > TILE_WORK / std::max<int64_t>(a->n, 1);
     if (pl.tile) {
         // the fewest groups of up to eight 32-row blocks, of even size
         const int64_t qb = cdiv(pl.rows, 32), blocks = cdiv(a->n, 64);
         pl.groups = (int)cdiv(qb, TILE_WAVES);
         pl.per_group = (int)cdiv(qb, pl.groups);
         const int64_t base = heads * pl.groups;
-        // splits whose rounds of 256 workgroups take least, in units of the time of 64
-        // keys; a workgroup's start and end cost some, and a merge its partials' traffic
+        // splits whose rounds of 256 workgroups take least, in units of the time of 64 keys
+        // (2.0 to 2.6 us): a workgroup's start and end cost five, a merge two and its
+        // partials' traffic (us with splits that fill half a round, one and two: 64 heads
+        // of 8,192 keys, 256 rows 155, 101, 118; 8 heads of 16,384, 512 rows 76, 63, 76;
+        // 32 heads of 4,096, 256 rows 48, 40, 75)
         double best = 0.0;
         const int64_t most = std::max<int64_t>(16, cdiv(256, std::max<int64_t>(base, 1)));
         for (int64_t s = 1; s <= most && (s == 1 || blocks >= 4 * s); ++s) {
-            const double merge = s == 1 ? 0.0 : 4.0 + (double)heads * pl.rows * s * 4e-4;
-            const double t = (double)cdiv(base * s, 256) * ((double)blocks / s + 6.0) + merge;
+            const double merge = s == 1 ? 0.0 : 2.0 + (double)heads * pl.rows * s * 2.5e-5;
+            const double t = (double)cdiv(base * s, 256) * ((double)blocks / s + 5.0) + merge;
             if (s == 1 || t < best) {
                 best = t;
                 pl.splits = (int)s;
@@ -988,11 +1024,20 @@ Plan attend_plan(const nkv_paged_attend_args* a) {
         pl.items = base * pl.splits;
         return pl;
     }
-    pl.two = pl.rows > 16;
+    // Two groups of 16 rows to a wave where there are more (us with one and two: 8 heads of
+    // 4,096 keys, 32 rows 11.3, 12.6, 64 rows 15.3, 14.8; 64 heads, 48 rows 43, 33).  Four
+    // waves a workgroup and one workgroup a CU: a start and a merge cost more than
+    // latency (8 heads of 4,096 keys, 4 rows: 128, 256, 512 workgroups 10.2, 9.3, 10.3 us;
+    // 2 heads of 262,144: 69, 46, 51); two of them where sequences have lengths of their
+    // own, so that CUs with short ones take more, or two groups much to do (16 heads of
+    // 4,096 keys, 256 rows: 40, 32); and eight waves in long calls of uneven sequences (32
+    // of up to 16,384 keys, 8 heads: 273, 249).
+    pl.two = pl.rows > 32;
     pl.groups = (int)cdiv(pl.rows, pl.two ? 32 : 16);
     const int64_t base = heads * pl.groups;
-    pl.eight = base * tiles >= 4096;
-    const int64_t slots = pl.eight && !a->length ? 256 : 512, waves = pl.eight ? 8 : 4;
+    const bool uneven = a->length && a->B > 1;
+    pl.eight = uneven && base * tiles >= 32768;
+    const int64_t slots = uneven || (pl.two && base * tiles > 8192) ? 512 : 256, waves = pl.eight ? 8 : 4;
     if (base > 0 && base < slots)
         pl.splits = (int)std::max<int64_t>(1, std::min(cdiv(slots, base), tiles / waves));
     pl.items = base * pl.splits;
@@ -1103,7 +1148,8 @@ void merge_run(const AttendParams& p, hipStream_t s) {
     auto grid = [&](int sg) {
         return dim3((unsigned)cdiv(p.rows, 16 / sg), (unsigned)p.H, (unsigned)p.B);
     };
-    if (p.splits > 8) merge_kernel<T, 16, 4><<<grid(16), 256, 0, s>>>(p);
+    if (p.splits > 64) merge_kernel<T, 16, 16><<<grid(16), 256, 0, s>>>(p);
+    else if (p.splits > 8) merge_kernel<T, 16, 4><<<grid(16), 256, 0, s>>>(p);
     else if (p.splits > 4) merge_kernel<T, 1, 8><<<grid(1), 256, 0, s>>>(p);
     else merge_kernel<T, 1, 4><<<grid(1), 256, 0, s>>>(p);
 }
@@ -1156,6 +1202,8 @@ extern "C" int nkv_paged_attend(void* stream, const nkv_paged_attend_args* a, vo
     p.rows = (int)pl.rows;
     p.page_d = c.page * c.D;
     p.per_group = pl.per_group;
+    p.by_G = divisor(a->G), p.by_H = divisor(c.H), p.by_BH = divisor((int64_t)a->B * c.H);
+    p.by_splits = divisor(pl.splits), p.by_groups = divisor(pl.groups);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     rc = c.dtype == NKV_ROWS_BF16 ? attend_width<Bf16>(p, pl, s) : attend_width<Fp16>(p, pl, s);
     if (rc) return rc;

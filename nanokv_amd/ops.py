@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from ctypes import byref
+from ctypes import byref, c_void_p
 from dataclasses import dataclass
 from typing import Optional
 
@@ -1658,13 +1658,13 @@ class PagedCache:
     def struct(self) -> NkvPagedCache:
         k, v = self.k, self.v
         code = _PAGED_CODES.get(k.dtype)
-        if code is None or v.dtype != k.dtype:
+        if code is None or v.dtype is not k.dtype:
             raise TypeError("cache pages must be bf16 or fp16, k and v alike")
         shape = k.shape
         if len(shape) != 4 or v.shape != shape:
             raise ValueError("cache pages must be [pages, H, page, head_dim], k and v alike")
         pages, H, page, D = shape
-        if page < 16 or page > 1024 or page & (page - 1):
+        if not 16 <= page <= 1024 or page & (page - 1):
             raise ValueError("page must be a power of two from 16 to 1,024")
         if D < 8 or D % 8 or D > 128 or pages < 1 or H < 1:
             raise ValueError("head_dim must be a multiple of 8, at most 128, with a page and a head")
@@ -1674,6 +1674,7 @@ class PagedCache:
 
 
 _PAGED_CODES = {torch.bfloat16: _lib.NKV_ROWS_BF16, torch.float16: _lib.NKV_ROWS_FP16}
+_NO_ROWS, _NO_INTS = (None, 0, 0, 0), (None, 0)
 
 
 def _int_rows(t: Optional[torch.Tensor], B: int, n: Optional[int], name: str):
@@ -1695,18 +1696,26 @@ def _int_rows(t: Optional[torch.Tensor], B: int, n: Optional[int], name: str):
 
 def _page_table(table: torch.Tensor):
     """(pointer, entries between items, width, B) of a page table."""
-    if len(table.shape) != 2:
+    if table.dtype is not torch.int32 or table.dim() != 2:
         raise ValueError("table must be an int32 tensor of [B, width]")
     B, width = table.shape
-    at, sb = _int_rows(table, B, None, "table")
-    return at, sb, width, B
+    sb, sw = table.stride()
+    if sw != 1 and width > 1:
+        raise ValueError("table must have contiguous columns")
+    return table.data_ptr(), sb if B > 1 else 0, width, B
 
 
-def _paged_rows(t: torch.Tensor, B: int, T: int, D: int, name: str):
-    shape = t.shape
-    if len(shape) != 4 or shape[0] != B or shape[1] != T or shape[3] != D:
-        raise ValueError(f"{name} must be [B, T, heads, head_dim] of the table's B and k's T")
-    return _strides_bthd(t, name) if t.numel() else (0, 0, 0)
+def _paged_rows(t: torch.Tensor, shape, name: str):
+    """(pointer, strides) of rows [B, T, heads, head_dim]."""
+    if t.shape != shape:
+        raise ValueError(f"{name} must be [B, T, heads, head_dim], B the table's, T k's")
+    sb, st, sh, sd = t.stride()
+    at = t.data_ptr()
+    if sd != 1 or at & 15 or (sb | st | sh) & 7:
+        if t.numel():
+            _strides_bthd(t, name)
+        sb = st = sh = 0
+    return at, sb, st, sh
 
 
 def paged_append(cache: PagedCache, table: torch.Tensor, k: torch.Tensor, v: torch.Tensor, start, *,
@@ -1733,18 +1742,20 @@ def paged_append(cache: PagedCache, table: torch.Tensor, k: torch.Tensor, v: tor
     given = start if isinstance(start, torch.Tensor) else None
     device = _require_gpu(cache.k, cache.v, table, k, v, given, counts, q, q_out, freqs, positions)
     c = cache.struct()
-    at, sb, width, B = _page_table(table)
-    if k.dtype not in (cache.k.dtype, torch.float32) or v.dtype != k.dtype:
+    table_args = _page_table(table)
+    B, D, kind = table_args[3], c.D, k.dtype
+    if v.dtype is not kind or kind is not cache.k.dtype and kind is not torch.float32:
         raise TypeError("k and v must both have the cache's type or be fp32")
-    if len(k.shape) != 4 or k.shape[2] != c.H or v.shape != k.shape:
-        raise ValueError("k and v must be [B, T, H, head_dim] of the cache's H and head_dim")
+    if k.dim() != 4:
+        raise ValueError("k must be [B, T, H, head_dim]")
     T = k.shape[1]
-    ks, vs = _paged_rows(k, B, T, c.D, "k"), _paged_rows(v, B, T, c.D, "v")
+    shape = (B, T, c.H, D)
+    ks, vs = _paged_rows(k, shape, "k"), _paged_rows(v, shape, "v")
     rot = heads = 0
-    qs = qos = (0, 0, 0)
+    qs = qos = _NO_ROWS
     if freqs is not None:
         _contig(freqs, torch.float32, "freqs")
-        if len(freqs.shape) != 1 or not 1 <= freqs.shape[0] <= c.D // 2:
+        if freqs.dim() != 1 or not 1 <= freqs.shape[0] <= D // 2:
             raise ValueError("freqs must be [rot / 2], rot at most head_dim")
         rot = 2 * freqs.shape[0]
         if rot % (8 if interleaved else 16):
@@ -1752,29 +1763,29 @@ def paged_append(cache: PagedCache, table: torch.Tensor, k: torch.Tensor, v: tor
     elif q is not None or positions is not None:
         raise ValueError("q and positions need freqs")
     if q is not None:
-        if q.dtype != k.dtype:
+        if q.dtype is not kind:
             raise TypeError("q must have k's type")
-        qs = _paged_rows(q, B, T, c.D, "q")
+        if q.dim() != 4 or q.shape[2] < 1:
+            raise ValueError("q must be [B, T, heads, head_dim]")
         heads = q.shape[2]
-        if heads < 1:
-            raise ValueError("q must have a head")
+        shape = (B, T, heads, D)
+        qs = _paged_rows(q, shape, "q")
         if q_out is None:
             make = torch.empty if counts is None else torch.zeros
-            q_out = make(q.shape, device=device, dtype=cache.k.dtype)
-            qos = (T * heads * c.D, heads * c.D, c.D)
-        elif q_out.shape != q.shape or q_out.dtype != cache.k.dtype:
-            raise ValueError("q_out must have q's shape and the cache's type")
+            q_out = make(shape, device=device, dtype=cache.k.dtype)
+            qos = q_out.data_ptr(), T * heads * D, heads * D, D
+        elif q_out.dtype is not cache.k.dtype:
+            raise ValueError("q_out must have the cache's type")
         else:
-            qos = _paged_rows(q_out, B, T, c.D, "q_out")
+            qos = _paged_rows(q_out, shape, "q_out")
     elif q_out is not None:
         raise ValueError("q_out needs q")
-    pos, pos_sb = _int_rows(positions, B, T, "positions")
-    a = NkvPagedAppendArgs(c, at, sb, width, k.data_ptr(), *ks, v.data_ptr(), *vs, _ptr(q), *qs,
-                           _ptr(q_out), *qos, _ptr(freqs), pos, pos_sb, T,
+    pos = _NO_INTS if positions is None else _int_rows(positions, B, T, "positions")
+    a = NkvPagedAppendArgs(c, *table_args[:3], *ks, *vs, *qs, *qos, _ptr(freqs), *pos, T,
                            0 if given is not None else int(start), _cache8_ints(given, B, "start"),
                            _cache8_ints(counts, B, "counts"), B, heads, rot, bool(interleaved),
-                           _ROW_CODES[k.dtype])
-    if k.numel():
+                           _ROW_CODES[kind])
+    if B and T:
         _device_call("nkv_paged_append", device, byref(a))
     return q_out
 
@@ -1805,7 +1816,7 @@ def paged_attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, length
                           length if isinstance(length, torch.Tensor) else None)
     c = cache.struct()
     at, sb, width, B = _page_table(table)
-    if q.dtype != cache.k.dtype:
+    if q.dtype is not cache.k.dtype:
         raise TypeError("q must have the cache's type")
     shape, H, D = q.shape, c.H, c.D
     if len(shape) != 4 or shape[0] != B or shape[3] != D or shape[2] == 0 or shape[2] % H:
@@ -1814,20 +1825,21 @@ def paged_attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, length
         raise ValueError("causal and parents exclude each other")
     _, Q, heads, _ = shape
     lengths, n = _cache8_bound(width * c.page, B, length, max_length)
-    strides = _strides_bthd(q, "q") if q.numel() else (0, 0, 0)
+    rows = _paged_rows(q, shape, "q")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        os = (Q * heads * D, heads * D, D)
-    elif out.shape != shape or out.dtype != q.dtype:
+        to = out.data_ptr(), Q * heads * D, heads * D, D
+    elif out.shape != shape or out.dtype is not q.dtype:
         raise ValueError("out must have q's shape and type")
     else:
-        os = _strides_bthd(out, "out") if q.numel() else (0, 0, 0)
-    lse = torch.empty((B, heads, Q), device=device, dtype=torch.float32) if return_lse else None
-    tree, tree_sb = _int_rows(parents, B, Q, "parents")
+        to = _paged_rows(out, shape, "out")
+    lse = torch.empty_strided((B, heads, Q), (heads * Q, Q, 1), device=device,
+                              dtype=torch.float32) if return_lse else None
+    tree = _NO_INTS if parents is None else _int_rows(parents, B, Q, "parents")
     scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
     a = NkvPagedAttendArgs(c, at, sb, width, B, heads // H, Q, n, lengths,
-                           _cache8_ints(counts, B, "counts"), tree, tree_sb, q.data_ptr(), *strides,
-                           out.data_ptr(), *os, _ptr(lse), scale, bool(causal))
+                           _cache8_ints(counts, B, "counts"), *tree, *rows, *to, _ptr(lse), scale,
+                           bool(causal))
     scratch, nbytes = _scratch("nkv_paged_attend_workspace_size", a, device, workspace)
     _device_call("nkv_paged_attend", device, byref(a), _ptr(scratch), nbytes)
     return out, lse
@@ -1845,24 +1857,26 @@ def paged_commit(caches, table: torch.Tensor, start, rows: torch.Tensor,
     caches = [caches] if isinstance(caches, PagedCache) else list(caches)
     if not caches:
         raise ValueError("a cache is required")
+    pools = [t for c in caches for t in (c.k, c.v)]
     given = start if isinstance(start, torch.Tensor) else None
-    device = _require_gpu(*(t for c in caches for t in (c.k, c.v)), table, rows, counts, given)
-    structs = [c.struct() for c in caches]
-    if any(c.k.shape != caches[0].k.shape or c.k.dtype != caches[0].k.dtype for c in caches):
-        raise ValueError("caches must have one shape and type")
+    device = _require_gpu(*pools, table, rows, counts, given)
+    c, shape, kind = caches[0].struct(), pools[0].shape, pools[0].dtype
+    for t in pools:
+        if t.shape != shape or t.dtype is not kind or not t.is_contiguous():
+            raise ValueError("caches must have one shape and type, and be contiguous")
     at, sb, width, B = _page_table(table)
-    if len(rows.shape) != 2:
+    if rows.dim() != 2:
         raise ValueError("rows must be an int32 tensor of [B, M]")
     M = rows.shape[1]
     if M > _lib.NKV_PAGED_COMMIT:
         raise ValueError(f"at most {_lib.NKV_PAGED_COMMIT} rows a sequence")
-    path, path_sb = _int_rows(rows, B, M, "rows")
+    path = _int_rows(rows, B, M, "rows")
     first, n = _cache8_ints(given, B, "start"), _cache8_ints(counts, B, "counts")
-    length = torch.empty((B,), device=device, dtype=torch.int32)
-    for i in range(0, len(structs), _lib.NKV_PAGED_CACHES):
-        part = structs[i:i + _lib.NKV_PAGED_CACHES]
-        a = NkvPagedCommitArgs((NkvPagedCache * len(part))(*part), len(part), at, sb, width, path,
-                               path_sb, 0 if given is not None else int(start), first, n,
+    length = torch.empty(B, device=device, dtype=torch.int32)
+    for i in range(0, len(pools), 2 * _lib.NKV_PAGED_CACHES):
+        part = [t.data_ptr() for t in pools[i:i + 2 * _lib.NKV_PAGED_CACHES]]
+        a = NkvPagedCommitArgs(c, (c_void_p * len(part))(*part), len(part) // 2, at, sb, width,
+                               *path, 0 if given is not None else int(start), first, n,
                                length.data_ptr(), B, M)
         _device_call("nkv_paged_commit", device, byref(a))
     return length

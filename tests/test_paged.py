@@ -65,8 +65,9 @@ def attend_args(**kw):
 def commit_args(caches=None, **kw):
     a = _lib.NkvPagedCommitArgs()
     caches = caches or [cache()]
-    a._held = (_lib.NkvPagedCache * len(caches))(*caches)
-    a.caches, a.n_caches = a._held, len(caches)
+    a.cache = caches[0]
+    a._held = (ctypes.c_void_p * (2 * len(caches)))(*(p for c in caches for p in (c.k, c.v)))
+    a.pools, a.n_caches = a._held, len(caches)
     a.table, a.table_sb, a.table_w = PTR + (3 << 24), 4, 4
     a.rows, a.rows_sb, a.out_length = PTR + (4 << 24), 3, PTR + (5 << 24)
     a.B, a.M, a.start = 2, 3, 0
@@ -185,14 +186,14 @@ def test_commit_refusals(kw, code, text):
     refused("nkv_paged_commit", commit_args(**kw), code, text)
 
 
-def test_commit_refuses_unlike_or_overlapping_caches():
+def test_commit_refuses_caches_that_overlap_or_are_too_many():
     other = PTR + (16 << 24)
-    for kw in (dict(pages=9), dict(H=1), dict(page=32), dict(D=128), dict(dtype=1)):
-        refused("nkv_paged_commit", commit_args([cache(), cache(at=other, **kw)]), INV, b"one geometry")
     refused("nkv_paged_commit", commit_args([cache(), cache()]), INV, b"overlap")
     refused("nkv_paged_commit", commit_args([cache(), cache(at=other), cache(at=PTR + 512)]), INV, b"overlap")
+    refused("nkv_paged_commit", commit_args([cache(), cache(at=other + 8)]), INV, b"aligned")
     many = [cache(at=other + (i << 26)) for i in range(65)]
     refused("nkv_paged_commit", commit_args(many), UNS, b"64 caches")
+    refused("nkv_paged_commit", commit_args(pools=None), INV, b"a cache")
 
 
 CALLS = r"""
