@@ -259,9 +259,12 @@ void append_run(const AppendParams& p, bool f32, unsigned grid, hipStream_t s) {
     else append_kernel<T, false><<<grid, 256, 0, s>>>(p);
 }
 
-// Threads that share a token's rows: as many as there are rows in small calls.
+// Threads that share a token's rows: as many as there are rows in small calls, above
+// them a third (us with one, two, three, four and eight rows a thread: 512 tokens of 48
+// heads' rows of 128 6.1, 6.0, 6.2, 6.8, 9.0; 1,024 9.0, 7.5, 7.3, 8.2, 11.5; 1,560 of 72
+// 16.3, 13.8, 13.6, 14.0, 14.9; 32,764 of 48 238, 170, 157, 157, 162).
 uint32_t append_slots(int64_t tokens, int units, int rows) {
-    const int64_t per = std::clamp<int64_t>(tokens * units * rows / (1 << 18), 1, 8);
+    const int64_t per = std::clamp<int64_t>(tokens * units * rows >> 17, 1, 3);
     return (uint32_t)cdiv(rows, per);
 }
 

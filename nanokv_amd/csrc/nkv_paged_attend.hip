@@ -573,13 +573,16 @@ constexpr int TILE_WAVES = 8, TILE_KEYS = 128;
 template <int P>
 struct TileLds {
     static constexpr int PITCH = P == 64 ? 128 : 256, CH = PITCH / 16, ROWS = 1024 / PITCH;  // rows of a copy
-    static constexpr int BUF = TILE_KEYS * PITCH, SMEM = 4 * BUF;                              // K0 K1 V0 V1
-    static constexpr int COPIES = 16 / ROWS;                                                   // of 16 keys
+    static constexpr int BUF = TILE_KEYS * PITCH, SMEM = 4 * BUF;                            // K0 K1 V0 V1
+    static constexpr int COPIES = 16 / ROWS;                                                 // of a wave's 16 rows
     static __device__ __forceinline__ int vswz(int row) { return P == 64 ? (row >> 1 & 1) << 2 : (row & 3) << 2; }
 };
 
 typedef short i16x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ u32x2 lds_columns(const unsigned char* p) {
+// (__restrict__: a read that might alias the copies in flight would wait for them all,
+// the next tile's among them; this one's are waited for at the barrier.  24 % of a call
+// that streams its pages from memory)
+__device__ __forceinline__ u32x2 lds_columns(const unsigned char* __restrict__ p) {
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                          (__attribute__((address_space(3))) i16x4*)p));
 }
@@ -631,12 +634,23 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
             reinterpret_cast<u32x4*>(smem)[i] = u32x4{};
         __syncthreads();
     }
-    // a tile's pages: lane l < 8 that of keys 16 l .. 16 l + 15
+    // The pages of 64 tiles, a lane each: that of this wave's rows, and a bit for each
+    // 16 keys whether theirs is one.
     const int32_t* table = p.table.at + b * p.table.sb;
     const int shift = p.table.shift, w = (int)p.table.w;
-    auto load_ids = [&](int tile) -> uint32_t {
-        const int entry = (tile * TILE_KEYS + 16 * (lane & 7)) >> shift;
-        return entry < w ? (uint32_t)table[entry] : ~0u;
+    int ids_of = 0;
+    uint32_t ids = 0, there = 0;
+    auto load_ids = [&](int tile) {
+        ids_of = tile;
+        there = 0;
+#pragma unroll
+        for (int i = 0; i < TILE_KEYS / 16; ++i) {
+            const int64_t entry = ((int64_t)(tile + lane) * TILE_KEYS + 16 * i) >> shift;
+            const uint32_t id = entry < w ? (uint32_t)table[entry] : ~0u;
+            there |= id < p.table.pages ? 1u << i : 0u;
+            if (i == wave) ids = id;
+        }
+        ids = ids < p.table.pages ? ids : 0;
     };
     // this lane's part of the wave's copies: row lr of each, 16-byte slot `slot`
     const int lr = lane / L::CH, slot = lane % L::CH;
@@ -655,10 +669,9 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
     }
     const int64_t head = (int64_t)hk * p.page_d;
     const int page_rows = 1 << shift;
-    auto issue = [&](int tile, int buf, uint32_t ids) {
-        uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)ids, wave);
-        id = id < p.table.pages ? id : 0;
-        const int key = tile * TILE_KEYS + 16 * wave;
+    auto issue = [&](int tile) {
+        const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)ids, tile - ids_of);
+        const int key = tile * TILE_KEYS + 16 * wave, buf = (tile - b0) & 1;
         const int64_t at = (int64_t)id * p.table.page_elems + head + (int64_t)(key & (page_rows - 1)) * p.D;
         uint32_t vo = voff, ko[L::COPIES];
 #pragma unroll
@@ -694,12 +707,9 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
 #pragma unroll
     for (int i = 0; i < DB; ++i) o[i] = f32x16{};
     Stat st{NONE, 0.0f};
-    uint32_t ids = 0, paged = 0, next_paged = 0;
     if (b0 < b1) {
-        ids = load_ids(b0);
-        next_paged = (uint32_t)__ballot(lane < 8 && ids < p.table.pages);
-        issue(b0, 0, ids);
-        ids = load_ids(b0 + 1);
+        load_ids(b0);
+        issue(b0);
     }
     if (qs.tree && b1 * TILE_KEYS > qs.least(g0, g1)) tree_bits(tree, parent, qs.nq, g0, g1 - g0 + 1);
     // Whether some row of the wave does not see some of the 32 keys from k0 on (there: their
@@ -792,13 +802,13 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
     constexpr int STEPS = TILE_KEYS / 32;
     // (one more turn than tiles, for what the lagging waves carry out of the last)
     for (int tile = b0; tile <= b1; ++tile) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        paged = next_paged;
+        // this tile's copies have arrived, and all reads of the other buffer
+        wait_vmcnt<0>();
+        lds_barrier();
+        const uint32_t paged = tile < b1 ? (uint32_t)__builtin_amdgcn_readlane((int)there, tile - ids_of) : 0;
         if (tile + 1 < b1) {
-            next_paged = (uint32_t)__ballot(lane < 8 && ids < p.table.pages);
-            issue(tile + 1, (tile + 1 - b0) & 1, ids);
-            ids = load_ids(tile + 2);
+            if (tile + 1 - ids_of >= 64) load_ids(tile + 1);
+            issue(tile + 1);
         }
         const int key0 = tile * TILE_KEYS;
         const int nsub = tile == b1 ? 0 : min(max(wlast - key0 + 31, 0) >> 5, STEPS);
@@ -863,16 +873,16 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
     if (apart)
 #pragma unroll 1
         for (int k0 = b0 * TILE_KEYS; k0 < min(b1 * TILE_KEYS, wlast); k0 += 32) {
-            uint32_t id[2], there = 0;
+            uint32_t id[2], pages = 0;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int entry = (k0 + 16 * h) >> shift;
                 id[h] = entry < w ? (uint32_t)table[entry] : ~0u;
-                if (id[h] < p.table.pages) there |= 1u << h;
+                if (id[h] < p.table.pages) pages |= 1u << h;
                 else id[h] = 0;
             }
-            if (!masked(k0, there)) continue;
-            const uint32_t seen = seen_word(k0, there);
+            if (!masked(k0, pages)) continue;
+            const uint32_t seen = seen_word(k0, pages);
 #pragma unroll 1
             for (int k = 0; k < 32; ++k) {
                 const int64_t at = (int64_t)id[k >> 4] * p.table.page_elems + head +

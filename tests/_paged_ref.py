@@ -1,6 +1,7 @@
 """Plain 64-bit forms of the paged cache's operators, on numpy arrays, with bounds of
 the kernels' errors derived from where they round."""
 import numpy as np
+import torch
 
 HALF = {"bf16": 2.0 ** -8, "fp16": 2.0 ** -11}      # half a step, relative
 
@@ -94,6 +95,38 @@ def attend(q, k, v, see, scale, u, W):
             otol[t, h] = (W + 4 * ez + 2 * adds) * a * 1.01 + u * np.abs(out[t, h]) + small + 1e-30
             lse[h, t] = m + np.log(tot)
             ltol[h, t] = 2 * ez + adds + 2.0 ** -22 * (abs(m) + abs(np.log(tot)) + 1)
+    return out, lse, otol, ltol
+
+
+def attend_gpu(q, k, v, see, scale, u, W):
+    """The same in torch on the tensors' device, for large sequences: q [Q, Hq, D], k and
+    v [H, n, D] float64, see [Q, n]."""
+    Q, Hq, D = q.shape
+    H, n, _ = k.shape
+    some = see.any(1)
+    out, otol = torch.zeros_like(q), torch.zeros_like(q)
+    lse = torch.full((Hq, Q), -np.inf, dtype=q.dtype, device=q.device)
+    ltol = torch.zeros_like(lse)
+    count = see.sum(1).to(q.dtype)
+    if n == 0:
+        return out, lse, otol, ltol
+    for h in range(Hq):
+        kk, vv = k[h // (Hq // H)], v[h // (Hq // H)]
+        z = (q[:, h] @ kk.T * scale).masked_fill(~see, -np.inf)
+        mag = (q[:, h].abs() @ kk.abs().T).masked_fill(~see, 0).amax(1) * scale
+        ez = (D + 4) * 2.0 ** -24 * mag + 2.0 ** -21
+        m = torch.where(some, z.amax(1), 0)
+        p = torch.exp(z - m[:, None])
+        tot = torch.where(some, p.sum(1), 1)
+        out[:, h] = p @ vv / tot[:, None]
+        a = p @ vv.abs() / tot[:, None]
+        adds = (count + 32) * 2.0 ** -24
+        top = (see[:, :, None] * vv.abs().amax(1)[None, :, None]).amax((1, 2))
+        small = count * 2.0 ** -37 * top + (2.0 ** -25 if u == 2.0 ** -11 else 0)
+        otol[:, h] = ((W + 4 * ez + 2 * adds)[:, None] * a * 1.01 + u * out[:, h].abs()
+                      + small[:, None] + 1e-30)
+        lse[h] = torch.where(some, m + torch.log(tot), -np.inf)
+        ltol[h] = 2 * ez + adds + 2.0 ** -22 * (m.abs() + torch.log(tot).abs() + 1)
     return out, lse, otol, ltol
 
 

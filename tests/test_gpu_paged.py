@@ -302,6 +302,123 @@ def test_attend_tree(dev, name, B, Hq, H, D, page, Q, lengths, counts):
     check(q, cache, table, lengths, out, lse, parents=np.array(parents[0]), counts=counts)
 
 
+def check_large(q, cache, table, lengths, out, lse, causal=False, parents=None, counts=None):
+    """check on the GPU, sequence by sequence."""
+    B, Q, Hq, D = q.shape
+    u = ref.HALF["bf16" if q.dtype == torch.bfloat16 else "fp16"]
+    pages, H, page, _ = cache.k.shape
+    for b in range(B):
+        n, c = lengths[b], Q if counts is None else counts[b]
+        see = torch.tensor(ref.visible(Q, n, c, causal, None if parents is None else parents[b]),
+                           device=q.device)
+        at = table[b, :-(-n // page)].long()
+        there = ((at >= 0) & (at < pages)).repeat_interleave(page)[:n]
+        see &= there
+        k, v = (x[at.clamp(0, pages - 1)].transpose(0, 1).reshape(H, -1, D)[:, :n].double().clone()
+                for x in (cache.k, cache.v))
+        unseen = ~see.any(0)
+        k[:, unseen] = 0
+        v[:, unseen] = 0
+        qq = q[b].double()
+        qq[c:] = 0
+        ro, rl, ot, lt = ref.attend_gpu(qq, k, v, see, D ** -0.5, u, u)
+        got, gl = out[b].double(), lse[b].double()
+        assert torch.isfinite(got).all()
+        assert ((got - ro).abs() <= ot).all(), (b, ((got - ro).abs() - ot).max().item())
+        empty = torch.isneginf(rl)
+        assert torch.equal(torch.isneginf(gl), empty)
+        assert (got.transpose(0, 1)[empty] == 0).all()
+        assert ((gl - rl).abs()[~empty] <= lt[~empty]).all()
+
+
+# more than 2^24 (row, key) pairs in all heads, and more than 64 rows of a key head
+LARGE = [
+    # B, Hq, H, D, page, Q, lengths, counts
+    (2, 16, 8, 128, 16, 256, [2300, 2111], None), (3, 12, 12, 64, 32, 333, [1800, 0, 2049], [333, 5, 100]),
+    (1, 32, 8, 96, 128, 130, [4097], None), (2, 16, 4, 80, 16, 111, [5000, 111], [111, 60]),
+    (1, 7, 1, 40, 64, 300, [9000], [300]), (4, 8, 8, 128, 64, 257, [3000, 257, 1, 2500], None),
+    (1, 24, 24, 120, 16, 100, [8200], None),
+]
+
+
+@pytest.mark.parametrize("name", ["bf16", "fp16"])
+@pytest.mark.parametrize("what", ["whole", "causal", "tree"])
+@pytest.mark.parametrize("B,Hq,H,D,page,Q,lengths,counts", LARGE)
+def test_attend_many_rows(dev, name, what, B, Hq, H, D, page, Q, lengths, counts):
+    if what == "tree":
+        Q = min(Q, 256)
+        counts = None if counts is None else [min(c, Q) for c in counts]
+    rng = np.random.default_rng(100)
+    cache, table = make_pool(dev, lengths, H, D, page, TYPES[name], 101)
+    q = queries(dev, B, Q, Hq, D, TYPES[name], 102)
+    ct = None
+    if counts:
+        for b, c in enumerate(counts):
+            q[b, c:] = float("nan")
+        ct = torch.tensor(counts, dtype=torch.int32, device=dev)
+    n = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    parents = [random_tree(rng, Q, b % 2 == 1) for b in range(B)] if what == "tree" else None
+    tree = None if parents is None else torch.tensor(parents, dtype=torch.int32, device=dev)
+    out, lse = ops.paged_attend(q, cache, table, n, causal=what == "causal", parents=tree, counts=ct)
+    check_large(q, cache, table, lengths, out, lse, what == "causal", parents, counts)
+    # some pages are none
+    for b, m in enumerate(lengths):
+        if m > 4 * page:
+            table[b, 1], table[b, m // page // 2], table[b, m // page - 1] = -1, 2 ** 31 - 1, cache.k.shape[0]
+    out, lse = ops.paged_attend(q, cache, table, n, causal=what == "causal", parents=tree, counts=ct)
+    check_large(q, cache, table, lengths, out, lse, what == "causal", parents, counts)
+
+
+@pytest.mark.parametrize("name", ["bf16", "fp16"])
+@pytest.mark.parametrize("what", ["causal", "tree"])
+def test_many_rows_that_are_not_seen_may_hold_anything(dev, what, name):
+    rng = np.random.default_rng(103)
+    dtype, n, Q, H = TYPES[name], 2200, 200, 40
+    cache, table = make_pool(dev, [n], H, 128, 16, dtype, 104)
+    q = queries(dev, 1, Q, H, 128, dtype, 105)
+    parents = random_tree(rng, Q)
+    kw = dict(causal=True) if what == "causal" else dict(
+        parents=torch.tensor(parents, dtype=torch.int32, device=dev))
+    clean = ops.paged_attend(q, cache, table, n, **kw)
+    see = ref.visible(Q, n, Q, what == "causal", None if what == "causal" else parents)
+    for x, row, value in ((cache.k, n - 2, "nan"), (cache.v, n - Q + 3, "nan"), (cache.v, n - 1, "inf"),
+                          (cache.v, n - 77, "-inf")):
+        p, r = ref.slots(table[0].tolist(), 16, row)
+        held = x[p, :, r, 21].clone()
+        x[p, :, r, 21] = float(value)
+        out, lse = ops.paged_attend(q, cache, table, n, **kw)
+        x[p, :, r, 21] = held
+        hit = torch.tensor(see[:, row], device=dev)
+        assert hit.any() and not hit.all()
+        assert torch.equal(out[0, ~hit], clean[0][0, ~hit])
+        assert torch.equal(lse[0][:, ~hit], clean[1][0][:, ~hit])
+        if x is cache.v:
+            got = out[0, hit][..., 21]
+            assert (got.isnan() if value == "nan" else got == float(value)).all()
+            others = torch.arange(128, device=dev) != 21
+            assert torch.equal(out[0, hit][..., others], clean[0][0, hit][..., others])
+            assert torch.equal(lse, clean[1])
+        else:
+            assert out[0, hit].isnan().all() and lse[0][:, hit].isnan().all()
+
+
+@pytest.mark.parametrize("name", ["bf16", "fp16"])
+def test_many_rows_of_large_scores(dev, name):
+    dtype = TYPES[name]
+    cache, table = make_pool(dev, [4200], 16, 128, 32, dtype, 106)
+    q = queries(dev, 1, 300, 16, 128, dtype, 107, scale=30.0)
+    out, lse = ops.paged_attend(q, cache, table, 4200)
+    check_large(q, cache, table, [4200], out, lse)
+    cache.k[..., 0] = -1.0
+    q[..., 0] = 3e4
+    out, lse = ops.paged_attend(q, cache, table, 4200, softmax_scale=1e5)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    for size in (16, 1 << 20):
+        work = torch.empty(size, dtype=torch.uint8, device=dev)
+        fewer = ops.paged_attend(q, cache, table, 4200, softmax_scale=1e5, workspace=work)
+        assert torch.isfinite(fewer[0]).all()
+
+
 @pytest.mark.parametrize("Q,G", [(5, 1), (48, 2), (200, 2)])
 def test_a_chain_is_the_causal_mask(dev, Q, G):
     cache, table = make_pool(dev, [333], 2, 128, 16, torch.bfloat16, 27)
