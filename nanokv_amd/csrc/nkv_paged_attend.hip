@@ -1035,21 +1035,29 @@ Plan attend_plan(const nkv_paged_attend_args* a) {
         return pl;
     }
     // Two groups of 16 rows to a wave where there are more (us with one and two: 8 heads of
-    // 4,096 keys, 32 rows 11.3, 12.6, 64 rows 15.3, 14.8; 64 heads, 48 rows 43, 33).  Four
-    // waves a workgroup and one workgroup a CU: a start and a merge cost more than
-    // latency (8 heads of 4,096 keys, 4 rows: 128, 256, 512 workgroups 10.2, 9.3, 10.3 us;
-    // 2 heads of 262,144: 69, 46, 51); two of them where sequences have lengths of their
-    // own, so that CUs with short ones take more, or two groups much to do (16 heads of
-    // 4,096 keys, 256 rows: 40, 32); and eight waves in long calls of uneven sequences (32
-    // of up to 16,384 keys, 8 heads: 273, 249).
+    // 4,096 keys, 32 rows 11.3, 12.6, 64 rows 15.3, 14.8; 64 heads, 48 rows 43, 33).
     pl.two = pl.rows > 32;
     pl.groups = (int)cdiv(pl.rows, pl.two ? 32 : 16);
-    const int64_t base = heads * pl.groups;
+    const int64_t base = heads * pl.groups, work = base * tiles;
     const bool uneven = a->length && a->B > 1;
-    pl.eight = uneven && base * tiles >= 32768;
-    const int64_t slots = uneven || (pl.two && base * tiles > 8192) ? 512 : 256, waves = pl.eight ? 8 : 4;
-    if (base > 0 && base < slots)
-        pl.splits = (int)std::max<int64_t>(1, std::min(cdiv(slots, base), tiles / waves));
+    // Up to 16 tiles no splits: the second launch and its workspace cost more than they save
+    // (8 heads of 512 keys 9.2 us without, 8.3 with them, but a call takes the host 10.5
+    // and 14; of 1,024 keys 13.5 and 9.2).
+    if (tiles <= 16) {
+        pl.eight = tiles > 8;
+        pl.items = base;
+        return pl;
+    }
+    // Else one workgroup a CU, as a start and a merge cost more than latency (8 heads of
+    // 4,096 keys, 4 rows: 128, 256, 512 workgroups 10.2, 9.3, 10.3 us; 2 heads of 262,144:
+    // 69, 46, 51), of four waves, or eight where sequences have lengths of their own (128
+    // heads of 2,048 keys 26.5, 24.4; of up to 4,096 34.1, 34.9); two a CU in long calls of
+    // those, so that CUs with short ones take more (32 of up to 16,384 keys, 8 heads: 273,
+    // 249), and for two groups with much to do (16 heads of 4,096 keys, 256 rows: 40, 32).
+    pl.eight = uneven && work >= 4096;
+    const int64_t slots = (uneven && work >= 32768) || (pl.two && work > 8192) ? 512 : 256;
+    if (base < slots)
+        pl.splits = (int)std::max<int64_t>(1, std::min(cdiv(slots, std::max<int64_t>(base, 1)), tiles / (pl.eight ? 8 : 4)));
     pl.items = base * pl.splits;
     return pl;
 }
