@@ -260,12 +260,17 @@ __device__ __forceinline__ Item item_of(const AttendParams& p) {
 
 // ---------------------------------------------------------------- few rows
 // W waves of a workgroup share NQ groups of 16 query rows and a range of 32-key tiles;
-// each wave walks a run of tiles of its own, straight from memory into registers, and
-// the waves' results are merged in LDS.  S^T = K Q^T on 16x16x32 MFMAs leaves lane (r,
-// g) = (lane % 16, lane / 16) the scores of row r and keys 16 t + 4 g + e, whose
-// weights are then the operand of O^T += V^T P^T without leaving the registers.  V's
-// columns 8 r .. 8 r + 7 are a lane's (4 r .. of narrow heads), so its transposition is
-// a choice of halves of eight rows' words.
+// each wave walks a run of tiles of its own, and the waves' results are merged in LDS.
+// S^T = K Q^T on 16x16x32 MFMAs leaves lane (r, g) = (lane % 16, lane / 16) the scores of
+// row r and keys 16 t + 4 g + e, whose weights are then the operand of O^T += V^T P^T
+// without leaving the registers.  V's columns 8 r .. 8 r + 7 are a lane's (4 r .. of
+// narrow heads), so its transposition is a choice of halves of eight rows' words, read
+// straight from memory, whole rows to 16 lanes.  K's operand has a row to each of 16
+// lanes: read from memory that is 64 accesses of the vector cache to a load (a CU then
+// moves 58 GB/s of a context, eight waves 75 us for 8,192 keys of 8 heads without
+// splits), so that K's rows pass through the wave's own LDS buffers (51 us).
+// Long calls are bound by memory: two heads of 262,144 keys, 268 MB, 41 us, 6.5 TB/s
+// beside a merge of 6; 32 ragged sequences up to 16,384, 1.47 GB, 246 us, 6.0 TB/s.
 constexpr int TILE = 32;
 
 // Page numbers of a run of tiles, 64 at a time, a lane each.
@@ -275,6 +280,8 @@ struct Pages {
     __device__ __forceinline__ void load(int entry) {
         first = entry;
         ids = w ? at[min(entry + (int)(threadIdx.x & 63), w - 1)] : -1;
+        // (has arrived where the branch around this ends: a use behind it would wait for all loads)
+        asm volatile("" : "+v"(ids));
     }
     // entry `entry` (uniform; never below that of the last call by more than it has)
     __device__ __forceinline__ uint32_t get(int entry) {
@@ -284,12 +291,30 @@ struct Pages {
     }
 };
 
-template <int D, int W, int NQ>
+// One 16-byte-per-lane copy from 16 rows of a page (their bytes from `rows` on) into LDS,
+// the 64 lanes' pieces one after the other, from `further` bytes on for all of them; a
+// lane whose offset is NO_ROW brings zeros.  (By the buffer form: behind a global one every wait for a load
+// becomes one for all loads.)
+constexpr uint32_t NO_ROW = 1u << 30;
+__device__ __forceinline__ void copy_rows(const uint16_t* rows, int bytes, uint32_t offset, int further,
+                                          void* l) {
+    const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(rows), 0, bytes, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, NKV_LDS(l), 16, (int)offset, further, 0, 0);
+}
+
+template <int P>
+struct KeyLds {
+    static constexpr int PITCH = 2 * P, CH = PITCH / 16, ROWS = 1024 / PITCH;   // rows of a copy
+    static constexpr int BUF = TILE * PITCH, COPIES = TILE / ROWS;
+};
+
+template <int P, int W, int NQ>
 struct RowsSmem {
     union {
-        float o[W][16 * NQ][D + 4];
-        TreeSmem<16 * NQ> tree;
+        unsigned char k[W][2][KeyLds<P>::BUF];
+        float o[W][16 * NQ][P + 4];
     };
+    TreeSmem<16 * NQ> tree;
     Stat st[W][16 * NQ];
 };
 
@@ -302,6 +327,7 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
     constexpr bool SPLIT = std::is_same_v<T, Bf16>;
     using x8 = typename T::x8;
     using V = Value<T>;
+    using L = KeyLds<P>;
     extern __shared__ __align__(16) unsigned char rows_smem[];
     RowsSmem<P, W, NQ>& sm = *reinterpret_cast<RowsSmem<P, W, NQ>*>(rows_smem);
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
@@ -340,10 +366,19 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
     const int w0 = b0 + (int)((uint32_t)(wave * (b1 - b0)) / W), w1 = b0 + (int)((uint32_t)((wave + 1) * (b1 - b0)) / W);
     const int shift = p.table.shift, page_rows = 1 << shift;
     Pages pages{p.table.at + b * p.table.sb, (int)p.table.w, 0, 0};
-    // lane offsets into a page's rows of the head (elements)
-    uint32_t koff[KS], voff[4];
+    // lane offsets into a page's rows of the head (elements): V's rows, and K's in the copies:
+    // row lr of each, whose 16-byte slot `slot` holds chunk slot ^ row
+    uint32_t koff[L::COPIES], voff[4];
+    const int lr = lane / L::CH, slot = lane % L::CH;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) koff[s] = r * p.D + (32 * s + 8 * g < p.D ? 32 * s + 8 * g : 0);
+    for (int e = 0; e < L::COPIES; ++e) {
+        const int row = L::ROWS * e + lr, c = slot ^ (row & (L::CH - 1));
+        koff[e] = 8 * c < p.D ? 2 * ((row & 15) * p.D + 8 * c) : NO_ROW;
+    }
+    // K's operands: row r (+ 16 t), chunk 4 s + g
+    uint32_t kofs[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) kofs[s] = r * L::PITCH + 16 * ((4 * s + g) ^ (r & (L::CH - 1)));
 #pragma unroll
     for (int j = 0; j < 4; ++j) voff[j] = (4 * g + j) * p.D + min(DB * r, p.D - DB);
     const int64_t head = (int64_t)hk * p.page_d;
@@ -355,17 +390,22 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
         id = there ? id : 0;
         return (int64_t)id * p.table.page_elems + head + (int64_t)(key & (page_rows - 1)) * p.D;
     };
-    u32x4 kr[2][KS];
+    // K's rows of a tile go into one of the wave's two buffers by copies of the memory
+    // system; V's into registers.  Each is issued a tile ahead, in this order, which the
+    // empty asm statements keep: behind a tile's copies there are its eight loads of V.
     uint32_t vr[8][WORDS];
     int64_t at[2];
     bool there[2], next_there[2];
     auto load_k = [&](int tile) {
+        unsigned char* to = sm.k[wave][(tile - w0) & 1];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             at[t] = at16(tile * TILE + 16 * t, next_there[t]);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) kr[t][s] = *reinterpret_cast<const u32x4*>(p.k + at[t] + koff[s]);
+            for (int e = t * L::COPIES / 2; e < (t + 1) * L::COPIES / 2; ++e)
+                copy_rows(p.k + at[t], 32 * p.D, koff[e], 0, to + 1024 * e);
         }
+        asm volatile("" ::: "memory");
     };
     auto load_v = [&]() {
 #pragma unroll
@@ -383,6 +423,7 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
                     vr[4 * t + j][1] = w[1];
                 }
             }
+        asm volatile("" ::: "memory");
     };
     f32x4 o[NQ][DB];
     // the largest score before its scale (a difference of scores is exact where it counts,
@@ -401,25 +442,30 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
     }
     // (behind the first loads, which it does not wait for)
     if (qs.tree && b1 * TILE > first) tree_bits(sm.tree, parent, qs.nq, t0, t1 - t0 + 1);
-    for (int tile = w0; tile < w1; ++tile) {
+    // (the last tile apart: with a branch around the loads of a tile to come, a wait for this
+    // one's would be one for all)
+    auto step = [&](int tile, auto more) {
         const int key0 = tile * TILE;
         there[0] = next_there[0], there[1] = next_there[1];
-        if (p.D != 32 * KS) {                 // (q is zero there, but not what was loaded)
-#pragma unroll
-            for (int s = 0; s < KS; ++s)
-                if (32 * s + 8 * g >= p.D) kr[0][s] = kr[1][s] = u32x4{};
-        }
+        // K's copies have arrived, V's loads need not have
+        asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        const unsigned char* kb = sm.k[wave][(tile - w0) & 1];
         f32x4 s[NQ][2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t) {
+            x8 kr[KS];
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+                kr[i] = *reinterpret_cast<const x8*>(kb + kofs[i] + 16 * t * L::PITCH);
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
                 s[n][t] = f32x4{};
 #pragma unroll
-                for (int i = 0; i < KS; ++i) s[n][t] = T::mfma16(as_x8<x8>(kr[t][i]), qf[n][i], s[n][t]);
+                for (int i = 0; i < KS; ++i) s[n][t] = T::mfma16(kr[i], qf[n][i], s[n][t]);
             }
-        // the next tile's keys go where this one's were
-        if (tile + 1 < w1) load_k(tile + 1);
+        }
+        // (into the other buffer, which the tile before this one was read from)
+        if constexpr (more) load_k(tile + 1);
         if (key0 + TILE > first || !there[0] || !there[1]) {
             const uint32_t paged = (there[0] ? 0xffffu : 0u) | (there[1] ? 0xffff0000u : 0u);
 #pragma unroll
@@ -516,8 +562,10 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
                 }
             }
         }
-        if (tile + 1 < w1) load_v();
-    }
+        if constexpr (more) load_v();
+    };
+    for (int tile = w0; tile < w1 - 1; ++tile) step(tile, std::true_type{});
+    if (w0 < w1) step(w1 - 1, std::false_type{});
     // merge of the waves: o[n][i][e] is column DB (4 g + e) + i of row 16 n + r
     __syncthreads();  // (the tree's bits are done with)
 #pragma unroll
@@ -567,7 +615,7 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
 // LDS: row k of a tile at PITCH k; K's 16-byte chunk c at c ^ (k mod chunks), V's 64-byte
 // chunk c at c ^ (k mod 4) (narrow rows: c ^ (k / 2 mod 2)), so that neither kind of
 // read meets a bank twice; the copies' lanes take their chunks from where that is.
-// Columns past D are zero from the start on.
+// Columns past D are zeros.
 constexpr int TILE_WAVES = 8, TILE_KEYS = 128;
 
 template <int P>
@@ -629,11 +677,6 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
         }
     }
     const uint32_t* bits = tree.bits[active && mine.there ? mine.t - g0 : 0];
-    if (p.D < P) {
-        for (int i = threadIdx.x; i < L::SMEM / 16; i += 64 * TILE_WAVES)
-            reinterpret_cast<u32x4*>(smem)[i] = u32x4{};
-        __syncthreads();
-    }
     // The pages of 64 tiles, a lane each: that of this wave's rows, and a bit for each
     // 16 keys whether theirs is one.
     const int32_t* table = p.table.at + b * p.table.sb;
@@ -655,17 +698,14 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
     // this lane's part of the wave's copies: row lr of each, 16-byte slot `slot`
     const int lr = lane / L::CH, slot = lane % L::CH;
     uint32_t koff[L::COPIES], voff;
-    bool kin[L::COPIES], vin;
 #pragma unroll
     for (int e = 0; e < L::COPIES; ++e) {
         const int r = L::ROWS * e + lr, c = slot ^ (r & (L::CH - 1));
-        kin[e] = 8 * c < p.D;
-        koff[e] = r * p.D + 8 * c;
+        koff[e] = 8 * c < p.D ? 2 * (r * p.D + 8 * c) : NO_ROW;
     }
     {
         const int c = slot ^ L::vswz(lr);
-        vin = 8 * c < p.D;
-        voff = lr * p.D + 8 * c;
+        voff = 8 * c < p.D ? 2 * (lr * p.D + 8 * c) : NO_ROW;
     }
     const int64_t head = (int64_t)hk * p.page_d;
     const int page_rows = 1 << shift;
@@ -673,18 +713,13 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
         const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)ids, tile - ids_of);
         const int key = tile * TILE_KEYS + 16 * wave, buf = (tile - b0) & 1;
         const int64_t at = (int64_t)id * p.table.page_elems + head + (int64_t)(key & (page_rows - 1)) * p.D;
-        uint32_t vo = voff, ko[L::COPIES];
-#pragma unroll
-        for (int e = 0; e < L::COPIES; ++e) { ko[e] = koff[e]; asm volatile("" : "+v"(ko[e])); }
-        asm volatile("" : "+v"(vo));
         unsigned char* kd = smem + buf * L::BUF + 16 * wave * L::PITCH;
         unsigned char* vd = kd + 2 * L::BUF;
 #pragma unroll
-        for (int e = 0; e < L::COPIES; ++e)
-            if (kin[e]) dma16(p.k + at + ko[e], kd + 1024 * e);
+        for (int e = 0; e < L::COPIES; ++e) copy_rows(p.k + at, 32 * p.D, koff[e], 0, kd + 1024 * e);
 #pragma unroll
         for (int e = 0; e < L::COPIES; ++e)
-            if (vin) dma16(p.v + at + L::ROWS * e * p.D + vo, vd + 1024 * e);
+            copy_rows(p.v + at, 32 * p.D, voff, 2 * L::ROWS * e * p.D, vd + 1024 * e);
     };
     // operand offsets in buffer 0: K row l32 (+ 32 j), chunk 2 kk + hf; V rows 4 hf +
     // lane % 16 / 4 (+ 32 j + 16 k, and 8 on), 32 columns i: column 16 (l32 / 16) on.  A
@@ -1035,27 +1070,30 @@ Plan attend_plan(const nkv_paged_attend_args* a) {
         return pl;
     }
     // Two groups of 16 rows to a wave where there are more (us with one and two: 8 heads of
-    // 4,096 keys, 32 rows 11.3, 12.6, 64 rows 15.3, 14.8; 64 heads, 48 rows 43, 33).
+    // 4,096 keys, 32 rows 11.3, 12.6, 64 rows 15.3, 14.8; 64 heads, 64 rows 34.2, 33.1).
     pl.two = pl.rows > 32;
     pl.groups = (int)cdiv(pl.rows, pl.two ? 32 : 16);
     const int64_t base = heads * pl.groups, work = base * tiles;
     const bool uneven = a->length && a->B > 1;
-    // Up to 16 tiles no splits: the second launch and its workspace cost more than they save
-    // (8 heads of 512 keys 9.2 us without, 8.3 with them, but a call takes the host 10.5
-    // and 14; of 1,024 keys 13.5 and 9.2).
-    if (tiles <= 16) {
+    // Up to 32 tiles no splits: the second launch and its workspace cost more than they save
+    // (8 heads of 1,024 keys 10.3 us without, 8.7 with them, but a call takes the host 10.5
+    // and 14; of 2,048 keys 16.2 and 7.9).
+    if (tiles <= 32) {
         pl.eight = tiles > 8;
         pl.items = base;
         return pl;
     }
     // Else one workgroup a CU, as a start and a merge cost more than latency (8 heads of
-    // 4,096 keys, 4 rows: 128, 256, 512 workgroups 10.2, 9.3, 10.3 us; 2 heads of 262,144:
-    // 69, 46, 51), of four waves, or eight where sequences have lengths of their own (128
-    // heads of 2,048 keys 26.5, 24.4; of up to 4,096 34.1, 34.9); two a CU in long calls of
-    // those, so that CUs with short ones take more (32 of up to 16,384 keys, 8 heads: 273,
-    // 249), and for two groups with much to do (16 heads of 4,096 keys, 256 rows: 40, 32).
+    // 4,096 keys, 4 rows: 128, 256, 512 workgroups 10.2, 8.7, 10.3 us), of four waves, or
+    // eight where sequences have lengths of their own: half as many of those in short calls
+    // (128 heads of 2,048 keys: 128, 256 workgroups 20.2, 21.4; 64 of 8,192: 37.4, 35.4), and
+    // two a CU in long ones, so that CUs with short sequences take more (32 of up to 16,384
+    // keys, 8 heads: 272, 251).  Two as well for two groups with much to do (16 heads of
+    // 4,096 keys, 256 rows: 40, 32).
     pl.eight = uneven && work >= 4096;
-    const int64_t slots = (uneven && work >= 32768) || (pl.two && work > 8192) ? 512 : 256;
+    int64_t slots = 256;
+    if (uneven) slots = work >= 32768 ? 512 : work >= 16384 ? 256 : 128;
+    else if (pl.two && work > 8192) slots = 512;
     if (base < slots)
         pl.splits = (int)std::max<int64_t>(1, std::min(cdiv(slots, std::max<int64_t>(base, 1)), tiles / (pl.eight ? 8 : 4)));
     pl.items = base * pl.splits;
