@@ -1031,12 +1031,16 @@ struct Plan {
     size_t part, ml;              // bytes
 };
 
-// The tile kernel takes calls of more than TILE_ROWS rows of a key head and more than
-// TILE_WORK (row, key) pairs in all heads: a workgroup's start costs it about 10 us (us
+// The tile kernel takes calls of more than TILE_ROWS rows of a key head that have more than
+// TILE_WORK (row, key) pairs in all heads, as a workgroup's start costs it about 10 us (us
 // with either, rows first; 8 heads of 4,096 keys: 128 rows 19.7, 23.4, 256 rows 25.4,
 // 32.2; 16 heads: 128 rows 24.8, 28.0; 32 heads: 128 rows 32.9, 32.0, 256 rows 51, 40; 64
-// heads: 64 rows 34, 41, 96 rows 51, 43; 64 heads of 8,192 keys, 128 rows: 99, 79).
-constexpr int64_t TILE_ROWS = 64, TILE_WORK = 1 << 24;
+// heads: 64 rows 34, 41, 96 rows 51, 43; 64 heads of 8,192 keys, 128 rows: 99, 79), or
+// more than TILE_BLOCKS times 32 rows, which the other kernel would give a workgroup each,
+// with three of its four waves idle over few keys (256 heads of 64 keys, 64 rows 8.8, 8.2,
+// 128 rows 15.4, 9.4; 184 heads of 16 keys, 2,360 rows 144, 58; 64 heads, 256 rows 8.9,
+// 9.5; 128 heads of 512 keys, 128 rows 18.6, 21.4, 256 rows 34, 26).
+constexpr int64_t TILE_ROWS = 64, TILE_WORK = 1 << 24, TILE_BLOCKS = 512;
 
 Plan attend_plan(const nkv_paged_attend_args* a) {
     const nkv_paged_cache& c = a->cache;
@@ -1044,7 +1048,8 @@ Plan attend_plan(const nkv_paged_attend_args* a) {
     pl.rows = a->Q * a->G;
     const int64_t heads = (int64_t)a->B * c.H, tiles = cdiv(a->n, TILE);
     pl.splits = 1;
-    pl.tile = pl.rows > TILE_ROWS && heads * pl.rows > TILE_WORK / std::max<int64_t>(a->n, 1);
+    pl.tile = pl.rows > TILE_ROWS && (heads * cdiv(pl.rows, 32) > TILE_BLOCKS ||
+                                      heads * pl.rows > TILE_WORK / std::max<int64_t>(a->n, 1));
     if (pl.tile) {
         // the fewest groups of up to eight 32-row blocks, of even size
         const int64_t qb = cdiv(pl.rows, 32), blocks = cdiv(a->n, 64);

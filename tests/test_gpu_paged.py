@@ -369,6 +369,21 @@ def test_attend_many_rows(dev, name, what, B, Hq, H, D, page, Q, lengths, counts
     check_large(q, cache, table, lengths, out, lse, what == "causal", parents, counts)
 
 
+# more than 512 times 32 rows, more than 64 of a key head, over few keys
+FEW_KEYS = [
+    (40, 64, 8, 128, 16, 11, [5, 0, 1, 16] * 10, None), (3, 24, 24, 96, 64, 300, [16, 0, 37], [300, 0, 5]),
+    (13, 16, 16, 72, 16, 96, [96, 130, 1, 0, 500, 97, 95, 17, 16, 15, 33, 129, 128], None),
+    (1, 16, 8, 64, 32, 1100, [64], None), (33, 32, 16, 40, 1024, 40, [1] * 33, [40, 1, 0] * 11),
+]
+
+
+@pytest.mark.parametrize("name", ["bf16", "fp16"])
+@pytest.mark.parametrize("what", ["whole", "causal", "tree"])
+@pytest.mark.parametrize("B,Hq,H,D,page,Q,lengths,counts", FEW_KEYS)
+def test_attend_many_rows_over_few_keys(dev, name, what, B, Hq, H, D, page, Q, lengths, counts):
+    test_attend_many_rows(dev, name, what, B, Hq, H, D, page, Q, lengths, counts)
+
+
 @pytest.mark.parametrize("name", ["bf16", "fp16"])
 @pytest.mark.parametrize("what", ["causal", "tree"])
 def test_many_rows_that_are_not_seen_may_hold_anything(dev, what, name):
