@@ -310,16 +310,18 @@ extern "C" int nkv_paged_append(void* stream, const nkv_paged_append_args* a) {
     if (Hq) {
         span = rows_span(a->o_sb, a->B, a->o_st, a->T, a->o_sh, Hq, c.D);
         NKV_REQUIRE(span > 0, NKV_ERR_INVALID, "q_out's rows overlap");
+        NKV_REQUIRE(a->q_out != a->k && a->q_out != a->v, NKV_ERR_INVALID, "q_out overlaps the rows");
         if (a->q_out == a->q)
             NKV_REQUIRE(a->dtype == c.dtype && a->q_sb == a->o_sb && a->q_st == a->o_st && a->q_sh == a->o_sh,
                         NKV_ERR_INVALID, "q_out over q must have its type and strides");
     }
     const Range pools[2] = {{c.k, pool_bytes(c)}, {c.v, pool_bytes(c)}};
     const Range q_out(a->q_out, Hq && span == rows * c.D ? span * 2 : 0);
-    const Range small[4] = {{a->table, table_bytes(a->B, a->table_sb, a->table_w)},
+    const Range small[5] = {{a->table, table_bytes(a->B, a->table_sb, a->table_w)},
                             {a->start_dev, a->start_dev ? a->B * 4 : 0},
                             {a->counts, a->counts ? a->B * 4 : 0},
-                            {a->freqs, a->freqs ? a->rot * 2 : 0}};
+                            {a->freqs, a->freqs ? a->rot * 2 : 0},
+                            {a->positions, a->positions ? table_bytes(a->B, a->pos_sb, a->T) : 0}};
     const int64_t es = a->dtype == NKV_ROWS_FP32 ? 4 : 2;
     // (the extents of rows: of any strides that are not negative)
     auto extent = [&](const void* at, int64_t sb, int64_t st, int64_t sh, int heads) {
@@ -338,7 +340,7 @@ extern "C" int nkv_paged_append(void* stream, const nkv_paged_append_args* a) {
                     "the pools overlap the rows");
         for (const Range& x : small)
             NKV_REQUIRE(!r.meets(x) && !q_out.meets(x), NKV_ERR_INVALID,
-                        "the pools or q_out overlap the table, start_dev, counts or freqs");
+                        "the pools or q_out overlap the table, start_dev, counts, freqs or positions");
     }
     if (a->q_out != a->q)
         NKV_REQUIRE(!q_out.meets(q) && !q_out.meets(k) && !q_out.meets(v), NKV_ERR_INVALID,

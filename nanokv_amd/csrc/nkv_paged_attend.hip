@@ -1121,8 +1121,9 @@ void attend_fit(const nkv_paged_attend_args* a, Plan& pl, size_t limit) {
     pl.ml = rows * pl.splits * sizeof(f32x2);
 }
 
-// Also plans the call where there is something to do (pl.items > 0).
-int check_attend(const nkv_paged_attend_args* a, Plan& pl) {
+// Also plans the call, for a workspace of that many bytes, where there is something to do
+// (pl.items > 0).
+int check_attend(const nkv_paged_attend_args* a, Plan& pl, const void* workspace, size_t bytes) {
     NKV_REQUIRE(a, NKV_ERR_INVALID, "args is null");
     const nkv_paged_cache& c = a->cache;
     int rc = paged_check(c, __func__);
@@ -1146,12 +1147,19 @@ int check_attend(const nkv_paged_attend_args* a, Plan& pl) {
     NKV_REQUIRE((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) % 16 == 0 &&
                     (a->q_sb | a->q_st | a->q_sh | a->o_sb | a->o_st | a->o_sh) % 8 == 0,
                 NKV_ERR_INVALID, "q and out must be 16-byte aligned with strides divisible by 8");
+    NKV_REQUIRE(a->q_sb >= 0 && a->q_st >= 0 && a->q_sh >= 0, NKV_ERR_INVALID,
+                "q's strides must not be negative");
+    NKV_REQUIRE((int64_t)a->B * c.H * cdiv(a->Q * a->G, 32 * TILE_WAVES) <= 1 << 22, NKV_ERR_UNSUPPORTED,
+                "too many query rows");
     pl = attend_plan(a);
     NKV_REQUIRE(pl.items <= 1 << 22, NKV_ERR_UNSUPPORTED, "too many query rows");
+    attend_fit(a, pl, bytes);
     const int64_t span = rows_span(a->o_sb, a->B, a->o_st, a->Q, a->o_sh, (int64_t)c.H * a->G, c.D);
     NKV_REQUIRE(span > 0, NKV_ERR_INVALID, "out's rows overlap");
-    // what is written and what is read; an out with gaps may have anything in them
+    // what is written and what is read; an out or q with gaps may have anything in them
     const int64_t rows = (int64_t)a->B * c.H * a->G * a->Q;
+    const bool packed = rows_span(a->q_sb, a->B, a->q_st, a->Q, a->q_sh, (int64_t)c.H * a->G, c.D) == rows * c.D;
+    const Range q(a->q, packed ? rows * c.D * 2 : 0);
     const Range in[6] = {{c.k, pool_bytes(c)}, {c.v, pool_bytes(c)},
                          {a->table, table_bytes(a->B, a->table_sb, a->table_w)},
                          {a->length, a->length ? a->B * 4 : 0}, {a->counts, a->counts ? a->B * 4 : 0},
@@ -1160,10 +1168,20 @@ int check_attend(const nkv_paged_attend_args* a, Plan& pl) {
     for (const Range& r : in)
         NKV_REQUIRE(!r.meets(lse) && !r.meets(out), NKV_ERR_INVALID,
                     "out or lse overlaps the cache, table, length, counts or parents");
-    NKV_REQUIRE(!lse.meets(out), NKV_ERR_INVALID, "lse overlaps out");
+    NKV_REQUIRE(!lse.meets(out) && !lse.meets(q), NKV_ERR_INVALID, "lse overlaps q or out");
+    NKV_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0 || pl.part == 0, NKV_ERR_INVALID,
+                "workspace must be 16-byte aligned");
+    const Range work(workspace, workspace ? pl.part + pl.ml : 0);
+    NKV_REQUIRE(!work.meets(q) && !work.meets(out) && !work.meets(lse), NKV_ERR_INVALID,
+                "workspace overlaps q, out or lse");
+    for (const Range& r : in)
+        NKV_REQUIRE(!work.meets(r), NKV_ERR_INVALID,
+                    "workspace overlaps the cache, table, length, counts or parents");
     if (a->out == a->q)
         NKV_REQUIRE(a->q_sb == a->o_sb && a->q_st == a->o_st && a->q_sh == a->o_sh, NKV_ERR_INVALID,
                     "out over q must have its strides");
+    else
+        NKV_REQUIRE(!out.meets(q), NKV_ERR_INVALID, "out overlaps q");
     return NKV_OK;
 }
 
@@ -1223,8 +1241,7 @@ using namespace nkv;
 extern "C" size_t nkv_paged_attend_workspace_size(const nkv_paged_attend_args* a) {
     clear_error();
     Plan pl{};
-    if (check_attend(a, pl) || pl.items == 0) return 0;
-    attend_fit(a, pl, SIZE_MAX);
+    if (check_attend(a, pl, nullptr, SIZE_MAX) || pl.items == 0) return 0;
     return pl.part + pl.ml;
 }
 
@@ -1232,12 +1249,9 @@ extern "C" int nkv_paged_attend(void* stream, const nkv_paged_attend_args* a, vo
                                 size_t workspace_bytes) {
     clear_error();
     Plan pl{};
-    int rc = check_attend(a, pl);
+    int rc = check_attend(a, pl, workspace, workspace ? workspace_bytes : 0);
     if (rc || pl.items == 0) return rc;
     const nkv_paged_cache& c = a->cache;
-    attend_fit(a, pl, workspace ? workspace_bytes : 0);
-    NKV_REQUIRE(pl.part == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, NKV_ERR_INVALID,
-                "workspace must be 16-byte aligned");
     AttendParams p{};
     p.table = page_table(c, a->table, a->table_sb, a->table_w);
     p.k = (const uint16_t*)c.k;

@@ -138,6 +138,14 @@ def test_append_refusals_of_queries(kw, code, text):
     refused("nkv_paged_append", rotated(**kw), code, text)
 
 
+def test_append_refuses_queries_over_rows_and_positions():
+    rows, at = PTR + (4 << 24), PTR + (6 << 24)
+    refused("nkv_paged_append", rotated(q=rows, q_out=rows), INV, b"overlaps the rows")
+    refused("nkv_paged_append", rotated(v=at, q_out=at), INV, b"overlaps the rows")
+    refused("nkv_paged_append", rotated(positions=PTR + (7 << 24) + 4, pos_sb=4), INV, b"positions")
+    refused("nkv_paged_append", rotated(positions=PTR + 4, pos_sb=4), INV, b"positions")
+
+
 def test_append_refuses_pools_that_overlap():
     c = cache()
     c.v = c.k + 1024
@@ -165,6 +173,27 @@ def test_attend_refusals(kw, code, text):
     lib = _lib.lib()
     assert lib.nkv_paged_attend_workspace_size(ctypes.byref(attend_args(**kw))) == 0
     assert text in lib.nkv_last_error()
+
+
+def packed(**kw):
+    a = attend_args(**kw)
+    a.q_sb, a.q_st, a.q_sh = a.o_sb, a.o_st, a.o_sh
+    return a
+
+
+def test_attend_refuses_what_overlaps_queries_or_workspace():
+    q, out = PTR + (4 << 24), PTR + (5 << 24)
+    refused("nkv_paged_attend", packed(out=q + 128), INV, b"out overlaps q", None, 0)
+    refused("nkv_paged_attend", packed(lse=q + 16), INV, b"lse overlaps q", None, 0)
+    a = packed(n=65536, table_w=4096, table_sb=4096, B=1, lse=PTR + (6 << 24), length=PTR + (7 << 24))
+    need = _lib.lib().nkv_paged_attend_workspace_size(ctypes.byref(a))
+    for at in (q, out - 16, PTR + (6 << 24) - 16):
+        refused("nkv_paged_attend", a, INV, b"workspace overlaps q, out or lse", at, need)
+    for at in (PTR, PTR + (1 << 24), PTR + (3 << 24), PTR + (7 << 24) - 16):
+        refused("nkv_paged_attend", a, INV, b"workspace overlaps the cache", at, need)
+    a.q_st = -64
+    refused("nkv_paged_attend", a, INV, b"negative", None, 0)
+    refused("nkv_paged_attend", attend_args(B=65535, Q=1 << 28, n=64), UNS, b"too many", None, 0)
 
 
 def test_workspace_sizes_and_alignment():
