@@ -970,10 +970,10 @@ typedef struct nkv_paged_cache {
  * the rest are not written, neither in the cache nor in q_out.  Rows past the table
  * are dropped where start or counts are in device memory, and refused where neither
  * is.
- * Rows are 16-byte aligned with strides divisible by 8.  q_out may be q itself and
- * overlaps nothing else of the call, nor do its rows each other; the pools overlap
- * neither each other nor anything else of the call, and no row is written twice:
- * no two sequences write into the same page.
+ * Rows are 16-byte aligned, strides divisible by 8 and not negative.  q_out may be q
+ * itself and overlaps nothing else of the call, nor do its rows each other; the pools
+ * overlap neither each other nor anything else of the call, and no row is written
+ * twice: no two sequences write into the same page.
  */
 typedef struct nkv_paged_append_args {
     nkv_paged_cache cache;
@@ -1027,8 +1027,8 @@ int nkv_paged_append(void* stream, const nkv_paged_append_args* args);
  * Scores, softmax and sums are fp32; for their product with the values the weights,
  * relative to the row's largest one, are rounded to the cache's type (bf16 caches
  * in calls of few rows: to twice its bits).
- * q and out are 16-byte aligned with strides divisible by 8; out's rows do not
- * overlap.  out may be q itself; otherwise out, lse and the workspace overlap
+ * q and out are 16-byte aligned, their strides divisible by 8 and not negative; out's
+ * rows do not overlap.  out may be q itself; otherwise out, lse and the workspace overlap
  * nothing of the call.
  */
 #define NKV_PAGED_TREE 256
@@ -1070,9 +1070,9 @@ int nkv_paged_attend(void* stream, const nkv_paged_attend_args* args, void* work
  *   rows        int32, device, M entries an item, M <= NKV_PAGED_COMMIT
  *   start_dev, counts: as nkv_paged_append's (NULL: start; M)
  *   out_length  [B] int32, start + counts (both as clamped), or NULL
- * pools is an array in host memory, of at most NKV_PAGED_CACHES caches.  The pools overlap neither each other nor
- * anything else of the call; no two sequences write into the same page, and none
- * into one that another reads here.
+ * pools is an array in host memory, of at most NKV_PAGED_CACHES caches.  The pools
+ * overlap neither each other nor anything else of the call; no two sequences write
+ * into the same page, and none into one that another reads here.
  */
 #define NKV_PAGED_COMMIT 256
 #define NKV_PAGED_CACHES 64

@@ -1042,11 +1042,17 @@ struct Plan {
 // 9.5; 128 heads of 512 keys, 128 rows 18.6, 21.4, 256 rows 34, 26).
 constexpr int64_t TILE_ROWS = 64, TILE_WORK = 1 << 24, TILE_BLOCKS = 512;
 
+// Workgroups that item_of gives an XCD at most.
+int64_t per_xcd(int64_t units, int64_t groups) {
+    return units >= UNITS ? cdiv(units, 8) * groups : cdiv(units * groups, 8);
+}
+
 Plan attend_plan(const nkv_paged_attend_args* a) {
     const nkv_paged_cache& c = a->cache;
     Plan pl{};
     pl.rows = a->Q * a->G;
     const int64_t heads = (int64_t)a->B * c.H, tiles = cdiv(a->n, TILE);
+    const bool uneven = a->length && a->B > 1;
     pl.splits = 1;
     pl.tile = pl.rows > TILE_ROWS && (heads * cdiv(pl.rows, 32) > TILE_BLOCKS ||
                                       heads * pl.rows > TILE_WORK / std::max<int64_t>(a->n, 1));
@@ -1056,16 +1062,20 @@ Plan attend_plan(const nkv_paged_attend_args* a) {
         pl.groups = (int)cdiv(qb, TILE_WAVES);
         pl.per_group = (int)cdiv(qb, pl.groups);
         const int64_t base = heads * pl.groups;
-        // splits whose rounds of 256 workgroups take least, in units of the time of 64 keys
-        // (2.0 to 2.6 us): a workgroup's start and end cost five, a merge two and its
-        // partials' traffic (us with splits that fill half a round, one and two: 64 heads
-        // of 8,192 keys, 256 rows 155, 101, 118; 8 heads of 16,384, 512 rows 76, 63, 76;
-        // 32 heads of 4,096, 256 rows 48, 40, 75)
+        // splits whose rounds of workgroups take least, in units of the time of 64 keys (2.0
+        // to 2.6 us): a workgroup's start and end cost five, a merge two and its partials'
+        // traffic (us with splits that fill half a round, one and two: 64 heads of 8,192
+        // keys, 256 rows 155, 101, 118; 8 heads of 16,384, 512 rows 76, 63, 76; 32 heads of
+        // 4,096, 256 rows 48, 40, 75).  A round is an XCD's 32 CUs over what item_of gives
+        // it (4 heads of 123,539 keys, 529 rows: 20 splits, 30 workgroups an XCD, 193 us; 21,
+        // of which four XCDs have 33, 340), or, of sequences that end where they please, all
+        // 256 CUs over all (5 of up to 18,847 keys, 3,142 rows: 6 splits 212, 7 165).
         double best = 0.0;
         const int64_t most = std::max<int64_t>(16, cdiv(256, std::max<int64_t>(base, 1)));
         for (int64_t s = 1; s <= most && (s == 1 || blocks >= 4 * s); ++s) {
             const double merge = s == 1 ? 0.0 : 2.0 + (double)heads * pl.rows * s * 2.5e-5;
-            const double t = (double)cdiv(base * s, 256) * ((double)blocks / s + 5.0) + merge;
+            const int64_t rounds = uneven ? cdiv(base * s, 256) : cdiv(per_xcd(heads * s, pl.groups), 32);
+            const double t = (double)rounds * ((double)blocks / s + 5.0) + merge;
             if (s == 1 || t < best) {
                 best = t;
                 pl.splits = (int)s;
@@ -1079,12 +1089,11 @@ Plan attend_plan(const nkv_paged_attend_args* a) {
     pl.two = pl.rows > 32;
     pl.groups = (int)cdiv(pl.rows, pl.two ? 32 : 16);
     const int64_t base = heads * pl.groups, work = base * tiles;
-    const bool uneven = a->length && a->B > 1;
     // Up to 32 tiles no splits: the second launch and its workspace cost more than they save
     // (8 heads of 1,024 keys 10.3 us without, 8.7 with them, but a call takes the host 10.5
     // and 14; of 2,048 keys 16.2 and 7.9).
     if (tiles <= 32) {
-        pl.eight = tiles > 8;
+        pl.eight = tiles > 8 && (!pl.two || base <= 256);
         pl.items = base;
         return pl;
     }
@@ -1093,14 +1102,21 @@ Plan attend_plan(const nkv_paged_attend_args* a) {
     // eight where sequences have lengths of their own: half as many of those in short calls
     // (128 heads of 2,048 keys: 128, 256 workgroups 20.2, 21.4; 64 of 8,192: 37.4, 35.4), and
     // two a CU in long ones, so that CUs with short sequences take more (32 of up to 16,384
-    // keys, 8 heads: 272, 251).  Two as well for two groups with much to do (16 heads of
-    // 4,096 keys, 256 rows: 40, 32).
-    pl.eight = uneven && work >= 4096;
-    int64_t slots = 256;
-    if (uneven) slots = work >= 32768 ? 512 : work >= 16384 ? 256 : 128;
-    else if (pl.two && work > 8192) slots = 512;
-    if (base < slots)
-        pl.splits = (int)std::max<int64_t>(1, std::min(cdiv(slots, std::max<int64_t>(base, 1)), tiles / (pl.eight ? 8 : 4)));
+    // keys, 8 heads: 272, 251).  Two groups of rows get eight waves and one workgroup a CU
+    // at most (four waves with one a CU, with two, eight with one: 8 heads of 4,096 keys, 256
+    // rows 23.0, 23.4, 20.4; 64 of 2,048, 64 rows 23.4, 22.7, 21.7; one CU with two: 12 of
+    // 3,426, 220 rows, 2 splits 22.8, 3 of 35 workgroups an XCD 32.6), or four where there
+    // are more (12 heads of 1,185 keys, 760 rows: eight 36, four 29).
+    const int64_t least = std::max<int64_t>(base, 1);
+    int64_t splits = 256 / least;
+    if (pl.two) {
+        pl.eight = base <= 256;
+        while (splits > 1 && per_xcd(heads * splits, pl.groups) > 32) --splits;
+    } else {
+        pl.eight = uneven && work >= 4096;
+        splits = cdiv(!uneven ? 256 : work >= 32768 ? 512 : work >= 16384 ? 256 : 128, least);
+    }
+    pl.splits = (int)std::max<int64_t>(1, std::min(splits, tiles / (pl.eight ? 8 : 4)));
     pl.items = base * pl.splits;
     return pl;
 }
@@ -1187,8 +1203,7 @@ int check_attend(const nkv_paged_attend_args* a, Plan& pl, const void* workspace
 
 // Blocks of a launch over p.items workgroups in item_of's order.
 unsigned item_blocks(const AttendParams& p) {
-    const int64_t units = p.items / p.groups;
-    return (unsigned)(units >= UNITS ? 8 * cdiv(units, 8) * p.groups : 8 * cdiv(p.items, 8));
+    return (unsigned)(8 * per_xcd(p.items / p.groups, p.groups));
 }
 
 template <typename T, int KS, int W, int NQ>
