@@ -230,10 +230,10 @@ __device__ __forceinline__ void store_partial(const AttendParams& p, int bh, int
 // The work of a workgroup: a group of query rows of a unit (head and key split).
 // Block i runs on XCD i % 8, and the groups of a unit take consecutive slots of one
 // XCD, whose L2 then serves all but the first read of its rows.  Units go to the XCDs
-// in turn, so that sequences of unlike lengths spread over them; with fewer than
-// UNITS units an XCD takes a run of (unit, group) pairs instead.
-constexpr int UNITS = 32;
-
+// in turn, so that sequences of unlike lengths spread over them; of the last ones, fewer
+// than eight, an XCD takes a run of (unit, group) pairs, so that none has more than its
+// eighth (4 heads of 123,539 keys, 529 rows, 252 workgroups: with 33 on some XCDs' 32 CUs
+// 340 us, with 32 186; 28 heads of 10,634, 1,292 rows, 504 workgroups 334, 237).
 struct Item {
     uint32_t unit;
     int group;
@@ -249,13 +249,11 @@ __device__ __forceinline__ void share_of(const AttendParams& p, int split, int n
 
 __device__ __forceinline__ Item item_of(const AttendParams& p) {
     const uint32_t x = blockIdx.x & 7, k = blockIdx.x >> 3, groups = (uint32_t)p.groups;
-    const uint32_t items = (uint32_t)p.items, units = p.by_groups.of(items);
-    if (units >= UNITS) {
-        const uint32_t u = p.by_groups.of(k), unit = u * 8 + x;
-        return {unit, (int)(k - u * groups), unit < units};
-    }
-    const uint32_t item = x * ((items + 7) >> 3) + k, u = p.by_groups.of(item);
-    return {u, (int)(item - u * groups), item < items && k < (items + 7) >> 3};
+    const uint32_t units = p.by_groups.of((uint32_t)p.items), whole = units >> 3, u = p.by_groups.of(k);
+    if (u < whole) return {u * 8 + x, (int)(k - u * groups), true};
+    const uint32_t rest = (units & 7) * groups, each = (rest + 7) >> 3, j = k - whole * groups;
+    const uint32_t item = x * each + j, v = p.by_groups.of(item);
+    return {whole * 8 + v, (int)(item - v * groups), j < each && item < rest};
 }
 
 // ---------------------------------------------------------------- few rows
@@ -1042,11 +1040,6 @@ struct Plan {
 // 9.5; 128 heads of 512 keys, 128 rows 18.6, 21.4, 256 rows 34, 26).
 constexpr int64_t TILE_ROWS = 64, TILE_WORK = 1 << 24, TILE_BLOCKS = 512;
 
-// Workgroups that item_of gives an XCD at most.
-int64_t per_xcd(int64_t units, int64_t groups) {
-    return units >= UNITS ? cdiv(units, 8) * groups : cdiv(units * groups, 8);
-}
-
 Plan attend_plan(const nkv_paged_attend_args* a) {
     const nkv_paged_cache& c = a->cache;
     Plan pl{};
@@ -1062,20 +1055,16 @@ Plan attend_plan(const nkv_paged_attend_args* a) {
         pl.groups = (int)cdiv(qb, TILE_WAVES);
         pl.per_group = (int)cdiv(qb, pl.groups);
         const int64_t base = heads * pl.groups;
-        // splits whose rounds of workgroups take least, in units of the time of 64 keys (2.0
-        // to 2.6 us): a workgroup's start and end cost five, a merge two and its partials'
-        // traffic (us with splits that fill half a round, one and two: 64 heads of 8,192
-        // keys, 256 rows 155, 101, 118; 8 heads of 16,384, 512 rows 76, 63, 76; 32 heads of
-        // 4,096, 256 rows 48, 40, 75).  A round is an XCD's 32 CUs over what item_of gives
-        // it (4 heads of 123,539 keys, 529 rows: 20 splits, 30 workgroups an XCD, 193 us; 21,
-        // of which four XCDs have 33, 340), or, of sequences that end where they please, all
-        // 256 CUs over all (5 of up to 18,847 keys, 3,142 rows: 6 splits 212, 7 165).
+        // splits whose rounds of 256 workgroups take least, in units of the time of 64 keys
+        // (2.0 to 2.6 us): a workgroup's start and end cost five, a merge two and its
+        // partials' traffic (us with splits that fill half a round, one and two: 64 heads
+        // of 8,192 keys, 256 rows 155, 101, 118; 8 heads of 16,384, 512 rows 76, 63, 76;
+        // 32 heads of 4,096, 256 rows 48, 40, 75)
         double best = 0.0;
         const int64_t most = std::max<int64_t>(16, cdiv(256, std::max<int64_t>(base, 1)));
         for (int64_t s = 1; s <= most && (s == 1 || blocks >= 4 * s); ++s) {
             const double merge = s == 1 ? 0.0 : 2.0 + (double)heads * pl.rows * s * 2.5e-5;
-            const int64_t rounds = uneven ? cdiv(base * s, 256) : cdiv(per_xcd(heads * s, pl.groups), 32);
-            const double t = (double)rounds * ((double)blocks / s + 5.0) + merge;
+            const double t = (double)cdiv(base * s, 256) * ((double)blocks / s + 5.0) + merge;
             if (s == 1 || t < best) {
                 best = t;
                 pl.splits = (int)s;
@@ -1104,14 +1093,12 @@ Plan attend_plan(const nkv_paged_attend_args* a) {
     // two a CU in long ones, so that CUs with short sequences take more (32 of up to 16,384
     // keys, 8 heads: 272, 251).  Two groups of rows get eight waves and one workgroup a CU
     // at most (four waves with one a CU, with two, eight with one: 8 heads of 4,096 keys, 256
-    // rows 23.0, 23.4, 20.4; 64 of 2,048, 64 rows 23.4, 22.7, 21.7; one CU with two: 12 of
-    // 3,426, 220 rows, 2 splits 22.8, 3 of 35 workgroups an XCD 32.6), or four where there
-    // are more (12 heads of 1,185 keys, 760 rows: eight 36, four 29).
+    // rows 23.0, 23.4, 20.4; 64 of 2,048, 64 rows 23.4, 22.7, 21.7), or four where there
+    // are more (12 heads of 1,185 keys, 760 rows: eight 36, four 23).
     const int64_t least = std::max<int64_t>(base, 1);
     int64_t splits = 256 / least;
     if (pl.two) {
         pl.eight = base <= 256;
-        while (splits > 1 && per_xcd(heads * splits, pl.groups) > 32) --splits;
     } else {
         pl.eight = uneven && work >= 4096;
         splits = cdiv(!uneven ? 256 : work >= 32768 ? 512 : work >= 16384 ? 256 : 128, least);
@@ -1202,9 +1189,7 @@ int check_attend(const nkv_paged_attend_args* a, Plan& pl, const void* workspace
 }
 
 // Blocks of a launch over p.items workgroups in item_of's order.
-unsigned item_blocks(const AttendParams& p) {
-    return (unsigned)(8 * per_xcd(p.items / p.groups, p.groups));
-}
+unsigned item_blocks(const AttendParams& p) { return (unsigned)(8 * cdiv(p.items, 8)); }
 
 template <typename T, int KS, int W, int NQ>
 int rows_run(const AttendParams& p, hipStream_t s) {
