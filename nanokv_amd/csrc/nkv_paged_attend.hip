@@ -291,8 +291,8 @@ struct Pages {
 
 // One 16-byte-per-lane copy from 16 rows of a page (their bytes from `rows` on) into LDS,
 // the 64 lanes' pieces one after the other, from `further` bytes on for all of them; a
-// lane whose offset is NO_ROW brings zeros.  (By the buffer form: behind a global one every wait for a load
-// becomes one for all loads.)
+// lane whose offset is NO_ROW brings zeros.  (By the buffer form: behind a global one every
+// wait for a load becomes one for all loads.)
 constexpr uint32_t NO_ROW = 1u << 30;
 __device__ __forceinline__ void copy_rows(const uint16_t* rows, int bytes, uint32_t offset, int further,
                                           void* l) {
@@ -361,7 +361,8 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
         }
     }
     // this wave's tiles
-    const int w0 = b0 + (int)((uint32_t)(wave * (b1 - b0)) / W), w1 = b0 + (int)((uint32_t)((wave + 1) * (b1 - b0)) / W);
+    const int w0 = b0 + (int)((uint32_t)(wave * (b1 - b0)) / W);
+    const int w1 = b0 + (int)((uint32_t)((wave + 1) * (b1 - b0)) / W);
     const int shift = p.table.shift, page_rows = 1 << shift;
     Pages pages{p.table.at + b * p.table.sb, (int)p.table.w, 0, 0};
     // lane offsets into a page's rows of the head (elements): V's rows, and K's in the copies:
@@ -612,22 +613,27 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
 //
 // LDS: row k of a tile at PITCH k; K's 16-byte chunk c at c ^ (k mod chunks), V's 64-byte
 // chunk c at c ^ (k mod 4) (narrow rows: c ^ (k / 2 mod 2)), so that neither kind of
-// read meets a bank twice; the copies' lanes take their chunks from where that is.
-// Columns past D are zeros.
+// read meets a bank twice (counted: none does); the copies' lanes take their chunks from
+// where that is.  Columns past D are zeros.
+//
+// 1,560 queries of 24 heads over 12,480 keys, 239 GFLOP, three splits: 268 us, 890
+// TFLOP/s, and a merge of 11.  The matrix units are busy 36 % of the SIMDs' cycles; the
+// softmax between their products bounds it.  16 sequences of 8,192 keys, 8 heads, 256
+// rows, 137 GFLOP and 537 MB: 178 us.
 constexpr int TILE_WAVES = 8, TILE_KEYS = 128;
 
 template <int P>
 struct TileLds {
-    static constexpr int PITCH = P == 64 ? 128 : 256, CH = PITCH / 16, ROWS = 1024 / PITCH;  // rows of a copy
-    static constexpr int BUF = TILE_KEYS * PITCH, SMEM = 4 * BUF;                            // K0 K1 V0 V1
-    static constexpr int COPIES = 16 / ROWS;                                                 // of a wave's 16 rows
+    static constexpr int PITCH = P == 64 ? 128 : 256, CH = PITCH / 16;
+    static constexpr int BUF = TILE_KEYS * PITCH, SMEM = 4 * BUF;        // K0 K1 V0 V1
+    static constexpr int ROWS = 1024 / PITCH, COPIES = 16 / ROWS;        // rows of a copy, a wave's
     static __device__ __forceinline__ int vswz(int row) { return P == 64 ? (row >> 1 & 1) << 2 : (row & 3) << 2; }
 };
 
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 // (__restrict__: a read that might alias the copies in flight would wait for them all,
-// the next tile's among them; this one's are waited for at the barrier.  24 % of a call
-// that streams its pages from memory)
+// the next tile's among them; this one's are waited for at the barrier.  16 sequences of
+// 8,192 keys, 8 heads, 256 rows: 178 us, 188 without it)
 __device__ __forceinline__ u32x2 lds_columns(const unsigned char* __restrict__ p) {
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                          (__attribute__((address_space(3))) i16x4*)p));
@@ -955,7 +961,10 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
 // The merge of the splits' partial results: a thread eight columns, SG groups of
 // threads share a row's splits and are joined in LDS, and a thread has AHEAD splits'
 // loads in flight.  With M the largest m, out = sum(2^(m - M) o) / sum(2^(m - M) l).
-template <typename T, int SG, int AHEAD>
+// 37,440 rows of three splits, 68 MB: 11 us; few rows of many splits 4 to 6, the chain of a
+// launch, loads and the exchange.
+constexpr int AHEAD = 4;
+template <typename T, int SG>
 __global__ void __launch_bounds__(256) merge_kernel(AttendParams p) {
     constexpr int PARTS = 16, ROWS = 256 / (PARTS * SG);
     const int row = blockIdx.x * ROWS + threadIdx.x / (PARTS * SG);
@@ -1222,15 +1231,15 @@ int attend_width(const AttendParams& p, const Plan& pl, hipStream_t s) {
                      : p.D <= 96 ? attend_run<T, 3>(p, pl, s) : attend_run<T, 4>(p, pl, s);
 }
 
+// Sixteen groups of threads to a row where there are few rows and splits to share (whole
+// calls, us with sixteen and one: 32 rows of 32 splits 8.7, 16.7, of 12 21.3, 24.0; 128
+// rows of 8 18.0, 19.2, of 4 46.1, 46.3; 2,048 rows of 16 50.9, 49.7; 37,440 of 3 378, 278).
 template <typename T>
 void merge_run(const AttendParams& p, hipStream_t s) {
-    auto grid = [&](int sg) {
-        return dim3((unsigned)cdiv(p.rows, 16 / sg), (unsigned)p.H, (unsigned)p.B);
-    };
-    if (p.splits > 64) merge_kernel<T, 16, 16><<<grid(16), 256, 0, s>>>(p);
-    else if (p.splits > 8) merge_kernel<T, 16, 4><<<grid(16), 256, 0, s>>>(p);
-    else if (p.splits > 4) merge_kernel<T, 1, 8><<<grid(1), 256, 0, s>>>(p);
-    else merge_kernel<T, 1, 4><<<grid(1), 256, 0, s>>>(p);
+    const bool share = p.splits > 4 && (int64_t)p.B * p.H * p.rows <= 1024;
+    const dim3 grid((unsigned)cdiv(p.rows, share ? 1 : 16), (unsigned)p.H, (unsigned)p.B);
+    if (share) merge_kernel<T, 16><<<grid, 256, 0, s>>>(p);
+    else merge_kernel<T, 1><<<grid, 256, 0, s>>>(p);
 }
 
 }  // namespace
