@@ -1811,7 +1811,8 @@ def paged_attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, length
     t - 1, is the causal mask.
     Returns (out like q, lse [B, heads, Q] fp32 or None); a query that sees nothing gets
     0 and -inf.  workspace: optional uint8 buffer, nkv_paged_attend_workspace_size bytes
-    or fewer (with fewer, fewer key splits)."""
+    or fewer (with fewer, fewer key splits); calls that may run at once, or captured
+    graphs, need one each."""
     device = _require_gpu(q, cache.k, cache.v, table, parents, counts, out,
                           length if isinstance(length, torch.Tensor) else None)
     c = cache.struct()
