@@ -1026,7 +1026,8 @@ int nkv_paged_append(void* stream, const nkv_paged_append_args* args);
  *   lse  [B, H*G, Q] fp32 natural-log row log-sum-exp, or NULL
  * Scores, softmax and sums are fp32; for their product with the values the weights,
  * relative to the row's largest one, are rounded to the cache's type (bf16 caches
- * in calls of few rows: to twice its bits).
+ * in calls of few rows: to twice its bits).  A row that sees a value that is not finite
+ * has one there, NaN in place of an infinity where its weight rounds to zero.
  * q and out are 16-byte aligned, their strides divisible by 8 and not negative; out's
  * rows do not overlap.  out may be q itself; otherwise out, lse and the workspace overlap
  * nothing of the call.

@@ -80,6 +80,8 @@ Divisor divisor(int64_t d) {
     return {(uint32_t)d, s ? (uint32_t)((((unsigned __int128)1 << (31 + s)) / d) + 1) : 0, s ? (uint32_t)s - 1 : 0};
 }
 
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+
 struct AttendParams {
     PageTable table;
     const uint16_t* k;
@@ -91,13 +93,14 @@ struct AttendParams {
     const uint16_t* q;
     uint16_t* out;
     float* lse;
-    // partial results of the splits, [B*H][splits][rows]: the output's D sums (in units
+    // partial results of the splits, [H][B * splits][rows]: the output's D sums (in units
     // of 2^(m - LIFT)), and (m, l)
     float* part;
     f32x2* part_ml;
+    i32x2* shares;                // [B] a sequence's first slot and splits, or null: all alike
     int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;
     int64_t items;
-    Divisor by_G, by_H, by_BH, by_splits, by_groups;
+    Divisor by_G, by_H, by_B, by_groups;
     float scale_log2;
     int B, H, G, D, Q, n, causal, splits, groups, rows;
     int page_d;
@@ -129,10 +132,6 @@ struct Queries {
         return t0 >= nq ? 0 : tree ? len : sees(min(t1, nq - 1));
     }
 };
-__device__ __forceinline__ Queries queries_of(const AttendParams& p, int b) {
-    return {c8_length(p.length, b, p.n), c8_length(p.counts, b, p.Q), p.causal, p.parents != nullptr};
-}
-
 // ---------------------------------------------------------------- trees
 // For each of a workgroup's tokens one bit for every token of the draft that it sees:
 // its own and those on the way to the root.
@@ -217,17 +216,89 @@ __device__ __forceinline__ void store_row(const AttendParams& p, int b, int hk, 
 static_assert(Value<Fp16>::LIFT == 12.0f, "store_row's 4,096");
 
 // The same as one split's partial result.
-__device__ __forceinline__ void store_partial(const AttendParams& p, int bh, int split, int row, int d,
+__device__ __forceinline__ void store_partial(const AttendParams& p, int hk, int slot, int row, int d,
                                               const Stat& st, const float (&o)[8]) {
     if (row >= p.rows || d >= p.D) return;
-    const int64_t i = ((int64_t)bh * p.splits + split) * p.rows + row;
+    const int64_t i = ((int64_t)hk * p.B * p.splits + slot) * p.rows + row;
     f32x4* to = reinterpret_cast<f32x4*>(p.part + i * p.D + d);
     to[0] = f32x4{o[0], o[1], o[2], o[3]};
     to[1] = f32x4{o[4], o[5], o[6], o[7]};
     if (d == 0) p.part_ml[i] = f32x2{st.m, st.l};
 }
 
-// The work of a workgroup: a group of query rows of a unit (head and key split).
+// ---------------------------------------------------------------- shares
+// One of a sequence's key splits, which have the slots from `first` on of the B * splits
+// that there are; and the sequence's length and queries.
+struct Part {
+    int b, split, splits, first;
+    bool there;
+    int len, nq;
+};
+__device__ __forceinline__ Queries queries_of(const AttendParams& p, const Part& part) {
+    return {part.len, part.nq, p.causal, p.parents != nullptr};
+}
+
+// Sum over the wave.
+__device__ __forceinline__ int wave_sum(int v) {
+    uint32_t x = (uint32_t)v;
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = a[0] + a[1];
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = b[0] + b[1];
+    x += (uint32_t)__builtin_amdgcn_mov_dpp(x, 0x128, 0xf, 0xf, true);
+    x += (uint32_t)__builtin_amdgcn_mov_dpp(x, 0x141, 0xf, 0xf, true);
+    x += (uint32_t)__builtin_amdgcn_mov_dpp(x, 0x4e, 0xf, 0xf, true);
+    x += (uint32_t)__builtin_amdgcn_mov_dpp(x, 0xb1, 0xf, 0xf, true);
+    return __builtin_amdgcn_readfirstlane((int)x);
+}
+
+// Where lengths are in device memory, sequences (up to a wave's lanes) share the slots by
+// them: a split takes 128 tau keys for the least tau, two at least, with which all fit.  tau
+// = sum / (slots - B) and one more always does, as a sequence of t takes at most t / tau + 1.
+// Each wave finds this for itself, a sequence to a lane; the merge is told.  us with equal
+// splits and with these, 8 heads: 16 sequences, 256 rows, one of 32,768 keys and the others
+// of 512 478, 87, lengths evenly up to 32,768 541, 395, all alike 663, 666; 32 sequences, 4
+// rows, one of 16,384 keys, the others of 256 61, 36; 4 sequences of 4,096 17.3, 18.7.
+// With more workgroups than CUs the splits stay equal unless the longest sequence's are
+// half as long again: a CU that is done early takes the next (32 sequences, evenly from 6,144
+// to 16,384 keys, 4 rows: 251, by length 278).
+constexpr int BALANCED = 64, LEAST_SHARE = 2;
+__device__ __forceinline__ Part part_of(const AttendParams& p, int slot) {
+    const int split = (int)p.by_B.of((uint32_t)slot), own = slot - split * p.B;
+    const Part equal{own, split, p.splits, own * p.splits, true, c8_length(p.length, own, p.n),
+                     c8_length(p.counts, own, p.Q)};
+    if (!p.shares) return equal;
+    const int lane = threadIdx.x & 63, slots = p.B * p.splits;
+    const bool in = lane < p.B;
+    const int len = in ? c8_length(p.length, lane, p.n) : 0, nq = in ? c8_length(p.counts, lane, p.Q) : 0;
+    const int t = nq > 0 ? (len + 127) >> 7 : 0, all = wave_sum(t);
+    auto splits = [&](int tau) { return in ? max(1, (int)((uint32_t)(t + tau - 1) / (uint32_t)tau)) : 0; };
+    int lo = max(LEAST_SHARE, (all + slots - 1) / slots), hi = max(lo, all / (slots - p.B) + 1);
+    while (lo < hi) {
+        const int tau = (lo + hi) >> 1;
+        if (wave_sum(splits(tau)) <= slots) hi = tau;
+        else lo = tau + 1;
+    }
+    const int longest = __builtin_amdgcn_readfirstlane((int)wave_umax((uint32_t)t));
+    if (p.items > 256 && 2 * longest < 3 * hi * p.splits) return equal;
+    const int mine = splits(hi);
+    int end = mine;
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) {
+        const int x = __shfl_up(end, i);
+        end += lane >= i ? x : 0;
+    }
+    const int past = __popcll(__ballot(in && end <= slot)), b = min(past, p.B - 1);
+    const int n = __builtin_amdgcn_readlane(mine, b), first = __builtin_amdgcn_readlane(end, b) - n;
+    return {b, slot - first, n, first, past < p.B, __builtin_amdgcn_readlane(len, b),
+            __builtin_amdgcn_readlane(nq, b)};
+}
+__device__ __forceinline__ void tell_merge(const AttendParams& p, const Part& part, int hk, int group) {
+    if (p.shares && part.split == 0 && hk == 0 && group == 0 && threadIdx.x == 0)
+        p.shares[part.b] = i32x2{part.first, part.splits};
+}
+
+// The work of a workgroup: a group of query rows of a unit (slot and head).
 // Block i runs on XCD i % 8, and the groups of a unit take consecutive slots of one
 // XCD, whose L2 then serves all but the first read of its rows.  Units go to the XCDs
 // in turn, so that sequences of unlike lengths spread over them; of the last ones, fewer
@@ -241,10 +312,10 @@ struct Item {
 };
 
 // Part `split` of n tiles: an even share, the first ones a tile more.
-__device__ __forceinline__ void share_of(const AttendParams& p, int split, int n, int& from, int& to) {
-    const int each = (int)p.by_splits.of(n), more = n - each * p.splits;
-    from = split * each + min(split, more);
-    to = from + each + (split < more);
+__device__ __forceinline__ void share_of(const Part& part, int n, int& from, int& to) {
+    const int each = (int)((uint32_t)n / (uint32_t)part.splits), more = n - each * part.splits;
+    from = part.split * each + min(part.split, more);
+    to = from + each + (part.split < more);
 }
 
 __device__ __forceinline__ Item item_of(const AttendParams& p) {
@@ -332,9 +403,12 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Item it = item_of(p);
     if (!it.there) return;
-    const int rg = it.group, bh = (int)p.by_splits.of(it.unit);
-    const int split = (int)it.unit - bh * p.splits, b = (int)p.by_H.of(bh), hk = bh - b * p.H;
-    const Queries qs = queries_of(p, b);
+    const int rg = it.group, at_slot = (int)p.by_H.of(it.unit), hk = (int)it.unit - at_slot * p.H;
+    const Part part = part_of(p, at_slot);
+    if (!part.there) return;
+    tell_merge(p, part, hk, rg);
+    const int b = part.b;
+    const Queries qs = queries_of(p, part);
     const int32_t parent = tree_parent(p, b);
     const int row0 = rg * ROWS;
     // tiles that some row of the group sees, and keys that every row does
@@ -342,7 +416,7 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
     const int last = max(0, qs.most(t0, t1)), first = qs.least(t0, t1);
     const int nt = (last + TILE - 1) / TILE;
     int b0, b1;
-    share_of(p, split, nt, b0, b1);
+    share_of(part, nt, b0, b1);
     x8 qf[NQ][KS];
     int end[NQ];                              // keys that the lane's row sees
     const uint32_t* bits[NQ];                 // and the draft's tokens
@@ -597,7 +671,7 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
         }
         // (l is in the weights' units: 2^LIFT too large)
         if constexpr (V::LIFT != 0.0f) all.l *= 1.0f / 4096.0f;
-        if (p.splits > 1) store_partial(p, bh, split, row0 + mr, d, all, acc);
+        if (p.splits > 1) store_partial(p, hk, part.first + part.split, row0 + mr, d, all, acc);
         else store_row<T>(p, b, hk, row0 + mr, d, all, acc);
     }
 }
@@ -652,9 +726,12 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Item it = item_of(p);
     if (!it.there) return;
-    const int rg = it.group, split = (int)p.by_BH.of(it.unit);
-    const int bh = (int)it.unit - split * p.B * p.H, b = (int)p.by_H.of(bh), hk = bh - b * p.H;
-    const Queries qs = queries_of(p, b);
+    const int rg = it.group, at_slot = (int)p.by_H.of(it.unit), hk = (int)it.unit - at_slot * p.H;
+    const Part part = part_of(p, at_slot);
+    if (!part.there) return;
+    tell_merge(p, part, hk, rg);
+    const int b = part.b;
+    const Queries qs = queries_of(p, part);
     const int32_t parent = tree_parent(p, b);
     const int row0 = rg * p.per_group * 32;
     const int rows_end = min(row0 + p.per_group * 32, p.rows);
@@ -663,7 +740,7 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
     const int last = max(0, qs.most(g0, g1));
     const int nt = (last + TILE_KEYS - 1) / TILE_KEYS;
     int b0, b1;
-    share_of(p, split, nt, b0, b1);
+    share_of(part, nt, b0, b1);
     const int wrow = row0 + 32 * wave, row = wrow + l32;
     const bool active = wrow < rows_end;
     const RowAt mine = row_at(p, row, hk);
@@ -953,7 +1030,7 @@ __global__ void __launch_bounds__(64 * TILE_WAVES) attend_tile_kernel(AttendPara
             float x[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) x[k] = o[i][8 * e + k];
-            if (p.splits > 1) store_partial(p, bh, split, row, d, st, x);
+            if (p.splits > 1) store_partial(p, hk, part.first + part.split, row, d, st, x);
             else store_row<T>(p, b, hk, row, d, st, x);
         }
 }
@@ -972,16 +1049,18 @@ __global__ void __launch_bounds__(256) merge_kernel(AttendParams p) {
     const int sg = threadIdx.x / PARTS % SG, part = threadIdx.x % PARTS, d = part * 8;
     const int b = blockIdx.z, hk = blockIdx.y;
     const bool in = row < p.rows && d < p.D;
-    const int64_t first = ((int64_t)b * p.H + hk) * p.splits * p.rows + row;
+    const i32x2 share = p.shares ? p.shares[b] : i32x2{b * p.splits, p.splits};
+    const int splits = share[1];
+    const int64_t first = ((int64_t)hk * p.B * p.splits + share[0]) * p.rows + row;
     Stat all{NONE, 0.0f};
     float acc[8] = {};
     if (in) {
-        for (int s0 = sg; s0 < p.splits; s0 += SG * AHEAD) {
+        for (int s0 = sg; s0 < splits; s0 += SG * AHEAD) {
             f32x2 ml[AHEAD];
             f32x4 x[AHEAD][2];
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
-                const int64_t i = first + (int64_t)min(s0 + SG * j, p.splits - 1) * p.rows;
+                const int64_t i = first + (int64_t)min(s0 + SG * j, splits - 1) * p.rows;
                 ml[j] = p.part_ml[i];
                 const f32x4* from = reinterpret_cast<const f32x4*>(p.part + i * p.D + d);
                 x[j][0] = from[0];
@@ -990,7 +1069,7 @@ __global__ void __launch_bounds__(256) merge_kernel(AttendParams p) {
             float m = all.m;
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j)
-                if (s0 + SG * j < p.splits) m = fmaxf(m, ml[j][0]);
+                if (s0 + SG * j < splits) m = fmaxf(m, ml[j][0]);
             const float f = weight(all.m, m);
             all.m = m;
             all.l *= f;
@@ -998,7 +1077,7 @@ __global__ void __launch_bounds__(256) merge_kernel(AttendParams p) {
             for (int k = 0; k < 8; ++k) acc[k] *= f;
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
-                if (s0 + SG * j >= p.splits) break;
+                if (s0 + SG * j >= splits) break;
                 const float w = weight(ml[j][0], m);
                 all.l += w * ml[j][1];
 #pragma unroll
@@ -1036,7 +1115,7 @@ struct Plan {
     bool tile, eight, two;        // the tile kernel; of the other, eight waves, two groups of rows
     int groups, splits, per_group;
     int64_t items, rows;
-    size_t part, ml;              // bytes
+    size_t part, ml, shares;      // bytes
 };
 
 // The tile kernel takes calls of more than TILE_ROWS rows of a key head that have more than
@@ -1097,21 +1176,20 @@ Plan attend_plan(const nkv_paged_attend_args* a) {
         return pl;
     }
     // Else one workgroup a CU, as a start and a merge cost more than latency (8 heads of
-    // 4,096 keys, 4 rows: 128, 256, 512 workgroups 10.2, 8.7, 10.3 us), of four waves, or
-    // eight where sequences have lengths of their own: half as many of those in short calls
-    // (128 heads of 2,048 keys: 128, 256 workgroups 20.2, 21.4; 64 of 8,192: 37.4, 35.4), and
-    // two a CU in long ones, so that CUs with short sequences take more (32 of up to 16,384
-    // keys, 8 heads: 272, 251).  Two groups of rows get eight waves and one workgroup a CU
-    // at most (four waves with one a CU, with two, eight with one: 8 heads of 4,096 keys, 256
-    // rows 23.0, 23.4, 20.4; 64 of 2,048, 64 rows 23.4, 22.7, 21.7), or four where there
-    // are more (12 heads of 1,185 keys, 760 rows: eight 36, four 23).
+    // 4,096 keys, 4 rows: 128, 256, 512 workgroups 10.2, 8.7, 10.3 us), of four waves; two a
+    // CU in long calls of unlike lengths (8 sequences evenly up to 32,768 keys, 8 heads: 103,
+    // 102), and there eight waves where sequences have one or two splits (32 up to 16,384:
+    // 228, 218).  Two groups of rows get eight waves and one workgroup a CU at most (four
+    // waves with one a CU, with two, eight with one: 8 heads of 4,096 keys, 256 rows 23.0,
+    // 23.4, 20.4; 64 of 2,048, 64 rows 23.4, 22.7, 21.7), or four where there are more (12
+    // heads of 1,185 keys, 760 rows: eight 36, four 23).
     const int64_t least = std::max<int64_t>(base, 1);
     int64_t splits = 256 / least;
     if (pl.two) {
         pl.eight = base <= 256;
     } else {
-        pl.eight = uneven && work >= 4096;
-        splits = cdiv(!uneven ? 256 : work >= 32768 ? 512 : work >= 16384 ? 256 : 128, least);
+        splits = cdiv(uneven && work >= 32768 ? 512 : 256, least);
+        pl.eight = uneven && work >= 4096 && splits <= 2;
     }
     pl.splits = (int)std::max<int64_t>(1, std::min(splits, tiles / (pl.eight ? 8 : 4)));
     pl.items = base * pl.splits;
@@ -1123,7 +1201,8 @@ Plan attend_plan(const nkv_paged_attend_args* a) {
 void attend_fit(const nkv_paged_attend_args* a, Plan& pl, size_t limit) {
     if (pl.splits == 1) return;
     const size_t rows = (size_t)a->B * a->cache.H * pl.rows;
-    const size_t most = limit / (rows * (sizeof(f32x2) + 4 * a->cache.D));
+    const size_t shares = a->length && a->B > 1 && a->B <= BALANCED ? a->B * sizeof(i32x2) : 0;
+    const size_t most = limit < shares ? 0 : (limit - shares) / (rows * (sizeof(f32x2) + 4 * a->cache.D));
     if (most < (size_t)pl.splits) {
         pl.items /= pl.splits;
         pl.splits = (int)std::max<size_t>(1, most);
@@ -1132,6 +1211,7 @@ void attend_fit(const nkv_paged_attend_args* a, Plan& pl, size_t limit) {
     }
     pl.part = rows * pl.splits * 4 * a->cache.D;
     pl.ml = rows * pl.splits * sizeof(f32x2);
+    pl.shares = shares;
 }
 
 // Also plans the call, for a workspace of that many bytes, where there is something to do
@@ -1184,7 +1264,7 @@ int check_attend(const nkv_paged_attend_args* a, Plan& pl, const void* workspace
     NKV_REQUIRE(!lse.meets(out) && !lse.meets(q), NKV_ERR_INVALID, "lse overlaps q or out");
     NKV_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0 || pl.part == 0, NKV_ERR_INVALID,
                 "workspace must be 16-byte aligned");
-    const Range work(workspace, workspace ? pl.part + pl.ml : 0);
+    const Range work(workspace, workspace ? pl.part + pl.ml + pl.shares : 0);
     NKV_REQUIRE(!work.meets(q) && !work.meets(out) && !work.meets(lse), NKV_ERR_INVALID,
                 "workspace overlaps q, out or lse");
     for (const Range& r : in)
@@ -1252,7 +1332,7 @@ extern "C" size_t nkv_paged_attend_workspace_size(const nkv_paged_attend_args* a
     clear_error();
     Plan pl{};
     if (check_attend(a, pl, nullptr, SIZE_MAX) || pl.items == 0) return 0;
-    return pl.part + pl.ml;
+    return pl.part + pl.ml + pl.shares;
 }
 
 extern "C" int nkv_paged_attend(void* stream, const nkv_paged_attend_args* a, void* workspace,
@@ -1287,8 +1367,8 @@ extern "C" int nkv_paged_attend(void* stream, const nkv_paged_attend_args* a, vo
     p.rows = (int)pl.rows;
     p.page_d = c.page * c.D;
     p.per_group = pl.per_group;
-    p.by_G = divisor(a->G), p.by_H = divisor(c.H), p.by_BH = divisor((int64_t)a->B * c.H);
-    p.by_splits = divisor(pl.splits), p.by_groups = divisor(pl.groups);
+    p.shares = pl.shares ? (i32x2*)((char*)workspace + pl.part + pl.ml) : nullptr;
+    p.by_G = divisor(a->G), p.by_H = divisor(c.H), p.by_B = divisor(a->B), p.by_groups = divisor(pl.groups);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     rc = c.dtype == NKV_ROWS_BF16 ? attend_width<Bf16>(p, pl, s) : attend_width<Fp16>(p, pl, s);
     if (rc) return rc;

@@ -92,6 +92,27 @@ def test_views_and_shared_pages(dev, Q, n):
     assert torch.equal(got[0], want[0]) and got[1] is None
 
 
+@pytest.mark.parametrize("Q,Hq", [(1, 8), (3, 16), (24, 8), (150, 16)])
+@pytest.mark.parametrize("lengths", [
+    [9000] + [17] * 9, [0, 5000, 0, 1, 129, 4999], [3000 + 128 * i for i in range(5)], [2500] * 4, [0, 0, 4000],
+    [1] * 63 + [6000], [40 * i for i in range(65)],
+])
+def test_sequences_of_unlike_lengths(dev, Q, Hq, lengths):
+    """Splits by length: one long among short ones, empty ones, as many as a wave's lanes
+    and one more; some without queries; in a smaller workspace too."""
+    B, H, D = len(lengths), 2, 64
+    cache, table = make_pool(dev, lengths, H, D, 64, torch.bfloat16, 11)
+    q = queries(dev, B, Q, Hq, D, torch.bfloat16, 12)
+    length = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    check_large(q, cache, table, lengths, *ops.paged_attend(q, cache, table, length))
+    counts = [Q if b % 3 else b % 2 * (Q // 2) for b in range(B)]
+    ct = torch.tensor(counts, dtype=torch.int32, device=dev)
+    for size in (None, 100, 8 * B + 3 * B * Hq * Q * (4 * D + 8)):
+        work = None if size is None else torch.empty(size, dtype=torch.uint8, device=dev)
+        out, lse = ops.paged_attend(q, cache, table, length, causal=True, counts=ct, workspace=work)
+        check_large(q, cache, table, lengths, out, lse, True, None, counts)
+
+
 def test_calls_on_several_streams_with_splits(dev):
     """Calls of both kernels with key splits, several at once: each has a workspace of its
     own."""
