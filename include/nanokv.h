@@ -1057,7 +1057,8 @@ typedef struct nkv_paged_attend_args {
 
 /* Bytes of workspace nkv_paged_attend wants for these arguments (0 if none), for
  * the partial results of its key splits; 16-byte aligned.  In a smaller one, or
- * none, it takes fewer splits (the same attention within rounding). */
+ * none, it takes fewer splits (the same attention within rounding; how a sequence's
+ * keys are split depends on the call's shape and the lengths of its sequences). */
 size_t nkv_paged_attend_workspace_size(const nkv_paged_attend_args* args);
 int nkv_paged_attend(void* stream, const nkv_paged_attend_args* args, void* workspace,
                      size_t workspace_bytes);

@@ -691,8 +691,8 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
 // of the cycles); the copies' lanes take their chunks from where that is.  Columns past
 // D are zeros.
 //
-// 1,560 queries of 24 heads over 12,480 keys, 239 GFLOP, three splits: 262 to 270
-// us, 890 to 910 TFLOP/s, and a merge of 11.  The matrix units are busy 36 % of the SIMDs'
+// 1,560 queries of 24 heads over 12,480 keys, 239 GFLOP, three splits: 261 to 275
+// us, 870 to 910 TFLOP/s, and a merge of 11.  The matrix units are busy 36 % of the SIMDs'
 // cycles and the vector units 40 %: the softmax runs beside the products too little.  16
 // sequences of 8,192 keys, 8 heads, 256 rows, 137 GFLOP and 537 MB: 178 us.
 constexpr int TILE_WAVES = 8, TILE_KEYS = 128;
