@@ -346,9 +346,8 @@ extern "C" int nkv_paged_append(void* stream, const nkv_paged_append_args* a) {
             NKV_REQUIRE(!r.meets(x) && !q_out.meets(x), NKV_ERR_INVALID,
                         "the pools or q_out overlap the table, start_dev, counts, freqs or positions");
     }
-    if (a->q_out != a->q)
-        NKV_REQUIRE(!q_out.meets(q) && !q_out.meets(k) && !q_out.meets(v), NKV_ERR_INVALID,
-                    "q_out overlaps the rows");
+    NKV_REQUIRE(!q_out.meets(k) && !q_out.meets(v) && (a->q_out == a->q || !q_out.meets(q)),
+                NKV_ERR_INVALID, "q_out overlaps the rows");
     AppendParams p{};
     p.table = table;
     p.pool_k = (uint16_t*)c.k;
