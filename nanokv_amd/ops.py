@@ -1846,6 +1846,24 @@ def paged_attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, length
     return out, lse
 
 
+def _paged_disjoint(pools: list, read: tuple) -> None:
+    """The refusals of nkv_paged_commit that depend on the pools, for all launches of a
+    call before the first: one that a later launch makes would find layers moved."""
+    nbytes = pools[0].numel() * pools[0].element_size()
+    at = sorted(t.data_ptr() for t in pools)
+    if any(p % 16 for p in at):
+        raise ValueError("cache pages must be 16-byte aligned")
+    if any(b - a < nbytes for a, b in zip(at, at[1:])):
+        raise ValueError("caches overlap")
+    for t in read:
+        if t is None or t.numel() == 0:
+            continue
+        lo = t.data_ptr()
+        hi = lo + 4 * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+        if any(p < hi and lo < p + nbytes for p in at):
+            raise ValueError("the caches overlap table, rows, start or counts")
+
+
 def paged_commit(caches, table: torch.Tensor, start, rows: torch.Tensor,
                  counts: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Keep the accepted tokens of a draft, in place (see nkv_paged_commit).
@@ -1854,7 +1872,8 @@ def paged_commit(caches, table: torch.Tensor, start, rows: torch.Tensor,
     start + rows[b, j] of sequence b moves to row start + j for j < counts[b].  rows:
     int32 [B, M], M at most 256, in any order; counts: int32 [B] (default: all M);
     start: an int or an int32 tensor [B], as paged_append's.  Returns the new lengths,
-    start + counts, int32 [B]."""
+    start + counts, int32 [B].  No two pools of the caches share memory; more than 64
+    caches take a launch for each 64, and what is refused is refused before the first."""
     caches = [caches] if isinstance(caches, PagedCache) else list(caches)
     if not caches:
         raise ValueError("a cache is required")
@@ -1874,6 +1893,8 @@ def paged_commit(caches, table: torch.Tensor, start, rows: torch.Tensor,
     path = _int_rows(rows, B, M, "rows")
     first, n = _cache8_ints(given, B, "start"), _cache8_ints(counts, B, "counts")
     length = torch.empty(B, device=device, dtype=torch.int32)
+    if len(caches) > _lib.NKV_PAGED_CACHES and B:
+        _paged_disjoint(pools, (table, rows, given, counts))
     for i in range(0, len(pools), 2 * _lib.NKV_PAGED_CACHES):
         part = [t.data_ptr() for t in pools[i:i + 2 * _lib.NKV_PAGED_CACHES]]
         a = NkvPagedCommitArgs(c, (c_void_p * len(part))(*part), len(part) // 2, at, sb, width,
