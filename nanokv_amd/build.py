@@ -14,6 +14,8 @@ import subprocess
 import sys
 from pathlib import Path
 
+from nanokv_amd._waits import check_waits
+
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 INCLUDE = HERE.parent / "include"
@@ -44,6 +46,10 @@ SOURCES = {
     "nkv_paged.hip": [],
     "nkv_paged_attend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
+
+# Sources with hand-written counted waits: their listing is kept beside the object, and
+# a library in which such a wait may come too early is not linked.
+COUNTED_WAITS = ("nkv_paged_attend.hip",)
 
 COMMON = [
     f"--offload-arch={ARCH}",
@@ -78,6 +84,11 @@ def _run(cmd: list[str]) -> None:
         print(out, file=sys.stderr)
 
 
+def listing(src: str) -> Path:
+    """The kernels' assembly listing of a source of COUNTED_WAITS, once it is built."""
+    return HERE / "_build" / f"{Path(src).stem}-hip-amdgcn-amd-amdhsa-{ARCH}.s"
+
+
 def build(verbose: bool = False, jobs: int | None = None) -> Path:
     """Compile every source and link the library; returns its path."""
     objdir = HERE / "_build"
@@ -88,6 +99,8 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
     for src, extra in SOURCES.items():
         obj = objdir / (Path(src).stem + ".o")
         objs.append(obj)
+        if src in COUNTED_WAITS:
+            extra = [*extra, "--save-temps=obj"]
         cmds.append([cc, *COMMON, *extra, "-c", str(CSRC / src), "-o", str(obj)])
     procs = []
     for cmd in cmds:
@@ -106,6 +119,9 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
             print(out, file=sys.stderr)
     if errors:
         raise RuntimeError("\n".join(errors))
+    for src in COUNTED_WAITS:
+        if not check_waits(listing(src).read_text()):
+            raise RuntimeError(f"{src}: no counted wait in its listing")
     lib = HERE / LIB_NAME
     tmp = HERE / (LIB_NAME + ".tmp")
     _run([cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)])

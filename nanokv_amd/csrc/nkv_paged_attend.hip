@@ -520,7 +520,8 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
     auto step = [&](int tile, auto more) {
         const int key0 = tile * TILE;
         there[0] = next_there[0], there[1] = next_there[1];
-        // K's copies have arrived, V's loads need not have
+        // K's copies have arrived, V's loads need not have (the build counts the loads behind
+        // the copies in the listing, and refuses fewer than eight)
         asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
         const unsigned char* kb = sm.k[wave][(tile - w0) & 1];
         f32x4 s[NQ][2];
