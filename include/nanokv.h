@@ -973,7 +973,8 @@ typedef struct nkv_paged_cache {
  * Rows are 16-byte aligned, strides divisible by 8 and not negative.  q_out may be q
  * itself and overlaps nothing else of the call, nor do its rows each other; the pools
  * overlap neither each other nor anything else of the call, and no row is written
- * twice: no two sequences write into the same page.
+ * twice: no two sequences write into the same page.  (Overlaps of memory are refused,
+ * but for rows of unlike strides that both have gaps, which are not compared.)
  */
 typedef struct nkv_paged_append_args {
     nkv_paged_cache cache;
@@ -1030,7 +1031,7 @@ int nkv_paged_append(void* stream, const nkv_paged_append_args* args);
  * has one there, NaN in place of an infinity where its weight rounds to zero.
  * q and out are 16-byte aligned, their strides divisible by 8 and not negative; out's
  * rows do not overlap.  out may be q itself; otherwise out, lse and the workspace overlap
- * nothing of the call.
+ * nothing of the call, which is refused as nkv_paged_append's overlaps are.
  */
 #define NKV_PAGED_TREE 256
 typedef struct nkv_paged_attend_args {

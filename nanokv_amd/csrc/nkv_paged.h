@@ -52,4 +52,24 @@ inline int64_t table_bytes(int B, int64_t sb, int64_t w) { return B ? ((B - 1) *
 // two of them overlap (or a stride is negative).
 int64_t rows_span(int64_t s0, int64_t n0, int64_t s1, int64_t n1, int64_t s2, int64_t n2, int D);
 
+// Rows of `bytes` bytes, some of them or none (bytes = 0), at `at` + multiples of three
+// strides, in bytes; they lie in the `span` bytes from there on (host).
+struct RowSet {
+    uintptr_t at = 0;
+    int64_t bytes = 0;
+    __int128 span = 0;
+    struct {
+        int64_t stride = 0, count = 1;
+    } dims[3];
+    // strides of elements of es bytes, not negative; none where p is null
+    RowSet(const void* p, int es, int D, int64_t s0, int64_t n0, int64_t s1, int64_t n1, int64_t s2, int64_t n2);
+    RowSet(const Range& r) : at(r.lo), bytes((int64_t)(r.hi - r.lo)), span(bytes) {}
+};
+
+// Whether two sets have a byte in common.  Exact for rows that do not overlap within their
+// set where one set has no gaps, or both have the same strides (slices of one projection);
+// rows that do overlap are taken for all that they span, and others of unlike strides, both
+// with gaps, for apart.
+bool rows_meet(const RowSet& a, const RowSet& b);
+
 }  // namespace nkv

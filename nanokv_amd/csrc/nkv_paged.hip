@@ -255,6 +255,87 @@ int64_t rows_span(int64_t s0, int64_t n0, int64_t s1, int64_t n1, int64_t s2, in
     return end > INT64_MAX / 8 ? -1 : (int64_t)end;
 }
 
+RowSet::RowSet(const void* p, int es, int D, int64_t s0, int64_t n0, int64_t s1, int64_t n1,
+               int64_t s2, int64_t n2) {
+    if (!p) return;
+    at = reinterpret_cast<uintptr_t>(p);
+    span = bytes = (int64_t)D * es;
+    const int64_t s[3] = {s0, s1, s2}, n[3] = {n0, n1, n2};
+    // (a dimension of stride 0 is the same rows again)
+    for (int i = 0; i < 3; ++i)
+        if (s[i] > 0 && n[i] > 1) {
+            dims[i].stride = std::min(s[i], INT64_MAX / 8) * es;
+            dims[i].count = n[i];
+            span += (__int128)dims[i].stride * (n[i] - 1);
+        }
+}
+
+namespace {
+
+struct Steps {
+    __int128 stride, count;
+};
+
+// A set's dimensions in descending order of their strides.
+struct Nest {
+    Steps d[3];
+    int n = 0;
+    bool apart = true, packed;             // no two rows overlap; no gaps either
+    explicit Nest(const RowSet& r) {
+        __int128 rows = 1, span = r.bytes;
+        for (const auto& x : r.dims)
+            if (x.count > 1) d[n++] = {x.stride, x.count};
+        std::sort(d, d + n, [](const Steps& a, const Steps& b) { return a.stride > b.stride; });
+        for (int i = n - 1; i >= 0; --i) {
+            apart = apart && d[i].stride >= span;
+            span += d[i].stride * (d[i].count - 1);
+            rows *= d[i].count;
+        }
+        packed = apart && span == rows * r.bytes;
+    }
+};
+
+// Whether one of the rows of `bytes` bytes at `at` + multiples of n strides (descending)
+// meets [lo, hi).  Of a dimension's parts only those that reach over an end of it are looked
+// into: a part inside it holds a row.
+bool steps_meet(const Steps* d, int n, __int128 at, __int128 bytes, __int128 lo, __int128 hi) {
+    if (n == 0) return at < hi && at + bytes > lo;
+    __int128 part = bytes;
+    for (int i = 1; i < n; ++i) part += d[i].stride * (d[i].count - 1);
+    const __int128 s = d[0].stride, before = lo - part - at;
+    if (hi <= at) return false;
+    const __int128 first = before < 0 ? 0 : before / s + 1, last = std::min((hi - 1 - at) / s, d[0].count - 1);
+    for (__int128 i = first; i <= last; ++i) {
+        const __int128 x = at + i * s;
+        if ((x >= lo && x + part <= hi) || steps_meet(d + 1, n - 1, x, bytes, lo, hi)) return true;
+    }
+    return false;
+}
+
+}  // namespace
+
+bool rows_meet(const RowSet& a, const RowSet& b) {
+    const __int128 ax = a.at, by = b.at;
+    if (a.bytes == 0 || b.bytes == 0 || ax >= by + b.span || by >= ax + a.span) return false;
+    const Nest x(a), y(b);
+    if (!x.apart || !y.apart) return true;
+    if (x.packed) return steps_meet(y.d, y.n, by, b.bytes, ax, ax + a.span);
+    if (y.packed) return steps_meet(x.d, x.n, ax, a.bytes, by, by + b.span);
+    // like strides: the distances between a row of each are steps of the same strides
+    Steps d[3];
+    int n = 0;
+    __int128 at = ax - by;
+    for (int i = 0; i < 3; ++i) {
+        const auto &p = a.dims[i], &q = b.dims[i];
+        if (p.count > 1 && q.count > 1 && p.stride != q.stride) return false;
+        const __int128 stride = p.count > 1 ? p.stride : q.stride;
+        at -= stride * (q.count - 1);
+        if (p.count > 1 || q.count > 1) d[n++] = {stride, (__int128)p.count + q.count - 1};
+    }
+    std::sort(d, d + n, [](const Steps& l, const Steps& r) { return l.stride > r.stride; });
+    return steps_meet(d, n, at, 1, 1 - (__int128)a.bytes, b.bytes);
+}
+
 namespace {
 
 template <typename T>
@@ -307,46 +388,41 @@ extern "C" int nkv_paged_append(void* stream, const nkv_paged_append_args* a) {
                     (a->k_sb | a->k_st | a->k_sh | a->v_sb | a->v_st | a->v_sh) % 8 == 0 &&
                     (Hq == 0 || (a->q_sb | a->q_st | a->q_sh | a->o_sb | a->o_st | a->o_sh) % 8 == 0),
                 NKV_ERR_INVALID, "rows must be 16-byte aligned with strides divisible by 8");
-    // what is written, the pools and q_out, and what is read; a q_out with gaps may
-    // have anything in them
-    const int64_t rows = (int64_t)a->B * a->T * Hq;
-    int64_t span = 0;
+    NKV_REQUIRE(a->k_sb >= 0 && a->k_st >= 0 && a->k_sh >= 0 && a->v_sb >= 0 && a->v_st >= 0 &&
+                    a->v_sh >= 0 && (Hq == 0 || (a->q_sb >= 0 && a->q_st >= 0 && a->q_sh >= 0)),
+                NKV_ERR_INVALID, "strides must not be negative");
+    // what is written, the pools and q_out, and what is read
     if (Hq) {
-        span = rows_span(a->o_sb, a->B, a->o_st, a->T, a->o_sh, Hq, c.D);
-        NKV_REQUIRE(span > 0, NKV_ERR_INVALID, "q_out's rows overlap");
+        NKV_REQUIRE(rows_span(a->o_sb, a->B, a->o_st, a->T, a->o_sh, Hq, c.D) > 0, NKV_ERR_INVALID,
+                    "q_out's rows overlap");
         NKV_REQUIRE(a->q_out != a->k && a->q_out != a->v, NKV_ERR_INVALID, "q_out overlaps the rows");
         if (a->q_out == a->q)
             NKV_REQUIRE(a->dtype == c.dtype && a->q_sb == a->o_sb && a->q_st == a->o_st && a->q_sh == a->o_sh,
                         NKV_ERR_INVALID, "q_out over q must have its type and strides");
     }
+    const int es = a->dtype == NKV_ROWS_FP32 ? 4 : 2;
+    const RowSet k(a->k, es, c.D, a->k_sb, a->B, a->k_st, a->T, a->k_sh, c.H);
+    const RowSet v(a->v, es, c.D, a->v_sb, a->B, a->v_st, a->T, a->v_sh, c.H);
+    const RowSet q(a->q, es, c.D, a->q_sb, a->B, a->q_st, a->T, a->q_sh, Hq);
+    const RowSet q_out(a->q_out, 2, c.D, a->o_sb, a->B, a->o_st, a->T, a->o_sh, Hq);
     const Range pools[2] = {{c.k, pool_bytes(c)}, {c.v, pool_bytes(c)}};
-    const Range q_out(a->q_out, Hq && span == rows * c.D ? span * 2 : 0);
     const Range small[5] = {{a->table, table_bytes(a->B, a->table_sb, a->table_w)},
                             {a->start_dev, a->start_dev ? a->B * 4 : 0},
                             {a->counts, a->counts ? a->B * 4 : 0},
                             {a->freqs, a->freqs ? a->rot * 2 : 0},
                             {a->positions, a->positions ? table_bytes(a->B, a->pos_sb, a->T) : 0}};
-    const int64_t es = a->dtype == NKV_ROWS_FP32 ? 4 : 2;
-    // (the extents of rows: of any strides that are not negative)
-    auto extent = [&](const void* at, int64_t sb, int64_t st, int64_t sh, int heads) {
-        const __int128 n = (__int128)(a->B - 1) * sb + (__int128)(a->T - 1) * st + (__int128)(heads - 1) * sh + c.D;
-        return Range(at, at ? es * (int64_t)std::min<__int128>(n, INT64_MAX / 8) : 0);
-    };
-    NKV_REQUIRE(a->k_sb >= 0 && a->k_st >= 0 && a->k_sh >= 0 && a->v_sb >= 0 && a->v_st >= 0 &&
-                    a->v_sh >= 0 && (Hq == 0 || (a->q_sb >= 0 && a->q_st >= 0 && a->q_sh >= 0)),
-                NKV_ERR_INVALID, "strides must not be negative");
-    const Range k = extent(a->k, a->k_sb, a->k_st, a->k_sh, c.H);
-    const Range v = extent(a->v, a->v_sb, a->v_st, a->v_sh, c.H);
-    const Range q = extent(a->q, a->q_sb, a->q_st, a->q_sh, std::max(Hq, 1));
     NKV_REQUIRE(!pools[0].meets(pools[1]), NKV_ERR_INVALID, "the pools overlap each other");
     for (const Range& r : pools) {
-        NKV_REQUIRE(!r.meets(k) && !r.meets(v) && !r.meets(q) && !r.meets(q_out), NKV_ERR_INVALID,
-                    "the pools overlap the rows");
+        NKV_REQUIRE(!rows_meet(r, k) && !rows_meet(r, v) && !rows_meet(r, q) && !rows_meet(r, q_out),
+                    NKV_ERR_INVALID, "the pools overlap the rows");
         for (const Range& x : small)
-            NKV_REQUIRE(!r.meets(x) && !q_out.meets(x), NKV_ERR_INVALID,
-                        "the pools or q_out overlap the table, start_dev, counts, freqs or positions");
+            NKV_REQUIRE(!r.meets(x), NKV_ERR_INVALID,
+                        "the pools overlap the table, start_dev, counts, freqs or positions");
     }
-    NKV_REQUIRE(!q_out.meets(k) && !q_out.meets(v) && (a->q_out == a->q || !q_out.meets(q)),
+    for (const Range& x : small)
+        NKV_REQUIRE(!rows_meet(q_out, x), NKV_ERR_INVALID,
+                    "q_out overlaps the table, start_dev, counts, freqs or positions");
+    NKV_REQUIRE(!rows_meet(q_out, k) && !rows_meet(q_out, v) && (a->q_out == a->q || !rows_meet(q_out, q)),
                 NKV_ERR_INVALID, "q_out overlaps the rows");
     AppendParams p{};
     p.table = table;

@@ -1248,25 +1248,26 @@ int check_attend(const nkv_paged_attend_args* a, Plan& pl, const void* workspace
     pl = attend_plan(a);
     NKV_REQUIRE(pl.items <= 1 << 22, NKV_ERR_UNSUPPORTED, "too many query rows");
     attend_fit(a, pl, bytes);
-    const int64_t span = rows_span(a->o_sb, a->B, a->o_st, a->Q, a->o_sh, (int64_t)c.H * a->G, c.D);
-    NKV_REQUIRE(span > 0, NKV_ERR_INVALID, "out's rows overlap");
-    // what is written and what is read; an out or q with gaps may have anything in them
-    const int64_t rows = (int64_t)a->B * c.H * a->G * a->Q;
-    const bool packed = rows_span(a->q_sb, a->B, a->q_st, a->Q, a->q_sh, (int64_t)c.H * a->G, c.D) == rows * c.D;
-    const Range q(a->q, packed ? rows * c.D * 2 : 0);
+    NKV_REQUIRE(rows_span(a->o_sb, a->B, a->o_st, a->Q, a->o_sh, (int64_t)c.H * a->G, c.D) > 0,
+                NKV_ERR_INVALID, "out's rows overlap");
+    // what is written and what is read
+    const int64_t heads = (int64_t)c.H * a->G;
+    const RowSet q(a->q, 2, c.D, a->q_sb, a->B, a->q_st, a->Q, a->q_sh, heads);
+    const RowSet out(a->out, 2, c.D, a->o_sb, a->B, a->o_st, a->Q, a->o_sh, heads);
     const Range in[6] = {{c.k, pool_bytes(c)}, {c.v, pool_bytes(c)},
                          {a->table, table_bytes(a->B, a->table_sb, a->table_w)},
                          {a->length, a->length ? a->B * 4 : 0}, {a->counts, a->counts ? a->B * 4 : 0},
                          {a->parents, a->parents ? table_bytes(a->B, a->parents_sb, a->Q) : 0}};
-    const Range lse(a->lse, a->lse ? rows * 4 : 0), out(a->out, span == rows * c.D ? rows * c.D * 2 : 0);
+    const Range lse(a->lse, a->lse ? a->B * heads * a->Q * 4 : 0);
     for (const Range& r : in)
-        NKV_REQUIRE(!r.meets(lse) && !r.meets(out), NKV_ERR_INVALID,
+        NKV_REQUIRE(!r.meets(lse) && !rows_meet(out, r), NKV_ERR_INVALID,
                     "out or lse overlaps the cache, table, length, counts or parents");
-    NKV_REQUIRE(!lse.meets(out) && !lse.meets(q), NKV_ERR_INVALID, "lse overlaps q or out");
+    NKV_REQUIRE(!rows_meet(out, lse) && !rows_meet(q, lse), NKV_ERR_INVALID,
+                "lse overlaps q or out");
     NKV_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0 || pl.part == 0, NKV_ERR_INVALID,
                 "workspace must be 16-byte aligned");
     const Range work(workspace, workspace ? pl.part + pl.ml + pl.shares : 0);
-    NKV_REQUIRE(!work.meets(q) && !work.meets(out) && !work.meets(lse), NKV_ERR_INVALID,
+    NKV_REQUIRE(!rows_meet(q, work) && !rows_meet(out, work) && !work.meets(lse), NKV_ERR_INVALID,
                 "workspace overlaps q, out or lse");
     for (const Range& r : in)
         NKV_REQUIRE(!work.meets(r), NKV_ERR_INVALID,
@@ -1275,7 +1276,7 @@ int check_attend(const nkv_paged_attend_args* a, Plan& pl, const void* workspace
         NKV_REQUIRE(a->q_sb == a->o_sb && a->q_st == a->o_st && a->q_sh == a->o_sh, NKV_ERR_INVALID,
                     "out over q must have its strides");
     else
-        NKV_REQUIRE(!out.meets(q), NKV_ERR_INVALID, "out overlaps q");
+        NKV_REQUIRE(!rows_meet(out, q), NKV_ERR_INVALID, "out overlaps q");
     return NKV_OK;
 }
 

@@ -1738,7 +1738,10 @@ def paged_append(cache: PagedCache, table: torch.Tensor, k: torch.Tensor, v: tor
     the cache's type, are returned (q_out: where they go, q itself allowed; rows past
     counts are left as they were there, and 0 in a new tensor).  Pairs are columns i and
     i + rot / 2, or 2 i and 2 i + 1 (interleaved).  positions: int32 [B, T] (or [T]),
-    default start + t."""
+    default start + t.
+    q_out may be q or lie between its rows (a slice of the same projection), and overlaps
+    nothing else; nor do the cache's pages.  Such overlaps are refused, but for those of
+    q_out with rows of other strides where both have gaps: that is the caller's to see to."""
     given = start if isinstance(start, torch.Tensor) else None
     device = _require_gpu(cache.k, cache.v, table, k, v, given, counts, q, q_out, freqs, positions)
     c = cache.struct()
@@ -1812,7 +1815,9 @@ def paged_attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, length
     Returns (out like q, lse [B, heads, Q] fp32 or None); a query that sees nothing gets
     0 and -inf.  workspace: optional uint8 buffer, nkv_paged_attend_workspace_size bytes
     or fewer (with fewer, fewer key splits); calls that may run at once, or captured
-    graphs, need one each."""
+    graphs, need one each.  out may be q or lie between its rows; it and workspace overlap
+    nothing else, which is refused but for an out and a q of unlike strides that both have
+    gaps."""
     device = _require_gpu(q, cache.k, cache.v, table, parents, counts, out,
                           length if isinstance(length, torch.Tensor) else None)
     c = cache.struct()
