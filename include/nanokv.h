@@ -1072,7 +1072,7 @@ int nkv_paged_attend(void* stream, const nkv_paged_attend_args* args, void* work
  * page, or comes from a negative row, is not written.
  *   rows        int32, device, M entries an item, M <= NKV_PAGED_COMMIT
  *   start_dev, counts: as nkv_paged_append's (NULL: start; M)
- *   out_length  [B] int32, start + counts (both as clamped), or NULL
+ *   out_length  [B] int32, start + counts (both as clamped; 2^31 - 1 at most), or NULL
  * pools is an array in host memory, of at most NKV_PAGED_CACHES caches.  The pools
  * overlap neither each other nor anything else of the call; no two sequences write
  * into the same page, and none into one that another reads here.

@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(256) commit_kernel(CommitParams p) {
     const int n = c8_length(p.counts, b, p.M);
     const int64_t start = paged_start(p.start_dev, b, p.start, p.table.cap());
     if (p.out_length && h == 0 && blockIdx.z == 0 && threadIdx.x == 0)
-        p.out_length[b] = (int32_t)(start + n);
+        p.out_length[b] = (int32_t)min(start + n, (int64_t)INT32_MAX);
     u32x4 x[ROUNDS][2];
     int64_t to[ROUNDS];
     uint16_t* const pk = p.pool[blockIdx.z][0];
