@@ -255,7 +255,11 @@ __device__ __forceinline__ int wave_sum(int v) {
 // Where lengths are in device memory, sequences (up to a wave's lanes) share the slots by
 // them: a split takes 128 tau keys for the least tau, two at least, with which all fit.  tau
 // = sum / (slots - B) and one more always does, as a sequence of t takes at most t / tau + 1.
-// Each wave finds this for itself, a sequence to a lane; the merge is told.  us with equal
+// Each wave finds this for itself, a sequence to a lane; the merge is told.  (Only where the
+// plan has splits to share: calls of 512 workgroups and more have none, and those of more
+// than 64 sequences equal ones, so that a long sequence sets the call's time: one of 131,072
+// keys and the others of 4,096, 8 heads, 63 sequences 287 us, 64 1,235; 4 heads, 64 167, 65
+// 642.)  us with equal
 // splits and with these, 8 heads: 16 sequences, 256 rows, one of 32,768 keys and the others
 // of 512 478, 87, lengths evenly up to 32,768 541, 395, all alike 663, 666; 32 sequences, 4
 // rows, one of 16,384 keys, the others of 256 61, 36; 4 sequences of 4,096 17.3, 18.7.
@@ -338,8 +342,11 @@ __device__ __forceinline__ Item item_of(const AttendParams& p) {
 // lanes: read from memory that is 64 accesses of the vector cache to a load (a CU then
 // moves 58 GB/s of a context, eight waves 75 us for 8,192 keys of 8 heads without
 // splits), so that K's rows pass through the wave's own LDS buffers (51 us).
-// Long calls are bound by memory: two heads of 262,144 keys, 268 MB, 41 us, 6.5 TB/s
-// beside a merge of 6; 32 ragged sequences up to 16,384, 1.47 GB, 246 us, 6.0 TB/s.
+// Long calls are bound by memory: two heads of 262,144 keys, 268 MB, 43 us, 6.2 TB/s
+// beside a merge of 6; 32 ragged sequences up to 16,384, 1.47 GB, 251 us, 5.9 TB/s.
+// Short ones by the start, the loads' latency and the exchange of the waves' rows: 8 heads
+// of 4,096 keys, one or two tiles to each wave of 256 workgroups, 16, 32 and 64 rows 6.9, 8.5
+// and 11.9 us (64 rows are eight waves' 135 KB through LDS), and a tree 0.3 to 0.8 more.
 constexpr int TILE = 32;
 
 // Page numbers of a run of tiles, 64 at a time, a lane each.
@@ -692,10 +699,17 @@ __global__ void __launch_bounds__(64 * W) attend_kernel(AttendParams p) {
 // of the cycles); the copies' lanes take their chunks from where that is.  Columns past
 // D are zeros.
 //
+// A weight is one number of the cache's type: bf16's 8 bits, rounded to the nearest, make a
+// result's error in norm 0.0018 to 0.0022 where its own rounding is 0.0017 (fp16's 11 bits
+// 0.0002 to 0.0003).  The other kernel's second bf16 number would add half again to the
+// products, which bound this one; sums and statistics are fp32.
+//
 // 1,560 queries of 24 heads over 12,480 keys, 239 GFLOP, three splits: 261 to 275
 // us, 870 to 910 TFLOP/s, and a merge of 11.  The matrix units are busy 36 % of the SIMDs'
-// cycles and the vector units 40 %: the softmax runs beside the products too little.  16
-// sequences of 8,192 keys, 8 heads, 256 rows, 137 GFLOP and 537 MB: 178 us.
+// cycles and the vector units 40 %: the softmax runs beside the products too little, and of
+// eight waves one has no rows (49 blocks of 32 are seven groups of seven).  16
+// sequences of 8,192 keys, 8 heads, 256 rows, 137 GFLOP and 537 MB: 178 us.  The form for
+// 128 columns fills the 256 registers of a lane, with six of them in scratch memory.
 constexpr int TILE_WAVES = 8, TILE_KEYS = 128;
 
 template <int P>
@@ -1314,7 +1328,9 @@ int attend_width(const AttendParams& p, const Plan& pl, hipStream_t s) {
                      : p.D <= 96 ? attend_run<T, 3>(p, pl, s) : attend_run<T, 4>(p, pl, s);
 }
 
-// Sixteen groups of threads to a row where there are few rows and splits to share (whole
+// Sixteen groups of threads to a row where there are few rows and splits to share, by the
+// mean of the sequences' splits (their number is known on the device only; a sequence may have
+// most of a call's, which one thread then reads four at a time) (whole
 // calls, us with sixteen and one: 32 rows of 32 splits 8.7, 16.7, of 12 21.3, 24.0; 128
 // rows of 8 18.0, 19.2, of 4 46.1, 46.3; 2,048 rows of 16 50.9, 49.7; 37,440 of 3 378, 278).
 template <typename T>

@@ -1812,6 +1812,8 @@ def paged_attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, length
     query t sees the rows before the draft, its own and those of its ancestors
     (parents[t] < t; anything else ends the way, -1 by custom).  A chain, parents[t] =
     t - 1, is the causal mask.
+    Scores and sums are fp32; softmax weights have the cache's type's bits for the product
+    with the values, bf16 ones twice as many in calls of few rows (see nkv_paged_attend).
     Returns (out like q, lse [B, heads, Q] fp32 or None); a query that sees nothing gets
     0 and -inf.  workspace: optional uint8 buffer, nkv_paged_attend_workspace_size bytes
     or fewer (with fewer, fewer key splits); calls that may run at once, or captured
