@@ -7,6 +7,7 @@ path: tensors must live on the GPU and the HIP library must be built.
 """
 from __future__ import annotations
 
+import bisect
 import ctypes
 import math
 from ctypes import byref, c_void_p
@@ -1853,11 +1854,11 @@ def paged_attend(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, length
     return out, lse
 
 
-def _paged_disjoint(pools: list, read: tuple) -> None:
-    """The refusals of nkv_paged_commit that depend on the pools, for all launches of a
-    call before the first: one that a later launch makes would find layers moved."""
-    nbytes = pools[0].numel() * pools[0].element_size()
-    at = sorted(t.data_ptr() for t in pools)
+def _paged_disjoint(pools: list, nbytes: int, read: tuple) -> None:
+    """The refusals of nkv_paged_commit that depend on the pools (pointers to that many
+    bytes each), for all launches of a call before the first: one that a later launch makes
+    would find layers moved."""
+    at = sorted(pools)
     if any(p % 16 for p in at):
         raise ValueError("cache pages must be 16-byte aligned")
     if any(b - a < nbytes for a, b in zip(at, at[1:])):
@@ -1867,7 +1868,8 @@ def _paged_disjoint(pools: list, read: tuple) -> None:
             continue
         lo = t.data_ptr()
         hi = lo + 4 * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-        if any(p < hi and lo < p + nbytes for p in at):
+        i = bisect.bisect_left(at, hi)           # the last pool that begins before hi
+        if i and lo < at[i - 1] + nbytes:
             raise ValueError("the caches overlap table, rows, start or counts")
 
 
@@ -1900,10 +1902,11 @@ def paged_commit(caches, table: torch.Tensor, start, rows: torch.Tensor,
     path = _int_rows(rows, B, M, "rows")
     first, n = _cache8_ints(given, B, "start"), _cache8_ints(counts, B, "counts")
     length = torch.empty(B, device=device, dtype=torch.int32)
+    pointers = [t.data_ptr() for t in pools]
     if len(caches) > _lib.NKV_PAGED_CACHES and B:
-        _paged_disjoint(pools, (table, rows, given, counts))
+        _paged_disjoint(pointers, pools[0].numel() * pools[0].element_size(), (table, rows, given, counts))
     for i in range(0, len(pools), 2 * _lib.NKV_PAGED_CACHES):
-        part = [t.data_ptr() for t in pools[i:i + 2 * _lib.NKV_PAGED_CACHES]]
+        part = pointers[i:i + 2 * _lib.NKV_PAGED_CACHES]
         a = NkvPagedCommitArgs(c, (c_void_p * len(part))(*part), len(part) // 2, at, sb, width,
                                *path, 0 if given is not None else int(start), first, n,
                                length.data_ptr(), B, M)
